@@ -661,6 +661,90 @@ KUIOPS_API int kuiops_decode_rows_batched(int64_t M, int64_t N, int64_t K, int d
                                const int64_t sv[3], int64_t cache_cap, void *workspace,
                                size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------- drafted trees, bounded caches --
+ * No reference counterparts: its app decodes one token at a time over a cache
+ * that only grows (infer.py:57-89).  Strides are in elements, batch / head /
+ * position, with contiguous rows; K / V rows must start 16-byte aligned.
+ *
+ * Attention of a tree of drafted tokens over a KV cache.  The last t of the
+ * L = kv_len[b] keys of a sequence (kv_len: device int32[n], at most s; null:
+ * s) are the nodes of its tree: node i is query i and key L - t + i.  parent
+ * (device int32[n][t]) gives each node's parent, an earlier node, or -1 for a
+ * node that follows the context directly.  Query i sees the L - t keys of the
+ * context, its ancestors and itself.  A node whose parent is below -1 or not
+ * an earlier node is absent, and so are its descendants: they see no key
+ * (output 0, lse -inf, their queries are not read).  Nodes whose key would lie
+ * before the first (kv_len[b] < t) are seen by nobody.  What the cache holds
+ * where a query does not look, NaN and infinities included, stays out of it.
+ * dtype BF16 / F16, e and ev multiples of 8 up to 256, t <= 256 and t <= s,
+ * scale > 0.  lse: fp32 [n][hq][t] (natural log) or null.  O must not overlap
+ * an input.  Workspace: kuiops_sdpa_tree_workspace bytes (may be 0), 16-byte
+ * aligned, no initialisation needed.                                       */
+KUIOPS_API size_t kuiops_sdpa_tree_workspace(int64_t n, int64_t hq, int64_t hkv, int64_t t, int64_t s, int64_t e,
+                                  int64_t ev);
+KUIOPS_API int kuiops_sdpa_tree(int64_t n, int64_t hq, int64_t hkv, int64_t t, int64_t s, int64_t e, int64_t ev,
+                     int dtype, const void *Q, const int64_t sq[3], const void *K, const int64_t sk[3],
+                     const void *V, const int64_t sv[3], void *O, const int64_t so[3], float *lse, float scale,
+                     const int32_t *parent, const int32_t *kv_len, void *workspace, size_t workspace_bytes,
+                     void *stream);
+
+/* Greedy acceptance of a drafted tree: the walk starts at node 0 (whose parent
+ * must be -1) and goes on to the lowest child whose token is target[] of the
+ * node it stands on (the model's choice after that node), until there is none.
+ * tokens, target: device int64[n][t]; parent: as above.  path (int32[n][t])
+ * gets the nodes in order, then -1; count (int32[n]) their number; next
+ * (int64[n]) the target of the last one (-1 if node 0 is absent).  t <= 256.  */
+KUIOPS_API int kuiops_tree_accept(int64_t n, int64_t t, const int64_t *tokens, const int32_t *parent,
+                       const int64_t *target, int32_t *path, int32_t *count, int64_t *next, void *stream);
+
+/* Moves the cache rows of an accepted path behind the context: with base =
+ * kv_len[b] - t, row base + path[b][i] goes to row base + i for every i before
+ * the path's end, its first entry that is below 0, not below t or outside the
+ * cache; len_out[b] = base + the path's length.  Any path is moved as if all
+ * rows were read first.  K / V have batch = a multiple of n entries (all
+ * layers' caches of n sequences): entry r belongs to sequence r % n.  krow /
+ * vrow: bytes of a row, multiples of 16; strides sk / sv in BYTES, multiples of
+ * 16, rows not overlapping.  path: device int32[n][p], p <= t, p <= 256.
+ * len_out must not overlap kv_len.  kv_len[b] < t: nothing moves and len_out[b]
+ * = kv_len[b].                                                             */
+KUIOPS_API int kuiops_kv_tree_commit(int64_t batch, int64_t n, int64_t hkv, int64_t cap, int64_t krow, int64_t vrow,
+                          void *K, const int64_t sk[3], void *V, const int64_t sv[3], int64_t p,
+                          const int32_t *path, int64_t t, const int32_t *kv_len, int32_t *len_out, void *stream);
+
+/* Decode attention (kuiops_sdpa_decode's semantics: causal queries are the
+ * last l of the kv_len[b] keys) that also adds to every key the weight that
+ * the queries of its KV head gave it: acc[b][g][j] += sum over the query heads
+ * h of group g and positions i of exp(scale q_i k_j - lse_i).  acc: fp32,
+ * strides sa = batch, head, unit key stride; keys at kv_len[b] and behind it
+ * keep theirs.  lse (required): fp32 [n][hq][l].  dtype, e, ev, scale and
+ * workspace as kuiops_sdpa_tree; causal needs l <= s.                      */
+KUIOPS_API size_t kuiops_sdpa_decode_accum_workspace(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s,
+                                          int64_t e, int64_t ev);
+KUIOPS_API int kuiops_sdpa_decode_accum(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e,
+                             int64_t ev, int dtype, const void *Q, const int64_t sq[3], const void *K,
+                             const int64_t sk[3], const void *V, const int64_t sv[3], void *O, const int64_t so[3],
+                             float *lse, float scale, int causal, const int32_t *kv_len, float *acc,
+                             const int64_t sa[2], void *workspace, size_t workspace_bytes, void *stream);
+
+/* Cuts every sequence with more than `budget` keys down to that many per KV
+ * head: the `recent` (<= budget) newest positions, those above the largest of
+ * pos[b][g][0 .. L) minus recent, then the keys with the largest acc (NaN above
+ * every number), the lowest slot winning a tie.  Kept rows at slots >= budget
+ * move into the freed slots below it, the i-th into the i-th, in place in K and
+ * V; their acc and pos go along into acc_out / pos_out, whose slots from the
+ * new length to the capacity become 0 and -1.  len_out[b] = min(kv_len[b],
+ * budget).  Slots of K / V from the budget on are not written.  acc_out, pos_out
+ * and len_out may be acc, pos and kv_len themselves, else must not overlap
+ * them.  krow / vrow / sk / sv as kuiops_kv_tree_commit (bytes); sa, sp, sao,
+ * spo: batch and head strides in elements, unit slot stride.  Workspace:
+ * kuiops_kv_evict_workspace(n, hkv, min(budget, cap)) bytes, no initialisation. */
+KUIOPS_API size_t kuiops_kv_evict_workspace(int64_t n, int64_t hkv, int64_t budget);
+KUIOPS_API int kuiops_kv_evict(int64_t n, int64_t hkv, int64_t cap, int64_t krow, int64_t vrow, void *K,
+                    const int64_t sk[3], void *V, const int64_t sv[3], const float *acc, const int64_t sa[2],
+                    const int32_t *pos, const int64_t sp[2], const int32_t *kv_len, int64_t budget,
+                    int64_t recent, float *acc_out, const int64_t sao[2], int32_t *pos_out, const int64_t spo[2],
+                    int32_t *len_out, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

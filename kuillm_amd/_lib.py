@@ -103,6 +103,18 @@ SIGNATURES = {
                                   _sz, _vp, _sz, _vp]),
     "kuiops_decode_step_error": (_int, [_vp, _i64, _vp]),
     "kuiops_decode_step_supported": (_int, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int]),
+    "kuiops_sdpa_tree_workspace": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "kuiops_sdpa_tree": (_int, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp, _i64p, _vp, _i64p, _vp, _i64p,
+                                _vp, _i64p, _vp, _flt, _vp, _vp, _vp, _sz, _vp]),
+    "kuiops_tree_accept": (_int, [_i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "kuiops_kv_tree_commit": (_int, [_i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64p, _vp, _i64p, _i64, _vp, _i64,
+                                     _vp, _vp, _vp]),
+    "kuiops_sdpa_decode_accum_workspace": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "kuiops_sdpa_decode_accum": (_int, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp, _i64p, _vp, _i64p, _vp,
+                                        _i64p, _vp, _i64p, _vp, _flt, _int, _vp, _vp, _i64p, _vp, _sz, _vp]),
+    "kuiops_kv_evict_workspace": (_sz, [_i64, _i64, _i64]),
+    "kuiops_kv_evict": (_int, [_i64, _i64, _i64, _i64, _i64, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp,
+                               _i64, _i64, _vp, _i64p, _vp, _i64p, _vp, _vp, _sz, _vp]),
 }
 
 

@@ -1,0 +1,363 @@
+// What happens to a KV cache besides attention, gfx950:
+//
+//   kuiops_tree_accept     the branch of a drafted tree that the model agrees with
+//   kuiops_kv_tree_commit  its rows moved behind the context
+//   kuiops_kv_evict        the cache cut down to the keys that weighed most
+//
+// All are copies and comparisons: results are exact, ties go to the lowest
+// index, and nothing depends on the order in which work-groups run.
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace kuiops {
+
+namespace {
+
+constexpr int kMaxTree = 256;                 // nodes of a tree
+
+// ------------------------------------------------------------ tree_accept
+// A wave per sequence, 4 nodes per lane.  A node is a candidate if its token is
+// the target of its parent; the walk from node 0 takes the lowest candidate
+// among the children, a ballot per 64 nodes and step.
+__global__ __launch_bounds__(64) void tree_accept_kernel(int t, const int64_t *tokens, const int32_t *parent,
+                                                         const int64_t *target, int32_t *path, int32_t *count, int64_t *next) {
+    constexpr int NW = kMaxTree / 64;
+    const int lane = threadIdx.x;
+    const int64_t b = blockIdx.x;
+    tokens += b * t;
+    parent += b * t;
+    target += b * t;
+    path += b * t;
+    int up[NW], mine[NW];                     // parent of a candidate (else -1); the path's node at this lane's place
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+        const int i = x * 64 + lane;
+        up[x] = mine[x] = -1;
+        if (i < t) {
+            const int p = parent[i];
+            if (p >= 0 && p < i && tokens[i] == target[p]) up[x] = p;
+        }
+    }
+    int at = parent[0] == -1 ? 0 : -1, last = -1, n = 0;
+    while (at >= 0) {
+#pragma unroll
+        for (int x = 0; x < NW; ++x)
+            if (n == x * 64 + lane) mine[x] = at;
+        ++n;
+        last = at;
+        at = -1;
+#pragma unroll
+        for (int x = NW - 1; x >= 0; --x) {
+            const uint64_t hits = __ballot(up[x] == last);
+            if (hits) at = x * 64 + __builtin_ctzll(hits);
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < NW; ++x)
+        if (x * 64 + lane < t) path[x * 64 + lane] = mine[x];
+    if (lane == 0) {
+        count[b] = n;
+        next[b] = last >= 0 ? target[last] : -1;
+    }
+}
+
+// --------------------------------------------------------- kv_tree_commit
+// A work-group has all rows of up to 512 bytes of a head's K or V: every row is
+// in registers before the first is written, so any path is right, whichever
+// rows it reads and overwrites.
+constexpr int kCommitThreads = 512, kCommitRegs = 16;       // x 16 bytes = 256 rows of 512
+struct CommitArgs {
+    int n, p, t;
+    int64_t cap;
+    char *K, *V;
+    int64_t sk0, sk1, sk2, sv0, sv1, sv2;     // bytes
+    int kcols, vcols, kblocks;                // 16-byte chunks of a row; work-groups of 32 chunks for K
+    const int32_t *path, *kv_len;
+    int32_t *len_out;
+};
+__global__ __launch_bounds__(kCommitThreads) void tree_commit_kernel(CommitArgs a) {
+    __shared__ int s_path[kMaxTree];
+    __shared__ int s_count;
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.z, head = blockIdx.y;
+    const int b = (int)(row % a.n);
+    const bool is_v = (int)blockIdx.x >= a.kblocks;
+    const int c0 = ((int)blockIdx.x - (is_v ? a.kblocks : 0)) * 32;
+    const int cols = min(32, (is_v ? a.vcols : a.kcols) - c0);
+    const int64_t len = a.kv_len[b], base = len - a.t;
+    if (tid == 0) s_count = a.p;
+    __syncthreads();
+    if (tid < a.p) {
+        const int x = a.path[(int64_t)b * a.p + tid];
+        s_path[tid] = x;
+        // the path ends at its first entry that is no row of the tree in the cache
+        if (x < 0 || x >= a.t || base < 0 || base + max(x, tid) >= a.cap) atomicMin(&s_count, tid);
+    }
+    __syncthreads();
+    const int count = s_count;
+    if (row < a.n && head == 0 && blockIdx.x == 0 && tid == 0) a.len_out[b] = (int)(base < 0 ? len : base + count);
+    char *p = is_v ? a.V + row * a.sv0 + head * a.sv1 : a.K + row * a.sk0 + head * a.sk1;
+    const int64_t st = is_v ? a.sv2 : a.sk2;
+    p += base * st + c0 * 16;
+    u32x4 r[kCommitRegs];
+#pragma unroll
+    for (int x = 0; x < kCommitRegs; ++x) {
+        const int i = x * kCommitThreads + tid, to = i / 32, c = i % 32;
+        if (to < count && c < cols && s_path[to] != to) r[x] = *reinterpret_cast<const u32x4 *>(p + s_path[to] * st + c * 16);
+    }
+    __builtin_amdgcn_s_waitcnt(0);            // read before any row is written
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < kCommitRegs; ++x) {
+        const int i = x * kCommitThreads + tid, to = i / 32, c = i % 32;
+        if (to < count && c < cols && s_path[to] != to) *reinterpret_cast<u32x4 *>(p + to * st + c * 16) = r[x];
+    }
+}
+
+// --------------------------------------------------------------- kv_evict
+// evict_select_kernel, a work-group per (sequence, KV head): the key of a slot
+// is its weight's bits in ascending order, or the largest of all for the
+// `recent` newest positions.  The budget-th largest key is found 8 bits at a
+// time with a histogram in LDS; slots with a larger key are kept, and of those
+// with the same key the first ones.  A pass in slot order then lists the freed
+// slots below the budget and the kept ones behind it: as many of one as of the
+// other, and the i-th kept row goes to the i-th freed slot.  Sources are at or
+// behind the budget and destinations below it, so the moves need no order.
+// evict_move_kernel moves the rows of K and V.
+constexpr int kEvictThreads = 1024;
+struct EvictArgs {
+    int n, hkv, budget, recent;
+    int64_t cap;
+    const int32_t *kv_len;
+    int32_t *len_out;
+    const float *acc;
+    const int32_t *pos;
+    float *acc_out;
+    int32_t *pos_out;
+    int64_t sa0, sa1, sp0, sp1, sao0, sao1, spo0, spo1;
+    int32_t *moves;            // [n * hkv][1 + 2 * budget]: count, destinations, sources
+    char *K, *V;
+    int64_t sk0, sk1, sk2, sv0, sv1, sv2;     // bytes
+    int kcols, vcols;                         // 16-byte chunks of a row
+};
+
+__device__ __forceinline__ uint32_t weight_key(float w) {
+    if (w != w) return 0xfffffffeu;           // NaN ranks above every number
+    const uint32_t u = __float_as_uint(w + 0.f);              // (-0 is 0)
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+__global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a) {
+    constexpr int NT = kEvictThreads, NW = NT / 64;
+    __shared__ int s_red[NW][3];
+    __shared__ int s_hist[256];
+    __shared__ uint32_t s_prefix;
+    __shared__ int s_need;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int b = blockIdx.x / a.hkv, hk = blockIdx.x % a.hkv, m = a.budget;
+    const int L = (int)max((int64_t)0, min((int64_t)a.kv_len[b], a.cap)), cap = (int)a.cap;
+    const float *acc = a.acc + b * a.sa0 + hk * a.sa1;
+    const int32_t *pos = a.pos + b * a.sp0 + hk * a.sp1;
+    float *acc_out = a.acc_out + b * a.sao0 + hk * a.sao1;
+    int32_t *pos_out = a.pos_out + b * a.spo0 + hk * a.spo1;
+    int32_t *moves = a.moves + (int64_t)blockIdx.x * (1 + 2 * m);
+    if (L <= m) {
+        for (int j = tid; j < cap; j += NT) {
+            acc_out[j] = j < L ? acc[j] : 0.f;
+            pos_out[j] = j < L ? pos[j] : -1;
+        }
+        if (tid == 0) moves[0] = 0;
+        return;
+    }
+    int newest = INT32_MIN;
+    for (int j = tid; j < L; j += NT) newest = max(newest, pos[j]);
+    newest = -wave_min_i32(-max(newest, -INT32_MAX));
+    if (lane == 0) s_red[wave][0] = newest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) newest = max(newest, s_red[w][0]);
+    const int64_t floor_pos = (int64_t)newest - a.recent;
+    auto key_of = [&](int j) -> uint32_t { return pos[j] > floor_pos ? 0xffffffffu : weight_key(acc[j]); };
+
+    uint32_t prefix = 0, mask = 0;
+    int need = m;                              // of the keys with this prefix, the need-th largest is sought
+    for (int sh = 24; sh >= 0; sh -= 8) {
+        if (tid < 256) s_hist[tid] = 0;
+        __syncthreads();
+        for (int j = tid; j < L; j += NT) {
+            const uint32_t k = key_of(j);
+            if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> sh) & 255], 1);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            int left = need, v = 255;
+            while (v > 0 && s_hist[v] < left) left -= s_hist[v--];
+            s_prefix = prefix | ((uint32_t)v << sh);
+            s_need = left;
+        }
+        __syncthreads();
+        prefix = s_prefix;
+        need = s_need;
+        mask |= 255u << sh;
+    }
+
+    // slots in order, 1024 at a time: running counts of equal keys, freed and far slots
+    int eq0 = 0, hole0 = 0, far0 = 0;
+    const uint64_t below = (1ull << lane) - 1;
+    for (int j0 = 0; j0 < L; j0 += NT) {
+        const int j = j0 + tid;
+        const uint32_t k = j < L ? key_of(j) : 0;
+        const bool eq = j < L && k == prefix;
+        const uint64_t eqs = __ballot(eq);
+        if (lane == 0) s_red[wave][0] = __popcll(eqs);
+        __syncthreads();
+        int eqr = eq0 + __popcll(eqs & below);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const int c = s_red[w][0];
+            if (w < wave) eqr += c;
+            eq0 += c;
+        }
+        const bool kept = j < L && (k > prefix || (eq && eqr < need));
+        const bool hole = j < m && !kept, far = j >= m && kept;
+        const uint64_t holes = __ballot(hole), fars = __ballot(far);
+        if (lane == 0) {
+            s_red[wave][1] = __popcll(holes);
+            s_red[wave][2] = __popcll(fars);
+        }
+        __syncthreads();
+        int hr = hole0 + __popcll(holes & below), fr = far0 + __popcll(fars & below);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            if (w < wave) { hr += s_red[w][1]; fr += s_red[w][2]; }
+            hole0 += s_red[w][1];
+            far0 += s_red[w][2];
+        }
+        if (hole) moves[1 + hr] = j;
+        if (far) moves[1 + m + fr] = j;
+        if (kept && !far) {
+            acc_out[j] = acc[j];
+            pos_out[j] = pos[j];
+        }
+    }
+    if (tid == 0) moves[0] = hole0;
+    __builtin_amdgcn_s_waitcnt(0);
+    __threadfence_block();
+    __syncthreads();
+    for (int i = tid; i < hole0; i += NT) {
+        const int to = moves[1 + i], from = moves[1 + m + i];
+        acc_out[to] = acc[from];
+        pos_out[to] = pos[from];
+    }
+    __builtin_amdgcn_s_waitcnt(0);             // (acc_out may be acc: read before it is cleared)
+    __syncthreads();
+    for (int j = m + tid; j < cap; j += NT) {
+        acc_out[j] = 0.f;
+        pos_out[j] = -1;
+    }
+}
+
+__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
+    const int bh = blockIdx.y, b = bh / a.hkv, hk = bh % a.hkv;
+    const int32_t *moves = a.moves + (int64_t)bh * (1 + 2 * a.budget);
+    const int count = moves[0], cols = a.kcols + a.vcols;
+    if (hk == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
+        const int len = a.kv_len[b];
+        a.len_out[b] = min(max(len, 0), (int)min((int64_t)a.budget, a.cap));
+    }
+    char *K = a.K + b * a.sk0 + hk * a.sk1, *V = a.V + b * a.sv0 + hk * a.sv1;
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < (int64_t)count * cols; x += (int64_t)gridDim.x * 256) {
+        const int i = (int)(x / cols), c = (int)(x % cols);
+        const int64_t to = moves[1 + i], from = moves[1 + a.budget + i];
+        if (c < a.kcols)
+            *reinterpret_cast<u32x4 *>(K + to * a.sk2 + c * 16) = *reinterpret_cast<const u32x4 *>(K + from * a.sk2 + c * 16);
+        else
+            *reinterpret_cast<u32x4 *>(V + to * a.sv2 + (c - a.kcols) * 16) =
+                *reinterpret_cast<const u32x4 *>(V + from * a.sv2 + (c - a.kcols) * 16);
+    }
+}
+
+bool rows_ok(const void *p, const int64_t *st, int64_t bytes) {
+    return aligned16(p) && bytes > 0 && bytes % 16 == 0 && st[0] % 16 == 0 && st[1] % 16 == 0 && st[2] % 16 == 0 &&
+           st[2] >= bytes && st[0] >= 0 && st[1] >= 0;
+}
+
+}  // namespace
+
+}  // namespace kuiops
+
+using namespace kuiops;
+
+extern "C" int kuiops_tree_accept(int64_t n, int64_t t, const int64_t *tokens, const int32_t *parent, const int64_t *target,
+                                  int32_t *path, int32_t *count, int64_t *next, void *stream) {
+    if (n < 0 || t <= 0) return KUIOPS_E_INVALID;
+    if (n == 0) return KUIOPS_OK;
+    if (!tokens || !parent || !target || !path || !count || !next) return KUIOPS_E_INVALID;
+    if (t > kMaxTree || n >= ((int64_t)1 << 31)) return KUIOPS_E_UNSUPPORTED;
+    hipLaunchKernelGGL(tree_accept_kernel, dim3((unsigned)n), dim3(64), 0, as_stream(stream), (int)t, tokens, parent, target,
+                       path, count, next);
+    return launch_status();
+}
+
+extern "C" int kuiops_kv_tree_commit(int64_t batch, int64_t n, int64_t hkv, int64_t cap, int64_t krow, int64_t vrow,
+                                     void *K, const int64_t sk[3], void *V, const int64_t sv[3], int64_t p,
+                                     const int32_t *path, int64_t t, const int32_t *kv_len, int32_t *len_out, void *stream) {
+    if (batch < 0 || n < 0 || hkv < 0 || cap < 0 || p < 0 || t <= 0 || !sk || !sv) return KUIOPS_E_INVALID;
+    if (n == 0 || batch == 0) return batch == n ? KUIOPS_OK : KUIOPS_E_INVALID;
+    if (batch % n || hkv == 0 || !path || !kv_len || !len_out || len_out == kv_len) return KUIOPS_E_INVALID;
+    if (cap > 0 && (!K || !V)) return KUIOPS_E_INVALID;
+    if (p > t) return KUIOPS_E_INVALID;
+    if (p > kMaxTree || batch > 65535 || hkv > 65535 || cap >= ((int64_t)1 << 31)) return KUIOPS_E_UNSUPPORTED;
+    if (!rows_ok(K, sk, krow) || !rows_ok(V, sv, vrow) || krow > (1 << 20) || vrow > (1 << 20)) return KUIOPS_E_UNSUPPORTED;
+    CommitArgs a{};
+    a.n = (int)n; a.p = (int)p; a.t = (int)std::min<int64_t>(t, INT32_MAX); a.cap = cap;
+    a.K = reinterpret_cast<char *>(K); a.V = reinterpret_cast<char *>(V);
+    a.sk0 = sk[0]; a.sk1 = sk[1]; a.sk2 = sk[2];
+    a.sv0 = sv[0]; a.sv1 = sv[1]; a.sv2 = sv[2];
+    a.kcols = (int)(krow / 16); a.vcols = (int)(vrow / 16); a.kblocks = (int)cdiv(a.kcols, 32);
+    a.path = path; a.kv_len = kv_len; a.len_out = len_out;
+    const dim3 grid((unsigned)(a.kblocks + cdiv(a.vcols, 32)), (unsigned)hkv, (unsigned)batch);
+    hipLaunchKernelGGL(tree_commit_kernel, grid, dim3(kCommitThreads), 0, as_stream(stream), a);
+    return launch_status();
+}
+
+extern "C" size_t kuiops_kv_evict_workspace(int64_t n, int64_t hkv, int64_t budget) {
+    if (n <= 0 || hkv <= 0 || budget <= 0) return 0;
+    return (size_t)n * hkv * (1 + 2 * budget) * sizeof(int32_t);
+}
+
+extern "C" int kuiops_kv_evict(int64_t n, int64_t hkv, int64_t cap, int64_t krow, int64_t vrow, void *K, const int64_t sk[3],
+                               void *V, const int64_t sv[3], const float *acc, const int64_t sa[2], const int32_t *pos,
+                               const int64_t sp[2], const int32_t *kv_len, int64_t budget, int64_t recent, float *acc_out,
+                               const int64_t sao[2], int32_t *pos_out, const int64_t spo[2], int32_t *len_out,
+                               void *workspace, size_t workspace_bytes, void *stream) {
+    if (n < 0 || hkv < 0 || cap < 0 || budget <= 0 || recent < 0 || recent > budget || !sk || !sv || !sa || !sp || !sao || !spo)
+        return KUIOPS_E_INVALID;
+    if (n == 0) return KUIOPS_OK;
+    if (hkv == 0 || !kv_len || !len_out) return KUIOPS_E_INVALID;
+    if (cap > 0 && (!K || !V || !acc || !pos || !acc_out || !pos_out)) return KUIOPS_E_INVALID;
+    if (n * hkv > 65535 || cap >= ((int64_t)1 << 30)) return KUIOPS_E_UNSUPPORTED;
+    if (!rows_ok(K, sk, krow) || !rows_ok(V, sv, vrow) || krow > (1 << 20) || vrow > (1 << 20)) return KUIOPS_E_UNSUPPORTED;
+    // (a budget past the capacity never evicts)
+    budget = std::min(budget, std::max<int64_t>(cap, 1));
+    recent = std::min(recent, budget);
+    if (!workspace || workspace_bytes < kuiops_kv_evict_workspace(n, hkv, budget) || (reinterpret_cast<uintptr_t>(workspace) & 3))
+        return KUIOPS_E_WORKSPACE;
+    EvictArgs a{};
+    a.n = (int)n; a.hkv = (int)hkv; a.budget = (int)budget; a.recent = (int)recent; a.cap = cap;
+    a.kv_len = kv_len; a.len_out = len_out; a.acc = acc; a.pos = pos; a.acc_out = acc_out; a.pos_out = pos_out;
+    a.sa0 = sa[0]; a.sa1 = sa[1]; a.sp0 = sp[0]; a.sp1 = sp[1];
+    a.sao0 = sao[0]; a.sao1 = sao[1]; a.spo0 = spo[0]; a.spo1 = spo[1];
+    a.moves = reinterpret_cast<int32_t *>(workspace);
+    a.K = reinterpret_cast<char *>(K); a.V = reinterpret_cast<char *>(V);
+    a.sk0 = sk[0]; a.sk1 = sk[1]; a.sk2 = sk[2];
+    a.sv0 = sv[0]; a.sv1 = sv[1]; a.sv2 = sv[2];
+    a.kcols = (int)(krow / 16); a.vcols = (int)(vrow / 16);
+    const int64_t most = std::max<int64_t>(0, std::min(budget, cap - budget)) * (a.kcols + a.vcols);
+    const int64_t per = std::max<int64_t>(1, cdiv(2048, n * hkv));
+    const dim3 grid((unsigned)std::max<int64_t>(1, std::min(per, cdiv(most, 256))), (unsigned)(n * hkv));
+    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)(n * hkv)), dim3(kEvictThreads), 0, as_stream(stream), a);
+    hipLaunchKernelGGL(evict_move_kernel, grid, dim3(256), 0, as_stream(stream), a);
+    return launch_status();
+}

@@ -1196,3 +1196,238 @@ def decode_rows_batched(x, W, x_kind="plain", out_kind="plain", in_add=None, nor
         _ptr(k_cache), sk, _ptr(v_cache), sv, k_cache.shape[2] if k_cache is not None else 0,
         _ptr(ws), ws.numel() if ws is not None else 0, _stream(x.device)))
     return out
+
+
+# ------------------------------------------- drafted trees, bounded caches
+# Workspaces here are plain scratch (no counters to start at zero), allocated
+# per call from torch's caching allocator: calls on several streams and graphs
+# captured one after another never share one, and nothing has to be run once
+# before a capture.
+
+def _on_device(name, status_of, device, *tensors):
+    """Checks that every tensor is on ``device``, a GPU, and enqueues
+    ``status_of(stream)`` there, whichever device is the current one."""
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if device.type != "cuda":
+        raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
+    if device.index == torch.cuda.current_device():
+        _lib.check(name, status_of(_stream(device)))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(name, status_of(_stream(device)))
+
+
+def _strides(t, count, scale=1):
+    """The first strides of t, 0 for axes of one entry (torch lets those be anything)."""
+    return (ctypes.c_int64 * count)(*[0 if t.shape[i] <= 1 else t.stride(i) * scale for i in range(count)])
+
+
+def _disjoint(t) -> bool:
+    """Whether no two elements of t share memory."""
+    if t.numel() <= 1:
+        return True
+    span = 1
+    for st, size in sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1):
+        if st < span:
+            return False
+        span = st * (size - 1) + span
+    return True
+
+
+def _own_rows(t) -> bool:
+    """Elements that share no memory, in rows of unit stride."""
+    return (t.shape[-1] <= 1 or t.stride(-1) == 1) and _disjoint(t)
+
+
+@functools.lru_cache(maxsize=4096)
+def _cache_attn_workspace(name, *dims) -> int:
+    return getattr(_lib_handle(), name)(*dims)
+
+
+def _cache_attn_check(name, q, k, v, kv_len, scale, out):
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or not (q.dtype == k.dtype == v.dtype):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    n, hq, l, e = q.shape
+    _, hkv, s, _ = k.shape
+    ev = v.shape[3]
+    if k.shape[0] != n or k.shape[3] != e or v.shape[:3] != k.shape[:3] or hkv == 0 or hq % hkv or e == 0 or ev == 0:
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if kv_len is not None and (kv_len.dtype != torch.int32 or kv_len.shape != (n,) or not kv_len.is_contiguous()):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if q.dtype not in HALF or k.stride(3) != 1 or v.stride(3) != 1:
+        raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
+    if out is not None and (out.shape != (n, hq, l, ev) or out.dtype != q.dtype or out.stride(3) != 1
+                            or not _disjoint(out) or out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr())):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    # a copy of the few query rows where the kernels cannot read them in place
+    if q.stride(3) != 1 or any(st % 8 for st in q.stride()[:3]) or q.data_ptr() % 16:
+        q = q.contiguous()
+    if scale is None:
+        scale = 1.0 / math.sqrt(e)
+    return q, (n, hq, hkv, l, s, e, ev), float(scale)
+
+
+def sdpa_tree(q, k, v, parent, kv_len=None, scale=None, return_lse=False, out=None):
+    """Attention of a tree of drafted tokens over a KV cache -> (out, lse).
+
+    q (n, hq, t, e) holds the t nodes' queries; k / v (n, hkv, s, e / ev) are the
+    caches, in which the nodes' keys are the last t of the first ``kv_len[b]``
+    (int32 [n] on the device, read when the kernel runs; None: s).  ``parent``
+    (int32 [n, t], or [t] for all sequences) names each node's parent, an
+    earlier node, or -1 for one that follows the context.  Node i sees the
+    context, its ancestors and itself; a chain (parent i - 1) is causal decode
+    attention.  A node with any other parent, -2 for instance, is absent, and its
+    descendants with it: output 0, lse -inf, so trees of several sizes share a
+    batch.  bf16 / f16, head dims multiples of 8 up to 256, t <= 256.  ``out``
+    ((n, hq, t, ev), unit last stride) receives the result in place."""
+    q, dims, scale = _cache_attn_check("sdpa_tree", q, k, v, kv_len, scale, out)
+    n, hq, hkv, t, s, e, ev = dims
+    if parent.dtype != torch.int32 or parent.shape not in ((n, t), (t,)) or t > s:
+        raise _lib.KuiopsError("sdpa_tree", _lib.E_INVALID)
+    if parent.dim() == 1:
+        parent = parent.expand(n, t)
+    parent = parent.contiguous()
+    if out is None:
+        out = torch.empty((n, hq, t, ev), dtype=q.dtype, device=q.device)
+    lse = torch.empty((n, hq, t), dtype=torch.float32, device=q.device) if return_lse else None
+    nbytes = _cache_attn_workspace("kuiops_sdpa_tree_workspace", *dims)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _on_device("sdpa_tree", lambda stream: _lib_handle().kuiops_sdpa_tree(
+        *dims, _dt(q.dtype), q.data_ptr(), _strides(q, 3), k.data_ptr(), _strides(k, 3), v.data_ptr(), _strides(v, 3),
+        out.data_ptr(), _strides(out, 3), _ptr(lse), scale, parent.data_ptr(), _ptr(kv_len), _ptr(ws), nbytes, stream),
+        q.device, k, v, parent, kv_len, out)
+    return out, lse
+
+
+def tree_accept(tokens, parent, target):
+    """Greedy acceptance of drafted trees -> (path int32 [n, t], count int32 [n],
+    next token int64 [n]).
+
+    ``tokens`` (int64 [n, t]) are the drafted tokens, ``parent`` (int32 [n, t]) as
+    in :func:`sdpa_tree`, ``target`` (int64 [n, t]) the model's choice after every
+    node.  From node 0 (the last token that is certain, parent -1) the walk goes
+    to the lowest child whose token is its parent's target, as far as there is
+    one.  ``path`` lists the nodes, then -1; the next token is the target of the
+    last one (-1 where node 0 is absent: count 0).  t <= 256."""
+    n, t = tokens.shape if tokens.dim() == 2 else (0, 0)
+    if t == 0 or tokens.dtype != torch.int64 or target.dtype != torch.int64 or parent.dtype != torch.int32 \
+            or parent.shape != (n, t) or target.shape != (n, t):
+        raise _lib.KuiopsError("tree_accept", _lib.E_INVALID)
+    tokens, parent, target = tokens.contiguous(), parent.contiguous(), target.contiguous()
+    path = torch.empty((n, t), dtype=torch.int32, device=tokens.device)
+    count = torch.empty(n, dtype=torch.int32, device=tokens.device)
+    follow = torch.empty(n, dtype=torch.int64, device=tokens.device)
+    _on_device("tree_accept", lambda stream: _lib_handle().kuiops_tree_accept(
+        n, t, tokens.data_ptr(), parent.data_ptr(), target.data_ptr(), path.data_ptr(), count.data_ptr(),
+        follow.data_ptr(), stream), tokens.device, parent, target)
+    return path, count, follow
+
+
+def _cache_rows(name, k, v):
+    """Both caches of (batch, hkv, capacity, e) with rows that are moved as bytes."""
+    if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or not _disjoint(k) or not _disjoint(v):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    for c in (k, v):
+        if c.numel() and (c.stride(3) != 1 and c.shape[3] > 1):
+            raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
+    return [(c.shape[3] * c.element_size(), c.data_ptr(), _strides_rows(c)) for c in (k, v)]
+
+
+def _strides_rows(c):
+    st = _strides(c, 3, c.element_size())
+    if c.shape[2] <= 1:
+        st[2] = c.shape[3] * c.element_size()
+    return st
+
+
+def kv_tree_commit(k, v, path, kv_len, tree):
+    """Moves the cache rows of an accepted path behind the context, in place, and
+    returns the new key counts (int32 [n]).
+
+    ``tree`` is the number t of drafted nodes, whose keys are the last t of the
+    first ``kv_len[b]`` (int32 [n]); ``path`` (int32 [n, p], p <= t) the accepted
+    ones in order, ended by -1 (:func:`tree_accept`'s).  With base = kv_len[b] - t,
+    row base + path[b, i] goes to row base + i; the new count is base plus the
+    path's length.  k / v (layers * n, hkv, capacity, e) may be all layers'
+    caches of the n sequences at once, layer after layer.  Any element type,
+    rows of multiples of 16 bytes; p <= 256."""
+    n = kv_len.numel()
+    (krow, kp, sk), (vrow, vp, sv) = _cache_rows("kv_tree_commit", k, v)
+    batch, hkv, cap, _ = k.shape
+    tree = int(tree)
+    if kv_len.dtype != torch.int32 or kv_len.dim() != 1 or not kv_len.is_contiguous() or path.dtype != torch.int32 \
+            or path.dim() != 2 or path.shape[0] != n or tree < 1 or path.shape[1] > tree \
+            or (batch % n if n else batch):
+        raise _lib.KuiopsError("kv_tree_commit", _lib.E_INVALID)
+    path = path.contiguous()
+    out = torch.empty_like(kv_len)
+    _on_device("kv_tree_commit", lambda stream: _lib_handle().kuiops_kv_tree_commit(
+        batch, n, hkv, cap, krow, vrow, kp, sk, vp, sv, path.shape[1], path.data_ptr(), tree, kv_len.data_ptr(),
+        out.data_ptr(), stream), k.device, v, path, kv_len)
+    return out
+
+
+def sdpa_decode_accum(q, k, v, acc, kv_len=None, scale=None, causal=True, return_lse=False, out=None):
+    """:func:`sdpa_decode` that also adds up how much each key was looked at:
+    ``acc[b, g, j]`` (fp32 [n, hkv, s], in place) grows by the softmax weights
+    that the queries of KV head g give key j, over its query heads and the l
+    positions.  -> (out, lse).  What :func:`kv_evict` decides by.
+
+    One call per decoded token (l = 1), per piece of a prompt, or for a whole
+    prompt (l = kv_len).  bf16 / f16, head dims multiples of 8 up to 256."""
+    q, dims, scale = _cache_attn_check("sdpa_decode_accum", q, k, v, kv_len, scale, out)
+    n, hq, hkv, l, s, e, ev = dims
+    if acc.dtype != torch.float32 or acc.shape != (n, hkv, s) or not _own_rows(acc) or (causal and l > s):
+        raise _lib.KuiopsError("sdpa_decode_accum", _lib.E_INVALID)
+    if out is None:
+        out = torch.empty((n, hq, l, ev), dtype=q.dtype, device=q.device)
+    lse = torch.empty((n, hq, l), dtype=torch.float32, device=q.device)
+    nbytes = _cache_attn_workspace("kuiops_sdpa_decode_accum_workspace", *dims)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _on_device("sdpa_decode_accum", lambda stream: _lib_handle().kuiops_sdpa_decode_accum(
+        *dims, _dt(q.dtype), q.data_ptr(), _strides(q, 3), k.data_ptr(), _strides(k, 3), v.data_ptr(), _strides(v, 3),
+        out.data_ptr(), _strides(out, 3), lse.data_ptr(), scale, 1 if causal else 0, _ptr(kv_len), acc.data_ptr(),
+        _strides(acc, 2), _ptr(ws), nbytes, stream), q.device, k, v, acc, kv_len, out)
+    return out, (lse if return_lse else None)
+
+
+def kv_evict(k, v, acc, pos, kv_len, budget, recent=0, acc_out=None, pos_out=None, len_out=None):
+    """Cuts the caches of sequences with more than ``budget`` keys down to that
+    many per KV head -> (acc_out, pos_out, len_out).
+
+    Kept are the ``recent`` (<= budget) newest positions (those above the largest
+    of ``pos`` minus recent) and then the keys with the largest ``acc`` (NaN ranks
+    highest), ties to the lowest slot.  Kept rows of k / v (n, hkv, capacity, e)
+    in slots from the budget on move into the freed slots below it, the i-th
+    into the i-th; the others stay where they are, so slots are in no order of
+    position afterwards: ``pos`` (int32 [n, hkv, capacity]) says which token a slot
+    holds.  ``acc`` (fp32) and ``pos`` go along and become 0 and -1 from the new
+    length (min(kv_len, budget)) on.  k and v change in place; acc, pos and kv_len
+    (int32 [n]) too, unless ``acc_out`` / ``pos_out`` / ``len_out`` are given."""
+    name = "kv_evict"
+    (krow, kp, sk), (vrow, vp, sv) = _cache_rows(name, k, v)
+    n, hkv, cap, _ = k.shape
+    acc_out, pos_out, len_out = (a if o is None else o for a, o in ((acc, acc_out), (pos, pos_out), (kv_len, len_out)))
+    budget, recent = int(budget), int(recent)
+    if budget < 1 or recent < 0 or recent > budget or kv_len.shape != (n,) or len_out.shape != (n,) \
+            or any(t.dtype != torch.int32 for t in (pos, pos_out, kv_len, len_out)) \
+            or any(t.dtype != torch.float32 for t in (acc, acc_out)) \
+            or any(t.shape != (n, hkv, cap) or not _own_rows(t) for t in (acc, acc_out, pos, pos_out)) \
+            or not kv_len.is_contiguous() or not len_out.is_contiguous():
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    for t, o in ((acc, acc_out), (pos, pos_out)):
+        # the same memory, then slot for slot; or another buffer
+        if o is not t and o.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() and n * hkv * cap > 0 \
+                and (o.data_ptr() != t.data_ptr() or o.stride() != t.stride()):
+            raise _lib.KuiopsError(name, _lib.E_INVALID)
+    budget = min(budget, max(cap, 1))
+    nbytes = n * hkv * (1 + 2 * budget) * 4
+    ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=k.device)
+    _on_device(name, lambda stream: _lib_handle().kuiops_kv_evict(
+        n, hkv, cap, krow, vrow, kp, sk, vp, sv, acc.data_ptr(), _strides(acc, 2), pos.data_ptr(), _strides(pos, 2),
+        kv_len.data_ptr(), budget, min(recent, budget), acc_out.data_ptr(), _strides(acc_out, 2), pos_out.data_ptr(),
+        _strides(pos_out, 2), len_out.data_ptr(), ws.data_ptr(), nbytes, stream),
+        k.device, v, acc, pos, kv_len, acc_out, pos_out, len_out)
+    return acc_out, pos_out, len_out

@@ -586,3 +586,150 @@ def llama_greedy(p: dict, prompt, n_new: int, cfg: dict):
         probs = softmax(lg)
         toks.append(int(topk(probs, 1)[1][0]))
     return toks[len(prompt):], steps
+
+
+# ------------------------------------------- drafted trees, bounded caches
+
+
+def tree_sees(parent):
+    """Per node of a drafted tree the nodes that it sees, ascending: its
+    ancestors and itself; none if it is absent (its parent is below -1 or not an
+    earlier node, or is absent itself)."""
+    sees = []
+    for i, p in enumerate(int(x) for x in parent):
+        if p == -1:
+            sees.append([i])
+        elif 0 <= p < i and sees[p]:
+            sees.append(sees[p] + [i])
+        else:
+            sees.append([])
+    return sees
+
+
+def _attend_rows(q, k, v, visible, scale):
+    """One sequence in fp64: q [hq, l, e], k / v [hkv, s, .], visible(i) -> the
+    keys that query i sees.  (out, lse, weights [hkv, s], out's sum of absolute
+    terms, the largest sum of absolute score terms)."""
+    hq, l, _ = q.shape
+    hkv, s, ev = v.shape
+    out, size = np.zeros((hq, l, ev)), np.zeros((hq, l, ev))
+    lse, acc, terms = np.full((hq, l), -np.inf), np.zeros((hkv, s)), 0.0
+    for h in range(hq):
+        g = h // (hq // hkv)
+        for i in range(l):
+            keys = np.asarray(visible(i), dtype=np.int64)
+            if keys.size == 0:
+                continue
+            kk, vv = k[g, keys].astype(np.float64), v[g, keys].astype(np.float64)
+            qi = q[h, i].astype(np.float64)
+            with np.errstate(all="ignore"):
+                x = (kk @ qi) * scale
+                top = x.max()
+                w = np.exp(x - top)
+                total = w.sum()
+                if not total > 0 and not np.isnan(total):
+                    continue
+                lse[h, i] = top + np.log(total)
+                w = w / total
+                out[h, i] = (w[:, None] * vv).sum(0)
+                size[h, i] = (w[:, None] * np.abs(vv)).sum(0)
+            acc[g, keys] += w
+            terms = max(terms, float((np.abs(kk) @ np.abs(qi)).max() * scale))
+    return out, lse, acc, size, terms
+
+
+def sdpa_tree(q, k, v, parent, kv_len=None, scale=None):
+    """Attention of drafted trees over a cache (kuiops_sdpa_tree): (out, lse,
+    sums of absolute output terms, largest sum of absolute score terms)."""
+    n, _, t, e = q.shape
+    scale = 1.0 / np.sqrt(e) if scale is None else scale
+    got = []
+    for b in range(n):
+        L = k.shape[2] if kv_len is None else min(max(int(kv_len[b]), 0), k.shape[2])
+        sees = tree_sees(parent[b])
+
+        def visible(i, L=L, sees=sees):
+            if not sees[i]:
+                return []
+            return list(range(max(0, L - t))) + [L - t + j for j in sees[i] if L - t + j >= 0]
+        got.append(_attend_rows(q[b], k[b], v[b], visible, scale))
+    return np.stack([x[0] for x in got]), np.stack([x[1] for x in got]), np.stack([x[3] for x in got]), max(x[4] for x in got)
+
+
+def sdpa_decode_accum(q, k, v, acc, kv_len=None, scale=None, causal=True):
+    """Decode attention with the weights added up per key
+    (kuiops_sdpa_decode_accum): (out, lse, new acc, sums of absolute output
+    terms, largest sum of absolute score terms)."""
+    n, _, l, e = q.shape
+    scale = 1.0 / np.sqrt(e) if scale is None else scale
+    got, new = [], np.array(acc, dtype=np.float64)
+    for b in range(n):
+        L = k.shape[2] if kv_len is None else min(max(int(kv_len[b]), 0), k.shape[2])
+        r = _attend_rows(q[b], k[b], v[b], lambda i, L=L: range(max(0, L - l + i + 1 if causal else L)), scale)
+        new[b] += r[2]
+        got.append(r)
+    return (np.stack([x[0] for x in got]), np.stack([x[1] for x in got]), new, np.stack([x[3] for x in got]),
+            max(x[4] for x in got))
+
+
+def tree_accept(tokens, parent, target):
+    """Greedy acceptance of drafted trees (kuiops_tree_accept)."""
+    n, t = np.shape(tokens)
+    path, count, follow = np.full((n, t), -1, np.int32), np.zeros(n, np.int32), np.full(n, -1, np.int64)
+    for b in range(n):
+        at = 0 if parent[b][0] == -1 else None
+        while at is not None:
+            path[b, count[b]] = at
+            count[b] += 1
+            follow[b] = target[b][at]
+            at = next((i for i in range(at + 1, t) if parent[b][i] == at and tokens[b][i] == target[b][at]), None)
+    return path, count, follow
+
+
+def kv_tree_commit(k, v, path, kv_len, tree):
+    """(k, v, key counts) with an accepted path's rows behind the context
+    (kuiops_kv_tree_commit)."""
+    k, v = np.array(k), np.array(v)
+    n, cap = len(kv_len), k.shape[2]
+    ends = np.array(kv_len, np.int32)
+    for b in range(n):
+        base = int(kv_len[b]) - tree
+        if base < 0:
+            continue
+        rows = []
+        for i, x in enumerate(int(x) for x in path[b]):
+            if x < 0 or x >= tree or base + max(x, i) >= cap:
+                break
+            rows.append(base + x)
+        for c in (k, v):
+            c[b::n, :, base:base + len(rows)] = c[b::n][:, :, rows]
+        ends[b] = base + len(rows)
+    return k, v, ends
+
+
+def kv_evict(k, v, acc, pos, kv_len, budget, recent=0):
+    """(k, v, acc, pos, key counts) cut down to the budget (kuiops_kv_evict)."""
+    k, v = np.array(k), np.array(v)
+    n, hkv, cap = np.shape(acc)
+    acc_out, pos_out = np.zeros((n, hkv, cap), np.float32), np.full((n, hkv, cap), -1, np.int32)
+    lens = np.array([min(max(int(x), 0), cap) for x in kv_len])
+    for b in range(n):
+        L = lens[b]
+        for g in range(hkv):
+            slots = list(range(L))
+            if L > budget:
+                newest = int(np.max(pos[b, g, :L]))
+
+                def order(i, b=b, g=g, newest=newest):
+                    if int(pos[b, g, i]) > newest - recent:
+                        return (0, 0.0, i)
+                    w = float(acc[b, g, i])
+                    return (1, 0.0, i) if np.isnan(w) else (2, -w, i)
+                kept = set(sorted(range(L), key=order)[:budget])
+                far = iter([i for i in range(budget, L) if i in kept])
+                slots = [i if i in kept else next(far) for i in range(budget)]
+            m = len(slots)
+            for c in (k, v):
+                c[b, g, :m] = c[b, g, slots]
+            acc_out[b, g, :m], pos_out[b, g, :m] = np.asarray(acc)[b, g, slots], np.asarray(pos)[b, g, slots]
+    return k, v, acc_out, pos_out, np.minimum(lens, budget).astype(np.int32)
