@@ -32,8 +32,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void *base, ui
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)bytes, 0x00020000);
 }
 // 16 bytes per lane into dst + 16 * lane; zeros past the descriptor's size
-__device__ __forceinline__ void dma16_buf(__amdgpu_buffer_rsrc_t r, uint32_t voff, const void *dst) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)to_lds(dst), 16, (int)voff, 0,
+__device__ __forceinline__ void dma16_buf(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff, const void *dst) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)to_lds(dst), 16, (int)voff, (int)soff,
                                              0, 0);
 }
 
@@ -59,18 +59,40 @@ struct CacheAttnArgs {
     float *ws_o;               // [splits][n * hq * l][HD]: unnormalised output
     float *acc;                // kuiops_sdpa_decode_accum: per key sums, strides sa0, sa1, 1
     int64_t sa0, sa1;
+    float *scores;             // [n][hkv][hq / hkv * l][spad]: q k, -inf where not seen; or null
+    int64_t spad;
 };
 
 __device__ __forceinline__ int keys_of(const CacheAttnArgs &a, int b) {
     return a.kv_len ? (int)max((int64_t)0, min((int64_t)a.kv_len[b], a.s)) : (int)a.s;
 }
 
-// Which nodes each node of the tree sees (itself and its ancestors), as bits,
-// by pointer doubling: after round r a node's word holds its 2^r nearest
-// ancestors and `up` the next one, so 8 rounds suffice for 256 nodes and a
+// Which nodes each node of the tree sees (itself and its ancestors), as bits, by
+// pointer doubling: after round r a node's word holds its 2^r nearest ancestors
+// and `up` the next one, so 6 rounds suffice for 64 nodes, 8 for 256, and a
 // shallow tree stops early.  A node is absent if its parent is below -1 or not
-// an earlier node, or if an ancestor of it is: it then sees nothing.  Thread i
-// has node i.
+// an earlier node, or if an ancestor of it is: it then sees nothing.
+//
+// Up to 64 nodes: lane i of every wave has node i, no LDS and no barrier, so the
+// first keys' loads stay in flight meanwhile.
+__device__ __forceinline__ uint64_t tree_bits_wave(const int32_t *parent, int t) {
+    const int i = threadIdx.x & 63;
+    const int p = i < t ? parent[i] : -1;
+    int bad = p < -1 || p >= i;
+    int up = bad ? -1 : p;
+    uint32_t lo = i < 32 ? 1u << i : 0u, hi = i < 32 ? 0u : 1u << (i - 32);
+    while (__any(up >= 0)) {
+        const int from = up >= 0 ? up : i;
+        const uint32_t l2 = __shfl(lo, from, 64), h2 = __shfl(hi, from, 64);
+        const int b2 = __shfl(bad, from, 64), u2 = __shfl(up, from, 64);
+        lo |= l2;
+        hi |= h2;
+        bad |= b2;
+        up = up >= 0 ? u2 : -1;
+    }
+    return bad ? 0 : (uint64_t)hi << 32 | lo;
+}
+// More nodes: thread i has node i, words in LDS.
 struct TreeBits {
     uint64_t w[kMaxTree][kTreeWords];
     int16_t up[kMaxTree];
@@ -119,9 +141,66 @@ __device__ __forceinline__ void tree_bits(TreeBits &tb, const int32_t *parent, i
     __syncthreads();
 }
 
+// The row's first n >= 0 of 64 keys.
+__device__ __forceinline__ uint64_t first_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+
+// Which of the keys k0 .. k0 + 63 a row sees, as bits: `mine` is its word of the
+// tree's nodes where the tree has at most 64, else the words are tb's.
+__device__ __forceinline__ uint64_t seen_word(const CacheAttnArgs &a, const TreeBits *tb, uint64_t mine, int pos, int k0, int L) {
+    const int first = L - a.l;
+    if (a.mode != kTree) return first_bits((a.mode == kCausal ? min(L, first + pos + 1) : L) - k0);
+    const int j0 = k0 - first;                // the tree's node of key k0
+    if (j0 <= -64) return ~0ull;
+    if (a.l <= 64) return j0 < 0 ? mine << -j0 | first_bits(-j0) : j0 < 64 ? mine >> j0 : 0;
+    if (j0 < 0) return tb->w[pos][0] << -j0 | first_bits(-j0);
+    const int w = j0 >> 6, sh = j0 & 63;
+    uint64_t r = w < kTreeWords ? tb->w[pos][w] >> sh : 0;
+    if (sh && w + 1 < kTreeWords) r |= tb->w[pos][w + 1] << (64 - sh);
+    return r;
+}
+
+// What a work-group works on: the row groups of a (sequence, KV head, split)
+// run on one XCD, whose L2 then has the keys for all but the first.
+struct Unit {
+    int b, hk, split, rg;
+    bool any;
+};
+__device__ __forceinline__ Unit unit_of(const CacheAttnArgs &a) {
+    const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;
+    const int unit = idx / a.row_groups * 8 + xcd;
+    Unit u;
+    u.any = unit < a.n * a.hkv * a.splits;
+    u.rg = idx % a.row_groups;
+    u.split = unit % a.splits;
+    const int bh = unit / a.splits;
+    u.b = bh / a.hkv;
+    u.hk = bh % a.hkv;
+    return u;
+}
+
+template <typename T> struct Shift;       // probabilities are relative to 2^(maximum + value)
+template <> struct Shift<bf16_t> { static constexpr float value = 0.f; };       // p <= 2^8 between rescales
+// p <= 2^15, so that f16's smallest step 2^-24 is 2^-39 of it
+template <> struct Shift<f16_t> { static constexpr float value = -7.f; };
+constexpr float kSlack = 8.f;       // a row's maximum may grow by 2^8 before its sums are rescaled
+
+// 4 output columns of a row: o * (1 / sum), and the row's log-sum-exp
+template <typename T>
+__device__ __forceinline__ void store_row(const CacheAttnArgs &a, int64_t b, int head, int i, int d, f32x4 o, float m, float l) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    if (d < a.ev) {
+        t4 w;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) w[y] = from_f32<T>(o[y] * inv);
+        *reinterpret_cast<t4 *>(reinterpret_cast<T *>(a.O) + b * a.so0 + head * a.so1 + i * a.so2 + d) = w;
+    }
+    if (a.lse && d == 0) a.lse[(b * a.hq + head) * a.l + i] = l != 0.f ? (m + __log2f(l)) * kLn2 : -INFINITY;
+}
+
 // ------------------------------------------------------------------------
-// cache_attn_kernel -- 4 waves, each with key steps of 32 of its own; all have
-// the same 16 * RT query rows.
+// cache_attn_kernel -- few rows per KV head: NWV waves, each with key steps of
+// 32 of its own; all have the same 16 * RT query rows.
 //   S = K Q^T (16x16x32 MFMA): K straight from memory to registers; a lane
 //   holds 8 scores of one row per 16-row tile, the row's maximum crosses lanes
 //   16 and 32 apart only.  O^T += V^T P^T: V through LDS (DMA), read transposed;
@@ -130,23 +209,11 @@ __device__ __forceinline__ void tree_bits(TreeBits &tb, const int32_t *parent, i
 //   each (2^-16 of it is lost in bf16, 2^-21 in f16): with the few rows of
 //   this kernel the K / V stream takes the time, not the MFMAs.
 // A part that is 0 times an infinite value is NaN, so is a masked NaN: a wave
-// whose sums are not finite goes over its keys again, `careful`: values that
-// are not finite are then taken out of the tile and multiplied by themselves,
-// for the rows that see them.
-template <typename T> struct Parts;
-template <> struct Parts<bf16_t> {
-    // p <= 2^8 between rescales
-    static constexpr float kShift = 0.f;
-};
-template <> struct Parts<f16_t> {
-    // p <= 2^15, so that f16's smallest step 2^-24 is 2^-39 of it
-    static constexpr float kShift = -7.f;
-};
-constexpr float kSlack = 8.f;       // a row's maximum may grow by 2^8 before its sums are rescaled
-
-template <typename T, int HD, int RT>
-__global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
-    constexpr int NWV = 4, KB = 32, R = 16 * RT;
+// whose sums are not finite goes over its keys again with the row maxima that
+// it found, multiplying value by value for the rows that see them.
+template <typename T, int HD, int RT, int NWV>
+__global__ __launch_bounds__(NWV * 64) void cache_attn_kernel(CacheAttnArgs a) {
+    constexpr int KB = 32, R = 16 * RT;
     constexpr int RB = HD * 2, VT = KB * RB;          // bytes per V row / wave tile
     constexpr int KK = HD / 32, DT = HD / 16, DV = VT / 1024;
     typedef typename Mfma<T>::frag frag;
@@ -157,58 +224,23 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lr = lane & 15, G4 = lane >> 4;
-
-    // The row groups of a (sequence, KV head, split) run on one XCD, whose L2
-    // then has the keys for all but the first.
-    const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;
-    const int unit = idx / a.row_groups * 8 + xcd, rg = idx % a.row_groups;
-    if (unit >= a.n * a.hkv * a.splits) return;
-    const int split = unit % a.splits, bh = unit / a.splits;
-    const int b = bh / a.hkv, hk = bh % a.hkv;
-    const int G = a.hq / a.hkv, rows_kv = G * a.l, r0 = rg * R;
+    const Unit u = unit_of(a);
+    if (!u.any) return;
+    const int b = u.b, hk = u.hk, split = u.split;
+    const int G = a.hq / a.hkv, rows_kv = G * a.l, r0 = u.rg * R;
 
     const int L = keys_of(a, b);
     const int steps = (L + KB - 1) / KB;
     // a sequence's steps are spread evenly over its splits, whole steps of the work-group
     const int chunk = (steps + a.splits * NWV - 1) / (a.splits * NWV) * NWV * KB;
     const int kbeg = min(L, split * chunk), kend = min(L, kbeg + chunk);
-    const int first_node = L - a.l;                    // kTree: key of node 0 (may be below 0)
-    const int free_end = a.mode == kFull ? L : a.mode == kCausal ? L - a.l + 1 : first_node;
-
-    if (a.mode == kTree) tree_bits<NWV * 64>(tb, a.parent + (int64_t)b * a.l, a.l);
+    // keys below free_end are seen by every row
+    const int free_end = a.mode == kFull ? L : a.mode == kCausal ? L - a.l + 1 : L - a.l;
 
     const T *Kp = reinterpret_cast<const T *>(a.K) + b * a.sk0 + hk * a.sk1 + (int64_t)kbeg * a.sk2;
     const T *Vp = reinterpret_cast<const T *>(a.V) + b * a.sv0 + hk * a.sv1 + (int64_t)kbeg * a.sv2;
     const uint32_t kbytes = kend > kbeg ? (uint32_t)(((int64_t)(kend - kbeg - 1) * a.sk2 + a.e) * 2) : 0u;
     const uint32_t vbytes = kend > kbeg ? (uint32_t)(((int64_t)(kend - kbeg - 1) * a.sv2 + a.ev) * 2) : 0u;
-    const __amdgpu_buffer_rsrc_t rsK = make_rsrc(Kp, kbytes), rsV = make_rsrc(Vp, vbytes);
-
-    // query rows r0 + 16 rt + lr (B operand; rows past the list are 0)
-    frag qf[RT][KK];
-    bool row_ok[RT];
-    int pos[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int rr = r0 + rt * 16 + lr;
-        row_ok[rt] = rr < rows_kv;
-        const int h = row_ok[rt] ? rr / a.l : 0;
-        pos[rt] = row_ok[rt] ? rr % a.l : 0;
-        // (an absent node's query is not read: whatever it holds stays out)
-        if (a.mode == kTree && row_ok[rt]) row_ok[rt] = (tb.w[pos[rt]][pos[rt] >> 6] >> (pos[rt] & 63)) & 1;
-        const T *q = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + (hk * G + h) * a.sq1 + pos[rt] * a.sq2;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            const int d = kk * 32 + G4 * 8;
-            qf[rt][kk] = as_frag<frag>(row_ok[rt] && d < a.e ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0});
-        }
-    }
-    auto sees = [&](int rt, int key) __attribute__((always_inline)) -> bool {
-        if (!row_ok[rt] || key >= kend) return false;
-        if (key < free_end) return true;
-        if (a.mode == kCausal) return key <= first_node + pos[rt];
-        const int j = key - first_node;
-        return (tb.w[pos[rt]][j >> 6] >> (j & 63)) & 1;
-    };
 
     // V tile: 16-byte chunk c of row r at position c ^ vsw(r): the 16 rows x 32
     // bytes of a transposing read fall on the 64 banks evenly.
@@ -235,53 +267,90 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
     // keys k0 .. k0 + 31 (nothing past kend): K into registers `slot`, V into tile sv
     auto issue = [&](int k0, int slot, char *sv) __attribute__((always_inline)) {
         const bool on = k0 < kend;
-        const uint32_t kb = on ? (uint32_t)((int64_t)(k0 - kbeg) * a.sk2 * 2) : kOut;
-        const uint32_t vb = on ? (uint32_t)((int64_t)(k0 - kbeg) * a.sv2 * 2) : kOut;
+        const uint32_t kb = on ? (uint32_t)((int64_t)(k0 - kbeg) * a.sk2 * 2) : 0u;
+        const uint32_t vb = on ? (uint32_t)((int64_t)(k0 - kbeg) * a.sv2 * 2) : 0u;
+        const __amdgpu_buffer_rsrc_t rsK = make_rsrc(Kp, on ? kbytes : 0u), rsV = make_rsrc(Vp, on ? vbytes : 0u);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
-                kr[slot][t][kk] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                    rsK, (int)((kb | offK[t][kk]) >= kOut ? kOut : kb + offK[t][kk]), 0, 0));
+                kr[slot][t][kk] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsK, (int)offK[t][kk], (int)kb, 0));
 #pragma unroll
-        for (int j = 0; j < DV; ++j)
-            dma16_buf(rsV, (vb | offV[j]) >= kOut ? kOut : vb + offV[j], sv + wave * VT + j * 1024);
+        for (int j = 0; j < DV; ++j) dma16_buf(rsV, offV[j], vb, sv + wave * VT + j * 1024);
         __builtin_amdgcn_sched_barrier(0);
     };
 
+    // query rows r0 + 16 rt + lr (B operand; rows past the list are 0)
+    frag qf[RT][KK];
+    bool row_ok[RT];
+    int pos[RT];
+    uint64_t mine[RT];
+    uint64_t nodes = 0;
+    if (a.mode == kTree) {
+        if (a.l <= 64) nodes = tree_bits_wave(a.parent + (int64_t)b * a.l, a.l);
+        else if constexpr (NWV * 64 >= kMaxTree) tree_bits<NWV * 64>(tb, a.parent + (int64_t)b * a.l, a.l);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int rr = r0 + rt * 16 + lr;
+        row_ok[rt] = rr < rows_kv;
+        const int h = row_ok[rt] ? rr / a.l : 0;
+        pos[rt] = row_ok[rt] ? rr - h * a.l : 0;
+        mine[rt] = 0;
+        if (a.mode == kTree) {
+            // (an absent node's query is not read: whatever it holds stays out)
+            if (a.l <= 64) {
+                mine[rt] = (uint64_t)__shfl((uint32_t)(nodes >> 32), pos[rt], 64) << 32 | __shfl((uint32_t)nodes, pos[rt], 64);
+                row_ok[rt] = row_ok[rt] && mine[rt] != 0;
+            } else {
+                row_ok[rt] = row_ok[rt] && (tb.w[pos[rt]][pos[rt] >> 6] >> (pos[rt] & 63)) & 1;
+            }
+        }
+        const T *q = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + (hk * G + h) * a.sq1 + pos[rt] * a.sq2;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const int d = kk * 32 + G4 * 8;
+            qf[rt][kk] = as_frag<frag>(row_ok[rt] && d < a.e ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0});
+        }
+    }
+
     f32x4 o[RT][DT];
     float m_used[RT], l_run[RT];
-    auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            m_used[rt] = -INFINITY;
-            l_run[rt] = 0.f;
+    for (int rt = 0; rt < RT; ++rt) {
+        m_used[rt] = -INFINITY;
+        l_run[rt] = 0.f;
 #pragma unroll
-            for (int t = 0; t < DT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < DT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // scores of a step: (t, i) is key k0 + 16 t + 4 G4 + i; unseen keys -inf
+    auto scores = [&](int k0, int slot, int rt, f32x4 *sc) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) sc[t] = Mfma<T>::m16(as_frag<frag>(kr[slot][t][kk]), qf[rt][kk], sc[t]);
+        }
+        if (k0 + KB > free_end) {
+            const uint32_t seen = (uint32_t)seen_word(a, &tb, mine[rt], pos[rt], k0, L) >> (4 * G4);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!(seen >> (16 * t + i) & 1)) sc[t][i] = -INFINITY;
         }
     };
-    clear();
-    bool careful = false;
+    float *keep = a.scores ? a.scores + (int64_t)(b * a.hkv + hk) * rows_kv * a.spad : nullptr;
     auto step = [&](int k0, int slot, char *sv) __attribute__((always_inline)) {
         t8 hi[RT], lo[RT];
-        float pk[RT][8];
-        const bool masked = k0 + KB > min(free_end, kend);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             f32x4 sc[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) sc[t] = Mfma<T>::m16(as_frag<frag>(kr[slot][t][kk]), qf[rt][kk], sc[t]);
-            }
-            // score (t, i): key k0 + 16 t + 4 G4 + i
-            if (masked) {
+            scores(k0, slot, rt, sc);
+            if (keep && row_ok[rt]) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!sees(rt, k0 + 16 * t + 4 * G4 + i)) sc[t][i] = -INFINITY;
+                    *reinterpret_cast<f32x4 *>(keep + (int64_t)(r0 + rt * 16 + lr) * a.spad + k0 + 16 * t + 4 * G4) = sc[t];
             }
             float mx = -INFINITY;
 #pragma unroll
@@ -299,14 +368,13 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
                     for (int i = 0; i < 4; ++i) o[rt][t][i] *= alpha;
                 m_used[rt] = m_new;
             }
-            const float mref = m_used[rt] == -INFINITY ? 0.f : m_used[rt] + Parts<T>::kShift;
+            const float mref = m_used[rt] == -INFINITY ? 0.f : m_used[rt] + Shift<T>::value;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float p = fast_exp2(__builtin_fmaf(sc[t][i], a.scale_log2, -mref));
                     l_run[rt] += p;
-                    pk[rt][4 * t + i] = p;
                     const T h = from_f32<T>(p);
                     hi[rt][4 * t + i] = h;
                     lo[rt][4 * t + i] = from_f32<T>(p - to_f32(h));
@@ -316,38 +384,6 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
         constexpr int Y = 2 * KK + DV;
         __builtin_amdgcn_s_waitcnt((Y & 15) | ((Y >> 4) << 14) | (7 << 4) | (15 << 8));
         __builtin_amdgcn_sched_barrier(0);
-        if (careful) {
-            // (d, key) of this lane's outputs: d = 16 dt + 4 G4 + i for row lr
-            for (int x = 0; x < 8; ++x)
-                for (int g = 0; g < 4; ++g) {
-                    const int kr_ = 16 * (x >> 2) + 4 * g + (x & 3);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const int d = dt * 16 + 4 * G4;
-                        T *vp = reinterpret_cast<T *>(sv + wave * VT + kr_ * RB + (((d >> 3) ^ vsw(kr_)) << 4) + (d & 4) * 2);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float val = to_f32(vp[i]);
-                            const bool odd = !(fabsf(val) < INFINITY);
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) {
-                                float p = pk[rt][0];
-#pragma unroll
-                                for (int y = 1; y < 8; ++y) p = x == y ? pk[rt][y] : p;
-                                p = __shfl(p, g * 16 + lr, 64);
-                                if (odd && sees(rt, k0 + kr_)) o[rt][dt][i] += p * val;
-                            }
-                        }
-                    }
-                }
-            __builtin_amdgcn_s_waitcnt(0xc07f);
-            for (int c = lane; c < VT / 2; c += 64) {
-                T *vp = reinterpret_cast<T *>(sv + wave * VT) + c;
-                if (!(fabsf(to_f32(*vp)) < INFINITY)) *vp = from_f32<T>(0.f);
-            }
-            __builtin_amdgcn_s_waitcnt(0xc07f);
-            __builtin_amdgcn_sched_barrier(0);
-        }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             const char *vb = sv + wave * VT + offVr[dt];
@@ -364,33 +400,64 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
     };
 
     constexpr int KS = NWV * KB;
-    for (;;) {
-        int k0 = kbeg + wave * KB;
-        issue(k0, 0, sV0);
-        for (; k0 < kend; k0 += 2 * KS) {
-            issue(k0 + KS, 1, sV1);
-            step(k0, 0, sV0);
-            // (this wave's reads of the tile are done before its refill)
-            __builtin_amdgcn_s_waitcnt(0xc07f);
-            __builtin_amdgcn_sched_barrier(0);
-            issue(k0 + 2 * KS, 0, sV0);
-            step(k0 + KS, 1, sV1);
-            __builtin_amdgcn_s_waitcnt(0xc07f);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        // no DMA is in flight past here
-        __builtin_amdgcn_s_waitcnt(0);
+    int k0 = kbeg + wave * KB;
+    issue(k0, 0, sV0);
+    for (; k0 < kend; k0 += 2 * KS) {
+        issue(k0 + KS, 1, sV1);
+        step(k0, 0, sV0);
+        // (this wave's reads of the tile are done before its refill)
+        __builtin_amdgcn_s_waitcnt(0xc07f);
         __builtin_amdgcn_sched_barrier(0);
-        float z = 0.f;                  // stays 0 if every sum is finite
+        issue(k0 + 2 * KS, 0, sV0);
+        if (k0 + KS < kend) step(k0 + KS, 1, sV1);
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // no DMA is in flight past here
+    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_sched_barrier(0);
+    float z = 0.f;                  // stays 0 if every sum is finite
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z = __builtin_fmaf(o[rt][t][i], 0.f, z);
+    if (__any(z != 0.f)) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
+            for (int t = 0; t < DT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (k0 = kbeg + wave * KB; k0 < kend; k0 += KS) {
+            issue(k0, 0, sV0);
+            __builtin_amdgcn_s_waitcnt(0);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) z = __builtin_fmaf(o[rt][t][i], 0.f, z);
-        if (careful || !__any(z != 0.f)) break;
-        careful = true;
-        clear();
+            for (int rt = 0; rt < RT; ++rt) {
+                f32x4 sc[2];
+                scores(k0, 0, rt, sc);
+                const float mref = m_used[rt] == -INFINITY ? 0.f : m_used[rt] + Shift<T>::value;
+                const uint32_t seen = (uint32_t)seen_word(a, &tb, mine[rt], pos[rt], k0, L);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const float p = fast_exp2(__builtin_fmaf(sc[x >> 2][x & 3], a.scale_log2, -mref));
+                    for (int g = 0; g < 4; ++g) {
+                        const int key = 16 * (x >> 2) + 4 * g + (x & 3);
+                        const float pk = __shfl(p, g * 16 + lr, 64);
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) {
+                            const int d = dt * 16 + 4 * G4;
+                            const T *vp = reinterpret_cast<const T *>(sV0 + wave * VT + key * RB + (((d >> 3) ^ vsw(key)) << 4) + (d & 4) * 2);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (seen >> key & 1) o[rt][dt][i] += pk * to_f32(vp[i]);
+                        }
+                    }
+                }
+            }
+            __builtin_amdgcn_s_waitcnt(0xc07f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 
     // the waves' sums merge through LDS, 16 rows at a time in the first tiles' place
@@ -402,7 +469,7 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
         // lanes of a row hold disjoint keys: row sums over the lane groups
         const float lsum = xor_add<32>(xor_add<16>(l_run[rt]));
         if (G4 == 0) {
-            sm[wave][rt * 16 + lr] = row_ok[rt] ? m_used[rt] + Parts<T>::kShift : -INFINITY;
+            sm[wave][rt * 16 + lr] = row_ok[rt] ? m_used[rt] + Shift<T>::value : -INFINITY;
             sl[wave][rt * 16 + lr] = row_ok[rt] ? lsum : 0.f;
         }
         __syncthreads();
@@ -428,27 +495,299 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
                 for (int i = 0; i < 4; ++i) oo[i] = __builtin_fmaf(ov[i], wgt, oo[i]);
             }
             const int head = hk * G + rr / a.l, i = rr % a.l;
-            const int64_t row = ((int64_t)b * a.hq + head) * a.l + i;
-            if (a.splits > 1) {
-                const int64_t st = (int64_t)split * a.n * a.hq * a.l + row;
-                *reinterpret_cast<f32x4 *>(&a.ws_o[st * HD + d]) = oo;
-                if (d == 0) {
-                    a.ws_ml[st * 2] = mm;
-                    a.ws_ml[st * 2 + 1] = ll;
-                }
-                continue;
-            }
-            const float inv = ll != 0.f ? 1.f / ll : 0.f;
-            if (d < a.ev) {
-                typedef T t4 __attribute__((ext_vector_type(4)));
-                t4 w;
-#pragma unroll
-                for (int y = 0; y < 4; ++y) w[y] = from_f32<T>(oo[y] * inv);
-                *reinterpret_cast<t4 *>(reinterpret_cast<T *>(a.O) + b * a.so0 + head * a.so1 + i * a.so2 + d) = w;
-            }
-            if (a.lse && d == 0) a.lse[row] = ll != 0.f ? (mm + __log2f(ll)) * kLn2 : -INFINITY;
+            if (a.splits == 1) store_row<T>(a, b, head, i, d, oo, mm, ll);
+            const int64_t st = (int64_t)split * a.n * a.hq * a.l + ((int64_t)b * a.hq + head) * a.l + i;
+            if (a.splits > 1) *reinterpret_cast<f32x4 *>(&a.ws_o[st * HD + d]) = oo;
+            if (d == 0 && a.ws_ml) *reinterpret_cast<f32x2 *>(&a.ws_ml[st * 2]) = f32x2{mm, ll};
         }
     }
+}
+
+// ------------------------------------------------------------------------
+// cache_rows_kernel -- many rows per KV head: 4 waves of 32 rows each over the
+// same keys, 64 at a time, K and V through LDS (two stages each, DMA).  32x32x16
+// MFMAs in the same transposed form: a lane holds 32 scores of one row, and its
+// maximum and sum cross lanes 32 apart only.  Step j runs the exponentials of
+// block j between the score MFMAs of block j + 1, then O^T += V^T P^T.  The
+// probability is one 16-bit value here: with this many rows the MFMAs and the
+// softmax's vector instructions bound the kernel, and a second part would cost
+// a third more of the one and a third of the other; each weight is off by at
+// most half a step of the output's type, as the output itself is.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void cache_rows_kernel(CacheAttnArgs a) {
+    constexpr int NWV = 4, KB = 64, R = 32 * NWV;
+    constexpr int RB = HD * 2, CPR = HD / 8, TILE = KB * RB;
+    constexpr int DPW = TILE / 1024 / NWV, RPB = 1024 / RB;
+    constexpr int DT = HD / 32, KS = HD / 16;
+    typedef typename Mfma<T>::frag frag;
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    // K rows are read 16 at a time (ds_read_b128), V rows 8 rows x 64 bytes
+    // (transposing): chunk c of row r sits at c ^ swizzle(r), all banks evenly
+    auto kswz = [](int r) { return CPR == 16 ? (r & 15) : ((r >> 1) & 7); };
+    auto vswz = [](int r) { return CPR == 16 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
+    __shared__ __attribute__((aligned(1024))) char sK0[TILE], sV0[TILE], sK1[TILE], sV1[TILE];
+    __shared__ TreeBits tb;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lq = lane & 31, lh = lane >> 5, G4 = lane >> 4, qq = lane & 15;
+    const Unit u = unit_of(a);
+    if (!u.any) return;
+    const int b = u.b, hk = u.hk, split = u.split;
+    const int G = a.hq / a.hkv, rows_kv = G * a.l, r0 = u.rg * R;
+
+    const int L = keys_of(a, b), first = L - a.l;
+    const int blocks_all = (L + KB - 1) / KB;
+    const int chunk = (blocks_all + a.splits - 1) / a.splits * KB;
+    const int kbeg = min(L, split * chunk);
+    int kend = min(L, kbeg + chunk);
+    if (a.mode == kCausal) {
+        // keys past the last position of the work-group's rows are seen by none
+        const int last = min(r0 + R, rows_kv) - 1;
+        if (r0 / a.l == last / a.l) kend = max(kbeg, min(kend, first + last % a.l + 1));
+    }
+    const int free_end = a.mode == kFull ? L : a.mode == kCausal ? first + 1 : first;
+    const int nkv = (kend - kbeg + KB - 1) / KB;
+
+    const T *Kp = reinterpret_cast<const T *>(a.K) + b * a.sk0 + hk * a.sk1 + (int64_t)kbeg * a.sk2;
+    const T *Vp = reinterpret_cast<const T *>(a.V) + b * a.sv0 + hk * a.sv1 + (int64_t)kbeg * a.sv2;
+    const uint32_t kbytes = kend > kbeg ? (uint32_t)(((int64_t)(min(L, kbeg + chunk) - kbeg - 1) * a.sk2 + a.e) * 2) : 0u;
+    const uint32_t vbytes = kend > kbeg ? (uint32_t)(((int64_t)(min(L, kbeg + chunk) - kbeg - 1) * a.sv2 + a.ev) * 2) : 0u;
+    const __amdgpu_buffer_rsrc_t rsK = make_rsrc(Kp, kbytes), rsV = make_rsrc(Vp, vbytes);
+    uint32_t offK[DPW], offV[DPW];
+#pragma unroll
+    for (int j = 0; j < DPW; ++j) {
+        const int r = (wave * DPW + j) * RPB + lane / CPR, p = lane % CPR;
+        const int ck = (p ^ kswz(r)) * 8, cv = (p ^ vswz(r)) * 8;
+        offK[j] = ck < a.e ? (uint32_t)((r * a.sk2 + ck) * 2) : kOut;
+        offV[j] = cv < a.ev ? (uint32_t)((r * a.sv2 + cv) * 2) : kOut;
+    }
+    auto issue_k = [&](int kt, char *sk) __attribute__((always_inline)) {
+        const uint32_t kb = (uint32_t)((int64_t)kt * KB * a.sk2 * 2);
+#pragma unroll
+        for (int j = 0; j < DPW; ++j) dma16_buf(rsK, offK[j], kb, sk + (wave * DPW + j) * 1024);
+    };
+    auto issue_v = [&](int kt, char *sv) __attribute__((always_inline)) {
+        const uint32_t vb = (uint32_t)((int64_t)kt * KB * a.sv2 * 2);
+#pragma unroll
+        for (int j = 0; j < DPW; ++j) dma16_buf(rsV, offV[j], vb, sv + (wave * DPW + j) * 1024);
+    };
+    if (nkv > 0) {
+        issue_k(0, sK0);
+        issue_v(0, sV0);
+        if (nkv > 1) issue_k(1, sK1);
+    }
+
+    // this lane's row
+    const int rr = r0 + wave * 32 + lq;
+    bool row_ok = rr < rows_kv;
+    const bool live = r0 + wave * 32 < rows_kv;
+    const int h = row_ok ? rr / a.l : 0, pos = row_ok ? rr - h * a.l : 0;
+    uint64_t mine = 0;
+    if (a.mode == kTree) {
+        if (a.l <= 64) {
+            const uint64_t nodes = tree_bits_wave(a.parent + (int64_t)b * a.l, a.l);
+            mine = (uint64_t)__shfl((uint32_t)(nodes >> 32), pos, 64) << 32 | __shfl((uint32_t)nodes, pos, 64);
+            row_ok = row_ok && mine != 0;
+        } else {
+            tree_bits<NWV * 64>(tb, a.parent + (int64_t)b * a.l, a.l);
+            row_ok = row_ok && (tb.w[pos][pos >> 6] >> (pos & 63)) & 1;
+        }
+    }
+    const T *q = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + (hk * G + h) * a.sq1 + pos * a.sq2;
+    frag qf[KS];
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+        const int d = kk * 16 + lh * 8;
+        qf[kk] = as_frag<frag>(row_ok && d < a.e ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0});
+    }
+
+    // LDS offsets: K row 32 t + lq, chunk 2 kk + lh; V^T row d = 32 dt + lq, whose
+    // 8 key slots of lane half lh are keys 4 lh .. + 3 and 8 + 4 lh .. + 3 of a
+    // 16-key step (the order the scores' registers hold them)
+    const int kpos = kswz(lq);                      // == kswz(32 t + lq)
+    int offVr[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+        const int krow = 4 * (G4 >> 1) + (qq >> 2), d = dt * 32 + 16 * (G4 & 1) + 4 * (qq & 3);
+        offVr[dt] = krow * RB + (((d >> 3) ^ vswz(krow)) << 4) + ((d >> 2) & 1) * 8;   // vswz(krow + 8 x) == vswz(krow)
+    }
+    auto load_k = [&](const char *pk, int kk, int t) __attribute__((always_inline)) {
+        return as_frag<frag>(*reinterpret_cast<const u32x4 *>(pk + (t * 32 + lq) * RB + (((2 * kk + lh) ^ kpos) << 4)));
+    };
+    // scores of a block: sc[t][x] is key kv0 + 32 t + 8 (x / 4) + 4 lh + x % 4
+    auto qk = [&](const char *pk, f32x16 *sc) __attribute__((always_inline)) {
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) sc[t] = Mfma<T>::m32(load_k(pk, kk, t), qf[kk], kk == 0 ? f32x16{} : sc[t]);
+    };
+    auto hide = [&](f32x16 *sc, int kv0) __attribute__((always_inline)) {
+        if (kv0 + KB <= free_end) return;
+        const uint64_t seen = seen_word(a, &tb, mine, pos, kv0, L) >> (4 * lh);
+        const uint32_t w[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+                if (!(w[t] >> (8 * (x >> 2) + (x & 3)) & 1)) sc[t][x] = -INFINITY;
+    };
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = f32x16{};
+    float m_used = -INFINITY, l_run = 0.f;
+    auto step = [&](f32x16 *cur, f32x16 *nxt, const char *pk, const char *pv, int kv0) __attribute__((always_inline)) {
+        hide(cur, kv0);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) mx = fmaxf(mx, cur[t][x]);
+        mx = xor_max<32>(mx) * a.scale_log2;
+        if (__any(mx > m_used + kSlack)) {
+            const float m_new = fmaxf(m_used, mx);
+            const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[t][x] *= alpha;
+            m_used = m_new;
+        }
+        const float mref = m_used == -INFINITY ? 0.f : m_used + Shift<T>::value;
+        float rs = 0.f;
+        constexpr int EPK = 32 / KS, KPF = 3;       // exponentials per MFMA pair; K fragments read ahead
+        frag kr[KPF][2];
+#pragma unroll
+        for (int kk = 0; kk < KPF - 1; ++kk)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) kr[kk][t] = load_k(pk, kk, t);
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            if (kk + KPF - 1 < KS)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) kr[(kk + KPF - 1) % KPF][t] = load_k(pk, kk + KPF - 1, t);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) nxt[t] = Mfma<T>::m32(kr[kk % KPF][t], qf[kk], kk == 0 ? f32x16{} : nxt[t]);
+#pragma unroll
+            for (int y = 0; y < EPK; ++y) {
+                const int idx = kk * EPK + y, t = idx >> 4, x = idx & 15;
+                const float p = fast_exp2(__builtin_fmaf(cur[t][x], a.scale_log2, -mref));
+                cur[t][x] = p;
+                rs += p;
+            }
+        }
+        l_run += rs;
+        constexpr int NV = 4 * DT, VPF = 3;
+        frag vr[VPF];
+        auto load_v = [&](int idx, frag &dst) __attribute__((always_inline)) {
+            const char *vb = pv + offVr[idx % DT] + idx / DT * 16 * RB;
+            const s16x4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)to_lds(vb));
+            const s16x4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)to_lds(vb + 8 * RB));
+            const u32x2 h0 = __builtin_bit_cast(u32x2, t0), h1 = __builtin_bit_cast(u32x2, t1);
+            dst = as_frag<frag>(u32x4{h0[0], h0[1], h1[0], h1[1]});
+        };
+#pragma unroll
+        for (int x = 0; x < VPF - 1; ++x) load_v(x, vr[x]);
+        frag pf;
+#pragma unroll
+        for (int idx = 0; idx < NV; ++idx) {
+            const int b16 = idx / DT;
+            if (idx % DT == 0) {
+                t8 p8;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) p8[x] = from_f32<T>(cur[b16 >> 1][8 * (b16 & 1) + x]);
+                pf = __builtin_bit_cast(frag, p8);
+            }
+            if (idx + VPF - 1 < NV) load_v(idx + VPF - 1, vr[(idx + VPF - 1) % VPF]);
+            o[idx % DT] = Mfma<T>::m32(vr[idx % VPF], pf, o[idx % DT]);
+        }
+    };
+
+    // LDS stages: K_j and V_j in stage j % 2.  Step j needs K_{j+1} and V_j; it
+    // refills stage j % 2 with K_{j+2} and the other one with V_{j+1}, both
+    // consumed a step earlier.  (The last step's next scores are never used.)
+    f32x16 scA[2], scB[2];
+    if (nkv > 0) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (live) qk(sK0, scA);
+    }
+    for (int j0 = 0; j0 < nkv; j0 += 2) {
+#pragma unroll
+        for (int hs = 0; hs < 2; ++hs) {
+            const int j = j0 + hs;
+            if (j >= nkv) break;
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            if (j + 2 < nkv) issue_k(j + 2, hs ? sK1 : sK0);
+            if (j + 1 < nkv) issue_v(j + 1, hs ? sV0 : sV1);
+            if (live) step(hs ? scB : scA, hs ? scA : scB, hs ? sK0 : sK1, hs ? sV1 : sV0, kbeg + j * KB);
+        }
+    }
+    float z = 0.f;                  // stays 0 if every sum is finite
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) z = __builtin_fmaf(o[t][x], 0.f, z);
+    if (__syncthreads_or(live && z != 0.f)) {
+        // as in cache_attn_kernel: again, value by value, for the rows that see them
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] = f32x16{};
+        const float mref = m_used == -INFINITY ? 0.f : m_used + Shift<T>::value;
+        for (int j = 0; j < nkv; ++j) {
+            const int kv0 = kbeg + j * KB;
+            __syncthreads();
+            issue_k(j, sK0);
+            issue_v(j, sV0);
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            if (!live) continue;
+            qk(sK0, scA);
+            hide(scA, kv0);
+            const uint64_t seen = seen_word(a, &tb, mine, pos, kv0, L);
+            // 32 keys' weights at a time through the second stages, [key][row]
+            float (*pw)[32] = reinterpret_cast<float (*)[32]>((wave < 2 ? sK1 : sV1) + (wave & 1) * 4096);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x)
+                    pw[8 * (x >> 2) + 4 * lh + (x & 3)][lq] = fast_exp2(__builtin_fmaf(scA[t][x], a.scale_log2, -mref));
+                __builtin_amdgcn_s_waitcnt(0xc07f);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+                for (int key = 32 * t; key < 32 * t + 32; ++key) {
+                    if (!(seen >> key & 1)) continue;
+                    const float pk = pw[key & 31][lq];
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) {
+                            const int d = dt * 32 + 8 * (y >> 2) + 4 * lh + (y & 3);
+                            o[dt][y] += pk * to_f32(*reinterpret_cast<const T *>(sV0 + key * RB + (((d >> 3) ^ vswz(key)) << 4) + (d & 7) * 2));
+                        }
+                }
+                __builtin_amdgcn_s_waitcnt(0xc07f);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+
+    if (rr >= rows_kv) return;
+    const float m = row_ok ? m_used + Shift<T>::value : -INFINITY;
+    const float l = row_ok ? xor_add<32>(l_run) : 0.f;
+    const int head = hk * G + h;
+    const int64_t st = (int64_t)split * a.n * a.hq * a.l + ((int64_t)b * a.hq + head) * a.l + pos;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            const int d = dt * 32 + 8 * y + 4 * lh;
+            const f32x4 v = row_ok ? f32x4{o[dt][4 * y], o[dt][4 * y + 1], o[dt][4 * y + 2], o[dt][4 * y + 3]} : f32x4{0.f, 0.f, 0.f, 0.f};
+            if (a.splits == 1) store_row<T>(a, b, head, pos, d, v, m, l);
+            else *reinterpret_cast<f32x4 *>(&a.ws_o[st * HD + d]) = v;
+        }
+    if (a.splits > 1 && lh == 0) *reinterpret_cast<f32x2 *>(&a.ws_ml[st * 2]) = f32x2{m, l};
 }
 
 // The splits' states of a row, merged in split order (the same bits whatever
@@ -475,65 +814,154 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
     }
     const int i = (int)(row % a.l), head = (int)(row / a.l % a.hq);
     const int64_t b = row / a.l / a.hq;
-    const float inv = ll != 0.f ? 1.f / ll : 0.f;
-    if (d < a.ev) {
-        typedef T t4 __attribute__((ext_vector_type(4)));
-        t4 w;
-#pragma unroll
-        for (int y = 0; y < 4; ++y) w[y] = from_f32<T>(oo[y] * inv);
-        *reinterpret_cast<t4 *>(reinterpret_cast<T *>(a.O) + b * a.so0 + head * a.so1 + i * a.so2 + d) = w;
-    }
-    if (a.lse && d == 0) a.lse[row] = ll != 0.f ? (mm + __log2f(ll)) * kLn2 : -INFINITY;
+    store_row<T>(a, b, head, i, d, oo, mm, ll);
 }
 
-// key_weights_kernel -- acc[key] += sum over the rows of its KV head of
-// exp(scale q k - lse).  A wave keeps 16 keys in registers (A operand) and goes
-// over the rows 16 at a time; the rows' sum crosses lanes once, at the end.
+// accum_merge_kernel -- the weights of a few rows' keys from the scores that
+// cache_attn_kernel kept, and the merge of its splits: a work-group has 512 keys
+// of a KV head and its share of the rows' outputs.  (Writing and reading the
+// scores costs 8 bytes a row and key, reading K again 2 e a key.)
+constexpr int kScoreRows = 32;
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void accum_merge_kernel(CacheAttnArgs a) {
+    constexpr int D4 = HD / 4, RPB = 256 / D4;
+    __shared__ float s_m[kScoreRows], s_l[kScoreRows];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int b = blockIdx.y / a.hkv, hk = blockIdx.y % a.hkv;
+    const int G = a.hq / a.hkv, rows = G * a.l;
+    const int64_t all = (int64_t)a.n * a.hq * a.l;
+    auto row_of = [&](int r) { return ((int64_t)b * a.hq + hk * G + r / a.l) * a.l + r % a.l; };
+    const int L = keys_of(a, b);
+    if (blockIdx.x > 0 && (int)blockIdx.x * 512 >= L && (int)blockIdx.x >= (rows + RPB - 1) / RPB) return;
+    for (int r = wave; r < rows; r += 4) {
+        const f32x2 ml = lane < a.splits ? *reinterpret_cast<const f32x2 *>(&a.ws_ml[(lane * all + row_of(r)) * 2]) : f32x2{-INFINITY, 0.f};
+        const float mm = wave_max(ml[0]), mu = mm == -INFINITY ? 0.f : mm;
+        const float ll = wave_sum(ml[1] * fast_exp2(ml[0] - mu));
+        if (lane == 0) {
+            s_m[r] = mu;
+            s_l[r] = ll;
+        }
+    }
+    __syncthreads();
+    const int key = blockIdx.x * 512 + tid * 2;
+    if (key < L) {
+        const float *sc = a.scores + (int64_t)(b * a.hkv + hk) * rows * a.spad + key;
+        f32x2 w = {0.f, 0.f};
+        for (int r = 0; r < rows; ++r) {
+            const f32x2 x = *reinterpret_cast<const f32x2 *>(sc + r * a.spad);
+            const float m = s_m[r], inv = s_l[r] != 0.f ? 1.f / s_l[r] : 0.f;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) w[y] += inv * fast_exp2(__builtin_fmaf(x[y], a.scale_log2, -m));
+        }
+        float *acc = a.acc + b * a.sa0 + hk * a.sa1 + key;
+        acc[0] += w[0];
+        if (key + 1 < L) acc[1] += w[1];
+    }
+    if (a.splits == 1) return;
+    const int d = tid % D4 * 4;
+    for (int r = blockIdx.x * RPB + tid / D4; r < rows; r += gridDim.x * RPB) {
+        const int64_t row = row_of(r);
+        f32x4 oo = {0.f, 0.f, 0.f, 0.f};
+        for (int z = 0; z < a.splits; ++z) {
+            const float wgt = fast_exp2(a.ws_ml[(z * all + row) * 2] - s_m[r]);
+            const f32x4 ov = *reinterpret_cast<const f32x4 *>(&a.ws_o[(z * all + row) * HD + d]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) oo[i] = __builtin_fmaf(ov[i], wgt, oo[i]);
+        }
+        // (s_m is 0 for a row that saw nothing: its sum is 0 too)
+        store_row<T>(a, b, hk * G + r / a.l, r % a.l, d, oo, s_m[r], s_l[r]);
+    }
+}
+
+// key_weights_kernel -- the weights of many rows' keys: acc[key] += sum over the
+// rows that see it of exp(scale q k - lse).  A work-group has 64 keys, in the
+// registers of each of its 4 waves (A operand, 32x32x16 MFMA); the waves take the
+// rows in turn, 32 at a time from memory (a head's rows are read by all
+// work-groups of its XCD's L2), and a lane adds up 32 keys of its row position:
+// the rows' sum crosses lanes and waves once, at the end, in a fixed order.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void key_weights_kernel(CacheAttnArgs a) {
-    constexpr int KK = HD / 32;
+    constexpr int KS = HD / 16;
     typedef typename Mfma<T>::frag frag;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int lr = lane & 15, G4 = lane >> 4;
-    const int b = blockIdx.y / a.hkv, hk = blockIdx.y % a.hkv;
-    const int G = a.hq / a.hkv, rows_kv = G * a.l;
+    __shared__ float s_sum[4][64];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lq = lane & 31, lh = lane >> 5;
+    const int b = blockIdx.y / a.hkv, hk = blockIdx.y % a.hkv, G = a.hq / a.hkv;
     const int L = keys_of(a, b), first = L - a.l;
-    const int k0 = blockIdx.x * 64 + wave * 16;
+    const int k0 = blockIdx.x * 64;
     if (k0 >= L) return;
-    frag kf[KK];
-    const bool key_ok = k0 + lr < L;
-    const T *kp = reinterpret_cast<const T *>(a.K) + b * a.sk0 + hk * a.sk1 + (int64_t)(k0 + lr) * a.sk2;
+    // rows before position i0 see none of these keys
+    const int i0 = a.mode == kCausal ? max(0, k0 - first) : 0, per = a.l - i0, rows = G * per;
+    frag kf[2][KS];
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-        const int d = kk * 32 + G4 * 8;
-        kf[kk] = as_frag<frag>(key_ok && d < a.e ? *reinterpret_cast<const u32x4 *>(kp + d) : u32x4{0, 0, 0, 0});
+    for (int t = 0; t < 2; ++t) {
+        const int key = k0 + 32 * t + lq;
+        const T *kp = reinterpret_cast<const T *>(a.K) + b * a.sk0 + hk * a.sk1 + (int64_t)key * a.sk2;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            const int d = kk * 16 + lh * 8;
+            kf[t][kk] = as_frag<frag>(key < L && d < a.e ? *reinterpret_cast<const u32x4 *>(kp + d) : u32x4{0, 0, 0, 0});
+        }
     }
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int r0 = 0; r0 < rows_kv; r0 += 16) {
-        const int rr = r0 + lr;
-        const bool ok = rr < rows_kv;
-        const int h = ok ? rr / a.l : 0, i = ok ? rr % a.l : 0;
+    u32x4 qn[KS];
+    float nl = -INFINITY;
+    int pn = 0;
+    auto load = [&](int r) __attribute__((always_inline)) {
+        const int rr = r + lq;
+        const bool ok = rr < rows;
+        const int h = ok ? rr / per : 0, i = ok ? i0 + rr - h * per : 0;
         const T *q = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + (hk * G + h) * a.sq1 + i * a.sq2;
-        const float lse = ok ? a.lse[((int64_t)b * a.hq + hk * G + h) * a.l + i] * kLog2e : -INFINITY;
-        f32x4 sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            const int d = kk * 32 + G4 * 8;
-            const frag qf = as_frag<frag>(ok && d < a.e ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0});
-            sc = Mfma<T>::m16(kf[kk], qf, sc);
+        for (int kk = 0; kk < KS; ++kk) {
+            const int d = kk * 16 + lh * 8;
+            qn[kk] = ok && d < a.e ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0};
+        }
+        // (a row that saw nothing, or none: weight 0)
+        const float lse = ok ? a.lse[((int64_t)b * a.hq + hk * G + h) * a.l + i] : -INFINITY;
+        nl = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+        pn = ok ? i : a.l;
+    };
+    f32x16 sum[2] = {f32x16{}, f32x16{}};
+    int r = wave * 32;
+    if (r < rows) load(r);
+    for (; r < rows; r += 128) {
+        frag qf[KS];
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) qf[kk] = as_frag<frag>(qn[kk]);
+        const float c = nl;
+        const int last = a.mode == kCausal ? first + pn - k0 : 64;       // the row's last key here
+        if (r + 128 < rows) load(r + 128);
+        f32x16 sc[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) sc[t] = Mfma<T>::m32(kf[t][kk], qf[kk], sc[t]);
+        if (__any(last < 63)) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int x = 0; x < 16; ++x)
+                    if (32 * t + 8 * (x >> 2) + 4 * lh + (x & 3) > last) sc[t][x] = -INFINITY;
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int key = k0 + 4 * G4 + x;
-            const bool vis = ok && lse != -INFINITY && (a.mode == kFull || key <= first + i);
-            sum[x] += vis ? fast_exp2(__builtin_fmaf(sc[x], a.scale_log2, -lse)) : 0.f;
-        }
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) sum[t][x] += fast_exp2(__builtin_fmaf(sc[t][x], a.scale_log2, c));
     }
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-        const float t = group_sum<16>(sum[x]);
-        const int key = k0 + 4 * G4 + x;
-        if (lr == 0 && key < L) a.acc[b * a.sa0 + hk * a.sa1 + key] += t;
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const float v = xor_add<16>(group_sum<16>(sum[t][x]));
+            if (lq == 0) s_sum[wave][32 * t + 8 * (x >> 2) + 4 * lh + (x & 3)] = v;
+        }
+    __syncthreads();
+    if (tid < 64 && k0 + tid < L) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v += s_sum[w][tid];
+        a.acc[b * a.sa0 + hk * a.sa1 + k0 + tid] += v;
     }
 }
 
@@ -543,40 +971,48 @@ constexpr int kGroupsWanted = 512;      // work-groups of a launch: two for each
 constexpr int kMaxSplits = 64;
 
 struct Plan {
-    int hd, rt, row_groups, splits;
+    int hd, rows;          // head dim and rows of a work-group: 16 or 32 (cache_attn_kernel), 128 (cache_rows_kernel)
+    int row_groups, splits;
     int64_t units;
+    size_t o_bytes, ml_bytes, score_bytes;        // of the workspace
 };
 
-// Rows of a work-group: 16, or 32 where there are more than 16.  Splits: as
-// many as fill the GPU, of at least 128 keys (a step of each wave).
-Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev) {
+Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev, bool accum) {
     Plan p{};
     const int64_t w = std::max(e, ev), rows = hq / hkv * l;
     p.hd = w <= 64 ? 64 : w <= 128 ? 128 : 256;
-    p.rt = rows > 16 && p.hd <= 128 ? 2 : 1;
-    p.row_groups = (int)cdiv(rows, 16 * p.rt);
+    p.rows = p.hd == 256 || rows <= 16 ? 16 : rows <= 64 ? 32 : 128;
+    p.row_groups = (int)cdiv(rows, p.rows);
     const int64_t groups = n * hkv * p.row_groups;
     p.splits = (int)std::max<int64_t>(1, std::min({(int64_t)kMaxSplits, kGroupsWanted / std::max<int64_t>(groups, 1), cdiv(s, 128)}));
     p.units = n * hkv * p.splits;
+    const bool keep = accum && rows <= kScoreRows;
+    p.o_bytes = p.splits > 1 ? (size_t)p.splits * n * hq * l * p.hd * 4 : 0;
+    p.score_bytes = keep ? (size_t)n * hkv * rows * (cdiv(s, 32) * 32) * 4 : 0;
+    p.ml_bytes = p.splits > 1 || keep ? (size_t)p.splits * n * hq * l * 8 : 0;
     return p;
 }
 
-size_t state_bytes(const Plan &p, int64_t rows) {
-    return p.splits > 1 ? (size_t)p.splits * rows * (p.hd + 2) * sizeof(float) + 32 : 0;
-}
+size_t state_bytes(const Plan &p) { return p.o_bytes + p.score_bytes + p.ml_bytes; }
 
 template <typename T, int HD>
 int launch_attn(const CacheAttnArgs &a, const Plan &p, hipStream_t st) {
     const dim3 grid((unsigned)(cdiv(p.units, 8) * 8 * p.row_groups));
-    if (p.rt == 1) hipLaunchKernelGGL((cache_attn_kernel<T, HD, 1>), grid, dim3(256), 0, st, a);
-    else if constexpr (HD <= 128) hipLaunchKernelGGL((cache_attn_kernel<T, HD, 2>), grid, dim3(256), 0, st, a);
+    if (p.rows == 16) hipLaunchKernelGGL((cache_attn_kernel<T, HD, 1, 4>), grid, dim3(256), 0, st, a);
+    if constexpr (HD <= 128) {
+        if (p.rows == 32) hipLaunchKernelGGL((cache_attn_kernel<T, HD, 2, 4>), grid, dim3(256), 0, st, a);
+        if (p.rows == 128) hipLaunchKernelGGL((cache_rows_kernel<T, HD>), grid, dim3(256), 0, st, a);
+    }
+    if (a.scores) {
+        hipLaunchKernelGGL((accum_merge_kernel<T, HD>), dim3((unsigned)cdiv(a.s, 512), (unsigned)(a.n * a.hkv)), dim3(256), 0, st, a);
+        return launch_status();
+    }
     if (p.splits > 1) {
         const int64_t rows = (int64_t)a.n * a.hq * a.l;
         hipLaunchKernelGGL((cache_merge_kernel<T, HD>), dim3((unsigned)cdiv(rows, 256 / (HD / 4))), dim3(256), 0, st, a);
     }
     if (a.acc)
-        hipLaunchKernelGGL((key_weights_kernel<T, HD>), dim3((unsigned)cdiv(a.s, 64), (unsigned)(a.n * a.hkv)), dim3(256),
-                           0, st, a);
+        hipLaunchKernelGGL((key_weights_kernel<T, HD>), dim3((unsigned)cdiv(a.s, 64), (unsigned)(a.n * a.hkv)), dim3(256), 0, st, a);
     return launch_status();
 }
 
@@ -626,8 +1062,12 @@ CacheAttnArgs fill_attn(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s
     a.scale_log2 = scale * kLog2e;
     a.kv_len = kv_len;
     a.splits = p.splits; a.row_groups = p.row_groups;
-    a.ws_o = reinterpret_cast<float *>(workspace);
-    a.ws_ml = p.splits > 1 ? a.ws_o + (int64_t)p.splits * n * hq * l * p.hd : nullptr;
+    // (o and the scores in multiples of 16 bytes)
+    char *ws = reinterpret_cast<char *>(workspace);
+    a.ws_o = p.o_bytes ? reinterpret_cast<float *>(ws) : nullptr;
+    a.scores = p.score_bytes ? reinterpret_cast<float *>(ws + p.o_bytes) : nullptr;
+    a.ws_ml = p.ml_bytes ? reinterpret_cast<float *>(ws + p.o_bytes + p.score_bytes) : nullptr;
+    a.spad = cdiv(s, 32) * 32;
     return a;
 }
 
@@ -639,7 +1079,7 @@ using namespace kuiops;
 
 extern "C" size_t kuiops_sdpa_tree_workspace(int64_t n, int64_t hq, int64_t hkv, int64_t t, int64_t s, int64_t e, int64_t ev) {
     if (n <= 0 || hq <= 0 || hkv <= 0 || t <= 0 || s < 0 || e <= 0 || ev <= 0) return 0;
-    return state_bytes(plan_of(n, hq, hkv, t, s, e, ev), n * hq * t);
+    return state_bytes(plan_of(n, hq, hkv, t, s, e, ev, false));
 }
 
 extern "C" int kuiops_sdpa_tree(int64_t n, int64_t hq, int64_t hkv, int64_t t, int64_t s, int64_t e, int64_t ev, int dtype,
@@ -652,9 +1092,9 @@ extern "C" int kuiops_sdpa_tree(int64_t n, int64_t hq, int64_t hkv, int64_t t, i
     if (n == 0 || hq == 0 || t == 0) return KUIOPS_OK;
     if (!parent || t > s) return KUIOPS_E_INVALID;
     if (t > kMaxTree) return KUIOPS_E_UNSUPPORTED;
-    const Plan p = plan_of(n, hq, hkv, t, s, e, ev);
+    const Plan p = plan_of(n, hq, hkv, t, s, e, ev, false);
     if (!split_fits(p, s, sk[2], sv[2])) return KUIOPS_E_UNSUPPORTED;
-    const size_t need = state_bytes(p, n * hq * t);
+    const size_t need = state_bytes(p);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KUIOPS_E_WORKSPACE;
     CacheAttnArgs a = fill_attn(n, hq, hkv, t, s, e, ev, Q, sq, K, sk, V, sv, O, so, lse, scale, kTree, kv_len, p, workspace);
     a.parent = parent;
@@ -664,7 +1104,7 @@ extern "C" int kuiops_sdpa_tree(int64_t n, int64_t hq, int64_t hkv, int64_t t, i
 extern "C" size_t kuiops_sdpa_decode_accum_workspace(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e,
                                                      int64_t ev) {
     if (n <= 0 || hq <= 0 || hkv <= 0 || l <= 0 || s < 0 || e <= 0 || ev <= 0) return 0;
-    return state_bytes(plan_of(n, hq, hkv, l, s, e, ev), n * hq * l);
+    return state_bytes(plan_of(n, hq, hkv, l, s, e, ev, true));
 }
 
 extern "C" int kuiops_sdpa_decode_accum(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev,
@@ -676,9 +1116,9 @@ extern "C" int kuiops_sdpa_decode_accum(int64_t n, int64_t hq, int64_t hkv, int6
     if (bad) return bad;
     if (n == 0 || hq == 0 || l == 0) return KUIOPS_OK;
     if (!lse || !sa || (s > 0 && !acc) || (causal && l > s)) return KUIOPS_E_INVALID;
-    const Plan p = plan_of(n, hq, hkv, l, s, e, ev);
+    const Plan p = plan_of(n, hq, hkv, l, s, e, ev, true);
     if (!split_fits(p, s, sk[2], sv[2])) return KUIOPS_E_UNSUPPORTED;
-    const size_t need = state_bytes(p, n * hq * l);
+    const size_t need = state_bytes(p);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KUIOPS_E_WORKSPACE;
     CacheAttnArgs a = fill_attn(n, hq, hkv, l, s, e, ev, Q, sq, K, sk, V, sv, O, so, lse, scale, causal ? kCausal : kFull,
                                 kv_len, p, workspace);
