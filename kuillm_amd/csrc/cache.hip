@@ -29,17 +29,27 @@ __global__ __launch_bounds__(64) void tree_accept_kernel(int t, const int64_t *t
     parent += b * t;
     target += b * t;
     path += b * t;
+    __shared__ int64_t s_target[kMaxTree];
     int up[NW], mine[NW];                     // parent of a candidate (else -1); the path's node at this lane's place
+    int64_t token[NW];
 #pragma unroll
     for (int x = 0; x < NW; ++x) {
         const int i = x * 64 + lane;
         up[x] = mine[x] = -1;
+        token[x] = 0;
         if (i < t) {
-            const int p = parent[i];
-            if (p >= 0 && p < i && tokens[i] == target[p]) up[x] = p;
+            up[x] = parent[i];
+            token[x] = tokens[i];
+            s_target[i] = target[i];
         }
     }
-    int at = parent[0] == -1 ? 0 : -1, last = -1, n = 0;
+    __syncthreads();
+    int at = __shfl(up[0], 0, 64) == -1 ? 0 : -1, last = -1, n = 0;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+        const int i = x * 64 + lane, p = up[x];
+        up[x] = i < t && p >= 0 && p < i && token[x] == s_target[p] ? p : -1;
+    }
     while (at >= 0) {
 #pragma unroll
         for (int x = 0; x < NW; ++x)
@@ -58,72 +68,89 @@ __global__ __launch_bounds__(64) void tree_accept_kernel(int t, const int64_t *t
         if (x * 64 + lane < t) path[x * 64 + lane] = mine[x];
     if (lane == 0) {
         count[b] = n;
-        next[b] = last >= 0 ? target[last] : -1;
+        next[b] = last >= 0 ? s_target[last] : -1;
     }
 }
 
 // --------------------------------------------------------- kv_tree_commit
-// A work-group has all rows of up to 512 bytes of a head's K or V: every row is
-// in registers before the first is written, so any path is right, whichever
-// rows it reads and overwrites.
-constexpr int kCommitThreads = 512, kCommitRegs = 16;       // x 16 bytes = 256 rows of 512
+// A wave has up to 512 bytes of each row of a head's K or V, and all rows of a
+// pass over their columns are in its registers before the first is written, so
+// any path is right, whichever rows it reads and overwrites.  As many columns a
+// pass as 16 registers of 16 bytes hold: all 32 for up to 32 rows.
+constexpr int kCommitRegs = 16, kCommitWaves = 4;
 struct CommitArgs {
-    int n, p, t;
-    int64_t cap;
+    int n, p, t, hkv;
+    int64_t cap, units;
     char *K, *V;
     int64_t sk0, sk1, sk2, sv0, sv1, sv2;     // bytes
-    int kcols, vcols, kblocks;                // 16-byte chunks of a row; work-groups of 32 chunks for K
+    int kcols, vcols, kblocks, blocks;        // 16-byte chunks of a row; waves of 32 chunks for K, for both
     const int32_t *path, *kv_len;
     int32_t *len_out;
 };
-__global__ __launch_bounds__(kCommitThreads) void tree_commit_kernel(CommitArgs a) {
-    __shared__ int s_path[kMaxTree];
-    __shared__ int s_count;
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.z, head = blockIdx.y;
+__global__ __launch_bounds__(kCommitWaves * 64) void tree_commit_kernel(CommitArgs a) {
+    constexpr int NW = kMaxTree / 64;
+    __shared__ int s_path[kCommitWaves][kMaxTree];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t unit = (int64_t)blockIdx.x * kCommitWaves + wave;
+    if (unit >= a.units) return;
+    const int blk = (int)(unit % a.blocks), head = (int)(unit / a.blocks % a.hkv);
+    const int64_t row = unit / a.blocks / a.hkv;
     const int b = (int)(row % a.n);
-    const bool is_v = (int)blockIdx.x >= a.kblocks;
-    const int c0 = ((int)blockIdx.x - (is_v ? a.kblocks : 0)) * 32;
+    const bool is_v = blk >= a.kblocks;
+    const int c0 = (blk - (is_v ? a.kblocks : 0)) * 32;
     const int cols = min(32, (is_v ? a.vcols : a.kcols) - c0);
     const int64_t len = a.kv_len[b], base = len - a.t;
-    if (tid == 0) s_count = a.p;
-    __syncthreads();
-    if (tid < a.p) {
-        const int x = a.path[(int64_t)b * a.p + tid];
-        s_path[tid] = x;
-        // the path ends at its first entry that is no row of the tree in the cache
-        if (x < 0 || x >= a.t || base < 0 || base + max(x, tid) >= a.cap) atomicMin(&s_count, tid);
+    // the path ends at its first entry that is no row of the tree in the cache
+    int count = a.p;
+#pragma unroll
+    for (int x = NW - 1; x >= 0; --x) {
+        const int i = x * 64 + lane;
+        int v = -1;
+        if (i < a.p) v = a.path[(int64_t)b * a.p + i];
+        s_path[wave][i] = v;
+        const uint64_t bad = __ballot(i < a.p && (v < 0 || v >= a.t || base < 0 || base + max(v, i) >= a.cap));
+        if (bad) count = x * 64 + __builtin_ctzll(bad);
     }
-    __syncthreads();
-    const int count = s_count;
-    if (row < a.n && head == 0 && blockIdx.x == 0 && tid == 0) a.len_out[b] = (int)(base < 0 ? len : base + count);
+    if (unit < (int64_t)a.n * a.hkv * a.blocks && head == 0 && blk == 0 && lane == 0)
+        a.len_out[b] = (int)(base < 0 ? len : base + count);
+    if (count == 0) return;
+    __builtin_amdgcn_s_waitcnt(0xc07f);           // (the wave's own LDS writes)
     char *p = is_v ? a.V + row * a.sv0 + head * a.sv1 : a.K + row * a.sk0 + head * a.sk1;
     const int64_t st = is_v ? a.sv2 : a.sk2;
     p += base * st + c0 * 16;
-    u32x4 r[kCommitRegs];
+    int sh = 5;                                   // 2^sh columns a pass
+    while ((count << sh) > kCommitRegs * 64) --sh;
+    while (sh > 0 && (1 << (sh - 1)) >= cols) --sh;
+    for (int cb = 0; cb < cols; cb += 1 << sh) {
+        u32x4 r[kCommitRegs];
 #pragma unroll
-    for (int x = 0; x < kCommitRegs; ++x) {
-        const int i = x * kCommitThreads + tid, to = i / 32, c = i % 32;
-        if (to < count && c < cols && s_path[to] != to) r[x] = *reinterpret_cast<const u32x4 *>(p + s_path[to] * st + c * 16);
-    }
-    __builtin_amdgcn_s_waitcnt(0);            // read before any row is written
-    __syncthreads();
+        for (int x = 0; x < kCommitRegs; ++x) {
+            const int i = x * 64 + lane, to = i >> sh, c = cb + (i & ((1 << sh) - 1));
+            if (to < count && c < cols) r[x] = *reinterpret_cast<const u32x4 *>(p + s_path[wave][to] * st + c * 16);
+        }
+        __builtin_amdgcn_s_waitcnt(0);            // read before any row is written
+        __builtin_amdgcn_sched_barrier(0);
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
 #pragma unroll
-    for (int x = 0; x < kCommitRegs; ++x) {
-        const int i = x * kCommitThreads + tid, to = i / 32, c = i % 32;
-        if (to < count && c < cols && s_path[to] != to) *reinterpret_cast<u32x4 *>(p + to * st + c * 16) = r[x];
+        for (int x = 0; x < kCommitRegs; ++x) {
+            const int i = x * 64 + lane, to = i >> sh, c = cb + (i & ((1 << sh) - 1));
+            if (to < count && c < cols && s_path[wave][to] != to) *reinterpret_cast<u32x4 *>(p + to * st + c * 16) = r[x];
+        }
     }
 }
 
 // --------------------------------------------------------------- kv_evict
 // evict_select_kernel, a work-group per (sequence, KV head): the key of a slot
 // is its weight's bits in ascending order, or the largest of all for the
-// `recent` newest positions.  The budget-th largest key is found 8 bits at a
-// time with a histogram in LDS; slots with a larger key are kept, and of those
-// with the same key the first ones.  A pass in slot order then lists the freed
-// slots below the budget and the kept ones behind it: as many of one as of the
-// other, and the i-th kept row goes to the i-th freed slot.  Sources are at or
-// behind the budget and destinations below it, so the moves need no order.
+// `recent` newest positions.  The budget-th largest key is found 11, 11 and 10
+// bits at a time with a histogram in LDS (as many bits as that spread weights,
+// which share a few exponents, over enough counters); slots with a larger key are
+// kept, and of those with the same key the first ones.  Ranks in slot order then
+// pair the freed slots below the budget with the kept ones behind it: as many of
+// one as of the other, and the i-th kept row goes to the i-th freed slot.  Sources
+// are at or behind the budget and destinations below it, so the moves need no
+// order.  Slots of 1024 x IPT keys stay in registers (thread t has t, t + 1024,
+// ...); longer caches are read again (from L2) in each of the six passes.
 // evict_move_kernel moves the rows of K and V.
 constexpr int kEvictThreads = 1024;
 struct EvictArgs {
@@ -148,12 +175,37 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
+// Exclusive sums of one value per thread, and their total (all threads).
+template <int NT>
+__device__ __forceinline__ int block_scan(int v, int *s_wave, int &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(incl, o, 64);
+        incl += lane >= o ? x : 0;
+    }
+    if (lane == 63) s_wave[wave] = incl;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+        const int c = s_wave[w];
+        before += w < wave ? c : 0;
+        total += c;
+    }
+    __syncthreads();
+    return before + incl - v;
+}
+
+template <int IPT>        // slots of a thread held in registers; 0: none, any number
 __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a) {
-    constexpr int NT = kEvictThreads, NW = NT / 64;
-    __shared__ int s_red[NW][3];
-    __shared__ int s_hist[256];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_need;
+    constexpr int NT = kEvictThreads, NW = NT / 64, NR = IPT > 0 ? IPT : 1;
+    constexpr int kBins = 2048;
+    __shared__ int s_wave[NW], s_hist[kBins];
+    __shared__ uint16_t s_rank[NW][2];
+    __shared__ int s_digit, s_left, s_same;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int b = blockIdx.x / a.hkv, hk = blockIdx.x % a.hkv, m = a.budget;
     const int L = (int)max((int64_t)0, min((int64_t)a.kv_len[b], a.cap)), cap = (int)a.cap;
@@ -170,75 +222,128 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a
         if (tid == 0) moves[0] = 0;
         return;
     }
-    int newest = INT32_MIN;
-    for (int j = tid; j < L; j += NT) newest = max(newest, pos[j]);
-    newest = -wave_min_i32(-max(newest, -INT32_MAX));
-    if (lane == 0) s_red[wave][0] = newest;
+    const int chunks = (L + NT - 1) / NT;
+    // this thread's slots
+    float ra[NR];
+    int32_t rp[NR];
+    uint32_t rk[NR];
+    int newest = -INT32_MAX;
+    if constexpr (IPT > 0) {
+#pragma unroll
+        for (int c = 0; c < IPT; ++c) {
+            const int j = c * NT + tid;
+            ra[c] = j < L ? acc[j] : 0.f;
+            rp[c] = j < L ? pos[j] : INT32_MIN;
+        }
+#pragma unroll
+        for (int c = 0; c < IPT; ++c) newest = max(newest, rp[c]);
+    } else {
+        for (int j = tid; j < L; j += NT) newest = max(newest, pos[j]);
+    }
+    for (int x = tid; x < kBins; x += NT) s_hist[x] = 0;
+    newest = -wave_min_i32(-newest);
+    if (lane == 0) s_wave[wave] = newest;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) newest = max(newest, s_red[w][0]);
+    for (int w = 0; w < NW; ++w) newest = max(newest, s_wave[w]);
     const int64_t floor_pos = (int64_t)newest - a.recent;
-    auto key_of = [&](int j) -> uint32_t { return pos[j] > floor_pos ? 0xffffffffu : weight_key(acc[j]); };
+    auto key_of = [&](float w, int32_t p) -> uint32_t { return p > floor_pos ? 0xffffffffu : weight_key(w); };
+    if constexpr (IPT > 0) {
+#pragma unroll
+        for (int c = 0; c < IPT; ++c) rk[c] = key_of(ra[c], rp[c]);
+    }
+    // f(slot, key) for this thread's slots, in slot order
+    auto each = [&](auto f) {
+        if constexpr (IPT > 0) {
+#pragma unroll
+            for (int c = 0; c < IPT; ++c)
+                if (c * NT + tid < L) f(c * NT + tid, rk[c]);
+        } else {
+            for (int j = tid; j < L; j += NT) f(j, key_of(acc[j], pos[j]));
+        }
+    };
 
     uint32_t prefix = 0, mask = 0;
-    int need = m;                              // of the keys with this prefix, the need-th largest is sought
-    for (int sh = 24; sh >= 0; sh -= 8) {
-        if (tid < 256) s_hist[tid] = 0;
+    int need = m, same = 0;                    // of the keys with this prefix, the need-th largest is sought
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        each([&](int, uint32_t k) {
+            if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> sh) & ((1 << bits) - 1)], 1);
+        });
         __syncthreads();
-        for (int j = tid; j < L; j += NT) {
-            const uint32_t k = key_of(j);
-            if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> sh) & 255], 1);
+        // thread t has the two largest counters that are left of it: kBins - 1 - 2 t and the next one below
+        const int hi = s_hist[kBins - 1 - 2 * tid], lo = s_hist[kBins - 2 - 2 * tid];
+        int total;
+        const int above = block_scan<NT>(hi + lo, s_wave, total);
+        if (above < need && need <= above + hi + lo) {
+            const bool first = need <= above + hi;
+            s_digit = kBins - 1 - 2 * tid - (first ? 0 : 1);
+            s_left = need - above - (first ? 0 : hi);
+            s_same = first ? hi : lo;
         }
+        s_hist[kBins - 1 - 2 * tid] = s_hist[kBins - 2 - 2 * tid] = 0;
         __syncthreads();
-        if (tid == 0) {
-            int left = need, v = 255;
-            while (v > 0 && s_hist[v] < left) left -= s_hist[v--];
-            s_prefix = prefix | ((uint32_t)v << sh);
-            s_need = left;
-        }
-        __syncthreads();
-        prefix = s_prefix;
-        need = s_need;
-        mask |= 255u << sh;
+        prefix |= (uint32_t)s_digit << sh;
+        mask |= ((1u << bits) - 1) << sh;
+        need = s_left;
+        same = s_same;
     }
 
-    // slots in order, 1024 at a time: running counts of equal keys, freed and far slots
+    // 1024 slots at a time: running counts of equal keys, and of freed and far slots
+    const bool ties = need < same;              // some of the equal keys are freed
     int eq0 = 0, hole0 = 0, far0 = 0;
     const uint64_t below = (1ull << lane) - 1;
-    for (int j0 = 0; j0 < L; j0 += NT) {
-        const int j = j0 + tid;
-        const uint32_t k = j < L ? key_of(j) : 0;
-        const bool eq = j < L && k == prefix;
-        const uint64_t eqs = __ballot(eq);
-        if (lane == 0) s_red[wave][0] = __popcll(eqs);
-        __syncthreads();
-        int eqr = eq0 + __popcll(eqs & below);
+    auto chunk = [&](int c, uint32_t k, bool reg, float av, int32_t pv) __attribute__((always_inline)) {
+        const int j = c * NT + tid;
+        const bool in = j < L;
+        int eqr = 0;
+        if (ties) {
+            const uint64_t eqs = __ballot(in && k == prefix);
+            if (lane == 0) s_wave[wave] = __popcll(eqs);
+            __syncthreads();
+            eqr = eq0 + __popcll(eqs & below);
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const int c = s_red[w][0];
-            if (w < wave) eqr += c;
-            eq0 += c;
+            for (int w = 0; w < NW; ++w) {
+                const int x = s_wave[w];
+                eqr += w < wave ? x : 0;
+                eq0 += x;
+            }
+            // (the barriers below separate these reads from the next chunk's writes)
         }
-        const bool kept = j < L && (k > prefix || (eq && eqr < need));
-        const bool hole = j < m && !kept, far = j >= m && kept;
+        const bool kept = in && (k > prefix || (k == prefix && eqr < need));
+        const bool hole = in && j < m && !kept, far = j >= m && kept;
         const uint64_t holes = __ballot(hole), fars = __ballot(far);
         if (lane == 0) {
-            s_red[wave][1] = __popcll(holes);
-            s_red[wave][2] = __popcll(fars);
+            s_rank[wave][0] = (uint16_t)__popcll(holes);
+            s_rank[wave][1] = (uint16_t)__popcll(fars);
         }
         __syncthreads();
         int hr = hole0 + __popcll(holes & below), fr = far0 + __popcll(fars & below);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            if (w < wave) { hr += s_red[w][1]; fr += s_red[w][2]; }
-            hole0 += s_red[w][1];
-            far0 += s_red[w][2];
+            const int x = s_rank[w][0], y = s_rank[w][1];
+            hr += w < wave ? x : 0;
+            fr += w < wave ? y : 0;
+            hole0 += x;
+            far0 += y;
         }
+        __syncthreads();
         if (hole) moves[1 + hr] = j;
         if (far) moves[1 + m + fr] = j;
         if (kept && !far) {
-            acc_out[j] = acc[j];
-            pos_out[j] = pos[j];
+            acc_out[j] = reg ? av : acc[j];
+            pos_out[j] = reg ? pv : pos[j];
+        }
+    };
+    if constexpr (IPT > 0) {
+#pragma unroll
+        for (int c = 0; c < IPT; ++c)
+            if (c < chunks) chunk(c, rk[c], true, ra[c], rp[c]);
+    } else {
+        for (int c = 0; c < chunks; ++c) {
+            const int j = c * NT + tid;
+            chunk(c, j < L ? key_of(acc[j], pos[j]) : 0, false, 0.f, 0);
         }
     }
     if (tid == 0) moves[0] = hole0;
@@ -316,9 +421,13 @@ extern "C" int kuiops_kv_tree_commit(int64_t batch, int64_t n, int64_t hkv, int6
     a.sk0 = sk[0]; a.sk1 = sk[1]; a.sk2 = sk[2];
     a.sv0 = sv[0]; a.sv1 = sv[1]; a.sv2 = sv[2];
     a.kcols = (int)(krow / 16); a.vcols = (int)(vrow / 16); a.kblocks = (int)cdiv(a.kcols, 32);
+    a.blocks = a.kblocks + (int)cdiv(a.vcols, 32);
+    a.hkv = (int)hkv;
+    a.units = batch * hkv * a.blocks;
     a.path = path; a.kv_len = kv_len; a.len_out = len_out;
-    const dim3 grid((unsigned)(a.kblocks + cdiv(a.vcols, 32)), (unsigned)hkv, (unsigned)batch);
-    hipLaunchKernelGGL(tree_commit_kernel, grid, dim3(kCommitThreads), 0, as_stream(stream), a);
+    if (cdiv(a.units, kCommitWaves) > INT32_MAX) return KUIOPS_E_UNSUPPORTED;
+    hipLaunchKernelGGL(tree_commit_kernel, dim3((unsigned)cdiv(a.units, kCommitWaves)), dim3(kCommitWaves * 64), 0,
+                       as_stream(stream), a);
     return launch_status();
 }
 
@@ -357,7 +466,11 @@ extern "C" int kuiops_kv_evict(int64_t n, int64_t hkv, int64_t cap, int64_t krow
     const int64_t most = std::max<int64_t>(0, std::min(budget, cap - budget)) * (a.kcols + a.vcols);
     const int64_t per = std::max<int64_t>(1, cdiv(2048, n * hkv));
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min(per, cdiv(most, 256))), (unsigned)(n * hkv));
-    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)(n * hkv)), dim3(kEvictThreads), 0, as_stream(stream), a);
+    const dim3 heads((unsigned)(n * hkv)), threads(kEvictThreads);
+    if (cap <= kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<1>), heads, threads, 0, as_stream(stream), a);
+    else if (cap <= 4 * kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<4>), heads, threads, 0, as_stream(stream), a);
+    else if (cap <= 16 * kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<16>), heads, threads, 0, as_stream(stream), a);
+    else hipLaunchKernelGGL((evict_select_kernel<0>), heads, threads, 0, as_stream(stream), a);
     hipLaunchKernelGGL(evict_move_kernel, grid, dim3(256), 0, as_stream(stream), a);
     return launch_status();
 }

@@ -54,7 +54,8 @@ struct CacheAttnArgs {
     float scale_log2;          // softmax scale * log2(e), > 0
     const int32_t *kv_len;     // [n] device, or null: s
     const int32_t *parent;     // kTree: [n][l]
-    int splits, row_groups;
+    int splits, row_groups;    // row groups that work-groups begin with: half of them with `pair`
+    int pair;
     float *ws_ml;              // [splits][n * hq * l][2]: maximum (log2 domain), sum
     float *ws_o;               // [splits][n * hq * l][HD]: unnormalised output
     float *acc;                // kuiops_sdpa_decode_accum: per key sums, strides sa0, sa1, 1
@@ -533,25 +534,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const Unit u = unit_of(a);
     if (!u.any) return;
     const int b = u.b, hk = u.hk, split = u.split;
-    const int G = a.hq / a.hkv, rows_kv = G * a.l, r0 = u.rg * R;
-
+    const int G = a.hq / a.hkv, rows_kv = G * a.l;
     const int L = keys_of(a, b), first = L - a.l;
     const int blocks_all = (L + KB - 1) / KB;
     const int chunk = (blocks_all + a.splits - 1) / a.splits * KB;
+
+    // a.pair: row groups p and last - p, whose causal lengths together are the same for every p
+    const int groups = (rows_kv + R - 1) / R;
+    for (int rg = u.rg;;) {
+    const int r0 = rg * R, last = min(r0 + R, rows_kv) - 1;
     const int kbeg = min(L, split * chunk);
     int kend = min(L, kbeg + chunk);
-    if (a.mode == kCausal) {
-        // keys past the last position of the work-group's rows are seen by none
-        const int last = min(r0 + R, rows_kv) - 1;
-        if (r0 / a.l == last / a.l) kend = max(kbeg, min(kend, first + last % a.l + 1));
-    }
-    const int free_end = a.mode == kFull ? L : a.mode == kCausal ? first + 1 : first;
+    // keys past the last position of the work-group's rows are seen by none
+    if (a.mode == kCausal && r0 / a.l == last / a.l) kend = max(kbeg, min(kend, first + last % a.l + 1));
+    // keys below free_end are seen by every row of the wave
+    const int w0 = r0 + wave * 32, w1 = min(w0 + 31, rows_kv - 1);
+    const int free_end = a.mode == kFull ? L : a.mode == kCausal ? first + 1 + (w0 / a.l == w1 / a.l ? w0 % a.l : 0) : first;
     const int nkv = (kend - kbeg + KB - 1) / KB;
 
     const T *Kp = reinterpret_cast<const T *>(a.K) + b * a.sk0 + hk * a.sk1 + (int64_t)kbeg * a.sk2;
     const T *Vp = reinterpret_cast<const T *>(a.V) + b * a.sv0 + hk * a.sv1 + (int64_t)kbeg * a.sv2;
-    const uint32_t kbytes = kend > kbeg ? (uint32_t)(((int64_t)(min(L, kbeg + chunk) - kbeg - 1) * a.sk2 + a.e) * 2) : 0u;
-    const uint32_t vbytes = kend > kbeg ? (uint32_t)(((int64_t)(min(L, kbeg + chunk) - kbeg - 1) * a.sv2 + a.ev) * 2) : 0u;
+    const uint32_t kbytes = kend > kbeg ? (uint32_t)(((int64_t)(kend - kbeg - 1) * a.sk2 + a.e) * 2) : 0u;
+    const uint32_t vbytes = kend > kbeg ? (uint32_t)(((int64_t)(kend - kbeg - 1) * a.sv2 + a.ev) * 2) : 0u;
     const __amdgpu_buffer_rsrc_t rsK = make_rsrc(Kp, kbytes), rsV = make_rsrc(Vp, vbytes);
     uint32_t offK[DPW], offV[DPW];
 #pragma unroll
@@ -578,9 +582,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 
     // this lane's row
-    const int rr = r0 + wave * 32 + lq;
+    const int rr = w0 + lq;
     bool row_ok = rr < rows_kv;
-    const bool live = r0 + wave * 32 < rows_kv;
+    const bool live = w0 < rows_kv;
     const int h = row_ok ? rr / a.l : 0, pos = row_ok ? rr - h * a.l : 0;
     uint64_t mine = 0;
     if (a.mode == kTree) {
@@ -773,25 +777,66 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
     }
 
-    if (rr >= rows_kv) return;
-    const float m = row_ok ? m_used + Shift<T>::value : -INFINITY;
-    const float l = row_ok ? xor_add<32>(l_run) : 0.f;
-    const int head = hk * G + h;
-    const int64_t st = (int64_t)split * a.n * a.hq * a.l + ((int64_t)b * a.hq + head) * a.l + pos;
+    const float l_all = xor_add<32>(l_run);
+    if (rr < rows_kv) {
+        const float m = row_ok ? m_used + Shift<T>::value : -INFINITY, l = row_ok ? l_all : 0.f;
+        const int head = hk * G + h;
+        const int64_t st = (int64_t)split * a.n * a.hq * a.l + ((int64_t)b * a.hq + head) * a.l + pos;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-            const int d = dt * 32 + 8 * y + 4 * lh;
-            const f32x4 v = row_ok ? f32x4{o[dt][4 * y], o[dt][4 * y + 1], o[dt][4 * y + 2], o[dt][4 * y + 3]} : f32x4{0.f, 0.f, 0.f, 0.f};
-            if (a.splits == 1) store_row<T>(a, b, head, pos, d, v, m, l);
-            else *reinterpret_cast<f32x4 *>(&a.ws_o[st * HD + d]) = v;
-        }
-    if (a.splits > 1 && lh == 0) *reinterpret_cast<f32x2 *>(&a.ws_ml[st * 2]) = f32x2{m, l};
+            for (int y = 0; y < 4; ++y) {
+                const int d = dt * 32 + 8 * y + 4 * lh;
+                const f32x4 v = row_ok ? f32x4{o[dt][4 * y], o[dt][4 * y + 1], o[dt][4 * y + 2], o[dt][4 * y + 3]} : f32x4{0.f, 0.f, 0.f, 0.f};
+                if (a.splits == 1) store_row<T>(a, b, head, pos, d, v, m, l);
+                else *reinterpret_cast<f32x4 *>(&a.ws_o[st * HD + d]) = v;
+            }
+        if (a.splits > 1 && lh == 0) *reinterpret_cast<f32x2 *>(&a.ws_ml[st * 2]) = f32x2{m, l};
+    }
+    if (!a.pair || rg != u.rg || groups - 1 - rg == rg) break;
+    rg = groups - 1 - rg;
+    __syncthreads();                // (the other group's first keys take the place of the last ones)
+    }
 }
 
-// The splits' states of a row, merged in split order (the same bits whatever
-// order the work-groups ended in): a thread has 4 columns of a row.
+// 4 columns of a row's splits, merged in split order (the same bits whatever order
+// the work-groups ended in); the splits' loads go out together, 8 at a time.
+template <int HD>
+__device__ __forceinline__ void merge_splits(const CacheAttnArgs &a, int64_t rows, int64_t row, int d, f32x4 &oo, float &mm, float &ll) {
+    oo = f32x4{0.f, 0.f, 0.f, 0.f};
+    mm = -INFINITY;
+    ll = 0.f;
+    for (int z0 = 0; z0 < a.splits; z0 += 8) {
+        f32x4 ov[8];
+        f32x2 ml[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            const int64_t st = (z0 + y) * rows + row;
+            ml[y] = f32x2{-INFINITY, 0.f};
+            if (z0 + y < a.splits) {
+                ml[y] = *reinterpret_cast<const f32x2 *>(&a.ws_ml[st * 2]);
+                ov[y] = *reinterpret_cast<const f32x4 *>(&a.ws_o[st * HD + d]);
+            }
+        }
+        float top = mm;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) top = fmaxf(top, ml[y][0]);
+        const float mu = top == -INFINITY ? 0.f : top, old = fast_exp2(mm - mu);
+        ll *= old;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) oo[i] *= old;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            if (z0 + y < a.splits) {
+                const float wgt = fast_exp2(ml[y][0] - mu);
+                ll = __builtin_fmaf(ml[y][1], wgt, ll);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) oo[i] = __builtin_fmaf(ov[y][i], wgt, oo[i]);
+            }
+        }
+        mm = top;
+    }
+}
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
     constexpr int D4 = HD / 4;
@@ -799,22 +844,11 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
     const int64_t row = (int64_t)blockIdx.x * (256 / D4) + threadIdx.x / D4;
     if (row >= rows) return;
     const int d = threadIdx.x % D4 * 4;
-    float mm = -INFINITY;
-    for (int z = 0; z < a.splits; ++z) mm = fmaxf(mm, a.ws_ml[(z * rows + row) * 2]);
-    const float mu = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f;
-    f32x4 oo = {0.f, 0.f, 0.f, 0.f};
-    for (int z = 0; z < a.splits; ++z) {
-        const f32x2 ml = *reinterpret_cast<const f32x2 *>(&a.ws_ml[(z * rows + row) * 2]);
-        const f32x4 ov = *reinterpret_cast<const f32x4 *>(&a.ws_o[(z * rows + row) * HD + d]);
-        const float wgt = fast_exp2(ml[0] - mu);
-        ll = __builtin_fmaf(ml[1], wgt, ll);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) oo[i] = __builtin_fmaf(ov[i], wgt, oo[i]);
-    }
-    const int i = (int)(row % a.l), head = (int)(row / a.l % a.hq);
-    const int64_t b = row / a.l / a.hq;
-    store_row<T>(a, b, head, i, d, oo, mm, ll);
+    f32x4 oo;
+    float mm, ll;
+    merge_splits<HD>(a, rows, row, d, oo, mm, ll);
+    const int i = (int)(row % a.l);
+    store_row<T>(a, row / a.l / a.hq, (int)(row / a.l % a.hq), i, d, oo, mm, ll);
 }
 
 // accum_merge_kernel -- the weights of a few rows' keys from the scores that
@@ -839,129 +873,192 @@ __global__ __launch_bounds__(256) void accum_merge_kernel(CacheAttnArgs a) {
         const float ll = wave_sum(ml[1] * fast_exp2(ml[0] - mu));
         if (lane == 0) {
             s_m[r] = mu;
-            s_l[r] = ll;
+            s_l[r] = ll != 0.f ? 1.f / ll : 0.f;
+        }
+    }
+    // the rows' outputs
+    if (a.splits > 1) {
+        const int d = tid % D4 * 4;
+        for (int r = blockIdx.x * RPB + tid / D4; r < rows; r += gridDim.x * RPB) {
+            f32x4 oo;
+            float mm, ll;
+            merge_splits<HD>(a, all, row_of(r), d, oo, mm, ll);
+            store_row<T>(a, b, hk * G + r / a.l, r % a.l, d, oo, mm, ll);
         }
     }
     __syncthreads();
     const int key = blockIdx.x * 512 + tid * 2;
-    if (key < L) {
-        const float *sc = a.scores + (int64_t)(b * a.hkv + hk) * rows * a.spad + key;
-        f32x2 w = {0.f, 0.f};
-        for (int r = 0; r < rows; ++r) {
-            const f32x2 x = *reinterpret_cast<const f32x2 *>(sc + r * a.spad);
-            const float m = s_m[r], inv = s_l[r] != 0.f ? 1.f / s_l[r] : 0.f;
+    if (key >= L) return;
+    const float *sc = a.scores + (int64_t)(b * a.hkv + hk) * rows * a.spad + key;
+    f32x2 w = {0.f, 0.f};
+    for (int r = 0; r < rows; r += 4) {
+        f32x2 x[4];
 #pragma unroll
-            for (int y = 0; y < 2; ++y) w[y] += inv * fast_exp2(__builtin_fmaf(x[y], a.scale_log2, -m));
-        }
-        float *acc = a.acc + b * a.sa0 + hk * a.sa1 + key;
-        acc[0] += w[0];
-        if (key + 1 < L) acc[1] += w[1];
-    }
-    if (a.splits == 1) return;
-    const int d = tid % D4 * 4;
-    for (int r = blockIdx.x * RPB + tid / D4; r < rows; r += gridDim.x * RPB) {
-        const int64_t row = row_of(r);
-        f32x4 oo = {0.f, 0.f, 0.f, 0.f};
-        for (int z = 0; z < a.splits; ++z) {
-            const float wgt = fast_exp2(a.ws_ml[(z * all + row) * 2] - s_m[r]);
-            const f32x4 ov = *reinterpret_cast<const f32x4 *>(&a.ws_o[(z * all + row) * HD + d]);
+        for (int y = 0; y < 4; ++y) x[y] = *reinterpret_cast<const f32x2 *>(sc + min(r + y, rows - 1) * a.spad);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) oo[i] = __builtin_fmaf(ov[i], wgt, oo[i]);
+        for (int y = 0; y < 4; ++y) {
+            if (r + y >= rows) break;
+            const float m = s_m[r + y], inv = s_l[r + y];
+#pragma unroll
+            for (int z = 0; z < 2; ++z) w[z] += inv * fast_exp2(__builtin_fmaf(x[y][z], a.scale_log2, -m));
         }
-        // (s_m is 0 for a row that saw nothing: its sum is 0 too)
-        store_row<T>(a, b, hk * G + r / a.l, r % a.l, d, oo, s_m[r], s_l[r]);
     }
+    float *acc = a.acc + b * a.sa0 + hk * a.sa1 + key;
+    acc[0] += w[0];
+    if (key + 1 < L) acc[1] += w[1];
 }
 
 // key_weights_kernel -- the weights of many rows' keys: acc[key] += sum over the
-// rows that see it of exp(scale q k - lse).  A work-group has 64 keys, in the
-// registers of each of its 4 waves (A operand, 32x32x16 MFMA); the waves take the
-// rows in turn, 32 at a time from memory (a head's rows are read by all
-// work-groups of its XCD's L2), and a lane adds up 32 keys of its row position:
-// the rows' sum crosses lanes and waves once, at the end, in a fixed order.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void key_weights_kernel(CacheAttnArgs a) {
-    constexpr int KS = HD / 16;
+// rows that see it of exp(scale q k - lse).  A tile is 32 * KT keys, in the
+// registers of each of the NWV waves (A operand, 32x32x16 MFMA); the waves take
+// the rows in turn, 32 at a time, and a lane adds up its keys of its row position:
+// the rows' sum crosses lanes and waves once, at the end, in a fixed order.  Rows
+// come through the wave's own LDS stages by DMA, whole rows at a time: loaded from
+// memory into the operand's lanes, 16 bytes of 32 rows each, their addresses alone
+// took three times the arithmetic's time.  A work-group takes tiles p and last - p:
+// causal keys are seen by the fewer rows the later they are, and two such tiles
+// always by about as many.  The exponentials bound it.
+template <typename T, int HD, int KT>
+__global__ __launch_bounds__(HD <= 128 ? 512 : 256) void key_weights_kernel(CacheAttnArgs a, int tiles) {
+    constexpr int KS = HD / 16, NWV = HD <= 128 ? 8 : 4, KEYS = 32 * KT, NS = HD <= 64 ? 3 : 2;
+    constexpr int RB = HD * 2, CPR = HD / 8, RPB = 1024 / RB, STAGE = 32 * RB, DPT = STAGE / 1024, STEP = NWV * 32;
     typedef typename Mfma<T>::frag frag;
-    __shared__ float s_sum[4][64];
+    auto swz = [](int r) { return CPR >= 16 ? (r & 15) : ((r >> 1) & 7); };     // as cache_rows_kernel's K
+    __shared__ __attribute__((aligned(1024))) char sQ[NS][NWV][STAGE];
+    __shared__ float s_sum[NWV][KEYS];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lq = lane & 31, lh = lane >> 5;
     const int b = blockIdx.y / a.hkv, hk = blockIdx.y % a.hkv, G = a.hq / a.hkv;
     const int L = keys_of(a, b), first = L - a.l;
-    const int k0 = blockIdx.x * 64;
-    if (k0 >= L) return;
-    // rows before position i0 see none of these keys
-    const int i0 = a.mode == kCausal ? max(0, k0 - first) : 0, per = a.l - i0, rows = G * per;
-    frag kf[2][KS];
+    const int p = blockIdx.x;
+    const T *Qp = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + hk * G * a.sq1;
+    const float *Lp = a.lse + ((int64_t)b * a.hq + hk * G) * a.l;
+    // this lane's row of a stage and its 16 bytes of it, per DMA instruction (columns
+    // past the head dim read others: they meet zeros of K)
+    int row_j[DPT], col_j[DPT];
+    int64_t off_j[DPT];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int key = k0 + 32 * t + lq;
-        const T *kp = reinterpret_cast<const T *>(a.K) + b * a.sk0 + hk * a.sk1 + (int64_t)key * a.sk2;
-#pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
-            const int d = kk * 16 + lh * 8;
-            kf[t][kk] = as_frag<frag>(key < L && d < a.e ? *reinterpret_cast<const u32x4 *>(kp + d) : u32x4{0, 0, 0, 0});
-        }
+    for (int j = 0; j < DPT; ++j) {
+        row_j[j] = j * RPB + lane / CPR;
+        const int c = ((lane % CPR) ^ swz(row_j[j])) * 8;
+        col_j[j] = c < a.e ? c : 0;
+        off_j[j] = row_j[j] * a.sq2 + col_j[j];
     }
-    u32x4 qn[KS];
-    float nl = -INFINITY;
-    int pn = 0;
-    auto load = [&](int r) __attribute__((always_inline)) {
-        const int rr = r + lq;
-        const bool ok = rr < rows;
-        const int h = ok ? rr / per : 0, i = ok ? i0 + rr - h * per : 0;
-        const T *q = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + (hk * G + h) * a.sq1 + i * a.sq2;
+    for (int tile = p;; tile = tiles - 1 - p) {
+        const int k0 = tile * KEYS;
+        if (k0 < L) {
+            // rows before position i0 see none of these keys
+            const int i0 = a.mode == kCausal ? max(0, k0 - first) : 0, per = a.l - i0, rows = G * per;
+            frag kf[KT][KS];
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
-            const int d = kk * 16 + lh * 8;
-            qn[kk] = ok && d < a.e ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0};
+            for (int t = 0; t < KT; ++t) {
+                const int key = k0 + 32 * t + lq;
+                const T *kp = reinterpret_cast<const T *>(a.K) + b * a.sk0 + hk * a.sk1 + (int64_t)key * a.sk2;
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk) {
+                    const int d = kk * 16 + lh * 8;
+                    kf[t][kk] = as_frag<frag>(key < L && d < a.e ? *reinterpret_cast<const u32x4 *>(kp + d) : u32x4{0, 0, 0, 0});
+                }
+            }
+            float ln[NS];
+            int pn[NS];
+            // the wave's next 32 rows into stage z.  Past the list a lane takes its last
+            // row (with a weight of 0, and for the keys only that this row sees: a NaN in
+            // it reaches no others), so every turn has the same loads.
+            int r0 = wave * 32, h0 = r0 / per, p0 = i0 + r0 - h0 * per;
+            auto load = [&](int z) __attribute__((always_inline)) {
+                const float *lp;
+                if (p0 + 31 < a.l && r0 + 31 < rows) {
+                    const T *q = Qp + h0 * a.sq1 + p0 * a.sq2;
+#pragma unroll
+                    for (int j = 0; j < DPT; ++j)
+                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(q + off_j[j]),
+                                                         (__attribute__((address_space(3))) void *)to_lds(sQ[z][wave] + j * 1024), 16, 0, 0);
+                    lp = Lp + (int64_t)h0 * a.l + p0 + lq;
+                    pn[z] = p0 + lq;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < DPT; ++j) {
+                        const int r = min(r0 + row_j[j], rows - 1), h = r / per;
+                        const T *q = Qp + h * a.sq1 + (i0 + r - h * per) * a.sq2 + col_j[j];
+                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)q,
+                                                         (__attribute__((address_space(3))) void *)to_lds(sQ[z][wave] + j * 1024), 16, 0, 0);
+                    }
+                    const int r = min(r0 + lq, rows - 1), h = r / per;
+                    pn[z] = i0 + r - h * per;
+                    lp = Lp + (int64_t)h * a.l + pn[z];
+                }
+                const float x = *lp;
+                ln[z] = r0 + lq < rows ? x : -INFINITY;
+                __builtin_amdgcn_sched_barrier(0);
+                r0 += STEP;
+                p0 += STEP;
+                while (r0 < rows && p0 >= a.l) {
+                    p0 -= per;
+                    ++h0;
+                }
+            };
+            f32x16 sum[KT];
+#pragma unroll
+            for (int t = 0; t < KT; ++t) sum[t] = f32x16{};
+#pragma unroll
+            for (int z = 0; z < NS - 1; ++z) load(z);
+            for (int rb = wave * 32; rb < rows; rb += NS * STEP) {
+#pragma unroll
+                for (int z = 0; z < NS; ++z) {
+                    if (rb + z * STEP >= rows) break;
+                    load((z + NS - 1) % NS);
+                    // this turn's rows have landed: only the later turns' loads are younger
+                    constexpr int Y = (NS - 1) * (DPT + 1);
+                    __builtin_amdgcn_s_waitcnt((Y & 15) | ((Y >> 4) << 14) | (7 << 4) | (15 << 8));
+                    __builtin_amdgcn_sched_barrier(0);
+                    // (a row that saw nothing, or none: weight 0)
+                    const float c = ln[z] == -INFINITY ? -INFINITY : -ln[z] * kLog2e;
+                    const int last = a.mode == kCausal ? first + pn[z] - k0 : KEYS;       // the row's last key here
+                    f32x16 sc[KT];
+#pragma unroll
+                    for (int kk = 0; kk < KS; ++kk) {
+                        const frag qf = as_frag<frag>(*reinterpret_cast<const u32x4 *>(sQ[z][wave] + lq * RB + (((2 * kk + lh) ^ swz(lq)) << 4)));
+#pragma unroll
+                        for (int t = 0; t < KT; ++t) sc[t] = Mfma<T>::m32(kf[t][kk], qf, kk == 0 ? f32x16{} : sc[t]);
+                    }
+                    if (__any(last < KEYS - 1)) {
+#pragma unroll
+                        for (int t = 0; t < KT; ++t)
+#pragma unroll
+                            for (int x = 0; x < 16; ++x)
+                                if (32 * t + 8 * (x >> 2) + 4 * lh + (x & 3) > last) sc[t][x] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int t = 0; t < KT; ++t)
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) sum[t][x] += fast_exp2(__builtin_fmaf(sc[t][x], a.scale_log2, c));
+                    // (the stage's reads are done before its refill)
+                    __builtin_amdgcn_s_waitcnt(0xc07f);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            // no DMA is in flight past here
+            __builtin_amdgcn_s_waitcnt(0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const float v = xor_add<16>(group_sum<16>(sum[t][x]));
+                    if (lq == 0) s_sum[wave][32 * t + 8 * (x >> 2) + 4 * lh + (x & 3)] = v;
+                }
+            __syncthreads();
+            if (tid < KEYS && k0 + tid < L) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < NWV; ++w) v += s_sum[w][tid];
+                a.acc[b * a.sa0 + hk * a.sa1 + k0 + tid] += v;
+            }
+            __syncthreads();
         }
-        // (a row that saw nothing, or none: weight 0)
-        const float lse = ok ? a.lse[((int64_t)b * a.hq + hk * G + h) * a.l + i] : -INFINITY;
-        nl = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
-        pn = ok ? i : a.l;
-    };
-    f32x16 sum[2] = {f32x16{}, f32x16{}};
-    int r = wave * 32;
-    if (r < rows) load(r);
-    for (; r < rows; r += 128) {
-        frag qf[KS];
-#pragma unroll
-        for (int kk = 0; kk < KS; ++kk) qf[kk] = as_frag<frag>(qn[kk]);
-        const float c = nl;
-        const int last = a.mode == kCausal ? first + pn - k0 : 64;       // the row's last key here
-        if (r + 128 < rows) load(r + 128);
-        f32x16 sc[2] = {f32x16{}, f32x16{}};
-#pragma unroll
-        for (int kk = 0; kk < KS; ++kk)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) sc[t] = Mfma<T>::m32(kf[t][kk], qf[kk], sc[t]);
-        if (__any(last < 63)) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int x = 0; x < 16; ++x)
-                    if (32 * t + 8 * (x >> 2) + 4 * lh + (x & 3) > last) sc[t][x] = -INFINITY;
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) sum[t][x] += fast_exp2(__builtin_fmaf(sc[t][x], a.scale_log2, c));
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-            const float v = xor_add<16>(group_sum<16>(sum[t][x]));
-            if (lq == 0) s_sum[wave][32 * t + 8 * (x >> 2) + 4 * lh + (x & 3)] = v;
-        }
-    __syncthreads();
-    if (tid < 64 && k0 + tid < L) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) v += s_sum[w][tid];
-        a.acc[b * a.sa0 + hk * a.sa1 + k0 + tid] += v;
+        if (tile != p || tiles - 1 - p <= p) break;
     }
 }
 
@@ -972,12 +1069,12 @@ constexpr int kMaxSplits = 64;
 
 struct Plan {
     int hd, rows;          // head dim and rows of a work-group: 16 or 32 (cache_attn_kernel), 128 (cache_rows_kernel)
-    int row_groups, splits;
+    int row_groups, splits, pair;
     int64_t units;
     size_t o_bytes, ml_bytes, score_bytes;        // of the workspace
 };
 
-Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev, bool accum) {
+Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev, int mode, bool accum) {
     Plan p{};
     const int64_t w = std::max(e, ev), rows = hq / hkv * l;
     p.hd = w <= 64 ? 64 : w <= 128 ? 128 : 256;
@@ -986,6 +1083,8 @@ Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e
     const int64_t groups = n * hkv * p.row_groups;
     p.splits = (int)std::max<int64_t>(1, std::min({(int64_t)kMaxSplits, kGroupsWanted / std::max<int64_t>(groups, 1), cdiv(s, 128)}));
     p.units = n * hkv * p.splits;
+    p.pair = p.rows == 128 && mode == kCausal && p.splits == 1 && p.row_groups > 1;
+    if (p.pair) p.row_groups = (p.row_groups + 1) / 2;
     const bool keep = accum && rows <= kScoreRows;
     p.o_bytes = p.splits > 1 ? (size_t)p.splits * n * hq * l * p.hd * 4 : 0;
     p.score_bytes = keep ? (size_t)n * hkv * rows * (cdiv(s, 32) * 32) * 4 : 0;
@@ -994,6 +1093,22 @@ Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e
 }
 
 size_t state_bytes(const Plan &p) { return p.o_bytes + p.score_bytes + p.ml_bytes; }
+
+// 64 keys a tile halve the rows' loads, 32 give twice the work-groups
+template <typename T, int HD>
+void launch_weights(const CacheAttnArgs &a, hipStream_t st) {
+    const int64_t heads = (int64_t)a.n * a.hkv;
+    const int kt = HD <= 128 && heads * cdiv(a.s, 128) >= 256 ? 2 : 1;
+    const int tiles = (int)cdiv(a.s, 32 * kt);
+    const dim3 grid((unsigned)cdiv(tiles, 2), (unsigned)heads);
+    if constexpr (HD <= 128) {
+        if (kt == 2) {
+            hipLaunchKernelGGL((key_weights_kernel<T, HD, 2>), grid, dim3(512), 0, st, a, tiles);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((key_weights_kernel<T, HD, 1>), grid, dim3(HD <= 128 ? 512 : 256), 0, st, a, tiles);
+}
 
 template <typename T, int HD>
 int launch_attn(const CacheAttnArgs &a, const Plan &p, hipStream_t st) {
@@ -1012,7 +1127,7 @@ int launch_attn(const CacheAttnArgs &a, const Plan &p, hipStream_t st) {
         hipLaunchKernelGGL((cache_merge_kernel<T, HD>), dim3((unsigned)cdiv(rows, 256 / (HD / 4))), dim3(256), 0, st, a);
     }
     if (a.acc)
-        hipLaunchKernelGGL((key_weights_kernel<T, HD>), dim3((unsigned)cdiv(a.s, 64), (unsigned)(a.n * a.hkv)), dim3(256), 0, st, a);
+        launch_weights<T, HD>(a, st);
     return launch_status();
 }
 
@@ -1061,7 +1176,7 @@ CacheAttnArgs fill_attn(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s
     a.lse = lse;
     a.scale_log2 = scale * kLog2e;
     a.kv_len = kv_len;
-    a.splits = p.splits; a.row_groups = p.row_groups;
+    a.splits = p.splits; a.row_groups = p.row_groups; a.pair = p.pair;
     // (o and the scores in multiples of 16 bytes)
     char *ws = reinterpret_cast<char *>(workspace);
     a.ws_o = p.o_bytes ? reinterpret_cast<float *>(ws) : nullptr;
@@ -1079,7 +1194,7 @@ using namespace kuiops;
 
 extern "C" size_t kuiops_sdpa_tree_workspace(int64_t n, int64_t hq, int64_t hkv, int64_t t, int64_t s, int64_t e, int64_t ev) {
     if (n <= 0 || hq <= 0 || hkv <= 0 || t <= 0 || s < 0 || e <= 0 || ev <= 0) return 0;
-    return state_bytes(plan_of(n, hq, hkv, t, s, e, ev, false));
+    return state_bytes(plan_of(n, hq, hkv, t, s, e, ev, kTree, false));
 }
 
 extern "C" int kuiops_sdpa_tree(int64_t n, int64_t hq, int64_t hkv, int64_t t, int64_t s, int64_t e, int64_t ev, int dtype,
@@ -1092,7 +1207,7 @@ extern "C" int kuiops_sdpa_tree(int64_t n, int64_t hq, int64_t hkv, int64_t t, i
     if (n == 0 || hq == 0 || t == 0) return KUIOPS_OK;
     if (!parent || t > s) return KUIOPS_E_INVALID;
     if (t > kMaxTree) return KUIOPS_E_UNSUPPORTED;
-    const Plan p = plan_of(n, hq, hkv, t, s, e, ev, false);
+    const Plan p = plan_of(n, hq, hkv, t, s, e, ev, kTree, false);
     if (!split_fits(p, s, sk[2], sv[2])) return KUIOPS_E_UNSUPPORTED;
     const size_t need = state_bytes(p);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KUIOPS_E_WORKSPACE;
@@ -1104,7 +1219,7 @@ extern "C" int kuiops_sdpa_tree(int64_t n, int64_t hq, int64_t hkv, int64_t t, i
 extern "C" size_t kuiops_sdpa_decode_accum_workspace(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e,
                                                      int64_t ev) {
     if (n <= 0 || hq <= 0 || hkv <= 0 || l <= 0 || s < 0 || e <= 0 || ev <= 0) return 0;
-    return state_bytes(plan_of(n, hq, hkv, l, s, e, ev, true));
+    return state_bytes(plan_of(n, hq, hkv, l, s, e, ev, kCausal, true));
 }
 
 extern "C" int kuiops_sdpa_decode_accum(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev,
@@ -1116,7 +1231,7 @@ extern "C" int kuiops_sdpa_decode_accum(int64_t n, int64_t hq, int64_t hkv, int6
     if (bad) return bad;
     if (n == 0 || hq == 0 || l == 0) return KUIOPS_OK;
     if (!lse || !sa || (s > 0 && !acc) || (causal && l > s)) return KUIOPS_E_INVALID;
-    const Plan p = plan_of(n, hq, hkv, l, s, e, ev, true);
+    const Plan p = plan_of(n, hq, hkv, l, s, e, ev, causal ? kCausal : kFull, true);
     if (!split_fits(p, s, sk[2], sv[2])) return KUIOPS_E_UNSUPPORTED;
     const size_t need = state_bytes(p);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KUIOPS_E_WORKSPACE;
