@@ -203,6 +203,7 @@ template <int IPT>        // slots of a thread held in registers; 0: none, any n
 __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a) {
     constexpr int NT = kEvictThreads, NW = NT / 64, NR = IPT > 0 ? IPT : 1;
     constexpr int kBins = 2048;
+    static_assert(IPT * NW < kBins, "the counts take the histogram's place");
     __shared__ int s_wave[NW], s_hist[kBins];
     __shared__ uint16_t s_rank[NW][2];
     __shared__ int s_digit, s_left, s_same;
@@ -290,67 +291,138 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a
         same = s_same;
     }
 
-    // 1024 slots at a time: running counts of equal keys, and of freed and far slots
     const bool ties = need < same;              // some of the equal keys are freed
-    int eq0 = 0, hole0 = 0, far0 = 0;
     const uint64_t below = (1ull << lane) - 1;
-    auto chunk = [&](int c, uint32_t k, bool reg, float av, int32_t pv) __attribute__((always_inline)) {
-        const int j = c * NT + tid;
-        const bool in = j < L;
-        int eqr = 0;
-        if (ties) {
-            const uint64_t eqs = __ballot(in && k == prefix);
-            if (lane == 0) s_wave[wave] = __popcll(eqs);
-            __syncthreads();
-            eqr = eq0 + __popcll(eqs & below);
-#pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const int x = s_wave[w];
-                eqr += w < wave ? x : 0;
-                eq0 += x;
-            }
-            // (the barriers below separate these reads from the next chunk's writes)
-        }
-        const bool kept = in && (k > prefix || (k == prefix && eqr < need));
-        const bool hole = in && j < m && !kept, far = j >= m && kept;
-        const uint64_t holes = __ballot(hole), fars = __ballot(far);
-        if (lane == 0) {
-            s_rank[wave][0] = (uint16_t)__popcll(holes);
-            s_rank[wave][1] = (uint16_t)__popcll(fars);
-        }
-        __syncthreads();
-        int hr = hole0 + __popcll(holes & below), fr = far0 + __popcll(fars & below);
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const int x = s_rank[w][0], y = s_rank[w][1];
-            hr += w < wave ? x : 0;
-            fr += w < wave ? y : 0;
-            hole0 += x;
-            far0 += y;
-        }
-        __syncthreads();
+    auto place = [&](int j, bool kept, bool hole, int hr, int fr, float w, int32_t p) __attribute__((always_inline)) {
+        const bool far = j >= m && kept;
         if (hole) moves[1 + hr] = j;
         if (far) moves[1 + m + fr] = j;
         if (kept && !far) {
-            acc_out[j] = reg ? av : acc[j];
-            pos_out[j] = reg ? pv : pos[j];
+            acc_out[j] = w;
+            pos_out[j] = p;
         }
     };
+    int holes_all = 0;
     if constexpr (IPT > 0) {
+        // counts per 1024 slots and wave, in slot order, and one scan of them all
+        // (wave 0), first of the equal keys, then of freed (low half) and far slots
+        uint32_t *s_count = reinterpret_cast<uint32_t *>(s_hist);
+        constexpr int NC = IPT * NW, PER = (NC + 63) / 64;
+        auto scan_counts = [&](uint32_t &total) __attribute__((always_inline)) {
+            __syncthreads();
+            if (wave == 0) {
+                uint32_t v[PER], sum = 0;
 #pragma unroll
-        for (int c = 0; c < IPT; ++c)
-            if (c < chunks) chunk(c, rk[c], true, ra[c], rp[c]);
+                for (int x = 0; x < PER; ++x) {
+                    v[x] = lane * PER + x < NC ? s_count[lane * PER + x] : 0;
+                    sum += v[x];
+                }
+                uint32_t incl = sum;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const uint32_t y = __shfl_up(incl, o, 64);
+                    incl += lane >= o ? y : 0;
+                }
+                uint32_t run = incl - sum;
+#pragma unroll
+                for (int x = 0; x < PER; ++x) {
+                    if (lane * PER + x < NC) s_count[lane * PER + x] = run;
+                    run += v[x];
+                }
+                if (lane == 63) s_count[NC] = run;
+            }
+            __syncthreads();
+            total = s_count[NC];
+        };
+        uint32_t keeps = 0;                    // of this thread's slots, as bits
+        uint32_t total;
+        if (ties) {
+#pragma unroll
+            for (int c = 0; c < IPT; ++c) {
+                const uint64_t eqs = __ballot(c * NT + tid < L && rk[c] == prefix);
+                if (lane == 0) s_count[c * NW + wave] = (uint32_t)__popcll(eqs);
+            }
+            scan_counts(total);
+        }
+#pragma unroll
+        for (int c = 0; c < IPT; ++c) {
+            const bool in = c * NT + tid < L;
+            bool kept = in && rk[c] >= prefix;
+            if (ties) {
+                const uint64_t eqs = __ballot(in && rk[c] == prefix);
+                kept = in && (rk[c] > prefix || (rk[c] == prefix && (int)s_count[c * NW + wave] + __popcll(eqs & below) < need));
+            }
+            keeps |= kept ? 1u << c : 0u;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < IPT; ++c) {
+            const int j = c * NT + tid;
+            const bool kept = keeps >> c & 1;
+            const uint32_t holes = (uint32_t)__popcll(__ballot(j < m && j < L && !kept)), fars = (uint32_t)__popcll(__ballot(j >= m && kept));
+            if (lane == 0) s_count[c * NW + wave] = fars << 16 | holes;
+        }
+        scan_counts(total);
+        holes_all = (int)(total & 0xffffu);
+#pragma unroll
+        for (int c = 0; c < IPT; ++c) {
+            const int j = c * NT + tid;
+            const bool kept = keeps >> c & 1, hole = j < m && j < L && !kept;
+            const uint64_t hb = __ballot(hole), fb = __ballot(j >= m && kept);
+            const uint32_t before = s_count[c * NW + wave];
+            place(j, kept, hole, (int)(before & 0xffffu) + __popcll(hb & below), (int)(before >> 16) + __popcll(fb & below), ra[c], rp[c]);
+        }
     } else {
+        // 1024 slots at a time, with running counts
+        int eq0 = 0, hole0 = 0, far0 = 0;
         for (int c = 0; c < chunks; ++c) {
             const int j = c * NT + tid;
-            chunk(c, j < L ? key_of(acc[j], pos[j]) : 0, false, 0.f, 0);
+            const bool in = j < L;
+            const float w = in ? acc[j] : 0.f;
+            const int32_t p = in ? pos[j] : 0;
+            const uint32_t k = in ? key_of(w, p) : 0;
+            const bool eq = in && k == prefix;
+            int eqr = 0;
+            if (ties) {
+                const uint64_t eqs = __ballot(eq);
+                if (lane == 0) s_wave[wave] = __popcll(eqs);
+                __syncthreads();
+                eqr = eq0 + __popcll(eqs & below);
+#pragma unroll
+                for (int v = 0; v < NW; ++v) {
+                    const int x = s_wave[v];
+                    eqr += v < wave ? x : 0;
+                    eq0 += x;
+                }
+                // (the barriers below separate these reads from the next writes)
+            }
+            const bool kept = in && (k > prefix || (eq && eqr < need));
+            const bool hole = in && j < m && !kept, far = j >= m && kept;
+            const uint64_t hb = __ballot(hole), fb = __ballot(far);
+            if (lane == 0) {
+                s_rank[wave][0] = (uint16_t)__popcll(hb);
+                s_rank[wave][1] = (uint16_t)__popcll(fb);
+            }
+            __syncthreads();
+            int hr = hole0 + __popcll(hb & below), fr = far0 + __popcll(fb & below);
+#pragma unroll
+            for (int v = 0; v < NW; ++v) {
+                const int x = s_rank[v][0], y = s_rank[v][1];
+                hr += v < wave ? x : 0;
+                fr += v < wave ? y : 0;
+                hole0 += x;
+                far0 += y;
+            }
+            __syncthreads();
+            place(j, kept, hole, hr, fr, w, p);
         }
+        holes_all = hole0;
     }
-    if (tid == 0) moves[0] = hole0;
+    if (tid == 0) moves[0] = holes_all;
     __builtin_amdgcn_s_waitcnt(0);
     __threadfence_block();
     __syncthreads();
-    for (int i = tid; i < hole0; i += NT) {
+    for (int i = tid; i < holes_all; i += NT) {
         const int to = moves[1 + i], from = moves[1 + m + i];
         acc_out[to] = acc[from];
         pos_out[to] = pos[from];

@@ -56,6 +56,7 @@ struct CacheAttnArgs {
     const int32_t *parent;     // kTree: [n][l]
     int splits, row_groups;    // row groups that work-groups begin with: half of them with `pair`
     int pair;
+    int head_tiles;            // cache_rows_kernel: row groups of a head where none crosses heads, else 0
     float *ws_ml;              // [splits][n * hq * l][2]: maximum (log2 domain), sum
     float *ws_o;               // [splits][n * hq * l][HD]: unnormalised output
     float *acc;                // kuiops_sdpa_decode_accum: per key sums, strides sa0, sa1, 1
@@ -200,11 +201,11 @@ __device__ __forceinline__ void store_row(const CacheAttnArgs &a, int64_t b, int
 }
 
 // ------------------------------------------------------------------------
-// cache_attn_kernel -- few rows per KV head: NWV waves, each with key steps of
-// 32 of its own; all have the same 16 * RT query rows.
+// cache_attn_kernel -- few rows per KV head: a work-group has 16 query rows, and
+// each of its 4 waves key steps of 32 of its own.
 //   S = K Q^T (16x16x32 MFMA): K straight from memory to registers; a lane
-//   holds 8 scores of one row per 16-row tile, the row's maximum crosses lanes
-//   16 and 32 apart only.  O^T += V^T P^T: V through LDS (DMA), read transposed;
+//   holds 8 scores of one row, the row's maximum crosses lanes 16 and 32 apart
+//   only.  O^T += V^T P^T: V through LDS (DMA), read transposed;
 //   the scores' registers are the other operand as they stand, keys numbered
 //   in that order.  The probability is the sum of two 16-bit parts, one MFMA
 //   each (2^-16 of it is lost in bf16, 2^-21 in f16): with the few rows of
@@ -212,9 +213,9 @@ __device__ __forceinline__ void store_row(const CacheAttnArgs &a, int64_t b, int
 // A part that is 0 times an infinite value is NaN, so is a masked NaN: a wave
 // whose sums are not finite goes over its keys again with the row maxima that
 // it found, multiplying value by value for the rows that see them.
-template <typename T, int HD, int RT, int NWV>
-__global__ __launch_bounds__(NWV * 64) void cache_attn_kernel(CacheAttnArgs a) {
-    constexpr int KB = 32, R = 16 * RT;
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
+    constexpr int NWV = 4, KB = 32, R = 16;
     constexpr int RB = HD * 2, VT = KB * RB;          // bytes per V row / wave tile
     constexpr int KK = HD / 32, DT = HD / 16, DV = VT / 1024;
     typedef typename Mfma<T>::frag frag;
@@ -281,59 +282,52 @@ __global__ __launch_bounds__(NWV * 64) void cache_attn_kernel(CacheAttnArgs a) {
         __builtin_amdgcn_sched_barrier(0);
     };
 
-    // query rows r0 + 16 rt + lr (B operand; rows past the list are 0)
-    frag qf[RT][KK];
-    bool row_ok[RT];
-    int pos[RT];
-    uint64_t mine[RT];
-    uint64_t nodes = 0;
-    if (a.mode == kTree) {
-        if (a.l <= 64) nodes = tree_bits_wave(a.parent + (int64_t)b * a.l, a.l);
-        else if constexpr (NWV * 64 >= kMaxTree) tree_bits<NWV * 64>(tb, a.parent + (int64_t)b * a.l, a.l);
-    }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int rr = r0 + rt * 16 + lr;
-        row_ok[rt] = rr < rows_kv;
-        const int h = row_ok[rt] ? rr / a.l : 0;
-        pos[rt] = row_ok[rt] ? rr - h * a.l : 0;
-        mine[rt] = 0;
-        if (a.mode == kTree) {
-            // (an absent node's query is not read: whatever it holds stays out)
-            if (a.l <= 64) {
-                mine[rt] = (uint64_t)__shfl((uint32_t)(nodes >> 32), pos[rt], 64) << 32 | __shfl((uint32_t)nodes, pos[rt], 64);
-                row_ok[rt] = row_ok[rt] && mine[rt] != 0;
-            } else {
-                row_ok[rt] = row_ok[rt] && (tb.w[pos[rt]][pos[rt] >> 6] >> (pos[rt] & 63)) & 1;
-            }
-        }
-        const T *q = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + (hk * G + h) * a.sq1 + pos[rt] * a.sq2;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            const int d = kk * 32 + G4 * 8;
-            qf[rt][kk] = as_frag<frag>(row_ok[rt] && d < a.e ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0});
-        }
-    }
+    constexpr int KS = NWV * KB;
+    int k0 = kbeg + wave * KB;
+    issue(k0, 0, sV0);
 
-    f32x4 o[RT][DT];
-    float m_used[RT], l_run[RT];
+    // query row r0 + lr (B operand; rows past the list are 0), loaded before the tree
+    // is looked at
+    const int rr = r0 + lr;
+    bool row_ok = rr < rows_kv;
+    const int h = row_ok ? rr / a.l : 0, pos = row_ok ? rr - h * a.l : 0;
+    const T *q = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + (hk * G + h) * a.sq1 + pos * a.sq2;
+    u32x4 qr[KK];
+    frag qf[KK];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m_used[rt] = -INFINITY;
-        l_run[rt] = 0.f;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int kk = 0; kk < KK; ++kk) {
+        const int d = kk * 32 + G4 * 8;
+        qr[kk] = row_ok && d < a.e ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0};
     }
+    uint64_t mine = 0;
+    if (a.mode == kTree) {
+        if (a.l <= 64) {
+            const uint64_t nodes = tree_bits_wave(a.parent + (int64_t)b * a.l, a.l);
+            mine = (uint64_t)__shfl((uint32_t)(nodes >> 32), pos, 64) << 32 | __shfl((uint32_t)nodes, pos, 64);
+            row_ok = row_ok && mine != 0;
+        } else {
+            tree_bits<NWV * 64>(tb, a.parent + (int64_t)b * a.l, a.l);
+            row_ok = row_ok && (tb.w[pos][pos >> 6] >> (pos & 63)) & 1;
+        }
+    }
+    // (whatever an absent node's query holds stays out)
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qf[kk] = as_frag<frag>(row_ok ? qr[kk] : u32x4{0, 0, 0, 0});
+
+    f32x4 o[DT];
+    float m_used = -INFINITY, l_run = 0.f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     // scores of a step: (t, i) is key k0 + 16 t + 4 G4 + i; unseen keys -inf
-    auto scores = [&](int k0, int slot, int rt, f32x4 *sc) __attribute__((always_inline)) {
+    auto scores = [&](int k0, int slot, f32x4 *sc) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) sc[t] = Mfma<T>::m16(as_frag<frag>(kr[slot][t][kk]), qf[rt][kk], sc[t]);
+            for (int kk = 0; kk < KK; ++kk) sc[t] = Mfma<T>::m16(as_frag<frag>(kr[slot][t][kk]), qf[kk], sc[t]);
         }
         if (k0 + KB > free_end) {
-            const uint32_t seen = (uint32_t)seen_word(a, &tb, mine[rt], pos[rt], k0, L) >> (4 * G4);
+            const uint32_t seen = (uint32_t)seen_word(a, &tb, mine, pos, k0, L) >> (4 * G4);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -341,50 +335,47 @@ __global__ __launch_bounds__(NWV * 64) void cache_attn_kernel(CacheAttnArgs a) {
                     if (!(seen >> (16 * t + i) & 1)) sc[t][i] = -INFINITY;
         }
     };
-    float *keep = a.scores ? a.scores + (int64_t)(b * a.hkv + hk) * rows_kv * a.spad : nullptr;
+    float *keep = a.scores ? a.scores + ((int64_t)(b * a.hkv + hk) * rows_kv + rr) * a.spad : nullptr;
     auto step = [&](int k0, int slot, char *sv) __attribute__((always_inline)) {
-        t8 hi[RT], lo[RT];
+        f32x4 sc[2];
+        scores(k0, slot, sc);
+        float mx = -INFINITY;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            f32x4 sc[2];
-            scores(k0, slot, rt, sc);
-            if (keep && row_ok[rt]) {
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    *reinterpret_cast<f32x4 *>(keep + (int64_t)(r0 + rt * 16 + lr) * a.spad + k0 + 16 * t + 4 * G4) = sc[t];
-            }
-            float mx = -INFINITY;
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[t][i]);
+        mx = xor_max<32>(xor_max<16>(mx)) * a.scale_log2;
+        if (__any(mx > m_used + kSlack)) {
+            const float m_new = fmaxf(m_used, mx);
+            const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
+            l_run *= alpha;
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < DT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[t][i]);
-            mx = xor_max<32>(xor_max<16>(mx)) * a.scale_log2;
-            if (__any(mx > m_used[rt] + kSlack)) {
-                const float m_new = fmaxf(m_used[rt], mx);
-                const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_used[rt] - m_new);
-                l_run[rt] *= alpha;
-#pragma unroll
-                for (int t = 0; t < DT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[rt][t][i] *= alpha;
-                m_used[rt] = m_new;
-            }
-            const float mref = m_used[rt] == -INFINITY ? 0.f : m_used[rt] + Shift<T>::value;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = fast_exp2(__builtin_fmaf(sc[t][i], a.scale_log2, -mref));
-                    l_run[rt] += p;
-                    const T h = from_f32<T>(p);
-                    hi[rt][4 * t + i] = h;
-                    lo[rt][4 * t + i] = from_f32<T>(p - to_f32(h));
-                }
+                for (int i = 0; i < 4; ++i) o[t][i] *= alpha;
+            m_used = m_new;
         }
+        const float mref = m_used == -INFINITY ? 0.f : m_used + Shift<T>::value;
+        t8 hi, lo;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = fast_exp2(__builtin_fmaf(sc[t][i], a.scale_log2, -mref));
+                l_run += p;
+                const T x = from_f32<T>(p);
+                hi[4 * t + i] = x;
+                lo[4 * t + i] = from_f32<T>(p - to_f32(x));
+            }
         // this step's V tile has landed: only the next step's loads are younger
         constexpr int Y = 2 * KK + DV;
         __builtin_amdgcn_s_waitcnt((Y & 15) | ((Y >> 4) << 14) | (7 << 4) | (15 << 8));
         __builtin_amdgcn_sched_barrier(0);
+        // (stored behind that wait, which counts stores too)
+        if (keep && row_ok) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) *reinterpret_cast<f32x4 *>(keep + k0 + 16 * t + 4 * G4) = sc[t];
+        }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             const char *vb = sv + wave * VT + offVr[dt];
@@ -392,17 +383,11 @@ __global__ __launch_bounds__(NWV * 64) void cache_attn_kernel(CacheAttnArgs a) {
             const s16x4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)to_lds(vb + 16 * RB));
             const u32x2 h0 = __builtin_bit_cast(u32x2, t0), h1 = __builtin_bit_cast(u32x2, t1);
             const frag vf = as_frag<frag>(u32x4{h0[0], h0[1], h1[0], h1[1]});
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                o[rt][dt] = Mfma<T>::m16(vf, __builtin_bit_cast(frag, hi[rt]), o[rt][dt]);
-                o[rt][dt] = Mfma<T>::m16(vf, __builtin_bit_cast(frag, lo[rt]), o[rt][dt]);
-            }
+            o[dt] = Mfma<T>::m16(vf, __builtin_bit_cast(frag, hi), o[dt]);
+            o[dt] = Mfma<T>::m16(vf, __builtin_bit_cast(frag, lo), o[dt]);
         }
     };
 
-    constexpr int KS = NWV * KB;
-    int k0 = kbeg + wave * KB;
-    issue(k0, 0, sV0);
     for (; k0 < kend; k0 += 2 * KS) {
         issue(k0 + KS, 1, sV1);
         step(k0, 0, sV0);
@@ -419,40 +404,33 @@ __global__ __launch_bounds__(NWV * 64) void cache_attn_kernel(CacheAttnArgs a) {
     __builtin_amdgcn_sched_barrier(0);
     float z = 0.f;                  // stays 0 if every sum is finite
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z = __builtin_fmaf(o[rt][t][i], 0.f, z);
+        for (int i = 0; i < 4; ++i) z = __builtin_fmaf(o[t][i], 0.f, z);
     if (__any(z != 0.f)) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int t = 0; t < DT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < DT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const float mref = m_used == -INFINITY ? 0.f : m_used + Shift<T>::value;
         for (k0 = kbeg + wave * KB; k0 < kend; k0 += KS) {
             issue(k0, 0, sV0);
             __builtin_amdgcn_s_waitcnt(0);
             __builtin_amdgcn_sched_barrier(0);
+            f32x4 sc[2];
+            scores(k0, 0, sc);
+            const uint32_t seen = (uint32_t)seen_word(a, &tb, mine, pos, k0, L);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                f32x4 sc[2];
-                scores(k0, 0, rt, sc);
-                const float mref = m_used[rt] == -INFINITY ? 0.f : m_used[rt] + Shift<T>::value;
-                const uint32_t seen = (uint32_t)seen_word(a, &tb, mine[rt], pos[rt], k0, L);
+            for (int x = 0; x < 8; ++x) {
+                const float p = fast_exp2(__builtin_fmaf(sc[x >> 2][x & 3], a.scale_log2, -mref));
+                for (int g = 0; g < 4; ++g) {
+                    const int key = 16 * (x >> 2) + 4 * g + (x & 3);
+                    const float pk = __shfl(p, g * 16 + lr, 64);
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const float p = fast_exp2(__builtin_fmaf(sc[x >> 2][x & 3], a.scale_log2, -mref));
-                    for (int g = 0; g < 4; ++g) {
-                        const int key = 16 * (x >> 2) + 4 * g + (x & 3);
-                        const float pk = __shfl(p, g * 16 + lr, 64);
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const int d = dt * 16 + 4 * G4;
+                        const T *vp = reinterpret_cast<const T *>(sV0 + wave * VT + key * RB + (((d >> 3) ^ vsw(key)) << 4) + (d & 4) * 2);
 #pragma unroll
-                        for (int dt = 0; dt < DT; ++dt) {
-                            const int d = dt * 16 + 4 * G4;
-                            const T *vp = reinterpret_cast<const T *>(sV0 + wave * VT + key * RB + (((d >> 3) ^ vsw(key)) << 4) + (d & 4) * 2);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (seen >> key & 1) o[rt][dt][i] += pk * to_f32(vp[i]);
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            if (seen >> key & 1) o[dt][i] += pk * to_f32(vp[i]);
                     }
                 }
             }
@@ -461,46 +439,42 @@ __global__ __launch_bounds__(NWV * 64) void cache_attn_kernel(CacheAttnArgs a) {
         }
     }
 
-    // the waves' sums merge through LDS, 16 rows at a time in the first tiles' place
+    // the waves' sums merge through LDS, in the first tiles' place
     constexpr int D4 = HD / 4;
-    float (*so)[16][HD] = reinterpret_cast<float (*)[16][HD]>(sV0);
-    static_assert(16 * HD * 4 == VT, "a wave's 16 rows take its V tile");
+    float (*so)[R][HD] = reinterpret_cast<float (*)[R][HD]>(sV0);
+    static_assert(R * HD * 4 == VT, "a wave's rows take its V tile");
+    // lanes of a row hold disjoint keys: row sums over the lane groups
+    l_run = xor_add<32>(xor_add<16>(l_run));
+    if (G4 == 0) {
+        sm[wave][lr] = row_ok ? m_used + Shift<T>::value : -INFINITY;
+        sl[wave][lr] = row_ok ? l_run : 0.f;
+    }
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        // lanes of a row hold disjoint keys: row sums over the lane groups
-        const float lsum = xor_add<32>(xor_add<16>(l_run[rt]));
-        if (G4 == 0) {
-            sm[wave][rt * 16 + lr] = row_ok[rt] ? m_used[rt] + Shift<T>::value : -INFINITY;
-            sl[wave][rt * 16 + lr] = row_ok[rt] ? lsum : 0.f;
+    for (int dt = 0; dt < DT; ++dt)
+        *reinterpret_cast<f32x4 *>(&so[wave][lr][dt * 16 + 4 * G4]) = row_ok ? o[dt] : f32x4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
+    for (int x = tid; x < R * D4; x += NWV * 64) {
+        const int r = x / D4, d = x % D4 * 4;
+        if (r0 + r >= rows_kv) continue;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NWV; ++w) mm = fmaxf(mm, sm[w][r]);
+        const float mu = mm == -INFINITY ? 0.f : mm;
+        float ll = 0.f;
+        f32x4 oo = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NWV; ++w) {
+            const float wgt = fast_exp2(sm[w][r] - mu);
+            ll = __builtin_fmaf(sl[w][r], wgt, ll);
+            const f32x4 ov = *reinterpret_cast<const f32x4 *>(&so[w][r][d]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) oo[i] = __builtin_fmaf(ov[i], wgt, oo[i]);
         }
-        __syncthreads();
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-            *reinterpret_cast<f32x4 *>(&so[wave][lr][dt * 16 + 4 * G4]) = row_ok[rt] ? o[rt][dt] : f32x4{0.f, 0.f, 0.f, 0.f};
-        __syncthreads();
-        for (int x = tid; x < 16 * D4; x += NWV * 64) {
-            const int r = x / D4, d = x % D4 * 4, rr = r0 + rt * 16 + r;
-            if (rr >= rows_kv) continue;
-            float mm = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < NWV; ++w) mm = fmaxf(mm, sm[w][rt * 16 + r]);
-            const float mu = mm == -INFINITY ? 0.f : mm;
-            float ll = 0.f;
-            f32x4 oo = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < NWV; ++w) {
-                const float wgt = fast_exp2(sm[w][rt * 16 + r] - mu);
-                ll = __builtin_fmaf(sl[w][rt * 16 + r], wgt, ll);
-                const f32x4 ov = *reinterpret_cast<const f32x4 *>(&so[w][r][d]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) oo[i] = __builtin_fmaf(ov[i], wgt, oo[i]);
-            }
-            const int head = hk * G + rr / a.l, i = rr % a.l;
-            if (a.splits == 1) store_row<T>(a, b, head, i, d, oo, mm, ll);
-            const int64_t st = (int64_t)split * a.n * a.hq * a.l + ((int64_t)b * a.hq + head) * a.l + i;
-            if (a.splits > 1) *reinterpret_cast<f32x4 *>(&a.ws_o[st * HD + d]) = oo;
-            if (d == 0 && a.ws_ml) *reinterpret_cast<f32x2 *>(&a.ws_ml[st * 2]) = f32x2{mm, ll};
-        }
+        const int head = hk * G + (r0 + r) / a.l, i = (r0 + r) % a.l;
+        const int64_t st = (int64_t)split * a.n * a.hq * a.l + ((int64_t)b * a.hq + head) * a.l + i;
+        if (a.splits == 1) store_row<T>(a, b, head, i, d, oo, mm, ll);
+        else *reinterpret_cast<f32x4 *>(&a.ws_o[st * HD + d]) = oo;
+        if (d == 0 && a.ws_ml) *reinterpret_cast<f32x2 *>(&a.ws_ml[st * 2]) = f32x2{mm, ll};
     }
 }
 
@@ -540,15 +514,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int chunk = (blocks_all + a.splits - 1) / a.splits * KB;
 
     // a.pair: row groups p and last - p, whose causal lengths together are the same for every p
-    const int groups = (rows_kv + R - 1) / R;
+    const int groups = a.head_tiles ? G * a.head_tiles : (rows_kv + R - 1) / R;
     for (int rg = u.rg;;) {
-    const int r0 = rg * R, last = min(r0 + R, rows_kv) - 1;
+    // rows r0 .. r0 + R - 1 of the KV head's list, up to the head's end with head_tiles
+    const int head = a.head_tiles ? rg / a.head_tiles : 0;
+    const int r0 = a.head_tiles ? head * a.l + (rg - head * a.head_tiles) * R : rg * R;
+    const int rend = min(r0 + R, a.head_tiles ? (head + 1) * a.l : rows_kv), last = rend - 1;
     const int kbeg = min(L, split * chunk);
     int kend = min(L, kbeg + chunk);
     // keys past the last position of the work-group's rows are seen by none
     if (a.mode == kCausal && r0 / a.l == last / a.l) kend = max(kbeg, min(kend, first + last % a.l + 1));
     // keys below free_end are seen by every row of the wave
-    const int w0 = r0 + wave * 32, w1 = min(w0 + 31, rows_kv - 1);
+    const int w0 = r0 + wave * 32, w1 = min(w0 + 31, last);
     const int free_end = a.mode == kFull ? L : a.mode == kCausal ? first + 1 + (w0 / a.l == w1 / a.l ? w0 % a.l : 0) : first;
     const int nkv = (kend - kbeg + KB - 1) / KB;
 
@@ -583,9 +560,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
     // this lane's row
     const int rr = w0 + lq;
-    bool row_ok = rr < rows_kv;
-    const bool live = w0 < rows_kv;
+    bool row_ok = rr < rend;
+    const bool live = w0 < rend;
     const int h = row_ok ? rr / a.l : 0, pos = row_ok ? rr - h * a.l : 0;
+    const T *q = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + (hk * G + h) * a.sq1 + pos * a.sq2;
+    u32x4 qr[KS];
+    frag qf[KS];
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+        const int d = kk * 16 + lh * 8;
+        qr[kk] = row_ok && d < a.e ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0};
+    }
     uint64_t mine = 0;
     if (a.mode == kTree) {
         if (a.l <= 64) {
@@ -597,13 +582,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             row_ok = row_ok && (tb.w[pos][pos >> 6] >> (pos & 63)) & 1;
         }
     }
-    const T *q = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + (hk * G + h) * a.sq1 + pos * a.sq2;
-    frag qf[KS];
 #pragma unroll
-    for (int kk = 0; kk < KS; ++kk) {
-        const int d = kk * 16 + lh * 8;
-        qf[kk] = as_frag<frag>(row_ok && d < a.e ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0});
-    }
+    for (int kk = 0; kk < KS; ++kk) qf[kk] = as_frag<frag>(row_ok ? qr[kk] : u32x4{0, 0, 0, 0});
 
     // LDS offsets: K row 32 t + lq, chunk 2 kk + lh; V^T row d = 32 dt + lq, whose
     // 8 key slots of lane half lh are keys 4 lh .. + 3 and 8 + 4 lh .. + 3 of a
@@ -778,17 +758,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 
     const float l_all = xor_add<32>(l_run);
-    if (rr < rows_kv) {
+    if (rr < rend) {
         const float m = row_ok ? m_used + Shift<T>::value : -INFINITY, l = row_ok ? l_all : 0.f;
-        const int head = hk * G + h;
-        const int64_t st = (int64_t)split * a.n * a.hq * a.l + ((int64_t)b * a.hq + head) * a.l + pos;
+        const int64_t st = (int64_t)split * a.n * a.hq * a.l + ((int64_t)b * a.hq + hk * G + h) * a.l + pos;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
                 const int d = dt * 32 + 8 * y + 4 * lh;
                 const f32x4 v = row_ok ? f32x4{o[dt][4 * y], o[dt][4 * y + 1], o[dt][4 * y + 2], o[dt][4 * y + 3]} : f32x4{0.f, 0.f, 0.f, 0.f};
-                if (a.splits == 1) store_row<T>(a, b, head, pos, d, v, m, l);
+                if (a.splits == 1) store_row<T>(a, b, hk * G + h, pos, d, v, m, l);
                 else *reinterpret_cast<f32x4 *>(&a.ws_o[st * HD + d]) = v;
             }
         if (a.splits > 1 && lh == 0) *reinterpret_cast<f32x2 *>(&a.ws_ml[st * 2]) = f32x2{m, l};
@@ -867,6 +846,18 @@ __global__ __launch_bounds__(256) void accum_merge_kernel(CacheAttnArgs a) {
     auto row_of = [&](int r) { return ((int64_t)b * a.hq + hk * G + r / a.l) * a.l + r % a.l; };
     const int L = keys_of(a, b);
     if (blockIdx.x > 0 && (int)blockIdx.x * 512 >= L && (int)blockIdx.x >= (rows + RPB - 1) / RPB) return;
+    // the first rows' scores and the sums, before the rows' maxima are known (the
+    // scores' rows are padded, with whatever they hold, past the last key)
+    const int key = blockIdx.x * 512 + tid * 2;
+    const float *sc = a.scores + (int64_t)(b * a.hkv + hk) * rows * a.spad + key;
+    float *acc = a.acc + b * a.sa0 + hk * a.sa1 + key;
+    f32x2 x[4] = {}, old = {0.f, 0.f};
+    if (key < a.s) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) x[y] = *reinterpret_cast<const f32x2 *>(sc + min(y, rows - 1) * a.spad);
+        old[0] = acc[0];
+        if (key + 1 < a.s) old[1] = acc[1];
+    }
     for (int r = wave; r < rows; r += 4) {
         const f32x2 ml = lane < a.splits ? *reinterpret_cast<const f32x2 *>(&a.ws_ml[(lane * all + row_of(r)) * 2]) : f32x2{-INFINITY, 0.f};
         const float mm = wave_max(ml[0]), mu = mm == -INFINITY ? 0.f : mm;
@@ -887,14 +878,13 @@ __global__ __launch_bounds__(256) void accum_merge_kernel(CacheAttnArgs a) {
         }
     }
     __syncthreads();
-    const int key = blockIdx.x * 512 + tid * 2;
     if (key >= L) return;
-    const float *sc = a.scores + (int64_t)(b * a.hkv + hk) * rows * a.spad + key;
     f32x2 w = {0.f, 0.f};
     for (int r = 0; r < rows; r += 4) {
-        f32x2 x[4];
+        if (r > 0) {
 #pragma unroll
-        for (int y = 0; y < 4; ++y) x[y] = *reinterpret_cast<const f32x2 *>(sc + min(r + y, rows - 1) * a.spad);
+            for (int y = 0; y < 4; ++y) x[y] = *reinterpret_cast<const f32x2 *>(sc + min(r + y, rows - 1) * a.spad);
+        }
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
             if (r + y >= rows) break;
@@ -903,9 +893,8 @@ __global__ __launch_bounds__(256) void accum_merge_kernel(CacheAttnArgs a) {
             for (int z = 0; z < 2; ++z) w[z] += inv * fast_exp2(__builtin_fmaf(x[y][z], a.scale_log2, -m));
         }
     }
-    float *acc = a.acc + b * a.sa0 + hk * a.sa1 + key;
-    acc[0] += w[0];
-    if (key + 1 < L) acc[1] += w[1];
+    acc[0] = old[0] + w[0];
+    if (key + 1 < L) acc[1] = old[1] + w[1];
 }
 
 // key_weights_kernel -- the weights of many rows' keys: acc[key] += sum over the
@@ -1064,28 +1053,52 @@ __global__ __launch_bounds__(HD <= 128 ? 512 : 256) void key_weights_kernel(Cach
 
 // ------------------------------------------------------------- host side
 
-constexpr int kGroupsWanted = 512;      // work-groups of a launch: two for each of the 256 CUs
-constexpr int kMaxSplits = 64;
-
 struct Plan {
-    int hd, rows;          // head dim and rows of a work-group: 16 or 32 (cache_attn_kernel), 128 (cache_rows_kernel)
-    int row_groups, splits, pair;
+    int hd, rows;          // head dim and rows of a work-group: 16 (cache_attn_kernel) or 128 (cache_rows_kernel)
+    int row_groups, splits, pair, head_tiles;
     int64_t units;
     size_t o_bytes, ml_bytes, score_bytes;        // of the workspace
 };
 
+// Which kernel.  16-row groups are several work-groups for more rows, each of
+// which reads the keys (from L2 behind the first), which fills the GPU soonest;
+// 128-row ones read them once and do far less per row.  The 16-row form wins up
+// to about 2^25 = (KV heads x 16-row groups x keys x head dim).  Measured around
+// it, us, best split counts, 16 against 128 rows: head dim 128, 8 KV heads, 256
+// rows, 2048 / 4096 keys 19.5 / 20.0 and 28.3 / 24.7; 32 heads, 64 rows, 1024 / 4096
+// 14.6 / 15.6 and 29.1 / 22.4; head dim 64, 32 heads, 256 rows, 1024 / 2048 15.1 / 16.4
+// and 23.3 / 19.2; 8 heads, 32 rows, 256 keys 6.1 / 8.3; 64 heads, 64 rows, 4000 keys
+// of 128 42.4 / 30.5.
+//
+// How many splits.  About one work-group per CU (twice that only while each
+// still has 2048 keys: 16 sequences of 64 nodes over 8064 keys 163 -> 149 us), of at
+// least 256 keys: 64 KV heads, 16 rows, 4000 keys of 128: 256 / 512 / 1024 work-groups
+// 25.8 / 25.7 / 31.4; 32 rows, 16-row groups, 256 / 512 / 1024 28.9 / 29.5 / 36.2.  Short
+// caches are not split, which saves the merge's launch: 8 heads, 32 rows, 640 keys
+// of 64 one split 7.7, four 8.6; 1024 keys 9.2 / 8.6; 256 of 128 8.5 / 10.3; 640 12.0 /
+// 11.0.
+constexpr int kCUs = 256;
 Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev, int mode, bool accum) {
     Plan p{};
     const int64_t w = std::max(e, ev), rows = hq / hkv * l;
     p.hd = w <= 64 ? 64 : w <= 128 ? 128 : 256;
-    p.rows = p.hd == 256 || rows <= 16 ? 16 : rows <= 64 ? 32 : 128;
+    p.rows = p.hd == 256 || rows <= 16 || n * hkv * cdiv(rows, 16) * s <= ((int64_t)1 << 25) / p.hd ? 16 : 128;
     p.row_groups = (int)cdiv(rows, p.rows);
-    const int64_t groups = n * hkv * p.row_groups;
-    p.splits = (int)std::max<int64_t>(1, std::min({(int64_t)kMaxSplits, kGroupsWanted / std::max<int64_t>(groups, 1), cdiv(s, 128)}));
+    // long causal pieces: no row group crosses heads (one that does sees the last
+    // row of one head next to the first of another, so every block of it is masked:
+    // a 1999-token prompt, 32 / 8 heads of 64: 47 -> 40 us); 7 groups a head waste an
+    // eighth of the rows at most
+    if (p.rows == 128 && mode == kCausal && l > 7 * 128) {
+        p.head_tiles = (int)cdiv(l, 128);
+        p.row_groups = (int)(hq / hkv) * p.head_tiles;
+    }
+    const int64_t groups = n * hkv * p.row_groups, want = cdiv(s * groups, 2 * kCUs) >= 2048 ? 2 * kCUs : kCUs;
+    p.splits = s * p.hd <= 640 * 64 ? 1 : (int)std::max<int64_t>(1, std::min(want / std::max<int64_t>(groups, 1), cdiv(s, 256)));
+    p.splits = std::min(p.splits, 64);          // (accum_merge_kernel has a lane for each)
     p.units = n * hkv * p.splits;
     p.pair = p.rows == 128 && mode == kCausal && p.splits == 1 && p.row_groups > 1;
     if (p.pair) p.row_groups = (p.row_groups + 1) / 2;
-    const bool keep = accum && rows <= kScoreRows;
+    const bool keep = accum && p.rows == 16 && rows <= kScoreRows;
     p.o_bytes = p.splits > 1 ? (size_t)p.splits * n * hq * l * p.hd * 4 : 0;
     p.score_bytes = keep ? (size_t)n * hkv * rows * (cdiv(s, 32) * 32) * 4 : 0;
     p.ml_bytes = p.splits > 1 || keep ? (size_t)p.splits * n * hq * l * 8 : 0;
@@ -1113,11 +1126,8 @@ void launch_weights(const CacheAttnArgs &a, hipStream_t st) {
 template <typename T, int HD>
 int launch_attn(const CacheAttnArgs &a, const Plan &p, hipStream_t st) {
     const dim3 grid((unsigned)(cdiv(p.units, 8) * 8 * p.row_groups));
-    if (p.rows == 16) hipLaunchKernelGGL((cache_attn_kernel<T, HD, 1, 4>), grid, dim3(256), 0, st, a);
-    if constexpr (HD <= 128) {
-        if (p.rows == 32) hipLaunchKernelGGL((cache_attn_kernel<T, HD, 2, 4>), grid, dim3(256), 0, st, a);
-        if (p.rows == 128) hipLaunchKernelGGL((cache_rows_kernel<T, HD>), grid, dim3(256), 0, st, a);
-    }
+    if (p.rows == 16) hipLaunchKernelGGL((cache_attn_kernel<T, HD>), grid, dim3(256), 0, st, a);
+    else if constexpr (HD <= 128) hipLaunchKernelGGL((cache_rows_kernel<T, HD>), grid, dim3(256), 0, st, a);
     if (a.scores) {
         hipLaunchKernelGGL((accum_merge_kernel<T, HD>), dim3((unsigned)cdiv(a.s, 512), (unsigned)(a.n * a.hkv)), dim3(256), 0, st, a);
         return launch_status();
@@ -1176,7 +1186,7 @@ CacheAttnArgs fill_attn(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s
     a.lse = lse;
     a.scale_log2 = scale * kLog2e;
     a.kv_len = kv_len;
-    a.splits = p.splits; a.row_groups = p.row_groups; a.pair = p.pair;
+    a.splits = p.splits; a.row_groups = p.row_groups; a.pair = p.pair; a.head_tiles = p.head_tiles;
     // (o and the scores in multiples of 16 bytes)
     char *ws = reinterpret_cast<char *>(workspace);
     a.ws_o = p.o_bytes ? reinterpret_cast<float *>(ws) : nullptr;
@@ -1219,7 +1229,8 @@ extern "C" int kuiops_sdpa_tree(int64_t n, int64_t hq, int64_t hkv, int64_t t, i
 extern "C" size_t kuiops_sdpa_decode_accum_workspace(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e,
                                                      int64_t ev) {
     if (n <= 0 || hq <= 0 || hkv <= 0 || l <= 0 || s < 0 || e <= 0 || ev <= 0) return 0;
-    return state_bytes(plan_of(n, hq, hkv, l, s, e, ev, kCausal, true));
+    return std::max(state_bytes(plan_of(n, hq, hkv, l, s, e, ev, kCausal, true)),
+                    state_bytes(plan_of(n, hq, hkv, l, s, e, ev, kFull, true)));
 }
 
 extern "C" int kuiops_sdpa_decode_accum(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev,

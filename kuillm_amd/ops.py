@@ -1203,70 +1203,107 @@ def decode_rows_batched(x, W, x_kind="plain", out_kind="plain", in_add=None, nor
 # per call from torch's caching allocator: calls on several streams and graphs
 # captured one after another never share one, and nothing has to be run once
 # before a capture.
+#
+# What follows from shapes, strides and types alone (their checks, the C
+# strides, the workspace's size) is worked out once per combination: a decoding
+# step calls with the same ones over and over, and they take twice the launches'
+# time (host time of a tree call: 25 us without, 11 with).
 
-def _on_device(name, status_of, device, *tensors):
-    """Checks that every tensor is on ``device``, a GPU, and enqueues
-    ``status_of(stream)`` there, whichever device is the current one."""
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise _lib.KuiopsError(name, _lib.E_INVALID)
-    if device.type != "cuda":
-        raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
-    if device.index == torch.cuda.current_device():
-        _lib.check(name, status_of(_stream(device)))
+def _meta(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
+def _enqueue(name, device, args):
+    """The C entry ``name`` with ``args`` and the current stream of GPU ``device``
+    (an index), which need not be the current device."""
+    fn = getattr(_lib_handle(), name)
+    if device == torch._C._cuda_getDevice():
+        status = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            _lib.check(name, status_of(_stream(device)))
+            status = fn(*args, _raw_stream(device))
+    if status:
+        _lib.check(name, status)
 
 
-def _strides(t, count, scale=1):
-    """The first strides of t, 0 for axes of one entry (torch lets those be anything)."""
-    return (ctypes.c_int64 * count)(*[0 if t.shape[i] <= 1 else t.stride(i) * scale for i in range(count)])
+def _gpu_of(name, t, *others) -> int:
+    """The index of the GPU that t and the others (or None) are all on."""
+    device = t.get_device()
+    for o in others:
+        if o is not None and o.get_device() != device:
+            raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if device < 0:
+        raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
+    return device
 
 
-def _disjoint(t) -> bool:
-    """Whether no two elements of t share memory."""
-    if t.numel() <= 1:
+def _c_strides(shape, stride, count, scale=1):
+    """The first strides, 0 for axes of one entry (torch lets those be anything)."""
+    return (ctypes.c_int64 * count)(*[0 if shape[i] <= 1 else stride[i] * scale for i in range(count)])
+
+
+def _disjoint(shape, stride) -> bool:
+    """Whether no two elements share memory."""
+    if math.prod(shape) <= 1:
         return True
     span = 1
-    for st, size in sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1):
+    for st, size in sorted((st, size) for st, size in zip(stride, shape) if size > 1):
         if st < span:
             return False
         span = st * (size - 1) + span
     return True
 
 
-def _own_rows(t) -> bool:
+def _own_rows(shape, stride) -> bool:
     """Elements that share no memory, in rows of unit stride."""
-    return (t.shape[-1] <= 1 or t.stride(-1) == 1) and _disjoint(t)
+    return (shape[-1] <= 1 or stride[-1] == 1) and _disjoint(shape, stride)
 
 
-@functools.lru_cache(maxsize=4096)
-def _cache_attn_workspace(name, *dims) -> int:
-    return getattr(_lib_handle(), name)(*dims)
+def _flat_ints(t, n) -> bool:
+    return t.dtype == torch.int32 and t.shape == (n,) and (n <= 1 or t.stride(0) == 1)
 
 
-def _cache_attn_check(name, q, k, v, kv_len, scale, out):
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or not (q.dtype == k.dtype == v.dtype):
+class _AttnPlan:
+    __slots__ = ("dims", "dtype", "scale", "sq", "sq_copy", "q_in_place", "sk", "sv", "so", "out_shape", "ws")
+
+
+@functools.lru_cache(maxsize=2048)
+def _attn_plan(name, q, k, v, out) -> _AttnPlan:
+    """Checks the (shape, stride, dtype) of sdpa_tree's / sdpa_decode_accum's tensors."""
+    (qs, qst, qd), (ks, kst, kd), (vs, vst, vd) = q, k, v
+    if len(qs) != 4 or len(ks) != 4 or len(vs) != 4 or not (qd == kd == vd):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
-    n, hq, l, e = q.shape
-    _, hkv, s, _ = k.shape
-    ev = v.shape[3]
-    if k.shape[0] != n or k.shape[3] != e or v.shape[:3] != k.shape[:3] or hkv == 0 or hq % hkv or e == 0 or ev == 0:
+    n, hq, l, e = qs
+    hkv, s, ev = ks[1], ks[2], vs[3]
+    if ks[0] != n or ks[3] != e or vs[:3] != ks[:3] or hkv == 0 or hq % hkv or e == 0 or ev == 0:
         raise _lib.KuiopsError(name, _lib.E_INVALID)
-    if kv_len is not None and (kv_len.dtype != torch.int32 or kv_len.shape != (n,) or not kv_len.is_contiguous()):
-        raise _lib.KuiopsError(name, _lib.E_INVALID)
-    if q.dtype not in HALF or k.stride(3) != 1 or v.stride(3) != 1:
+    if qd not in HALF or (e > 1 and kst[3] != 1) or (ev > 1 and vst[3] != 1):
         raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
-    if out is not None and (out.shape != (n, hq, l, ev) or out.dtype != q.dtype or out.stride(3) != 1
-                            or not _disjoint(out) or out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr())):
+    p = _AttnPlan()
+    p.dims, p.dtype, p.scale = (n, hq, hkv, l, s, e, ev), _dt(qd), 1.0 / math.sqrt(e)
+    p.out_shape = (n, hq, l, ev)
+    if out is not None and (out[0] != p.out_shape or out[2] != qd or not _own_rows(out[0], out[1])):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
+    flat = (hq * l * e, l * e, e, 1)
+    p.q_in_place = (e <= 1 or qst[3] == 1) and not any(st % 8 for st, size in zip(qst[:3], qs) if size > 1)
+    p.sq, p.sq_copy = _c_strides(qs, qst, 3), _c_strides(qs, flat, 3)
+    p.sk, p.sv = _c_strides(ks, kst, 3), _c_strides(vs, vst, 3)
+    p.so = _c_strides(p.out_shape, (hq * l * ev, l * ev, ev, 1) if out is None else out[1], 3)
+    p.ws = getattr(_lib_handle(), f"kuiops_{name}_workspace")(*p.dims)
+    return p
+
+
+def _attn_call(name, q, k, v, kv_len, out):
+    """(plan, q and its C strides as the kernels read it, out)."""
+    p = _attn_plan(name, _meta(q), _meta(k), _meta(v), _meta(out))
+    if kv_len is not None and not _flat_ints(kv_len, p.dims[0]):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if out is not None and out.numel() and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if p.q_in_place and q.data_ptr() % 16 == 0:
+        return p, q, p.sq
     # a copy of the few query rows where the kernels cannot read them in place
-    if q.stride(3) != 1 or any(st % 8 for st in q.stride()[:3]) or q.data_ptr() % 16:
-        q = q.contiguous()
-    if scale is None:
-        scale = 1.0 / math.sqrt(e)
-    return q, (n, hq, hkv, l, s, e, ev), float(scale)
+    return p, torch.empty(q.shape, dtype=q.dtype, device=q.device).copy_(q), p.sq_copy
 
 
 def sdpa_tree(q, k, v, parent, kv_len=None, scale=None, return_lse=False, out=None):
@@ -1280,24 +1317,24 @@ def sdpa_tree(q, k, v, parent, kv_len=None, scale=None, return_lse=False, out=No
     context, its ancestors and itself; a chain (parent i - 1) is causal decode
     attention.  A node with any other parent, -2 for instance, is absent, and its
     descendants with it: output 0, lse -inf, so trees of several sizes share a
-    batch.  bf16 / f16, head dims multiples of 8 up to 256, t <= 256.  ``out``
-    ((n, hq, t, ev), unit last stride) receives the result in place."""
-    q, dims, scale = _cache_attn_check("sdpa_tree", q, k, v, kv_len, scale, out)
-    n, hq, hkv, t, s, e, ev = dims
+    batch.  bf16 / f16, head dims multiples of 8 up to 256, t <= 256, scale > 0.
+    ``out`` ((n, hq, t, ev), unit last stride) receives the result in place; it
+    must not overlap q, k or v."""
+    p, q, sq = _attn_call("sdpa_tree", q, k, v, kv_len, out)
+    n, hq, _, t, s, _, _ = p.dims
     if parent.dtype != torch.int32 or parent.shape not in ((n, t), (t,)) or t > s:
         raise _lib.KuiopsError("sdpa_tree", _lib.E_INVALID)
+    device = _gpu_of("sdpa_tree", q, k, v, parent, kv_len, out)
     if parent.dim() == 1:
         parent = parent.expand(n, t)
     parent = parent.contiguous()
     if out is None:
-        out = torch.empty((n, hq, t, ev), dtype=q.dtype, device=q.device)
+        out = torch.empty(p.out_shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((n, hq, t), dtype=torch.float32, device=q.device) if return_lse else None
-    nbytes = _cache_attn_workspace("kuiops_sdpa_tree_workspace", *dims)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _on_device("sdpa_tree", lambda stream: _lib_handle().kuiops_sdpa_tree(
-        *dims, _dt(q.dtype), q.data_ptr(), _strides(q, 3), k.data_ptr(), _strides(k, 3), v.data_ptr(), _strides(v, 3),
-        out.data_ptr(), _strides(out, 3), _ptr(lse), scale, parent.data_ptr(), _ptr(kv_len), _ptr(ws), nbytes, stream),
-        q.device, k, v, parent, kv_len, out)
+    ws = torch.empty(p.ws, dtype=torch.uint8, device=q.device) if p.ws else None
+    _enqueue("kuiops_sdpa_tree", device, (
+        *p.dims, p.dtype, q.data_ptr(), sq, k.data_ptr(), p.sk, v.data_ptr(), p.sv, out.data_ptr(), p.so, _ptr(lse),
+        p.scale if scale is None else float(scale), parent.data_ptr(), _ptr(kv_len), _ptr(ws), p.ws))
     return out, lse
 
 
@@ -1311,35 +1348,36 @@ def tree_accept(tokens, parent, target):
     to the lowest child whose token is its parent's target, as far as there is
     one.  ``path`` lists the nodes, then -1; the next token is the target of the
     last one (-1 where node 0 is absent: count 0).  t <= 256."""
-    n, t = tokens.shape if tokens.dim() == 2 else (0, 0)
-    if t == 0 or tokens.dtype != torch.int64 or target.dtype != torch.int64 or parent.dtype != torch.int32 \
-            or parent.shape != (n, t) or target.shape != (n, t):
+    shape = tokens.shape
+    if len(shape) != 2 or shape[1] == 0 or tokens.dtype != torch.int64 or target.dtype != torch.int64 \
+            or parent.dtype != torch.int32 or parent.shape != shape or target.shape != shape:
         raise _lib.KuiopsError("tree_accept", _lib.E_INVALID)
+    device = _gpu_of("tree_accept", tokens, parent, target)
+    n, t = shape
     tokens, parent, target = tokens.contiguous(), parent.contiguous(), target.contiguous()
-    path = torch.empty((n, t), dtype=torch.int32, device=tokens.device)
+    path = torch.empty(shape, dtype=torch.int32, device=tokens.device)
     count = torch.empty(n, dtype=torch.int32, device=tokens.device)
     follow = torch.empty(n, dtype=torch.int64, device=tokens.device)
-    _on_device("tree_accept", lambda stream: _lib_handle().kuiops_tree_accept(
-        n, t, tokens.data_ptr(), parent.data_ptr(), target.data_ptr(), path.data_ptr(), count.data_ptr(),
-        follow.data_ptr(), stream), tokens.device, parent, target)
+    _enqueue("kuiops_tree_accept", device, (n, t, tokens.data_ptr(), parent.data_ptr(), target.data_ptr(),
+                                            path.data_ptr(), count.data_ptr(), follow.data_ptr()))
     return path, count, follow
 
 
+@functools.lru_cache(maxsize=2048)
 def _cache_rows(name, k, v):
-    """Both caches of (batch, hkv, capacity, e) with rows that are moved as bytes."""
-    if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or not _disjoint(k) or not _disjoint(v):
+    """(bytes of a row, strides in bytes) of both caches (batch, hkv, capacity, e),
+    whose rows are moved as bytes."""
+    if len(k[0]) != 4 or len(v[0]) != 4 or k[0][:3] != v[0][:3] or not _disjoint(*k[:2]) or not _disjoint(*v[:2]):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
-    for c in (k, v):
-        if c.numel() and (c.stride(3) != 1 and c.shape[3] > 1):
+    got = []
+    for shape, stride, dtype in (k, v):
+        if math.prod(shape) and shape[3] > 1 and stride[3] != 1:
             raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
-    return [(c.shape[3] * c.element_size(), c.data_ptr(), _strides_rows(c)) for c in (k, v)]
-
-
-def _strides_rows(c):
-    st = _strides(c, 3, c.element_size())
-    if c.shape[2] <= 1:
-        st[2] = c.shape[3] * c.element_size()
-    return st
+        st = _c_strides(shape, stride, 3, dtype.itemsize)
+        if shape[2] <= 1:
+            st[2] = shape[3] * dtype.itemsize
+        got.append((shape[3] * dtype.itemsize, st))
+    return got
 
 
 def kv_tree_commit(k, v, path, kv_len, tree):
@@ -1353,20 +1391,27 @@ def kv_tree_commit(k, v, path, kv_len, tree):
     path's length.  k / v (layers * n, hkv, capacity, e) may be all layers'
     caches of the n sequences at once, layer after layer.  Any element type,
     rows of multiples of 16 bytes; p <= 256."""
-    n = kv_len.numel()
-    (krow, kp, sk), (vrow, vp, sv) = _cache_rows("kv_tree_commit", k, v)
+    name = "kv_tree_commit"
+    (krow, sk), (vrow, sv) = _cache_rows(name, _meta(k), _meta(v))
     batch, hkv, cap, _ = k.shape
-    tree = int(tree)
-    if kv_len.dtype != torch.int32 or kv_len.dim() != 1 or not kv_len.is_contiguous() or path.dtype != torch.int32 \
-            or path.dim() != 2 or path.shape[0] != n or tree < 1 or path.shape[1] > tree \
-            or (batch % n if n else batch):
-        raise _lib.KuiopsError("kv_tree_commit", _lib.E_INVALID)
+    n, tree = kv_len.numel(), int(tree)
+    if not _flat_ints(kv_len, n) or path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != n or tree < 1 \
+            or path.shape[1] > tree or (batch % n if n else batch):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    device = _gpu_of(name, k, v, path, kv_len)
     path = path.contiguous()
-    out = torch.empty_like(kv_len)
-    _on_device("kv_tree_commit", lambda stream: _lib_handle().kuiops_kv_tree_commit(
-        batch, n, hkv, cap, krow, vrow, kp, sk, vp, sv, path.shape[1], path.data_ptr(), tree, kv_len.data_ptr(),
-        out.data_ptr(), stream), k.device, v, path, kv_len)
+    out = torch.empty(n, dtype=torch.int32, device=k.device)
+    _enqueue("kuiops_kv_tree_commit", device, (
+        batch, n, hkv, cap, krow, vrow, k.data_ptr(), sk, v.data_ptr(), sv, path.shape[1], path.data_ptr(), tree,
+        kv_len.data_ptr(), out.data_ptr()))
     return out
+
+
+@functools.lru_cache(maxsize=2048)
+def _acc_strides(name, dims, acc):
+    if acc[2] != torch.float32 or acc[0] != dims or not _own_rows(*acc[:2]):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    return _c_strides(*acc[:2], 2)
 
 
 def sdpa_decode_accum(q, k, v, acc, kv_len=None, scale=None, causal=True, return_lse=False, out=None):
@@ -1376,21 +1421,41 @@ def sdpa_decode_accum(q, k, v, acc, kv_len=None, scale=None, causal=True, return
     positions.  -> (out, lse).  What :func:`kv_evict` decides by.
 
     One call per decoded token (l = 1), per piece of a prompt, or for a whole
-    prompt (l = kv_len).  bf16 / f16, head dims multiples of 8 up to 256."""
-    q, dims, scale = _cache_attn_check("sdpa_decode_accum", q, k, v, kv_len, scale, out)
-    n, hq, hkv, l, s, e, ev = dims
-    if acc.dtype != torch.float32 or acc.shape != (n, hkv, s) or not _own_rows(acc) or (causal and l > s):
-        raise _lib.KuiopsError("sdpa_decode_accum", _lib.E_INVALID)
+    prompt (l = kv_len).  bf16 / f16, head dims multiples of 8 up to 256,
+    scale > 0; ``out`` must not overlap q, k or v."""
+    name = "sdpa_decode_accum"
+    p, q, sq = _attn_call(name, q, k, v, kv_len, out)
+    n, hq, hkv, l, s, _, _ = p.dims
+    sa = _acc_strides(name, (n, hkv, s), _meta(acc))
+    if causal and l > s:
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    device = _gpu_of(name, q, k, v, acc, kv_len, out)
     if out is None:
-        out = torch.empty((n, hq, l, ev), dtype=q.dtype, device=q.device)
+        out = torch.empty(p.out_shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((n, hq, l), dtype=torch.float32, device=q.device)
-    nbytes = _cache_attn_workspace("kuiops_sdpa_decode_accum_workspace", *dims)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _on_device("sdpa_decode_accum", lambda stream: _lib_handle().kuiops_sdpa_decode_accum(
-        *dims, _dt(q.dtype), q.data_ptr(), _strides(q, 3), k.data_ptr(), _strides(k, 3), v.data_ptr(), _strides(v, 3),
-        out.data_ptr(), _strides(out, 3), lse.data_ptr(), scale, 1 if causal else 0, _ptr(kv_len), acc.data_ptr(),
-        _strides(acc, 2), _ptr(ws), nbytes, stream), q.device, k, v, acc, kv_len, out)
+    ws = torch.empty(p.ws, dtype=torch.uint8, device=q.device) if p.ws else None
+    _enqueue("kuiops_sdpa_decode_accum", device, (
+        *p.dims, p.dtype, q.data_ptr(), sq, k.data_ptr(), p.sk, v.data_ptr(), p.sv, out.data_ptr(), p.so,
+        lse.data_ptr(), p.scale if scale is None else float(scale), 1 if causal else 0, _ptr(kv_len), acc.data_ptr(), sa,
+        _ptr(ws), p.ws))
     return out, (lse if return_lse else None)
+
+
+@functools.lru_cache(maxsize=2048)
+def _evict_plan(name, dims, acc, pos, acc_out, pos_out):
+    for t, dtype in ((acc, torch.float32), (pos, torch.int32), (acc_out, torch.float32), (pos_out, torch.int32)):
+        if t[2] != dtype or t[0] != dims or not _own_rows(*t[:2]):
+            raise _lib.KuiopsError(name, _lib.E_INVALID)
+    return [_c_strides(*t[:2], 2) for t in (acc, pos, acc_out, pos_out)]
+
+
+def _same_or_apart(t, o) -> bool:
+    """Whether o is t's own memory, element for element, or another buffer."""
+    if o is t or not t.numel():
+        return True
+    if o.untyped_storage().data_ptr() != t.untyped_storage().data_ptr():
+        return True
+    return o.data_ptr() == t.data_ptr() and o.stride() == t.stride()
 
 
 def kv_evict(k, v, acc, pos, kv_len, budget, recent=0, acc_out=None, pos_out=None, len_out=None):
@@ -1407,27 +1472,22 @@ def kv_evict(k, v, acc, pos, kv_len, budget, recent=0, acc_out=None, pos_out=Non
     length (min(kv_len, budget)) on.  k and v change in place; acc, pos and kv_len
     (int32 [n]) too, unless ``acc_out`` / ``pos_out`` / ``len_out`` are given."""
     name = "kv_evict"
-    (krow, kp, sk), (vrow, vp, sv) = _cache_rows(name, k, v)
+    (krow, sk), (vrow, sv) = _cache_rows(name, _meta(k), _meta(v))
     n, hkv, cap, _ = k.shape
-    acc_out, pos_out, len_out = (a if o is None else o for a, o in ((acc, acc_out), (pos, pos_out), (kv_len, len_out)))
+    acc_out = acc if acc_out is None else acc_out
+    pos_out = pos if pos_out is None else pos_out
+    len_out = kv_len if len_out is None else len_out
     budget, recent = int(budget), int(recent)
-    if budget < 1 or recent < 0 or recent > budget or kv_len.shape != (n,) or len_out.shape != (n,) \
-            or any(t.dtype != torch.int32 for t in (pos, pos_out, kv_len, len_out)) \
-            or any(t.dtype != torch.float32 for t in (acc, acc_out)) \
-            or any(t.shape != (n, hkv, cap) or not _own_rows(t) for t in (acc, acc_out, pos, pos_out)) \
-            or not kv_len.is_contiguous() or not len_out.is_contiguous():
+    if budget < 1 or recent < 0 or recent > budget or not _flat_ints(kv_len, n) or not _flat_ints(len_out, n) \
+            or not _same_or_apart(acc, acc_out) or not _same_or_apart(pos, pos_out) or not _same_or_apart(kv_len, len_out):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
-    for t, o in ((acc, acc_out), (pos, pos_out)):
-        # the same memory, then slot for slot; or another buffer
-        if o is not t and o.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() and n * hkv * cap > 0 \
-                and (o.data_ptr() != t.data_ptr() or o.stride() != t.stride()):
-            raise _lib.KuiopsError(name, _lib.E_INVALID)
+    sa, sp, sao, spo = _evict_plan(name, (n, hkv, cap), _meta(acc), _meta(pos), _meta(acc_out), _meta(pos_out))
+    device = _gpu_of(name, k, v, acc, pos, kv_len, acc_out, pos_out, len_out)
     budget = min(budget, max(cap, 1))
     nbytes = n * hkv * (1 + 2 * budget) * 4
     ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=k.device)
-    _on_device(name, lambda stream: _lib_handle().kuiops_kv_evict(
-        n, hkv, cap, krow, vrow, kp, sk, vp, sv, acc.data_ptr(), _strides(acc, 2), pos.data_ptr(), _strides(pos, 2),
-        kv_len.data_ptr(), budget, min(recent, budget), acc_out.data_ptr(), _strides(acc_out, 2), pos_out.data_ptr(),
-        _strides(pos_out, 2), len_out.data_ptr(), ws.data_ptr(), nbytes, stream),
-        k.device, v, acc, pos, kv_len, acc_out, pos_out, len_out)
+    _enqueue("kuiops_kv_evict", device, (
+        n, hkv, cap, krow, vrow, k.data_ptr(), sk, v.data_ptr(), sv, acc.data_ptr(), sa, pos.data_ptr(), sp,
+        kv_len.data_ptr(), budget, min(recent, budget), acc_out.data_ptr(), sao, pos_out.data_ptr(), spo,
+        len_out.data_ptr(), ws.data_ptr(), nbytes))
     return acc_out, pos_out, len_out

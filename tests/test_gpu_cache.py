@@ -59,9 +59,17 @@ def trees(n, t, seed, absent=0):
     return p
 
 
-def one_part(hq, hkv, rows):
-    """Whether the call's probabilities are single 16-bit values: more than 64 query rows share a KV head."""
-    return hq // hkv * rows > 64
+def wide_capacity(n, hq, hkv, rows, e, ev):
+    """A cache capacity with which a call of more than 16 rows runs on the
+    128-row kernel (whose probabilities are single 16-bit values); the smaller
+    ones of these tests run on the 16-row kernel."""
+    groups = n * hkv * -(-(hq // hkv * rows) // 16)
+    return 2 ** 25 // ((64 if max(e, ev) <= 64 else 128) * groups) + 64
+
+
+def padded(x, cap):
+    """x with its third axis padded to the capacity with NaN."""
+    return torch.cat([x, torch.full((*x.shape[:2], cap - x.shape[2], x.shape[3]), math.nan, dtype=x.dtype)], 2)
 
 
 TREES = [  # n, hq, hkv, t, s, e, ev, lens, absent, chain
@@ -84,18 +92,26 @@ TREES = [  # n, hq, hkv, t, s, e, ev, lens, absent, chain
 ]
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("n,hq,hkv,t,s,e,ev,lens,absent,chain", TREES)
-def test_sdpa_tree(cuda, n, hq, hkv, t, s, e, ev, lens, absent, chain, dtype):
+def test_sdpa_tree(cuda, n, hq, hkv, t, s, e, ev, lens, absent, chain, dtype, wide):
     q, k, v = gen((n, hq, t, e), dtype, 1), gen((n, hkv, s, e), dtype, 2), gen((n, hkv, s, ev), dtype, 3)
+    if wide:
+        if hq // hkv * t <= 16 or max(e, ev) > 128:
+            return      # these have the 16-row kernel alone
+        lens = lens or (s,) * n
     parent = trees(n, t, 4, absent)
     if chain:
         parent = np.where(parent >= -1, np.arange(t) - 1, parent).astype(np.int32)
     ref, lref, size, terms = O.sdpa_tree(npy(q), npy(k), npy(v), parent, lens)
     kv_len = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=cuda)
+    if wide:
+        cap = wide_capacity(n, hq, hkv, t, e, ev)
+        k, v = padded(k, cap), padded(v, cap)
     out, lse = ops.sdpa_tree(q.to(cuda), k.to(cuda), v.to(cuda), torch.from_numpy(parent).to(cuda), kv_len, return_lse=True)
     assert out.dtype == dtype and lse.dtype == torch.float32
-    close_out(out, ref, size, terms, e, one_part(hq, hkv, t))
+    close_out(out, ref, size, terms, e, wide)
     close_lse(lse, lref, terms, e)
 
 
@@ -109,6 +125,20 @@ def test_sdpa_tree_long_cache_splits(cuda):
                                  torch.tensor([L], dtype=torch.int32, device=cuda), return_lse=True)
         close_out(out, ref, size, terms, 64, False)
         close_lse(lse, lref, terms, 64)
+
+
+@pytest.mark.parametrize("L", [7, 63, 64, 65, 200, 1000, 4097])
+def test_sdpa_tree_splits_of_the_wide_kernel(cuda, L):
+    # 128-row kernel, the keys over several work-groups, the tree across block ends
+    n, hq, hkv, t, e = 1, 16, 2, 7, 64
+    q, k, v = gen((n, hq, t, e), BF, 1), gen((n, hkv, L, e), BF, 2), gen((n, hkv, L, e), BF, 3)
+    parent = trees(n, t, 4)
+    ref, lref, size, terms = O.sdpa_tree(npy(q), npy(k), npy(v), parent, (L,))
+    cap = wide_capacity(n, hq, hkv, t, e, e)
+    out, lse = ops.sdpa_tree(q.to(cuda), padded(k, cap).to(cuda), padded(v, cap).to(cuda), torch.from_numpy(parent).to(cuda),
+                             torch.tensor([L], dtype=torch.int32, device=cuda), return_lse=True)
+    close_out(out, ref, size, terms, e, True)
+    close_lse(lse, lref, terms, e)
 
 
 def test_sdpa_tree_layouts(cuda):
@@ -130,10 +160,11 @@ def test_sdpa_tree_layouts(cuda):
     close_out(got, ref, size, terms, e, False)
 
 
-@pytest.mark.parametrize("hq", [2, 24])
+@pytest.mark.parametrize("e", [64, 128])
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dtype", [BF, HF])
-def test_sdpa_tree_values_that_are_not_finite_where_no_query_looks(cuda, dtype, hq):
-    n, hkv, t, s, e, L = 1, 2, 6, 120, 64, 100
+def test_sdpa_tree_values_that_are_not_finite_where_no_query_looks(cuda, dtype, wide, e):
+    n, hq, hkv, t, s, L = 1, 24, 2, 6, 120, 100
     q, k, v = gen((n, hq, t, e), dtype, 1), gen((n, hkv, s, e), dtype, 2), gen((n, hkv, s, e), dtype, 3)
     parent = np.array([[-1, 0, 0, 1, -2, 4]], np.int32)
     ref, lref, size, terms = O.sdpa_tree(npy(q), npy(k), npy(v), parent, (L,))
@@ -141,9 +172,12 @@ def test_sdpa_tree_values_that_are_not_finite_where_no_query_looks(cuda, dtype, 
     for j in list(range(L, s)) + [L - 2, L - 1]:
         k[:, :, j], v[:, :, j] = (math.nan, math.inf) if j % 2 else (-math.inf, math.nan)
     q[:, :, 4:] = math.nan
+    if wide:
+        cap = wide_capacity(n, hq, hkv, t, e, e)
+        k, v = padded(k, cap), padded(v, cap)
     args = k.to(cuda), v.to(cuda), torch.from_numpy(parent).to(cuda), torch.tensor([L], dtype=torch.int32, device=cuda)
     out, lse = ops.sdpa_tree(q.to(cuda), *args, return_lse=True)
-    close_out(out, ref, size, terms, e, one_part(hq, hkv, t))
+    close_out(out, ref, size, terms, e, wide)
     close_lse(lse, lref, terms, e)
     # node 2's value: seen by node 2 alone
     v[:, :, L - t + 2, 5], v[:, :, L - t + 2, 6], v[:, :, L - t + 2, 7] = math.inf, -math.inf, math.nan
@@ -151,7 +185,7 @@ def test_sdpa_tree_values_that_are_not_finite_where_no_query_looks(cuda, dtype, 
     got = npy(out)
     assert (got[:, :, 2, 5] == math.inf).all() and (got[:, :, 2, 6] == -math.inf).all() and np.isnan(got[:, :, 2, 7]).all()
     got[:, :, 2, 5:8] = ref[:, :, 2, 5:8]
-    close_out(torch.from_numpy(got).to(dtype), ref, size, terms, e, one_part(hq, hkv, t))
+    close_out(torch.from_numpy(got).to(dtype), ref, size, terms, e, wide)
 
 
 def test_sdpa_tree_an_infinite_value_of_the_context_reaches_every_row(cuda):
@@ -201,19 +235,29 @@ ACCUM = [  # n, hq, hkv, l, s, e, ev, lens, causal
     (2, 4, 1, 70, 333, 128, 128, (333, 70), True),        # a piece of one
     (1, 4, 2, 33, 90, 80, 40, (90,), True),
     (1, 2, 2, 3, 90, 256, 256, (90,), True),
+    (1, 2, 1, 60, 130, 256, 192, (130,), True),
+    (1, 8, 4, 1000, 1000, 64, 64, None, True),            # row groups that end with a head
+    (1, 4, 1, 897, 1500, 128, 128, (1400,), True),
 ]
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("n,hq,hkv,l,s,e,ev,lens,causal", ACCUM)
-def test_sdpa_decode_accum(cuda, n, hq, hkv, l, s, e, ev, lens, causal, dtype):
+def test_sdpa_decode_accum(cuda, n, hq, hkv, l, s, e, ev, lens, causal, dtype, wide):
     q, k, v = gen((n, hq, l, e), dtype, 1), gen((n, hkv, s, e), dtype, 2), gen((n, hkv, s, ev), dtype, 3)
-    acc = torch.rand(n, hkv, s, generator=torch.Generator().manual_seed(4))
+    if wide:
+        if hq // hkv * l <= 16 or max(e, ev) > 128:
+            return      # these have the 16-row kernel alone
+        lens = lens or (s,) * n
+        cap = max(s, wide_capacity(n, hq, hkv, l, e, ev))
+        k, v = padded(k, cap), padded(v, cap)
+    acc = torch.rand(n, hkv, k.shape[2], generator=torch.Generator().manual_seed(4))
     ref, lref, aref, size, terms = O.sdpa_decode_accum(npy(q), npy(k), npy(v), npy(acc), lens, causal=causal)
     kv_len = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=cuda)
     got = acc.to(cuda)
     out, lse = ops.sdpa_decode_accum(q.to(cuda), k.to(cuda), v.to(cuda), got, kv_len, causal=causal, return_lse=True)
-    close_out(out, ref, size, terms, e, one_part(hq, hkv, l))
+    close_out(out, ref, size, terms, e, wide or 2 ** 25 // 128 < n * hkv * -(-(hq // hkv * l) // 16) * s)
     close_lse(lse, lref, terms, e)
     rows = hq // hkv * l
     grown = aref - npy(acc)
@@ -221,7 +265,7 @@ def test_sdpa_decode_accum(cuda, n, hq, hkv, l, s, e, ev, lens, causal, dtype):
     assert (np.abs(npy(got) - aref) <= tol).all()
     # keys behind the length keep their sums, to the bit
     for b in range(n):
-        L = s if lens is None else lens[b]
+        L = k.shape[2] if lens is None else lens[b]
         assert torch.equal(got[b, :, L:].cpu(), acc[b, :, L:])
 
 
