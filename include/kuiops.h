@@ -667,8 +667,8 @@ KUIOPS_API int kuiops_decode_rows_batched(int64_t M, int64_t N, int64_t K, int d
  * position, with contiguous rows; K / V rows must start 16-byte aligned.
  *
  * Attention of a tree of drafted tokens over a KV cache.  The last t of the
- * L = kv_len[b] keys of a sequence (kv_len: device int32[n], at most s; null:
- * s) are the nodes of its tree: node i is query i and key L - t + i.  parent
+ * L = kv_len[b] keys of a sequence (kv_len: device int32[n], taken as 0 .. s;
+ * null: s) are the nodes of its tree: node i is query i and key L - t + i.  parent
  * (device int32[n][t]) gives each node's parent, an earlier node, or -1 for a
  * node that follows the context directly.  Query i sees the L - t keys of the
  * context, its ancestors and itself.  A node whose parent is below -1 or not
@@ -702,7 +702,8 @@ KUIOPS_API int kuiops_tree_accept(int64_t n, int64_t t, const int64_t *tokens, c
  * the path's end, its first entry that is below 0, not below t or outside the
  * cache; len_out[b] = base + the path's length.  Any path is moved as if all
  * rows were read first.  K / V have batch = a multiple of n entries (all
- * layers' caches of n sequences): entry r belongs to sequence r % n.  krow /
+ * layers' caches of n sequences): entry r belongs to sequence r % n; K and V must
+ * not overlap.  krow /
  * vrow: bytes of a row, multiples of 16; strides sk / sv in BYTES, multiples of
  * 16, rows not overlapping.  path: device int32[n][p], p <= t, p <= 256.
  * len_out must not overlap kv_len.  kv_len[b] < t: nothing moves and len_out[b]

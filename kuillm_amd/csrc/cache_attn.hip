@@ -1156,7 +1156,7 @@ int check_attn(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t
     if (!Q || !O || (s > 0 && (!K || !V))) return KUIOPS_E_INVALID;
     if (dtype != KUIOPS_BF16 && dtype != KUIOPS_F16) return KUIOPS_E_UNSUPPORTED;
     if (e % 8 || ev % 8 || e > 256 || ev > 256) return KUIOPS_E_UNSUPPORTED;
-    if (!(scale > 0.f) || !(scale < INFINITY)) return KUIOPS_E_UNSUPPORTED;
+    if (!(scale > 0.f) || !(scale * kLog2e < INFINITY)) return KUIOPS_E_UNSUPPORTED;
     if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || (reinterpret_cast<uintptr_t>(O) & 7)) return KUIOPS_E_UNSUPPORTED;
     for (int i = 0; i < 3; ++i)
         if (sq[i] % 8 || sk[i] % 8 || sv[i] % 8 || so[i] % 4 || sk[i] < 0 || sv[i] < 0) return KUIOPS_E_UNSUPPORTED;

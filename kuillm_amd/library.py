@@ -13,7 +13,9 @@ back silently.
 Schemas follow the aten ops they replace (mm, addmm, bmm, _softmax over the
 last dim, scaled-dot-product attention returning (out, lse), topk, gather,
 index, the elementwise maps, last-axis mean, cat) with the reference's argument meaning
-(kuipy/kuiops.py:403-754).
+(kuipy/kuiops.py:403-754).  The drafted-tree and bounded-cache ops (sdpa_tree,
+tree_accept, kv_tree_commit, sdpa_decode_accum, kv_evict) have no aten counterpart;
+those that change a cache in place say so in their schemas.
 """
 from __future__ import annotations
 
@@ -43,6 +45,14 @@ _SCHEMAS = {
                    "float s0=1.0, float s1=0.0) -> Tensor",
     "mean_lastdim": "mean_lastdim(Tensor x, bool keepdim=False) -> Tensor",
     "cat": "cat(Tensor[] tensors, int dim=0) -> Tensor",
+    "sdpa_tree": "sdpa_tree(Tensor q, Tensor k, Tensor v, Tensor parent, Tensor? kv_len=None, float? scale=None) "
+                 "-> (Tensor, Tensor)",
+    "tree_accept": "tree_accept(Tensor tokens, Tensor parent, Tensor target) -> (Tensor, Tensor, Tensor)",
+    "kv_tree_commit": "kv_tree_commit(Tensor(a!) k, Tensor(b!) v, Tensor path, Tensor kv_len, int tree) -> Tensor",
+    "sdpa_decode_accum": "sdpa_decode_accum(Tensor q, Tensor k, Tensor v, Tensor(a!) acc, Tensor? kv_len=None, "
+                         "float? scale=None, bool causal=True) -> (Tensor, Tensor)",
+    "kv_evict": "kv_evict(Tensor(a!) k, Tensor(b!) v, Tensor(c!) acc, Tensor(d!) pos, Tensor(e!) kv_len, int budget, "
+                "int recent=0) -> ()",
 }
 for _s in _SCHEMAS.values():
     _LIB.define(_s)
@@ -121,11 +131,25 @@ def _cat(tensors, dim=0):
     return ops.cat(list(tensors), dim)
 
 
+def _sdpa_tree(q, k, v, parent, kv_len=None, scale=None):
+    return ops.sdpa_tree(q, k, v, parent, kv_len=kv_len, scale=scale, return_lse=True)
+
+
+def _sdpa_decode_accum(q, k, v, acc, kv_len=None, scale=None, causal=True):
+    return ops.sdpa_decode_accum(q, k, v, acc, kv_len=kv_len, scale=scale, causal=causal, return_lse=True)
+
+
+def _kv_evict(k, v, acc, pos, kv_len, budget, recent=0):
+    ops.kv_evict(k, v, acc, pos, kv_len, budget, recent)
+
+
 for _name, _fn in (("mm", _mm), ("addmm", _addmm), ("bmm", _bmm), ("softmax", _softmax),
                    ("sdpa", _sdpa), ("sdpa_decode", _sdpa_decode), ("topk", _topk),
                    ("gather", _gather), ("index", _index), ("index_multi", _index_multi), ("scatter", _scatter), ("sort", _sort),
                    ("cumsum", _cumsum), ("multinomial", _multinomial), ("elementwise", _elementwise),
-                   ("mean_lastdim", _mean_lastdim), ("cat", _cat)):
+                   ("mean_lastdim", _mean_lastdim), ("cat", _cat), ("sdpa_tree", _sdpa_tree),
+                   ("tree_accept", ops.tree_accept), ("kv_tree_commit", ops.kv_tree_commit),
+                   ("sdpa_decode_accum", _sdpa_decode_accum), ("kv_evict", _kv_evict)):
     _LIB.impl(_name, _fn, "CUDA")
 
 
@@ -230,3 +254,29 @@ def _cat_fake(tensors, dim=0):
 def _index_multi_fake(inp, first, idxs):
     bshape = torch.broadcast_shapes(*[tuple(t.shape) for t in idxs])
     return inp.new_empty((*inp.shape[:first], *bshape, *inp.shape[first + len(idxs):]))
+
+
+@_fake("sdpa_tree")
+def _sdpa_tree_fake(q, k, v, parent, kv_len=None, scale=None):
+    return q.new_empty((*q.shape[:3], v.shape[-1])), q.new_empty(q.shape[:3], dtype=torch.float32)
+
+
+@_fake("tree_accept")
+def _tree_accept_fake(tokens, parent, target):
+    n, t = tokens.shape
+    return tokens.new_empty((n, t), dtype=torch.int32), tokens.new_empty(n, dtype=torch.int32), tokens.new_empty(n)
+
+
+@_fake("kv_tree_commit")
+def _kv_tree_commit_fake(k, v, path, kv_len, tree):
+    return kv_len.new_empty(kv_len.shape)
+
+
+@_fake("sdpa_decode_accum")
+def _sdpa_decode_accum_fake(q, k, v, acc, kv_len=None, scale=None, causal=True):
+    return q.new_empty((*q.shape[:3], v.shape[-1])), q.new_empty(q.shape[:3], dtype=torch.float32)
+
+
+@_fake("kv_evict")
+def _kv_evict_fake(k, v, acc, pos, kv_len, budget, recent=0):
+    return None

@@ -1311,7 +1311,8 @@ def sdpa_tree(q, k, v, parent, kv_len=None, scale=None, return_lse=False, out=No
 
     q (n, hq, t, e) holds the t nodes' queries; k / v (n, hkv, s, e / ev) are the
     caches, in which the nodes' keys are the last t of the first ``kv_len[b]``
-    (int32 [n] on the device, read when the kernel runs; None: s).  ``parent``
+    (int32 [n] on the device, read when the kernel runs and taken as 0 .. s; None:
+    s).  ``parent``
     (int32 [n, t], or [t] for all sequences) names each node's parent, an
     earlier node, or -1 for one that follows the context.  Node i sees the
     context, its ancestors and itself; a chain (parent i - 1) is causal decode
@@ -1389,14 +1390,14 @@ def kv_tree_commit(k, v, path, kv_len, tree):
     ones in order, ended by -1 (:func:`tree_accept`'s).  With base = kv_len[b] - t,
     row base + path[b, i] goes to row base + i; the new count is base plus the
     path's length.  k / v (layers * n, hkv, capacity, e) may be all layers'
-    caches of the n sequences at once, layer after layer.  Any element type,
-    rows of multiples of 16 bytes; p <= 256."""
+    caches of the n sequences at once, layer after layer; they must not overlap.
+    Any element type, rows of multiples of 16 bytes; p <= 256."""
     name = "kv_tree_commit"
     (krow, sk), (vrow, sv) = _cache_rows(name, _meta(k), _meta(v))
     batch, hkv, cap, _ = k.shape
     n, tree = kv_len.numel(), int(tree)
     if not _flat_ints(kv_len, n) or path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != n or tree < 1 \
-            or path.shape[1] > tree or (batch % n if n else batch):
+            or path.shape[1] > tree or (batch % n if n else batch) or (k.numel() and k.data_ptr() == v.data_ptr()):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     device = _gpu_of(name, k, v, path, kv_len)
     path = path.contiguous()
@@ -1450,12 +1451,14 @@ def _evict_plan(name, dims, acc, pos, acc_out, pos_out):
 
 
 def _same_or_apart(t, o) -> bool:
-    """Whether o is t's own memory, element for element, or another buffer."""
-    if o is t or not t.numel():
+    """Whether o is t's own memory, element for element, or shares none with it."""
+    if o is t or not t.numel() or not o.numel():
         return True
-    if o.untyped_storage().data_ptr() != t.untyped_storage().data_ptr():
-        return True
-    return o.data_ptr() == t.data_ptr() and o.stride() == t.stride()
+    if o.data_ptr() == t.data_ptr():
+        return o.stride() == t.stride() and o.shape == t.shape
+    first, second = (t, o) if t.data_ptr() < o.data_ptr() else (o, t)
+    span = sum((size - 1) * st for size, st in zip(first.shape, first.stride())) + 1
+    return first.data_ptr() + span * first.element_size() <= second.data_ptr()
 
 
 def kv_evict(k, v, acc, pos, kv_len, budget, recent=0, acc_out=None, pos_out=None, len_out=None):

@@ -142,6 +142,7 @@ def test_kv_tree_commit_refuses():
     for args in ((k[0], v[0], path, n, 3), (k, v[:, :, :9], path, n, 3), (k, v, path.long(), n, 3), (k, v, path, n.long(), 3),
                  (k, v, path[:1], n, 3), (k, v, path, n, 0), (k, v, path, n, 2),           # a path longer than the tree
                  (torch.cat([k, k[:1]]), torch.cat([v, v[:1]]), path, n, 3),               # 3 entries of 2 sequences
+                 (k, k, path, n, 3),                                                       # one cache for both
                  (k[:, :, :1].expand(-1, -1, 10, -1), v, path, n, 3)):                     # rows on one another
         refuses(INVALID, ops.kv_tree_commit, *args)
     refuses(UNSUPPORTED, ops.kv_tree_commit, k.transpose(2, 3).contiguous().transpose(2, 3), v, path, n, 3)
@@ -154,9 +155,13 @@ def test_kv_evict_refuses():
     both = torch.zeros(2, 2, 12)
     for kw in (dict(budget=0), dict(recent=-1), dict(recent=5), dict(acc=acc.double()), dict(pos=pos.long()), dict(acc=acc[..., :9]),
                dict(kv_len=n.long()), dict(kv_len=n[:1]), dict(acc_out=acc.half()), dict(pos_out=pos[:1]), dict(len_out=n.long()),
-               dict(acc_out=both[..., 1:11], acc=both[..., :10]), dict(k=k[:, :, :1].expand(-1, -1, 10, -1)), dict(v=v[:, :1])):
+               dict(acc_out=both[..., 1:11], acc=both[..., :10]), dict(pos_out=pos.view(-1)[:40].view(2, 2, 10).transpose(0, 1)), dict(k=k[:, :, :1].expand(-1, -1, 10, -1)), dict(v=v[:, :1])):
         refuses(INVALID, ops.kv_evict, **{**dict(k=k, v=v, acc=acc, pos=pos, kv_len=n, budget=4), **kw})
     refuses(UNSUPPORTED, ops.kv_evict, k, v, acc, pos, n, 4)
+    # another part of the same buffer is another buffer
+    refuses(UNSUPPORTED, ops.kv_evict, k, v, torch.zeros(2, 2, 2, 10)[0], pos, n, 4, acc_out=torch.zeros(2, 2, 2, 10)[1])
+    pair = torch.zeros(2, 2, 2, 10)
+    refuses(UNSUPPORTED, ops.kv_evict, k, v, pair[0], pos, n, 4, acc_out=pair[1])
 
 
 def test_c_entries_refuse_on_the_host(lib):
@@ -189,9 +194,9 @@ def test_c_entries_refuse_on_the_host(lib):
 
     r3, q = _lib.strides3(0, 0, 128), ctypes.c_void_p(1 << 21)
 
-    def commit(batch=2, n=2, krow=128, sk=r3, np=3, t=4, ln=p, out=q):
-        return lib.kuiops_kv_tree_commit(batch, n, 2, 40, krow, 128, p, sk, p, r3, np, p, t, ln, out, null)
-    assert commit(batch=3) == commit(np=5) == commit(t=0) == commit(out=p) == commit(ln=null) == INVALID
+    def commit(batch=2, n=2, krow=128, sk=r3, np=3, t=4, ln=p, out=q, vp=q):
+        return lib.kuiops_kv_tree_commit(batch, n, 2, 40, krow, 128, p, sk, vp, r3, np, p, t, ln, out, null)
+    assert commit(vp=p) == commit(batch=3) == commit(np=5) == commit(t=0) == commit(out=p) == commit(ln=null) == INVALID
     assert commit(krow=120) == commit(sk=_lib.strides3(0, 0, 64)) == commit(sk=_lib.strides3(0, 8, 128)) == commit(np=257, t=300) == UNSUPPORTED
 
     s2 = _lib.strides3(0, 0, 0)
@@ -201,3 +206,35 @@ def test_c_entries_refuse_on_the_host(lib):
     assert evict(budget=0) == evict(recent=9) == evict(recent=-1) == evict(acc=null) == INVALID
     assert evict(krow=8) == UNSUPPORTED
     assert evict(ws=null) == evict(nb=lib.kuiops_kv_evict_workspace(1, 2, 8) - 1) == _lib.E_WORKSPACE
+
+
+# ------------------------------------------------------------- custom ops
+
+def test_custom_ops_trace_without_a_device():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from kuillm_amd import library  # noqa: F401
+    with FakeTensorMode():
+        q, k, v = attn()
+        par, n = tree(), torch.zeros(2, dtype=torch.int32)
+        op = torch.ops.kuiops
+        out, lse = op.sdpa_tree(q, k, v, par, n)
+        assert out.shape == (2, 4, 3, 64) and out.dtype == BF and lse.shape == (2, 4, 3) and lse.dtype == torch.float32
+        tok = torch.zeros(2, 3, dtype=torch.int64)
+        path, count, follow = op.tree_accept(tok, par, tok)
+        assert path.shape == (2, 3) and path.dtype == count.dtype == torch.int32 and follow.shape == (2,) and follow.dtype == torch.int64
+        assert op.kv_tree_commit(k, v, path, n, 3).shape == (2,)
+        acc = torch.zeros(2, 2, 10)
+        out, lse = op.sdpa_decode_accum(q, k, v, acc, n)
+        assert out.shape == (2, 4, 3, 64) and lse.shape == (2, 4, 3)
+        assert op.kv_evict(k, v, acc, torch.zeros(2, 2, 10, dtype=torch.int32), n, 4) is None
+    for name, changed in (("kv_tree_commit", 2), ("sdpa_decode_accum", 1), ("kv_evict", 5), ("sdpa_tree", 0), ("tree_accept", 0)):
+        schema = getattr(torch.ops.kuiops, name).default._schema
+        assert sum(a.alias_info is not None and a.alias_info.is_write for a in schema.arguments) == changed
+
+
+def test_custom_ops_have_no_cpu_kernel():
+    from kuillm_amd import library  # noqa: F401
+    q, k, v = attn()
+    with pytest.raises(NotImplementedError):
+        torch.ops.kuiops.sdpa_tree(q, k, v, tree())

@@ -524,3 +524,46 @@ def test_empty_calls(cuda):
     got = ops.kv_evict(k, k.clone(), torch.zeros(1, 2, 0, device=cuda), torch.zeros(1, 2, 0, dtype=torch.int32, device=cuda),
                        torch.zeros(1, dtype=torch.int32, device=cuda), 4)
     assert got[2].tolist() == [0]
+
+
+def test_custom_ops_run_the_same_kernels(cuda):
+    from kuillm_amd import library  # noqa: F401
+    op = torch.ops.kuiops
+    q, k, v = (x.to(cuda) for x in (gen((2, 4, 5, 64), BF, 1), gen((2, 2, 60, 64), BF, 2), gen((2, 2, 60, 64), BF, 3)))
+    parent, lens = torch.from_numpy(trees(2, 5, 4)).to(cuda), torch.tensor([60, 33], dtype=torch.int32, device=cuda)
+    for a, b in zip(op.sdpa_tree(q, k, v, parent, lens), ops.sdpa_tree(q, k, v, parent, lens, return_lse=True)):
+        assert torch.equal(a, b)
+    tok = torch.randint(0, 2, (2, 5), device=cuda)
+    path, count, follow = op.tree_accept(tok, parent, tok.flip(0).contiguous())
+    for a, b in zip((path, count, follow), ops.tree_accept(tok, parent, tok.flip(0))):
+        assert torch.equal(a, b)
+    sides = [[k.clone(), v.clone()] for _ in range(2)]
+    assert torch.equal(op.kv_tree_commit(*sides[0], path, lens, 5), ops.kv_tree_commit(*sides[1], path, lens, 5))
+    accs = [torch.zeros(2, 2, 60, device=cuda) for _ in range(2)]
+    for a, b in zip(op.sdpa_decode_accum(q, k, v, accs[0], lens), ops.sdpa_decode_accum(q, k, v, accs[1], lens, return_lse=True)):
+        assert torch.equal(a, b)
+    pos = [torch.arange(60, dtype=torch.int32, device=cuda).repeat(2, 2, 1) for _ in range(2)]
+    ends = [lens.clone(), lens.clone()]
+    op.kv_evict(*sides[0], accs[0], pos[0], ends[0], 20, 4)
+    ops.kv_evict(*sides[1], accs[1], pos[1], ends[1], 20, 4)
+    for a, b in zip((*sides[0], accs[0], pos[0], ends[0]), (*sides[1], accs[1], pos[1], ends[1])):
+        assert torch.equal(a, b)
+    assert ends[0].tolist() == [20, 20]
+
+
+def test_another_current_device_or_stream_is_not_used(cuda):
+    # a side stream's call runs behind that stream's own work
+    q, k, v = (x.to(cuda) for x in (gen((1, 4, 5, 64), BF, 1), gen((1, 2, 600, 64), BF, 2), gen((1, 2, 600, 64), BF, 3)))
+    parent = torch.from_numpy(trees(1, 5, 4)).to(cuda)
+    ref, _ = ops.sdpa_tree(q, k, v, parent)
+    side = torch.cuda.Stream()
+    late = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        big = torch.randn(4096, 4096, device=cuda)
+        for _ in range(10):
+            big = big @ big * 1e-4
+        late.copy_(q)
+        got, _ = ops.sdpa_tree(late, k, v, parent)
+    side.synchronize()
+    assert torch.equal(got, ref)
