@@ -151,7 +151,10 @@ __global__ __launch_bounds__(kCommitWaves * 64) void tree_commit_kernel(CommitAr
 // are at or behind the budget and destinations below it, so the moves need no
 // order.  Slots of 1024 x IPT keys stay in registers (thread t has t, t + 1024,
 // ...); longer caches are read again (from L2) in each of the six passes.
-// evict_move_kernel moves the rows of K and V.
+// evict_move_kernel moves the rows of K and V (few of them move in the first kernel).
+// What bounds them: a few hundred slots, one work-group's latency (576 keys: 7.4 us with
+// the move); 64 heads of 8000, select 16 us, of it the histograms about half; the moves
+// the memory, 5.9 TB/s read and written.
 constexpr int kEvictThreads = 1024;
 struct EvictArgs {
     int n, hkv, budget, recent;
@@ -167,7 +170,26 @@ struct EvictArgs {
     char *K, *V;
     int64_t sk0, sk1, sk2, sv0, sv1, sv2;     // bytes
     int kcols, vcols;                         // 16-byte chunks of a row
+    int move_here;                            // evict_select_kernel moves its head's rows too
 };
+
+// Rows first .. of a head's moves, 16 bytes a thread, `step` apart.
+__device__ __forceinline__ void move_rows(const EvictArgs &a, int b, int hk, const int32_t *moves, int count, int64_t first, int64_t step) {
+    const int cols = a.kcols + a.vcols;
+    char *K = a.K + b * a.sk0 + hk * a.sk1, *V = a.V + b * a.sv0 + hk * a.sv1;
+    for (int64_t x = first; x < (int64_t)count * cols; x += step) {
+        const int i = (int)(x / cols), c = (int)(x % cols);
+        const int64_t to = moves[1 + i], from = moves[1 + a.budget + i];
+        if (c < a.kcols)
+            *reinterpret_cast<u32x4 *>(K + to * a.sk2 + c * 16) = *reinterpret_cast<const u32x4 *>(K + from * a.sk2 + c * 16);
+        else
+            *reinterpret_cast<u32x4 *>(V + to * a.sv2 + (c - a.kcols) * 16) =
+                *reinterpret_cast<const u32x4 *>(V + from * a.sv2 + (c - a.kcols) * 16);
+    }
+}
+__device__ __forceinline__ int new_length(const EvictArgs &a, int b) {
+    return min(max(a.kv_len[b], 0), (int)min((int64_t)a.budget, a.cap));
+}
 
 __device__ __forceinline__ uint32_t weight_key(float w) {
     if (w != w) return 0xfffffffeu;           // NaN ranks above every number
@@ -215,6 +237,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a
     float *acc_out = a.acc_out + b * a.sao0 + hk * a.sao1;
     int32_t *pos_out = a.pos_out + b * a.spo0 + hk * a.spo1;
     int32_t *moves = a.moves + (int64_t)blockIdx.x * (1 + 2 * m);
+    if (a.move_here && hk == 0 && tid == 0) a.len_out[b] = new_length(a, b);
     if (L <= m) {
         for (int j = tid; j < cap; j += NT) {
             acc_out[j] = j < L ? acc[j] : 0.f;
@@ -427,6 +450,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a
         acc_out[to] = acc[from];
         pos_out[to] = pos[from];
     }
+    if (a.move_here) move_rows(a, b, hk, moves, holes_all, tid, NT);
     __builtin_amdgcn_s_waitcnt(0);             // (acc_out may be acc: read before it is cleared)
     __syncthreads();
     for (int j = m + tid; j < cap; j += NT) {
@@ -438,21 +462,8 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
     const int bh = blockIdx.y, b = bh / a.hkv, hk = bh % a.hkv;
     const int32_t *moves = a.moves + (int64_t)bh * (1 + 2 * a.budget);
-    const int count = moves[0], cols = a.kcols + a.vcols;
-    if (hk == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
-        const int len = a.kv_len[b];
-        a.len_out[b] = min(max(len, 0), (int)min((int64_t)a.budget, a.cap));
-    }
-    char *K = a.K + b * a.sk0 + hk * a.sk1, *V = a.V + b * a.sv0 + hk * a.sv1;
-    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < (int64_t)count * cols; x += (int64_t)gridDim.x * 256) {
-        const int i = (int)(x / cols), c = (int)(x % cols);
-        const int64_t to = moves[1 + i], from = moves[1 + a.budget + i];
-        if (c < a.kcols)
-            *reinterpret_cast<u32x4 *>(K + to * a.sk2 + c * 16) = *reinterpret_cast<const u32x4 *>(K + from * a.sk2 + c * 16);
-        else
-            *reinterpret_cast<u32x4 *>(V + to * a.sv2 + (c - a.kcols) * 16) =
-                *reinterpret_cast<const u32x4 *>(V + from * a.sv2 + (c - a.kcols) * 16);
-    }
+    if (hk == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.len_out[b] = new_length(a, b);
+    move_rows(a, b, hk, moves, moves[0], (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
 bool rows_ok(const void *p, const int64_t *st, int64_t bytes) {
@@ -536,6 +547,12 @@ extern "C" int kuiops_kv_evict(int64_t n, int64_t hkv, int64_t cap, int64_t krow
     a.sv0 = sv[0]; a.sv1 = sv[1]; a.sv2 = sv[2];
     a.kcols = (int)(krow / 16); a.vcols = (int)(vrow / 16);
     const int64_t most = std::max<int64_t>(0, std::min(budget, cap - budget)) * (a.kcols + a.vcols);
+    // Few rows to move: the selecting work-group moves them itself, one launch less
+    // (us, two launches / one, graph replays: 8 heads of 64, 512 of 576 keys 9.4 / 7.6, 1792 of 2048
+    // 10.9 / 10.2, 1024 of 2048 11.2 / 12.7; 64 heads of 128, 512 of 640 10.3 / 9.2, 512 of 1024 13.0 /
+    // 15.2).  Not where len_out is kv_len: a head's work-group that starts late would read
+    // the new length of its sequence, so that one needs the second launch.
+    a.move_here = len_out != kv_len && most <= 4 * kEvictThreads;
     const int64_t per = std::max<int64_t>(1, cdiv(2048, n * hkv));
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min(per, cdiv(most, 256))), (unsigned)(n * hkv));
     const dim3 heads((unsigned)(n * hkv)), threads(kEvictThreads);
@@ -543,6 +560,6 @@ extern "C" int kuiops_kv_evict(int64_t n, int64_t hkv, int64_t cap, int64_t krow
     else if (cap <= 4 * kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<4>), heads, threads, 0, as_stream(stream), a);
     else if (cap <= 16 * kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<16>), heads, threads, 0, as_stream(stream), a);
     else hipLaunchKernelGGL((evict_select_kernel<0>), heads, threads, 0, as_stream(stream), a);
-    hipLaunchKernelGGL(evict_move_kernel, grid, dim3(256), 0, as_stream(stream), a);
+    if (!a.move_here) hipLaunchKernelGGL(evict_move_kernel, grid, dim3(256), 0, as_stream(stream), a);
     return launch_status();
 }

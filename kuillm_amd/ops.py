@@ -1356,7 +1356,7 @@ def tree_accept(tokens, parent, target):
     device = _gpu_of("tree_accept", tokens, parent, target)
     n, t = shape
     tokens, parent, target = tokens.contiguous(), parent.contiguous(), target.contiguous()
-    path = torch.empty(shape, dtype=torch.int32, device=tokens.device)
+    path = torch.empty_like(parent)
     count = torch.empty(n, dtype=torch.int32, device=tokens.device)
     follow = torch.empty(n, dtype=torch.int64, device=tokens.device)
     _enqueue("kuiops_tree_accept", device, (n, t, tokens.data_ptr(), parent.data_ptr(), target.data_ptr(),
@@ -1442,23 +1442,33 @@ def sdpa_decode_accum(q, k, v, acc, kv_len=None, scale=None, causal=True, return
     return out, (lse if return_lse else None)
 
 
+class _EvictPlan:
+    __slots__ = ("krow", "sk", "vrow", "sv", "strides", "acc_apart", "pos_apart")
+
+
+def _span(shape, stride) -> int:
+    """Elements from the first to the last one."""
+    return sum((size - 1) * st for size, st in zip(shape, stride)) + 1 if math.prod(shape) else 0
+
+
 @functools.lru_cache(maxsize=2048)
-def _evict_plan(name, dims, acc, pos, acc_out, pos_out):
+def _evict_plan(k, v, acc, pos, acc_out, pos_out) -> _EvictPlan:
+    """Checks the (shape, stride, dtype) of kv_evict's tensors."""
+    name, p = "kv_evict", _EvictPlan()
+    (p.krow, p.sk), (p.vrow, p.sv) = _cache_rows(name, k, v)
     for t, dtype in ((acc, torch.float32), (pos, torch.int32), (acc_out, torch.float32), (pos_out, torch.int32)):
-        if t[2] != dtype or t[0] != dims or not _own_rows(*t[:2]):
+        if t[2] != dtype or t[0] != k[0][:3] or not _own_rows(*t[:2]):
             raise _lib.KuiopsError(name, _lib.E_INVALID)
-    return [_c_strides(*t[:2], 2) for t in (acc, pos, acc_out, pos_out)]
+    p.strides = [_c_strides(*t[:2], 2) for t in (acc, pos, acc_out, pos_out)]
+    # (same layout, bytes of the input's extent, of the output's)
+    p.acc_apart, p.pos_apart = ((t[1] == o[1], 4 * _span(*t[:2]), 4 * _span(*o[:2])) for t, o in ((acc, acc_out), (pos, pos_out)))
+    return p
 
 
-def _same_or_apart(t, o) -> bool:
-    """Whether o is t's own memory, element for element, or shares none with it."""
-    if o is t or not t.numel() or not o.numel():
-        return True
-    if o.data_ptr() == t.data_ptr():
-        return o.stride() == t.stride() and o.shape == t.shape
-    first, second = (t, o) if t.data_ptr() < o.data_ptr() else (o, t)
-    span = sum((size - 1) * st for size, st in zip(first.shape, first.stride())) + 1
-    return first.data_ptr() + span * first.element_size() <= second.data_ptr()
+def _same_or_apart(a: int, b: int, same_layout: bool, a_bytes: int, b_bytes: int) -> bool:
+    """Whether a buffer at address b is the one at a, element for element, or
+    shares no memory with it."""
+    return (same_layout if a == b else b >= a + a_bytes or a >= b + b_bytes) or not a_bytes
 
 
 def kv_evict(k, v, acc, pos, kv_len, budget, recent=0, acc_out=None, pos_out=None, len_out=None):
@@ -1475,22 +1485,24 @@ def kv_evict(k, v, acc, pos, kv_len, budget, recent=0, acc_out=None, pos_out=Non
     length (min(kv_len, budget)) on.  k and v change in place; acc, pos and kv_len
     (int32 [n]) too, unless ``acc_out`` / ``pos_out`` / ``len_out`` are given."""
     name = "kv_evict"
-    (krow, sk), (vrow, sv) = _cache_rows(name, _meta(k), _meta(v))
-    n, hkv, cap, _ = k.shape
     acc_out = acc if acc_out is None else acc_out
     pos_out = pos if pos_out is None else pos_out
     len_out = kv_len if len_out is None else len_out
+    p = _evict_plan(_meta(k), _meta(v), _meta(acc), _meta(pos), _meta(acc_out), _meta(pos_out))
+    n, hkv, cap, _ = k.shape
     budget, recent = int(budget), int(recent)
+    acc_at, pos_at, len_at = acc.data_ptr(), pos.data_ptr(), kv_len.data_ptr()
+    acc_to, pos_to, len_to = acc_out.data_ptr(), pos_out.data_ptr(), len_out.data_ptr()
     if budget < 1 or recent < 0 or recent > budget or not _flat_ints(kv_len, n) or not _flat_ints(len_out, n) \
-            or not _same_or_apart(acc, acc_out) or not _same_or_apart(pos, pos_out) or not _same_or_apart(kv_len, len_out):
+            or not _same_or_apart(acc_at, acc_to, *p.acc_apart) or not _same_or_apart(pos_at, pos_to, *p.pos_apart) \
+            or not _same_or_apart(len_at, len_to, True, 4 * n, 4 * n):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
-    sa, sp, sao, spo = _evict_plan(name, (n, hkv, cap), _meta(acc), _meta(pos), _meta(acc_out), _meta(pos_out))
     device = _gpu_of(name, k, v, acc, pos, kv_len, acc_out, pos_out, len_out)
     budget = min(budget, max(cap, 1))
     nbytes = n * hkv * (1 + 2 * budget) * 4
     ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=k.device)
+    sa, sp, sao, spo = p.strides
     _enqueue("kuiops_kv_evict", device, (
-        n, hkv, cap, krow, vrow, k.data_ptr(), sk, v.data_ptr(), sv, acc.data_ptr(), sa, pos.data_ptr(), sp,
-        kv_len.data_ptr(), budget, min(recent, budget), acc_out.data_ptr(), sao, pos_out.data_ptr(), spo,
-        len_out.data_ptr(), ws.data_ptr(), nbytes))
+        n, hkv, cap, p.krow, p.vrow, k.data_ptr(), p.sk, v.data_ptr(), p.sv, acc_at, sa, pos_at, sp, len_at, budget,
+        min(recent, budget), acc_to, sao, pos_to, spo, len_to, ws.data_ptr(), nbytes))
     return acc_out, pos_out, len_out
