@@ -64,6 +64,7 @@ struct CacheAttnArgs {
     float *scores;             // [n][hkv][hq / hkv * l][spad]: q k, -inf where not seen; or null
     int sum_here;              // a work-group has all rows and keys of its KV head: it adds up the weights itself
     int64_t spad;
+    float *part_sums;          // key_weights_kernel: [parts][n][hkv][spad], or null
 };
 
 __device__ __forceinline__ int keys_of(const CacheAttnArgs &a, int b) {
@@ -923,11 +924,15 @@ __global__ __launch_bounds__(256) void accum_merge_kernel(CacheAttnArgs a) {
 // memory into the operand's lanes, 16 bytes of 32 rows each, their addresses alone
 // took three times the arithmetic's time.  A work-group takes tiles p and last - p:
 // causal keys are seen by the fewer rows the later they are, and two such tiles
-// always by about as many.  The exponentials bound it.
+// always by about as many.  What bounds it: the exponentials (a turn of 32 rows and 64
+// keys, head dim 64: about 770 cycles of vector instructions, 256 of MFMA), and for
+// 32-key tiles the rows' traffic from L2, 8 to 10 TB/s.  With `parts` > 1 that many
+// work-groups share a tile's rows, and sum_parts_kernel adds up their sums.
 template <typename T, int HD, int KT>
-__global__ __launch_bounds__(HD <= 128 ? 512 : 256) void key_weights_kernel(CacheAttnArgs a, int tiles) {
+__global__ __launch_bounds__(HD <= 128 ? 512 : 256) void key_weights_kernel(CacheAttnArgs a, int tiles, int parts) {
     constexpr int KS = HD / 16, NWV = HD <= 128 ? 8 : 4, KEYS = 32 * KT, NS = HD <= 64 ? 3 : 2;
-    constexpr int RB = HD * 2, CPR = HD / 8, RPB = 1024 / RB, STAGE = 32 * RB, DPT = STAGE / 1024, STEP = NWV * 32;
+    constexpr int RB = HD * 2, CPR = HD / 8, RPB = 1024 / RB, STAGE = 32 * RB, DPT = STAGE / 1024;
+    const int part = blockIdx.x % parts, STEP = NWV * parts * 32;
     typedef typename Mfma<T>::frag frag;
     auto swz = [](int r) { return CPR >= 16 ? (r & 15) : ((r >> 1) & 7); };     // as cache_rows_kernel's K
     __shared__ __attribute__((aligned(1024))) char sQ[NS][NWV][STAGE];
@@ -937,7 +942,7 @@ __global__ __launch_bounds__(HD <= 128 ? 512 : 256) void key_weights_kernel(Cach
     const int lq = lane & 31, lh = lane >> 5;
     const int b = blockIdx.y / a.hkv, hk = blockIdx.y % a.hkv, G = a.hq / a.hkv;
     const int L = keys_of(a, b), first = L - a.l;
-    const int p = blockIdx.x;
+    const int p = blockIdx.x / parts, mine = part * NWV + wave;       // the wave among the tile's
     const T *Qp = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + hk * G * a.sq1;
     const float *Lp = a.lse + ((int64_t)b * a.hq + hk * G) * a.l;
     // this lane's row of a stage and its 16 bytes of it, per DMA instruction (columns
@@ -972,7 +977,7 @@ __global__ __launch_bounds__(HD <= 128 ? 512 : 256) void key_weights_kernel(Cach
             // the wave's next 32 rows into stage z.  Past the list a lane takes its last
             // row (with a weight of 0, and for the keys only that this row sees: a NaN in
             // it reaches no others), so every turn has the same loads.
-            int r0 = wave * 32, h0 = r0 / per, p0 = i0 + r0 - h0 * per;
+            int r0 = mine * 32, h0 = r0 / per, p0 = i0 + r0 - h0 * per;
             auto load = [&](int z) __attribute__((always_inline)) {
                 const float *lp;
                 if (p0 + 31 < a.l && r0 + 31 < rows) {
@@ -1010,7 +1015,7 @@ __global__ __launch_bounds__(HD <= 128 ? 512 : 256) void key_weights_kernel(Cach
             for (int t = 0; t < KT; ++t) sum[t] = f32x16{};
 #pragma unroll
             for (int z = 0; z < NS - 1; ++z) load(z);
-            for (int rb = wave * 32; rb < rows; rb += NS * STEP) {
+            for (int rb = mine * 32; rb < rows; rb += NS * STEP) {
 #pragma unroll
                 for (int z = 0; z < NS; ++z) {
                     if (rb + z * STEP >= rows) break;
@@ -1060,12 +1065,21 @@ __global__ __launch_bounds__(HD <= 128 ? 512 : 256) void key_weights_kernel(Cach
                 float v = 0.f;
 #pragma unroll
                 for (int w = 0; w < NWV; ++w) v += s_sum[w][tid];
-                a.acc[b * a.sa0 + hk * a.sa1 + k0 + tid] += v;
+                if (parts == 1) a.acc[b * a.sa0 + hk * a.sa1 + k0 + tid] += v;
+                else a.part_sums[((int64_t)part * a.n * a.hkv + blockIdx.y) * a.spad + k0 + tid] = v;
             }
             __syncthreads();
         }
         if (tile != p || tiles - 1 - p <= p) break;
     }
+}
+
+__global__ __launch_bounds__(256) void sum_parts_kernel(CacheAttnArgs a, int parts) {
+    const int b = blockIdx.y / a.hkv, hk = blockIdx.y % a.hkv, key = blockIdx.x * 256 + threadIdx.x;
+    if (key >= keys_of(a, b)) return;
+    float v = 0.f;
+    for (int x = 0; x < parts; ++x) v += a.part_sums[((int64_t)x * a.n * a.hkv + blockIdx.y) * a.spad + key];
+    a.acc[b * a.sa0 + hk * a.sa1 + key] += v;
 }
 
 // ------------------------------------------------------------- host side
@@ -1074,7 +1088,8 @@ struct Plan {
     int hd, rows;          // head dim and rows of a work-group: 16 (cache_attn_kernel) or 128 (cache_rows_kernel)
     int row_groups, splits, pair, head_tiles, sum_here;
     int64_t units;
-    size_t o_bytes, ml_bytes, score_bytes;        // of the workspace
+    int kt, parts;         // key_weights_kernel: 32-key blocks of a tile, work-groups of a tile
+    size_t o_bytes, ml_bytes, score_bytes, part_bytes;        // of the workspace
 };
 
 // Which kernel.  16-row groups are several work-groups for more rows, each of
@@ -1122,25 +1137,36 @@ Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e
     // and all: 16.3 -> 12.5 us)
     p.sum_here = keep && p.splits == 1 && p.row_groups == 1;
     p.ml_bytes = p.splits > 1 || (keep && !p.sum_here) ? (size_t)p.splits * n * hq * l * 8 : 0;
+    // Tiles of 64 keys halve the rows' traffic where there are enough of them, or
+    // enough rows to share among the work-groups of a tile; parts: a work-group for
+    // every CU, of two turns of its waves at least.  Whole calls, us, 32 keys one part / 32
+    // keys parts / 64 keys one part / 64 keys parts, 32 / 8 heads of 64 if not said: a
+    // 1999-token prompt 69.0 / 77.3 / 74.4 / 64.7 (f16, run after run: 63.6 / - / - / 66.5), two
+    // of them 113.6 / 124 / 94.2 / 106.5, 1000 tokens 42.7 / 41.9 / 49.9 / 43.9, 512 29.8 / 28.9 /
+    // 35.6 / 32.3, 128 behind 1920 23.9 / 31.8 / 28.6 / 27.8, 1000 tokens of 14 / 2 heads 47.9 /
+    // 38.4 / 58.6 / 42.7; heads of 128, 1999 tokens 104 / 106 / 101 / 92.
+    p.kt = p.parts = 1;
+    if (accum && !keep) {
+        const int64_t groups32 = n * hkv * cdiv(cdiv(s, 32), 2);
+        if (p.hd <= 128 && (groups32 >= 2 * kCUs || (p.hd == 128 && groups32 >= kCUs && rows >= 4096))) p.kt = 2;
+        const int64_t pairs = n * hkv * cdiv(cdiv(s, 32 * p.kt), 2), turns = cdiv(rows, 256);
+        p.parts = (int)std::max<int64_t>(1, std::min({(int64_t)8, kCUs / pairs, turns / 2}));
+        if (p.parts > 1) p.part_bytes = (size_t)p.parts * n * hkv * (cdiv(s, 32) * 32) * 4;
+    }
     return p;
 }
 
-size_t state_bytes(const Plan &p) { return p.o_bytes + p.score_bytes + p.ml_bytes; }
+size_t state_bytes(const Plan &p) { return p.o_bytes + p.score_bytes + p.ml_bytes + p.part_bytes; }
 
-// 64 keys a tile halve the rows' loads, 32 give twice the work-groups
 template <typename T, int HD>
-void launch_weights(const CacheAttnArgs &a, hipStream_t st) {
-    const int64_t heads = (int64_t)a.n * a.hkv;
-    const int kt = HD <= 128 && heads * cdiv(a.s, 128) >= 256 ? 2 : 1;
-    const int tiles = (int)cdiv(a.s, 32 * kt);
-    const dim3 grid((unsigned)cdiv(tiles, 2), (unsigned)heads);
+void launch_weights(const CacheAttnArgs &a, const Plan &p, hipStream_t st) {
+    const unsigned heads = (unsigned)(a.n * a.hkv), tiles = (unsigned)cdiv(a.s, 32 * p.kt);
+    const dim3 grid((tiles + 1) / 2 * p.parts, heads), threads(HD <= 128 ? 512 : 256);
     if constexpr (HD <= 128) {
-        if (kt == 2) {
-            hipLaunchKernelGGL((key_weights_kernel<T, HD, 2>), grid, dim3(512), 0, st, a, tiles);
-            return;
-        }
+        if (p.kt == 2) hipLaunchKernelGGL((key_weights_kernel<T, HD, 2>), grid, threads, 0, st, a, (int)tiles, p.parts);
     }
-    hipLaunchKernelGGL((key_weights_kernel<T, HD, 1>), grid, dim3(HD <= 128 ? 512 : 256), 0, st, a, tiles);
+    if (p.kt == 1) hipLaunchKernelGGL((key_weights_kernel<T, HD, 1>), grid, threads, 0, st, a, (int)tiles, p.parts);
+    if (p.parts > 1) hipLaunchKernelGGL(sum_parts_kernel, dim3((unsigned)cdiv(a.s, 256), heads), dim3(256), 0, st, a, p.parts);
 }
 
 template <typename T, int HD>
@@ -1158,7 +1184,7 @@ int launch_attn(const CacheAttnArgs &a, const Plan &p, hipStream_t st) {
         hipLaunchKernelGGL((cache_merge_kernel<T, HD>), dim3((unsigned)cdiv(rows, 256 / (HD / 4))), dim3(256), 0, st, a);
     }
     if (a.acc)
-        launch_weights<T, HD>(a, st);
+        launch_weights<T, HD>(a, p, st);
     return launch_status();
 }
 
@@ -1213,6 +1239,8 @@ CacheAttnArgs fill_attn(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s
     a.ws_o = p.o_bytes ? reinterpret_cast<float *>(ws) : nullptr;
     a.scores = p.score_bytes ? reinterpret_cast<float *>(ws + p.o_bytes) : nullptr;
     a.ws_ml = p.ml_bytes ? reinterpret_cast<float *>(ws + p.o_bytes + p.score_bytes) : nullptr;
+    // (behind the row sums, which are multiples of 8 bytes)
+    a.part_sums = p.part_bytes ? reinterpret_cast<float *>(ws + p.o_bytes + p.score_bytes + p.ml_bytes) : nullptr;
     a.spad = cdiv(s, 32) * 32;
     return a;
 }
