@@ -238,6 +238,8 @@ ACCUM = [  # n, hq, hkv, l, s, e, ev, lens, causal
     (1, 2, 1, 60, 130, 256, 192, (130,), True),
     (1, 8, 4, 1000, 1000, 64, 64, None, True),            # row groups that end with a head
     (1, 4, 1, 897, 1500, 128, 128, (1400,), True),
+    (2, 8, 4, 20, 70, 64, 64, (70, 25), True),
+    (1, 2, 1, 700, 700, 256, 256, None, True),            # a tile's rows over two work-groups
 ]
 
 
