@@ -212,6 +212,10 @@ __device__ __forceinline__ void store_row(const CacheAttnArgs &a, int64_t b, int
 //   in that order.  The probability is the sum of two 16-bit parts, one MFMA
 //   each (2^-16 of it is lost in bf16, 2^-21 in f16): with the few rows of
 //   this kernel the K / V stream takes the time, not the MFMAs.
+// K needs no LDS because a wave shares its keys with no other; V does, as the MFMA
+// wants 8 keys of a column in a lane.  Measured: 4 sequences of 1000 to 2000 keys, 32 / 32
+// heads of 128, 13 rows: 24.5 us, 4.3 TB/s; 8 rows over 500 keys, one sequence: 7.8 us, all
+// of it latency (key count, query, first keys, three steps of them, waves' merge).
 // A part that is 0 times an infinite value is NaN, so is a masked NaN: a wave
 // whose sums are not finite goes over its keys again with the row maxima that
 // it found, multiplying value by value for the rows that see them.
@@ -506,8 +510,16 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
 // softmax's vector instructions bound the kernel, and a second part would cost
 // a third more of the one and a third of the other; each weight is off by at
 // most half a step of the output's type, as the output itself is.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void cache_rows_kernel(CacheAttnArgs a) {
+// With two key groups (KG) 8 waves take blocks 2 j and 2 j + 1 and join their sums
+// through LDS in the end, half the columns each, in a fixed order.
+// Measured: 256 rows per head over 60000 keys, 8 heads of 128: 78 us, 800 TFLOP/s
+// and 3.1 TB/s; with all blocks in L2 it takes as long, and the MFMA pipes are
+// busy 36% of the time with one or two waves a SIMD: a step of 64 keys is 1024 cycles of MFMA
+// and about 900 of exponentials and other vector instructions, which overlap only in
+// part.  Deeper prefetch from LDS changed nothing; 512 registers and one wave a SIMD cost
+// 15 to 35% (accumulators copied to and fro).
+template <typename T, int HD, int KG>
+__global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2, 2))) void cache_rows_kernel(CacheAttnArgs a) {
     constexpr int NWV = 4, KB = 64, R = 32 * NWV;
     constexpr int RB = HD * 2, CPR = HD / 8, TILE = KB * RB;
     constexpr int DPW = TILE / 1024 / NWV, RPB = 1024 / RB;
@@ -518,18 +530,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // (transposing): chunk c of row r sits at c ^ swizzle(r), all banks evenly
     auto kswz = [](int r) { return CPR == 16 ? (r & 15) : ((r >> 1) & 7); };
     auto vswz = [](int r) { return CPR == 16 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
-    __shared__ __attribute__((aligned(1024))) char sK0[TILE], sV0[TILE], sK1[TILE], sV1[TILE];
+    __shared__ __attribute__((aligned(1024))) char stages[KG * 4 * TILE];
+    __shared__ f32x2 s_ml[KG][R];
     __shared__ TreeBits tb;
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NWV, kg = __builtin_amdgcn_readfirstlane(tid >> 6) / NWV;
+    char *const sK0 = stages + kg * 4 * TILE, *const sV0 = sK0 + TILE, *const sK1 = sV0 + TILE, *const sV1 = sK1 + TILE;
     const int lq = lane & 31, lh = lane >> 5, G4 = lane >> 4, qq = lane & 15;
     const Unit u = unit_of(a);
     if (!u.any) return;
     const int b = u.b, hk = u.hk, split = u.split;
     const int G = a.hq / a.hkv, rows_kv = G * a.l;
     const int L = keys_of(a, b), first = L - a.l;
-    const int blocks_all = (L + KB - 1) / KB;
-    const int chunk = (blocks_all + a.splits - 1) / a.splits * KB;
+    const int blocks_all = (L + KB * KG - 1) / (KB * KG);
+    const int chunk = (blocks_all + a.splits - 1) / a.splits * KB * KG;
 
     // a.pair: row groups p and last - p, whose causal lengths together are the same for every p
     const int groups = a.head_tiles ? G * a.head_tiles : (rows_kv + R - 1) / R;
@@ -545,7 +559,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // keys below free_end are seen by every row of the wave
     const int w0 = r0 + wave * 32, w1 = min(w0 + 31, last);
     const int free_end = a.mode == kFull ? L : a.mode == kCausal ? first + 1 + (w0 / a.l == w1 / a.l ? w0 % a.l : 0) : first;
-    const int nkv = (kend - kbeg + KB - 1) / KB;
+    const int nkv = (kend - kbeg + KB * KG - 1) / (KB * KG);
 
     const T *Kp = reinterpret_cast<const T *>(a.K) + b * a.sk0 + hk * a.sk1 + (int64_t)kbeg * a.sk2;
     const T *Vp = reinterpret_cast<const T *>(a.V) + b * a.sv0 + hk * a.sv1 + (int64_t)kbeg * a.sv2;
@@ -561,12 +575,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         offV[j] = cv < a.ev ? (uint32_t)((r * a.sv2 + cv) * 2) : kOut;
     }
     auto issue_k = [&](int kt, char *sk) __attribute__((always_inline)) {
-        const uint32_t kb = (uint32_t)((int64_t)kt * KB * a.sk2 * 2);
+        const uint32_t kb = (uint32_t)((int64_t)(kt * KG + kg) * KB * a.sk2 * 2);
 #pragma unroll
         for (int j = 0; j < DPW; ++j) dma16_buf(rsK, offK[j], kb, sk + (wave * DPW + j) * 1024);
     };
     auto issue_v = [&](int kt, char *sv) __attribute__((always_inline)) {
-        const uint32_t vb = (uint32_t)((int64_t)kt * KB * a.sv2 * 2);
+        const uint32_t vb = (uint32_t)((int64_t)(kt * KG + kg) * KB * a.sv2 * 2);
 #pragma unroll
         for (int j = 0; j < DPW; ++j) dma16_buf(rsV, offV[j], vb, sv + (wave * DPW + j) * 1024);
     };
@@ -596,7 +610,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             mine = (uint64_t)__shfl((uint32_t)(nodes >> 32), pos, 64) << 32 | __shfl((uint32_t)nodes, pos, 64);
             row_ok = row_ok && mine != 0;
         } else {
-            tree_bits<NWV * 64>(tb, a.parent + (int64_t)b * a.l, a.l);
+            tree_bits<NWV * KG * 64>(tb, a.parent + (int64_t)b * a.l, a.l);
             row_ok = row_ok && (tb.w[pos][pos >> 6] >> (pos & 63)) & 1;
         }
     }
@@ -724,7 +738,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             __syncthreads();
             if (j + 2 < nkv) issue_k(j + 2, hs ? sK1 : sK0);
             if (j + 1 < nkv) issue_v(j + 1, hs ? sV0 : sV1);
-            if (live) step(hs ? scB : scA, hs ? scA : scB, hs ? sK0 : sK1, hs ? sV1 : sV0, kbeg + j * KB);
+            if (live) step(hs ? scB : scA, hs ? scA : scB, hs ? sK0 : sK1, hs ? sV1 : sV0, kbeg + (j * KG + kg) * KB);
         }
     }
     float z = 0.f;                  // stays 0 if every sum is finite
@@ -738,7 +752,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int t = 0; t < DT; ++t) o[t] = f32x16{};
         const float mref = m_used == -INFINITY ? 0.f : m_used + Shift<T>::value;
         for (int j = 0; j < nkv; ++j) {
-            const int kv0 = kbeg + j * KB;
+            const int kv0 = kbeg + (j * KG + kg) * KB;
             __syncthreads();
             issue_k(j, sK0);
             issue_v(j, sV0);
@@ -776,11 +790,45 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 
     const float l_all = xor_add<32>(l_run);
-    if (rr < rend) {
-        const float m = row_ok ? m_used + Shift<T>::value : -INFINITY, l = row_ok ? l_all : 0.f;
-        const int64_t st = (int64_t)split * a.n * a.hq * a.l + ((int64_t)b * a.hq + hk * G + h) * a.l + pos;
+    float m = row_ok ? m_used + Shift<T>::value : -INFINITY, l = row_ok ? l_all : 0.f;
+    const int64_t st = (int64_t)split * a.n * a.hq * a.l + ((int64_t)b * a.hq + hk * G + h) * a.l + pos;
+    if constexpr (KG == 2) {
+        // each key group has half the columns of both groups' sums in the end
+        f32x4 *part = reinterpret_cast<f32x4 *>(stages);        // [wave][DT * 4][lane]
+        __syncthreads();
+        if (lh == 0) s_ml[kg][wave * 32 + lq] = f32x2{m, l};
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+        for (int half = 0; half < 2; ++half) {
+            if (half == kg) continue;
+#pragma unroll
+            for (int dt = half * DT / 2; dt < (half + 1) * DT / 2; ++dt)
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                    part[(wave * DT * 4 + dt * 4 + y) * 64 + lane] = f32x4{o[dt][4 * y], o[dt][4 * y + 1], o[dt][4 * y + 2], o[dt][4 * y + 3]};
+        }
+        __syncthreads();
+        const f32x2 other = s_ml[1 - kg][wave * 32 + lq];
+        const float top = fmaxf(m, other[0]), mu = top == -INFINITY ? 0.f : top;
+        const float w0 = fast_exp2(m - mu), w1 = fast_exp2(other[0] - mu);
+        m = top;
+        l = kg == 0 ? __builtin_fmaf(other[1], w1, l * w0) : __builtin_fmaf(l, w0, other[1] * w1);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (half != kg) continue;
+#pragma unroll
+            for (int dt = half * DT / 2; dt < (half + 1) * DT / 2; ++dt)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const f32x4 ov = part[(wave * DT * 4 + dt * 4 + y) * 64 + lane];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) o[dt][4 * y + x] = __builtin_fmaf(ov[x], w1, o[dt][4 * y + x] * w0);
+                }
+        }
+    }
+    if (rr < rend) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            if (KG == 2 && dt / (DT / 2) != kg) continue;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
                 const int d = dt * 32 + 8 * y + 4 * lh;
@@ -788,7 +836,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 if (a.splits == 1) store_row<T>(a, b, hk * G + h, pos, d, v, m, l);
                 else *reinterpret_cast<f32x4 *>(&a.ws_o[st * HD + d]) = v;
             }
-        if (a.splits > 1 && lh == 0) *reinterpret_cast<f32x2 *>(&a.ws_ml[st * 2]) = f32x2{m, l};
+        }
+        if (a.splits > 1 && lh == 0 && kg == 0) *reinterpret_cast<f32x2 *>(&a.ws_ml[st * 2]) = f32x2{m, l};
     }
     if (!a.pair || rg != u.rg || groups - 1 - rg == rg) break;
     rg = groups - 1 - rg;
@@ -797,7 +846,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 }
 
 // 4 columns of a row's splits, merged in split order (the same bits whatever order
-// the work-groups ended in); the splits' loads go out together, 8 at a time.
+// the work-groups ended in); the splits' loads go out together, 8 at a time: 5.6 us
+// for 2048 rows of 128 in 16 splits, 4.1 us for fewer (latency).
 template <int HD>
 __device__ __forceinline__ void merge_splits(const CacheAttnArgs &a, int64_t rows, int64_t row, int d, f32x4 &oo, float &mm, float &ll) {
     oo = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -851,7 +901,8 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
 // accum_merge_kernel -- the weights of a few rows' keys from the scores that
 // cache_attn_kernel kept, and the merge of its splits: a work-group has 512 keys
 // of a KV head and its share of the rows' outputs.  (Writing and reading the
-// scores costs 8 bytes a row and key, reading K again 2 e a key.)
+// scores costs 8 bytes a row and key, reading K again 2 e a key.)  7.1 us for 16 sequences
+// of 8 heads, 4 rows, 4000 keys: of which 8 MB of scores take about 2.
 constexpr int kScoreRows = 32;
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void accum_merge_kernel(CacheAttnArgs a) {
@@ -1088,6 +1139,7 @@ struct Plan {
     int hd, rows;          // head dim and rows of a work-group: 16 (cache_attn_kernel) or 128 (cache_rows_kernel)
     int row_groups, splits, pair, head_tiles, sum_here;
     int64_t units;
+    int key_groups;        // cache_rows_kernel: groups of 4 waves
     int kt, parts;         // key_weights_kernel: 32-key blocks of a tile, work-groups of a tile
     size_t o_bytes, ml_bytes, score_bytes, part_bytes;        // of the workspace
 };
@@ -1102,13 +1154,21 @@ struct Plan {
 // and 23.3 / 19.2; 8 heads, 32 rows, 256 keys 6.1 / 8.3; 64 heads, 64 rows, 4000 keys
 // of 128 42.4 / 30.5.
 //
-// How many splits.  About one work-group per CU (twice that only while each
-// still has 2048 keys: 16 sequences of 64 nodes over 8064 keys 163 -> 149 us), of at
+// How many splits.  About one work-group per CU (of 16-row ones twice that while each
+// still has 2048 keys), of at
 // least 256 keys: 64 KV heads, 16 rows, 4000 keys of 128: 256 / 512 / 1024 work-groups
 // 25.8 / 25.7 / 31.4; 32 rows, 16-row groups, 256 / 512 / 1024 28.9 / 29.5 / 36.2.  Short
 // caches are not split, which saves the merge's launch: 8 heads, 32 rows, 640 keys
 // of 64 one split 7.7, four 8.6; 1024 keys 9.2 / 8.6; 256 of 128 8.5 / 10.3; 640 12.0 /
 // 11.0.
+//
+// How many key groups.  A 128-row work-group that has a CU for itself takes the keys
+// with two groups of 4 waves, unless its keys are few, as the second group's first
+// loads and the joining of the sums take their time: one / two groups, kernel alone, 16 row
+// groups over 60000 keys of 128 in 16 splits 83.4 / 78.2; a 1999-token prompt, 32 / 8
+// heads of 64 39.5 / 35.7; 64 row groups, 1000 keys each 33.4 / 36.0; 256 row groups of 8000
+// keys 163 / 145 (one group and two splits 137 and 12 of merge).  With more work-groups
+// two of them share a CU: 512 of 4000 keys 137 / 150.
 constexpr int kCUs = 256;
 Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev, int mode, bool accum) {
     Plan p{};
@@ -1124,12 +1184,13 @@ Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e
         p.head_tiles = (int)cdiv(l, 128);
         p.row_groups = (int)(hq / hkv) * p.head_tiles;
     }
-    const int64_t groups = n * hkv * p.row_groups, want = cdiv(s * groups, 2 * kCUs) >= 2048 ? 2 * kCUs : kCUs;
+    const int64_t groups = n * hkv * p.row_groups, want = p.rows == 16 && cdiv(s * groups, 2 * kCUs) >= 2048 ? 2 * kCUs : kCUs;
     p.splits = s * p.hd <= 640 * 64 ? 1 : (int)std::max<int64_t>(1, std::min(want / std::max<int64_t>(groups, 1), cdiv(s, 256)));
     p.splits = std::min(p.splits, 64);          // (accum_merge_kernel has a lane for each)
     p.units = n * hkv * p.splits;
     p.pair = p.rows == 128 && mode == kCausal && p.splits == 1 && p.row_groups > 1;
     if (p.pair) p.row_groups = (p.row_groups + 1) / 2;
+    p.key_groups = p.rows == 128 && p.units * p.row_groups <= kCUs && cdiv(s, p.splits) >= 1536 ? 2 : 1;
     const bool keep = accum && p.rows == 16 && rows <= kScoreRows;
     p.o_bytes = p.splits > 1 ? (size_t)p.splits * n * hq * l * p.hd * 4 : 0;
     p.score_bytes = keep ? (size_t)n * hkv * rows * (cdiv(s, 32) * 32) * 4 : 0;
@@ -1173,7 +1234,10 @@ template <typename T, int HD>
 int launch_attn(const CacheAttnArgs &a, const Plan &p, hipStream_t st) {
     const dim3 grid((unsigned)(cdiv(p.units, 8) * 8 * p.row_groups));
     if (p.rows == 16) hipLaunchKernelGGL((cache_attn_kernel<T, HD>), grid, dim3(256), 0, st, a);
-    else if constexpr (HD <= 128) hipLaunchKernelGGL((cache_rows_kernel<T, HD>), grid, dim3(256), 0, st, a);
+    else if constexpr (HD <= 128) {
+        if (p.key_groups == 2) hipLaunchKernelGGL((cache_rows_kernel<T, HD, 2>), grid, dim3(512), 0, st, a);
+        else hipLaunchKernelGGL((cache_rows_kernel<T, HD, 1>), grid, dim3(256), 0, st, a);
+    }
     if (a.sum_here) return launch_status();
     if (a.scores) {
         hipLaunchKernelGGL((accum_merge_kernel<T, HD>), dim3((unsigned)cdiv(a.s, 512), (unsigned)(a.n * a.hkv)), dim3(256), 0, st, a);
@@ -1212,10 +1276,11 @@ int check_attn(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t
     return KUIOPS_OK;
 }
 
-// A split's keys are addressed with 31-bit byte offsets from its first one.
-bool split_fits(const Plan &p, int64_t s, int64_t sk2, int64_t sv2) {
+// A split's keys are addressed with 31-bit byte offsets from its first one, and a
+// launch has fewer than 2^32 threads.
+bool plan_fits(const Plan &p, int64_t s, int64_t sk2, int64_t sv2) {
     const int64_t chunk = (cdiv(cdiv(s, 32), (int64_t)p.splits * 4) * 4 + 8) * 32;
-    return chunk * std::max(sk2, sv2) * 2 + 1024 < ((int64_t)1 << 31);
+    return chunk * std::max(sk2, sv2) * 2 + 1024 < ((int64_t)1 << 31) && cdiv(p.units, 8) * 8 * p.row_groups < ((int64_t)1 << 24);
 }
 
 CacheAttnArgs fill_attn(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev, const void *Q,
@@ -1267,7 +1332,7 @@ extern "C" int kuiops_sdpa_tree(int64_t n, int64_t hq, int64_t hkv, int64_t t, i
     if (!parent || t > s) return KUIOPS_E_INVALID;
     if (t > kMaxTree) return KUIOPS_E_UNSUPPORTED;
     const Plan p = plan_of(n, hq, hkv, t, s, e, ev, kTree, false);
-    if (!split_fits(p, s, sk[2], sv[2])) return KUIOPS_E_UNSUPPORTED;
+    if (!plan_fits(p, s, sk[2], sv[2])) return KUIOPS_E_UNSUPPORTED;
     const size_t need = state_bytes(p);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KUIOPS_E_WORKSPACE;
     CacheAttnArgs a = fill_attn(n, hq, hkv, t, s, e, ev, Q, sq, K, sk, V, sv, O, so, lse, scale, kTree, kv_len, p, workspace);
@@ -1292,7 +1357,7 @@ extern "C" int kuiops_sdpa_decode_accum(int64_t n, int64_t hq, int64_t hkv, int6
     if (n == 0 || hq == 0 || l == 0) return KUIOPS_OK;
     if (!lse || !sa || (s > 0 && !acc) || (causal && l > s)) return KUIOPS_E_INVALID;
     const Plan p = plan_of(n, hq, hkv, l, s, e, ev, causal ? kCausal : kFull, true);
-    if (!split_fits(p, s, sk[2], sv[2])) return KUIOPS_E_UNSUPPORTED;
+    if (!plan_fits(p, s, sk[2], sv[2])) return KUIOPS_E_UNSUPPORTED;
     const size_t need = state_bytes(p);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KUIOPS_E_WORKSPACE;
     CacheAttnArgs a = fill_attn(n, hq, hkv, l, s, e, ev, Q, sq, K, sk, V, sv, O, so, lse, scale, causal ? kCausal : kFull,

@@ -41,6 +41,22 @@ def test_a_chain_is_causal_decode_attention():
     np.testing.assert_allclose(acc, 2.0)
 
 
+def test_the_attention_is_torchs():
+    r = np.random.default_rng(1)
+    q, k, v = (r.standard_normal(s) for s in ((2, 4, 9, 8), (2, 2, 9, 8), (2, 2, 9, 6)))
+    wide = [torch.from_numpy(np.repeat(x, 2, 1)) for x in (k, v)]
+    ref = torch.nn.functional.scaled_dot_product_attention(torch.from_numpy(q), *wide, is_causal=True)
+    np.testing.assert_allclose(O.sdpa_decode_accum(q, k, v, np.zeros((2, 2, 9)))[0], ref.numpy(), rtol=1e-10)
+    # a tree's rows: its nodes' keys alone behind the context
+    parent = [-1, 0, 0, 1, -1]
+    mask = torch.zeros(5, 9, dtype=torch.bool)
+    mask[:, :4] = True
+    for i, seen in enumerate(O.tree_sees(parent)):
+        mask[i, [4 + j for j in seen]] = True
+    ref = torch.nn.functional.scaled_dot_product_attention(torch.from_numpy(q[:, :, :5]), *wide, attn_mask=mask)
+    np.testing.assert_allclose(O.sdpa_tree(q[:, :, :5], k, v, [parent] * 2)[0], ref.numpy(), rtol=1e-10)
+
+
 def test_accept_and_commit_by_hand():
     #      0 -> 1, 2; 1 -> 3; 2 -> 4, 5
     parent, tokens, target = [-1, 0, 0, 1, 2, 2], [7, 8, 9, 5, 5, 6], [9, 1, 6, 1, 1, 3]
@@ -206,6 +222,15 @@ def test_c_entries_refuse_on_the_host(lib):
     assert evict(budget=0) == evict(recent=9) == evict(recent=-1) == evict(acc=null) == INVALID
     assert evict(krow=8) == UNSUPPORTED
     assert evict(ws=null) == evict(nb=lib.kuiops_kv_evict_workspace(1, 2, 8) - 1) == _lib.E_WORKSPACE
+
+
+def test_c_entries_refuse_launches_of_2_32_threads(lib):
+    p, null, s3 = ctypes.c_void_p(1 << 20), None, _lib.strides3(0, 0, 512)
+    assert lib.kuiops_sdpa_tree(128, 1 << 15, 1, 256, 300, 256, 256, _lib.BF16, p, s3, p, s3, p, s3, p, s3, null, 0.1, p, null,
+                                null, 0, null) == UNSUPPORTED
+    assert lib.kuiops_tree_accept(1 << 26, 1, p, p, p, p, p, p, null) == UNSUPPORTED
+    assert lib.kuiops_kv_tree_commit(65535, 1, 65535, 40, 512, 512, p, s3, ctypes.c_void_p(1 << 21), _lib.strides3(0, 0, 512), 3, p,
+                                     4, p, ctypes.c_void_p(1 << 22), null) == UNSUPPORTED
 
 
 # ------------------------------------------------------------- custom ops

@@ -127,6 +127,27 @@ def test_sdpa_tree_long_cache_splits(cuda):
         close_lse(lse, lref, terms, 64)
 
 
+@pytest.mark.parametrize("n,hq,hkv,t,s,e,ev,lens,absent,chain", [x for x in TREES if x[1] // x[2] * x[3] > 16 and max(x[5], x[6]) <= 128])
+def test_sdpa_tree_key_groups(cuda, n, hq, hkv, t, s, e, ev, lens, absent, chain):
+    # 128-row kernel with at least 1536 keys a work-group: two groups of waves share them
+    q, k, v = gen((n, hq, t, e), BF, 1), gen((n, hkv, s, e), BF, 2), gen((n, hkv, s, ev), BF, 3)
+    parent = trees(n, t, 4, absent)
+    if chain:           # an infinite value that only the last node sees
+        parent = np.where(parent >= -1, np.arange(t) - 1, parent).astype(np.int32)
+        v[0, 0, (lens or (s,))[0] - 1] = math.inf
+    lens = lens or (s,) * n
+    ref, lref, size, terms = O.sdpa_tree(npy(q), npy(k), npy(v), parent, lens)
+    cap = max(wide_capacity(n, hq, hkv, t, e, ev), 1536 * min(64, 256 // (n * hkv * -(-(hq // hkv * t) // 128))) + 31)
+    out, lse = ops.sdpa_tree(q.to(cuda), padded(k, cap).to(cuda), padded(v, cap).to(cuda), torch.from_numpy(parent).to(cuda),
+                             torch.tensor(lens, dtype=torch.int32, device=cuda), return_lse=True)
+    ok = np.isfinite(ref)
+    assert chain or ok.all()
+    assert (npy(out)[~ok] == math.inf).all()
+    out = torch.where(torch.from_numpy(ok).to(cuda), out, torch.zeros_like(out))
+    close_out(out, np.where(ok, ref, 0), np.where(ok, size, 0), terms, e, True)
+    close_lse(lse, lref, terms, e)
+
+
 @pytest.mark.parametrize("L", [7, 63, 64, 65, 200, 1000, 4097])
 def test_sdpa_tree_splits_of_the_wide_kernel(cuda, L):
     # 128-row kernel, the keys over several work-groups, the tree across block ends
@@ -239,6 +260,7 @@ ACCUM = [  # n, hq, hkv, l, s, e, ev, lens, causal
     (1, 8, 4, 1000, 1000, 64, 64, None, True),            # row groups that end with a head
     (1, 4, 1, 897, 1500, 128, 128, (1400,), True),
     (2, 8, 4, 20, 70, 64, 64, (70, 25), True),
+    (3, 4, 2, 1540, 1600, 64, 64, (1600, 1541, 700), True),     # paired row groups with two key groups
     (1, 2, 1, 700, 700, 256, 256, None, True),            # a tile's rows over two work-groups
 ]
 
