@@ -155,9 +155,9 @@ __global__ __launch_bounds__(kCommitWaves * 64) void tree_commit_kernel(CommitAr
 // order.  Slots of 1024 x IPT keys stay in registers (thread t has t, t + 1024,
 // ...); longer caches are read again (from L2) in each of the six passes.
 // evict_move_kernel moves the rows of K and V (few of them move in the first kernel).
-// What bounds them: a few hundred slots, one work-group's latency (576 keys: 7.4 us with
-// the move); 64 heads of 8000, select 16 us, of it the histograms about half; the moves
-// the memory, 5.9 TB/s read and written.
+// What bounds them: a few hundred slots, one work-group's latency (576 keys: 8.0 us with
+// the move); 64 heads of 8000, select 17.7 us, of it the histograms about half; the moves
+// the memory, 91 MB read and written in 20 us.
 constexpr int kEvictThreads = 1024;
 struct EvictArgs {
     int n, hkv, budget, recent;

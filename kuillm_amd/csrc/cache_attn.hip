@@ -213,7 +213,7 @@ __device__ __forceinline__ void store_row(const CacheAttnArgs &a, int64_t b, int
 //   each (2^-16 of it is lost in bf16, 2^-21 in f16): with the few rows of
 //   this kernel the K / V stream takes the time, not the MFMAs.
 // K needs no LDS because a wave shares its keys with no other; V does, as the MFMA
-// wants 8 keys of a column in a lane.  Measured: 4 sequences of 1000 to 2000 keys, 32 / 32
+// wants 8 keys of a column in a lane.  Measured: 4 sequences of 1153 to 2013 keys, 32 / 32
 // heads of 128, 13 rows: 24.5 us, 4.3 TB/s; 8 rows over 500 keys, one sequence: 7.8 us, all
 // of it latency (key count, query, first keys, three steps of them, waves' merge).
 // A part that is 0 times an infinite value is NaN, so is a masked NaN: a wave
