@@ -156,7 +156,7 @@ __global__ __launch_bounds__(kCommitWaves * 64) void tree_commit_kernel(CommitAr
 // ...); longer caches are read again (from L2) in each of the six passes.
 // evict_move_kernel moves the rows of K and V (few of them move in the first kernel).
 // What bounds them: a few hundred slots, one work-group's latency (576 keys: 8.0 us with
-// the move); 64 heads of 8000, select 17.7 us, of it the histograms about half; the moves
+// the move); 64 heads of 8000, select 13.3 us, of it the histograms about half; the moves
 // the memory, 91 MB read and written in 20 us.
 constexpr int kEvictThreads = 1024;
 struct EvictArgs {
@@ -559,8 +559,12 @@ extern "C" int kuiops_kv_evict(int64_t n, int64_t hkv, int64_t cap, int64_t krow
     const int64_t per = std::max<int64_t>(1, cdiv(2048, n * hkv));
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min(per, cdiv(most, 256))), (unsigned)(n * hkv));
     const dim3 heads((unsigned)(n * hkv)), threads(kEvictThreads);
+    // (slots of registers as the capacity needs: 8000 slots, 16 against 8 per thread 16.1 / 13.3 us;
+    // 2000, 4 against 2 10.9 / 10.0)
     if (cap <= kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<1>), heads, threads, 0, as_stream(stream), a);
+    else if (cap <= 2 * kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<2>), heads, threads, 0, as_stream(stream), a);
     else if (cap <= 4 * kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<4>), heads, threads, 0, as_stream(stream), a);
+    else if (cap <= 8 * kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<8>), heads, threads, 0, as_stream(stream), a);
     else if (cap <= 16 * kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<16>), heads, threads, 0, as_stream(stream), a);
     else hipLaunchKernelGGL((evict_select_kernel<0>), heads, threads, 0, as_stream(stream), a);
     if (!a.move_here) hipLaunchKernelGGL(evict_move_kernel, grid, dim3(256), 0, as_stream(stream), a);
