@@ -574,13 +574,16 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2, 2))
         offK[j] = ck < a.e ? (uint32_t)((r * a.sk2 + ck) * 2) : kOut;
         offV[j] = cv < a.ev ? (uint32_t)((r * a.sv2 + cv) * 2) : kOut;
     }
+    // (the second key group's last block may begin past the last key: its offset is the
+    // descriptor's size then, so every byte of it is past the end, and not beyond, where
+    // what is left of the size would be negative)
     auto issue_k = [&](int kt, char *sk) __attribute__((always_inline)) {
-        const uint32_t kb = (uint32_t)((int64_t)(kt * KG + kg) * KB * a.sk2 * 2);
+        const uint32_t k0 = (uint32_t)((int64_t)(kt * KG + kg) * KB * a.sk2 * 2), kb = KG == 1 ? k0 : min(k0, kbytes);
 #pragma unroll
         for (int j = 0; j < DPW; ++j) dma16_buf(rsK, offK[j], kb, sk + (wave * DPW + j) * 1024);
     };
     auto issue_v = [&](int kt, char *sv) __attribute__((always_inline)) {
-        const uint32_t vb = (uint32_t)((int64_t)(kt * KG + kg) * KB * a.sv2 * 2);
+        const uint32_t v0 = (uint32_t)((int64_t)(kt * KG + kg) * KB * a.sv2 * 2), vb = KG == 1 ? v0 : min(v0, vbytes);
 #pragma unroll
         for (int j = 0; j < DPW; ++j) dma16_buf(rsV, offV[j], vb, sv + (wave * DPW + j) * 1024);
     };
