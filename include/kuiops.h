@@ -712,8 +712,8 @@ KUIOPS_API int kuiops_kv_tree_commit(int64_t batch, int64_t n, int64_t hkv, int6
                           void *K, const int64_t sk[3], void *V, const int64_t sv[3], int64_t p,
                           const int32_t *path, int64_t t, const int32_t *kv_len, int32_t *len_out, void *stream);
 
-/* Decode attention (kuiops_sdpa_decode's semantics: causal queries are the
- * last l of the kv_len[b] keys) that also adds to every key the weight that
+/* Decode attention (kuiops_sdpa_decode's semantics, fp32 weights: causal queries
+ * are the last l of the kv_len[b] keys) that also adds to every key the weight that
  * the queries of its KV head gave it: acc[b][g][j] += sum over the query heads
  * h of group g and positions i of exp(scale q_i k_j - lse_i).  acc: fp32,
  * strides sa = batch, head, unit key stride; keys at kv_len[b] and behind it

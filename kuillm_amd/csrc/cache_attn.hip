@@ -182,9 +182,33 @@ __device__ __forceinline__ Unit unit_of(const CacheAttnArgs &a) {
     return u;
 }
 
+// A probability p as a sum of 16-bit parts, one MFMA each, which keeps fp32's bits.
+//   bf16: three parts, each the leading 8 bits of what is left, cut off: p exactly.
+//   f16: two, rounded: 11 bits, and 11 of a remainder that has 12 and a sign: 2^-23 of
+//   p is lost, and no more than half of f16's smallest step 2^-24 (see Shift).
+template <typename T> struct Parts;
+template <> struct Parts<bf16_t> {
+    static constexpr int N = 3;
+    static __device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+    static __device__ __forceinline__ void split(float p, bf16_t (&x)[N]) {
+        const float h = cut(p), r = p - h, m = cut(r);
+        x[0] = (bf16_t)h;
+        x[1] = (bf16_t)m;
+        x[2] = (bf16_t)(r - m);
+    }
+};
+template <> struct Parts<f16_t> {
+    static constexpr int N = 2;
+    static __device__ __forceinline__ void split(float p, f16_t (&x)[N]) {
+        x[0] = from_f32<f16_t>(p);
+        x[1] = from_f32<f16_t>(p - to_f32(x[0]));
+    }
+};
+
 template <typename T> struct Shift;       // probabilities are relative to 2^(maximum + value)
 template <> struct Shift<bf16_t> { static constexpr float value = 0.f; };       // p <= 2^8 between rescales
-// p <= 2^15, so that f16's smallest step 2^-24 is 2^-39 of it
+// p <= 2^15, and the row's largest is 2^7 at least: f16's smallest step 2^-24 is 2^-39 to
+// 2^-31 of it
 template <> struct Shift<f16_t> { static constexpr float value = -7.f; };
 constexpr float kSlack = 8.f;       // a row's maximum may grow by 2^8 before its sums are rescaled
 
@@ -209,9 +233,10 @@ __device__ __forceinline__ void store_row(const CacheAttnArgs &a, int64_t b, int
 //   holds 8 scores of one row, the row's maximum crosses lanes 16 and 32 apart
 //   only.  O^T += V^T P^T: V through LDS (DMA), read transposed;
 //   the scores' registers are the other operand as they stand, keys numbered
-//   in that order.  The probability is the sum of two 16-bit parts, one MFMA
-//   each (2^-16 of it is lost in bf16, 2^-21 in f16): with the few rows of
-//   this kernel the K / V stream takes the time, not the MFMAs.
+//   in that order.  The probability is the sum of 16-bit parts that keep fp32's
+//   bits, one MFMA each (see Parts): with the few rows of this kernel the K / V
+//   stream takes the time, not the MFMAs (bf16, two parts against three, calls, us: 8
+//   rows over 500 keys 11.1 / 11.1, 16 sequences of 4000 keys with weights 54.5 / 54.6).
 // K needs no LDS because a wave shares its keys with no other; V does, as the MFMA
 // wants 8 keys of a column in a lane.  Measured: 4 sequences of 1153 to 2013 keys, 32 / 32
 // heads of 128, 13 rows: 24.5 us, 4.3 TB/s; 8 rows over 500 keys, one sequence: 7.8 us, all
@@ -223,7 +248,7 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
     constexpr int NWV = 4, KB = 32, R = 16;
     constexpr int RB = HD * 2, VT = KB * RB;          // bytes per V row / wave tile
-    constexpr int KK = HD / 32, DT = HD / 16, DV = VT / 1024;
+    constexpr int KK = HD / 32, DT = HD / 16, DV = VT / 1024, NP = Parts<T>::N;
     typedef typename Mfma<T>::frag frag;
     typedef T t8 __attribute__((ext_vector_type(8)));
     __shared__ __attribute__((aligned(1024))) char sV0[NWV * VT], sV1[NWV * VT];
@@ -362,16 +387,17 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
             m_used = m_new;
         }
         const float mref = m_used == -INFINITY ? 0.f : m_used + Shift<T>::value;
-        t8 hi, lo;
+        t8 part[NP];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float p = fast_exp2(__builtin_fmaf(sc[t][i], a.scale_log2, -mref));
                 l_run += p;
-                const T x = from_f32<T>(p);
-                hi[4 * t + i] = x;
-                lo[4 * t + i] = from_f32<T>(p - to_f32(x));
+                T x[NP];
+                Parts<T>::split(p, x);
+#pragma unroll
+                for (int y = 0; y < NP; ++y) part[y][4 * t + i] = x[y];
             }
         // this step's V tile has landed: only the next step's loads are younger
         constexpr int Y = 2 * KK + DV;
@@ -389,8 +415,8 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
             const s16x4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)to_lds(vb + 16 * RB));
             const u32x2 h0 = __builtin_bit_cast(u32x2, t0), h1 = __builtin_bit_cast(u32x2, t1);
             const frag vf = as_frag<frag>(u32x4{h0[0], h0[1], h1[0], h1[1]});
-            o[dt] = Mfma<T>::m16(vf, __builtin_bit_cast(frag, hi), o[dt]);
-            o[dt] = Mfma<T>::m16(vf, __builtin_bit_cast(frag, lo), o[dt]);
+#pragma unroll
+            for (int y = 0; y < NP; ++y) o[dt] = Mfma<T>::m16(vf, __builtin_bit_cast(frag, part[y]), o[dt]);
         }
     };
 
@@ -505,11 +531,13 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
 // same keys, 64 at a time, K and V through LDS (two stages each, DMA).  32x32x16
 // MFMAs in the same transposed form: a lane holds 32 scores of one row, and its
 // maximum and sum cross lanes 32 apart only.  Step j runs the exponentials of
-// block j between the score MFMAs of block j + 1, then O^T += V^T P^T.  The
-// probability is one 16-bit value here: with this many rows the MFMAs and the
-// softmax's vector instructions bound the kernel, and a second part would cost
-// a third more of the one and a third of the other; each weight is off by at
-// most half a step of the output's type, as the output itself is.
+// block j between the score MFMAs of block j + 1, then O^T += V^T P^T, with the
+// probability's parts (see Parts) one behind the other.  One 16-bit value instead would
+// cost the weights 2^-9 (bf16) and the outputs 1.4 times the error of an fp32
+// product, and which kernel a call runs on would show in its bits; it took, calls, us, one
+// part / two / three in bf16: 256 rows a head over 60000 keys 88 / 112 / 130, 16 sequences
+// of 8000 145 / 188 / 224, 104 rows over 4000 38 / 41.5 / 45; f16, one / two: a 1999-token
+// prompt with weights 61 / 69.
 // With two key groups (KG) 8 waves take blocks 2 j and 2 j + 1 and join their sums
 // through LDS in the end, half the columns each, in a fixed order.
 // Measured: 256 rows per head over 60000 keys, 8 heads of 128: 78 us, 800 TFLOP/s
@@ -523,7 +551,7 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2, 2))
     constexpr int NWV = 4, KB = 64, R = 32 * NWV;
     constexpr int RB = HD * 2, CPR = HD / 8, TILE = KB * RB;
     constexpr int DPW = TILE / 1024 / NWV, RPB = 1024 / RB;
-    constexpr int DT = HD / 32, KS = HD / 16;
+    constexpr int DT = HD / 32, KS = HD / 16, NP = Parts<T>::N;
     typedef typename Mfma<T>::frag frag;
     typedef T t8 __attribute__((ext_vector_type(8)));
     // K rows are read 16 at a time (ds_read_b128), V rows 8 rows x 64 bytes
@@ -697,7 +725,7 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2, 2))
             }
         }
         l_run += rs;
-        constexpr int NV = 4 * DT, VPF = 3;
+        constexpr int NV = 4 * DT, VPF = 2;
         frag vr[VPF];
         auto load_v = [&](int idx, frag &dst) __attribute__((always_inline)) {
             const char *vb = pv + offVr[idx % DT] + idx / DT * 16 * RB;
@@ -708,18 +736,25 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2, 2))
         };
 #pragma unroll
         for (int x = 0; x < VPF - 1; ++x) load_v(x, vr[x]);
-        frag pf;
+        frag pf[NP];
 #pragma unroll
         for (int idx = 0; idx < NV; ++idx) {
             const int b16 = idx / DT;
             if (idx % DT == 0) {
-                t8 p8;
+                t8 p8[NP];
 #pragma unroll
-                for (int x = 0; x < 8; ++x) p8[x] = from_f32<T>(cur[b16 >> 1][8 * (b16 & 1) + x]);
-                pf = __builtin_bit_cast(frag, p8);
+                for (int x = 0; x < 8; ++x) {
+                    T part[NP];
+                    Parts<T>::split(cur[b16 >> 1][8 * (b16 & 1) + x], part);
+#pragma unroll
+                    for (int y = 0; y < NP; ++y) p8[y][x] = part[y];
+                }
+#pragma unroll
+                for (int y = 0; y < NP; ++y) pf[y] = __builtin_bit_cast(frag, p8[y]);
             }
             if (idx + VPF - 1 < NV) load_v(idx + VPF - 1, vr[(idx + VPF - 1) % VPF]);
-            o[idx % DT] = Mfma<T>::m32(vr[idx % VPF], pf, o[idx % DT]);
+#pragma unroll
+            for (int y = 0; y < NP; ++y) o[idx % DT] = Mfma<T>::m32(vr[idx % VPF], pf[y], o[idx % DT]);
         }
     };
 
