@@ -1245,7 +1245,7 @@ Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e
     // 35.6 / 32.3, 128 behind 1920 23.9 / 31.8 / 28.6 / 27.8, 1000 tokens of 14 / 2 heads 47.9 /
     // 38.4 / 58.6 / 42.7; heads of 128, 1999 tokens 104 / 106 / 101 / 92.
     p.kt = p.parts = 1;
-    if (accum && !keep) {
+    if (accum && !keep && s > 0) {
         const int64_t groups32 = n * hkv * cdiv(cdiv(s, 32), 2);
         if (p.hd <= 128 && (groups32 >= 2 * kCUs || (p.hd == 128 && groups32 >= kCUs && rows >= 4096))) p.kt = 2;
         const int64_t pairs = n * hkv * cdiv(cdiv(s, 32 * p.kt), 2), turns = cdiv(rows, 256);

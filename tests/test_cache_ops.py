@@ -263,3 +263,20 @@ def test_custom_ops_have_no_cpu_kernel():
     q, k, v = attn()
     with pytest.raises(NotImplementedError):
         torch.ops.kuiops.sdpa_tree(q, k, v, tree())
+
+
+# ------------------------------------------------------------ empty caches
+
+def test_an_empty_cache_has_a_plan(lib):
+    # rows per KV head below 16, up to 32 (whose maxima and sums are kept, 8 bytes each) and beyond: no
+    # division by the cache's tiles
+    for l, held in ((1, 0), (4, 0), (8, 32 * 8 * 8), (16, 0), (100, 0), (2000, 0)):
+        assert lib.kuiops_sdpa_decode_accum_workspace(1, 32, 8, l, 0, 64, 64) == held
+        assert lib.kuiops_sdpa_tree_workspace(1, 32, 8, l, 0, 64, 64) == 0
+
+
+@pytest.mark.parametrize("l", [1, 8, 16, 100])
+def test_sdpa_decode_accum_of_an_empty_cache_refuses_causal_queries(l):
+    q, k, v = attn(n=1, hq=32, hkv=8, l=l, s=0)
+    refuses(INVALID, ops.sdpa_decode_accum, q, k, v, torch.zeros(1, 8, 0))
+    refuses(UNSUPPORTED, ops.sdpa_decode_accum, q, k, v, torch.zeros(1, 8, 0), causal=False)        # not on a GPU

@@ -82,3 +82,12 @@ def test_weights_keep_the_bits_of_fp32(cuda, n, hq, hkv, t, e, kernel, dtype):
     if kernel == "16 rows" and e < 256:        # what sdpa_decode gives for the same rows
         same, _ = ops.sdpa_decode(q, k, v, scale=scale, kv_len=ends)
         close_bits(same, ref, size)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("hq,l,e", [(8, 5, 64), (8, 9, 128), (8, 100, 64), (2, 300, 256)])
+def test_sdpa_decode_accum_of_an_empty_cache(cuda, hq, l, e, dtype):
+    # 20, 36, 400 and 300 rows a KV head that see no key
+    q, k = gen((2, hq, l, e), dtype, 1).to(cuda), torch.zeros(2, 2, 0, e, dtype=dtype, device=cuda)
+    out, lse = ops.sdpa_decode_accum(q, k, k.clone(), torch.zeros(2, 2, 0, device=cuda), causal=False, return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()
