@@ -163,6 +163,12 @@ __device__ __forceinline__ uint64_t seen_word(const CacheAttnArgs &a, const Tree
     return r;
 }
 
+// How many of the first L keys a row of causal or full attention sees.  Its weights go
+// to them alone: a row of NaN leaves the other keys' sums as they are.
+__device__ __forceinline__ int keys_seen(const CacheAttnArgs &a, int pos, int L) {
+    return a.mode == kCausal ? min(L, L - a.l + pos + 1) : L;
+}
+
 // What a work-group works on: the row groups of a (sequence, KV head, split)
 // run on one XCD, whose L2 then has the keys for all but the first.
 struct Unit {
@@ -253,6 +259,7 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
     typedef T t8 __attribute__((ext_vector_type(8)));
     __shared__ __attribute__((aligned(1024))) char sV0[NWV * VT], sV1[NWV * VT];
     __shared__ float sm[NWV][R], sl[NWV][R], s_max[R], s_inv[R];
+    __shared__ int s_seen[R];
     __shared__ TreeBits tb;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -510,6 +517,7 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
         if (d == 0) {
             s_max[r] = mu;
             s_inv[r] = ll != 0.f ? 1.f / ll : 0.f;
+            s_seen[r] = keys_seen(a, i, L);
         }
     }
     if (!a.sum_here) return;
@@ -521,7 +529,10 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
     float *acc = a.acc + b * a.sa0 + hk * a.sa1;
     for (int key = tid; key < L; key += NWV * 64) {
         float w = 0.f;
-        for (int r = 0; r < rows_kv; ++r) w += s_inv[r] * fast_exp2(__builtin_fmaf(sc[r * a.spad + key], a.scale_log2, -s_max[r]));
+        for (int r = 0; r < rows_kv; ++r) {
+            const float p = s_inv[r] * fast_exp2(__builtin_fmaf(sc[r * a.spad + key], a.scale_log2, -s_max[r]));
+            w += key < s_seen[r] ? p : 0.f;
+        }
         acc[key] += w;
     }
 }
@@ -946,6 +957,7 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256) void accum_merge_kernel(CacheAttnArgs a) {
     constexpr int D4 = HD / 4, RPB = 256 / D4;
     __shared__ float s_m[kScoreRows], s_l[kScoreRows];
+    __shared__ int s_seen[kScoreRows];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int b = blockIdx.y / a.hkv, hk = blockIdx.y % a.hkv;
     const int G = a.hq / a.hkv, rows = G * a.l;
@@ -972,6 +984,7 @@ __global__ __launch_bounds__(256) void accum_merge_kernel(CacheAttnArgs a) {
         if (lane == 0) {
             s_m[r] = mu;
             s_l[r] = ll != 0.f ? 1.f / ll : 0.f;
+            s_seen[r] = keys_seen(a, r % a.l, L);
         }
     }
     // the rows' outputs
@@ -997,7 +1010,10 @@ __global__ __launch_bounds__(256) void accum_merge_kernel(CacheAttnArgs a) {
             if (r + y >= rows) break;
             const float m = s_m[r + y], inv = s_l[r + y];
 #pragma unroll
-            for (int z = 0; z < 2; ++z) w[z] += inv * fast_exp2(__builtin_fmaf(x[y][z], a.scale_log2, -m));
+            for (int z = 0; z < 2; ++z) {
+                const float p = inv * fast_exp2(__builtin_fmaf(x[y][z], a.scale_log2, -m));
+                w[z] += key + z < s_seen[r + y] ? p : 0.f;
+            }
         }
     }
     acc[0] = old[0] + w[0];
@@ -1114,7 +1130,7 @@ __global__ __launch_bounds__(HD <= 128 ? 512 : 256) void key_weights_kernel(Cach
                     __builtin_amdgcn_s_waitcnt((Y & 15) | ((Y >> 4) << 14) | (7 << 4) | (15 << 8));
                     __builtin_amdgcn_sched_barrier(0);
                     // (a row that saw nothing, or none: weight 0)
-                    const float c = ln[z] == -INFINITY ? -INFINITY : -ln[z] * kLog2e;
+                    float c = ln[z] == -INFINITY ? -INFINITY : -ln[z] * kLog2e;
                     const int last = a.mode == kCausal ? first + pn[z] - k0 : KEYS;       // the row's last key here
                     f32x16 sc[KT];
 #pragma unroll
@@ -1124,11 +1140,14 @@ __global__ __launch_bounds__(HD <= 128 ? 512 : 256) void key_weights_kernel(Cach
                         for (int t = 0; t < KT; ++t) sc[t] = Mfma<T>::m32(kf[t][kk], qf, kk == 0 ? f32x16{} : sc[t]);
                     }
                     if (__any(last < KEYS - 1)) {
+                        // (NaN of the row's lse goes to the scores that it sees)
+                        const float bad = c != c ? c : 0.f;
+                        c = c != c ? 0.f : c;
 #pragma unroll
                         for (int t = 0; t < KT; ++t)
 #pragma unroll
                             for (int x = 0; x < 16; ++x)
-                                if (32 * t + 8 * (x >> 2) + 4 * lh + (x & 3) > last) sc[t][x] = -INFINITY;
+                                sc[t][x] = 32 * t + 8 * (x >> 2) + 4 * lh + (x & 3) > last ? -INFINITY : sc[t][x] + bad;
                     }
 #pragma unroll
                     for (int t = 0; t < KT; ++t)

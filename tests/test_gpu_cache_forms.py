@@ -1,5 +1,7 @@
 """Forms of the cache operators that a call reaches by its sizes alone, against
 the fp64 oracle; tolerances as tests/test_gpu_cache.py counts them."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -91,3 +93,38 @@ def test_sdpa_decode_accum_of_an_empty_cache(cuda, hq, l, e, dtype):
     q, k = gen((2, hq, l, e), dtype, 1).to(cuda), torch.zeros(2, 2, 0, e, dtype=dtype, device=cuda)
     out, lse = ops.sdpa_decode_accum(q, k, k.clone(), torch.zeros(2, 2, 0, device=cuda), causal=False, return_lse=True)
     assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n,hq,hkv,l,s,e,bad", [
+    (1, 2, 2, 5, 90, 64, 1),          # one launch: a work-group has all rows and keys of its KV head
+    (2, 4, 2, 8, 1500, 64, 3),        # kept scores, several splits
+    (1, 4, 2, 12, 150, 128, 0),       # kept scores of two row groups
+    (1, 8, 2, 50, 200, 64, 17),       # scores computed again
+    (1, 4, 4, 300, 300, 64, 100),
+    (1, 2, 1, 70, 130, 256, 69),
+    (40, 8, 8, 40, 800, 64, 20),      # tiles of 64 keys
+])
+def test_sdpa_decode_accum_a_row_of_nan_reaches_the_keys_that_it_sees_alone(cuda, n, hq, hkv, l, s, e, bad, dtype):
+    q, k, v = gen((n, hq, l, e), dtype, 1), gen((n, hkv, s, e), dtype, 2), gen((n, hkv, s, e), dtype, 3)
+    head, L = hq - 1, s - 3                       # the last head's row at position `bad`, in sequence 0
+    lens = torch.full((n,), L, dtype=torch.int32, device=cuda)
+    acc = torch.rand(n, hkv, s, generator=torch.Generator().manual_seed(4)).to(cuda)
+    args = k.to(cuda), v.to(cuda)
+    clean, dirty = acc.clone(), acc.clone()
+    ref, _ = ops.sdpa_decode_accum(q.to(cuda), *args, clean, lens)
+    clean_q = q.clone()
+    q[0, head, bad] = math.nan
+    out, lse = ops.sdpa_decode_accum(q.to(cuda), *args, dirty, lens, return_lse=True)
+    assert out[0, head, bad].isnan().all() and lse[0, head, bad].isnan()
+    out[0, head, bad] = ref[0, head, bad]
+    # (a wave with a row of NaN sums its rows again, value by value: other roundings of the same fp32 sums)
+    want, _, _, size, terms = O.sdpa_decode_accum(npy(clean_q[:1]), npy(k[:1]), npy(v[:1]), np.zeros((1, hkv, s)), (L,))
+    close_out(out[:1], want, size, terms, e, False)
+    assert torch.equal(out[1:], ref[1:])
+    sees = L - l + bad + 1
+    assert dirty[0, -1, :sees].isnan().all()
+    # the keys behind lose this row's weight, which is none, and nothing else
+    assert torch.equal(dirty[0, -1, sees:], clean[0, -1, sees:])
+    dirty[0, -1, :sees] = clean[0, -1, :sees]
+    assert torch.equal(dirty, clean)
