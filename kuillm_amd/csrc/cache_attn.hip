@@ -1198,6 +1198,7 @@ struct Plan {
     int64_t units;
     int key_groups;        // cache_rows_kernel: groups of 4 waves
     int kt, parts;         // key_weights_kernel: 32-key blocks of a tile, work-groups of a tile
+    int64_t weight_groups; // its work-groups of a KV head, 0 without it
     size_t o_bytes, ml_bytes, score_bytes, part_bytes;        // of the workspace
 };
 
@@ -1270,6 +1271,7 @@ Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e
         const int64_t pairs = n * hkv * cdiv(cdiv(s, 32 * p.kt), 2), turns = cdiv(rows, 256);
         p.parts = (int)std::max<int64_t>(1, std::min({(int64_t)8, kCUs / pairs, turns / 2}));
         if (p.parts > 1) p.part_bytes = (size_t)p.parts * n * hkv * (cdiv(s, 32) * 32) * 4;
+        p.weight_groups = cdiv(cdiv(s, 32 * p.kt), 2) * p.parts;
     }
     return p;
 }
@@ -1279,7 +1281,7 @@ size_t state_bytes(const Plan &p) { return p.o_bytes + p.score_bytes + p.ml_byte
 template <typename T, int HD>
 void launch_weights(const CacheAttnArgs &a, const Plan &p, hipStream_t st) {
     const unsigned heads = (unsigned)(a.n * a.hkv), tiles = (unsigned)cdiv(a.s, 32 * p.kt);
-    const dim3 grid((tiles + 1) / 2 * p.parts, heads), threads(HD <= 128 ? 512 : 256);
+    const dim3 grid((unsigned)p.weight_groups, heads), threads(HD <= 128 ? 512 : 256);
     if constexpr (HD <= 128) {
         if (p.kt == 2) hipLaunchKernelGGL((key_weights_kernel<T, HD, 2>), grid, threads, 0, st, a, (int)tiles, p.parts);
     }
@@ -1337,7 +1339,8 @@ int check_attn(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t
 // launch has fewer than 2^32 threads.
 bool plan_fits(const Plan &p, int64_t s, int64_t sk2, int64_t sv2) {
     const int64_t chunk = (cdiv(cdiv(s, 32), (int64_t)p.splits * 4) * 4 + 8) * 32;
-    return chunk * std::max(sk2, sv2) * 2 + 1024 < ((int64_t)1 << 31) && cdiv(p.units, 8) * 8 * p.row_groups < ((int64_t)1 << 24);
+    return chunk * std::max(sk2, sv2) * 2 + 1024 < ((int64_t)1 << 31) && cdiv(p.units, 8) * 8 * p.row_groups < ((int64_t)1 << 24) &&
+           p.weight_groups * (p.hd <= 128 ? 512 : 256) < ((int64_t)1 << 32);
 }
 
 CacheAttnArgs fill_attn(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev, const void *Q,
