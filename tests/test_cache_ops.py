@@ -286,9 +286,10 @@ def test_sdpa_decode_accum_of_an_empty_cache_refuses_causal_queries(l):
 
 @pytest.mark.parametrize("e", [64, 128, 256])
 def test_weights_of_caches_past_a_launch_are_refused_before_anything_runs(lib, e):
-    # rows of 8 read as heads of e: 2^30 - 64 keys have more tiles than a launch of 2^32 threads
+    # rows of 8 read as heads of e: pairs of 32- or 64-key tiles, 512 threads each, or 256 at head dim 256: 2^24 of
+    # those for 2^30 - 1 keys (one less, and a launch that fits, for 2^30 - 64)
     p, null, s3, s2 = ctypes.c_void_p(1 << 20), None, _lib.strides3(0, 0, 8), _lib.strides3(0, 0, 0)
     for l in (40, 100):
-        got = lib.kuiops_sdpa_decode_accum(1, 1, 1, l, (1 << 30) - 64, e, e, _lib.BF16, p, s3, p, s3, p, s3, p, s3, p, 0.1, 1, null, p, s2,
+        got = lib.kuiops_sdpa_decode_accum(1, 1, 1, l, (1 << 30) - 1, e, e, _lib.BF16, p, s3, p, s3, p, s3, p, s3, p, 0.1, 1, null, p, s2,
                                            p, 1 << 50, null)
         assert got == UNSUPPORTED
