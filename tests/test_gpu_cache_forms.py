@@ -8,7 +8,8 @@ import torch
 
 from kuillm_amd import ops
 from oracle import kuiops_oracle as O
-from test_gpu_cache import BF, HF, close_lse, close_out, gen, npy, padded, trees, wide_capacity
+from test_gpu_cache import (ACCUM, BF, HF, TREES, close_lse, close_out, gen, npy, padded, score_error, trees,
+                            wide_capacity)
 
 pytestmark = pytest.mark.gpu
 
@@ -128,3 +129,144 @@ def test_sdpa_decode_accum_a_row_of_nan_reaches_the_keys_that_it_sees_alone(cuda
     assert torch.equal(dirty[0, -1, sees:], clean[0, -1, sees:])
     dirty[0, -1, :sees] = clean[0, -1, :sees]
     assert torch.equal(dirty, clean)
+
+
+# The lists of test_gpu_cache.py on the 128-row kernel, at the tolerance of weights that keep fp32's bits.
+
+def wide_cases(cases):
+    return [c for c in cases if c[1] // c[2] * c[3] > 16 and max(c[5], c[6]) <= 128]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n,hq,hkv,t,s,e,ev,lens,absent,chain", wide_cases(TREES))
+def test_sdpa_tree_128_rows(cuda, n, hq, hkv, t, s, e, ev, lens, absent, chain, dtype):
+    q, k, v = gen((n, hq, t, e), dtype, 1), gen((n, hkv, s, e), dtype, 2), gen((n, hkv, s, ev), dtype, 3)
+    parent, lens = trees(n, t, 4, absent), lens or (s,) * n
+    ref, lref, size, terms = O.sdpa_tree(npy(q), npy(k), npy(v), parent, lens)
+    cap = wide_capacity(n, hq, hkv, t, e, ev)
+    out, lse = ops.sdpa_tree(q.to(cuda), padded(k, cap).to(cuda), padded(v, cap).to(cuda), torch.from_numpy(parent).to(cuda),
+                             torch.tensor(lens, dtype=torch.int32, device=cuda), return_lse=True)
+    close_out(out, ref, size, terms, e, False)
+    close_lse(lse, lref, terms, e)
+
+
+def close_sums(got, ref, start, rows, terms, e):
+    grown = ref - start
+    tol = grown * (4 * score_error(e, terms) + 2.0 ** -19 + rows * 2.0 ** -24) + 2.0 ** -23 * np.abs(ref)
+    assert (np.abs(npy(got) - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n,hq,hkv,l,s,e,ev,lens,causal", wide_cases(ACCUM))
+def test_sdpa_decode_accum_128_rows(cuda, n, hq, hkv, l, s, e, ev, lens, causal, dtype):
+    q, k, v = gen((n, hq, l, e), dtype, 1), gen((n, hkv, s, e), dtype, 2), gen((n, hkv, s, ev), dtype, 3)
+    lens, cap = lens or (s,) * n, max(s, wide_capacity(n, hq, hkv, l, e, ev))
+    k, v = padded(k, cap), padded(v, cap)
+    acc = torch.rand(n, hkv, cap, generator=torch.Generator().manual_seed(4))
+    got = acc.to(cuda)
+    out, lse = ops.sdpa_decode_accum(q.to(cuda), k.to(cuda), v.to(cuda), got, torch.tensor(lens, dtype=torch.int32, device=cuda),
+                                     causal=causal, return_lse=True)
+    ref, lref, aref, size, terms = O.sdpa_decode_accum(npy(q), npy(k), npy(v), npy(acc), lens, causal=causal)
+    close_out(out, ref, size, terms, e, False)
+    close_lse(lse, lref, terms, e)
+    close_sums(got, aref, npy(acc), hq // hkv * l, terms, e)
+    for b in range(n):
+        assert torch.equal(got[b, :, lens[b]:].cpu(), acc[b, :, lens[b]:])
+
+
+def head_on_device(q, k, v, causal):
+    """One KV head in 64 bits on the device: q (G, l, e), k / v (L, e) -> out, lse, sums of the weights per key, sums
+    of absolute output terms, the largest sum of absolute score terms."""
+    G, l, e = q.shape
+    rows, L = q.double().reshape(G * l, e), k.shape[0]
+    x = rows @ k.double().t().contiguous() / math.sqrt(e)
+    terms = float((rows.abs() @ k.double().abs().t().contiguous()).max()) / math.sqrt(e) if L else 0.0
+    if causal:
+        at = torch.arange(l, device=q.device).repeat(G)[:, None] + L - l
+        x.masked_fill_(torch.arange(L, device=q.device)[None] > at, -math.inf)
+    lse = torch.logsumexp(x, 1)
+    w = (x - torch.where(lse > -math.inf, lse, 0.0)[:, None]).exp_()
+    return ((w @ v.double()).view(G, l, -1), lse.view(G, l), w.sum(0), (w @ v.double().abs()).view(G, l, -1), terms)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n,hq,hkv,l,s,e,lens,causal", [
+    # paired row groups, one group of waves: 3 groups (the middle one alone), and 4
+    (8, 8, 8, 320, 450, 64, (450, 449, 320, 385, 1, 400, 333, 384), True),
+    (8, 8, 8, 400, 460, 128, (460, 459, 400, 385, 384, 123, 0, 257), True),
+    # the same at 1600 keys, with as many work-groups as keep one group of waves; two prompts, by heads
+    (14, 8, 8, 513, 1600, 64, tuple(1600 - 91 * b for b in range(14)), True),
+    (2, 32, 8, 1999, 2036, 64, (1999, 2001), True),
+    # paired row groups, two groups of waves, and 64-key tiles whose rows two work-groups share
+    (1, 32, 8, 1999, 2036, 128, (1999,), True),
+    (1, 32, 1, 128, 16384, 128, (15001,), True),
+    # 32-key tiles whose rows three work-groups share
+    (1, 32, 8, 512, 550, 64, (540,), True),
+    # 64-key tiles, both of a work-group's live: 5 and 3 tiles, the middle one alone
+    (16, 8, 8, 40, 260, 64, (260, 257, 256, 193, 192, 129, 128, 65, 64, 40, 3, 0, 100, 200, 250, 259), True),
+    (22, 8, 8, 33, 190, 128, tuple(190 - 8 * b for b in range(22)), False),
+])
+def test_sdpa_decode_accum_forms(cuda, n, hq, hkv, l, s, e, lens, causal, dtype):
+    q, k, v = (gen(x, dtype, i).to(cuda) for i, x in enumerate(((n, hq, l, e), (n, hkv, s, e), (n, hkv, s, e))))
+    acc = torch.rand(n, hkv, s, generator=torch.Generator().manual_seed(4)).to(cuda)
+    got, G = acc.clone(), hq // hkv
+    out, lse = ops.sdpa_decode_accum(q, k, v, got, torch.tensor(lens, dtype=torch.int32, device=cuda), causal=causal, return_lse=True)
+    for b, L in enumerate(lens):
+        for h in range(hkv):
+            heads = slice(h * G, (h + 1) * G)
+            ref, lref, sums, size, terms = head_on_device(q[b, heads], k[b, h, :L], v[b, h, :L], causal)
+            close_out(out[b, heads], npy(ref), npy(size), terms, e, False)
+            close_lse(lse[b, heads], npy(lref), terms, e)
+            want = acc[b, h].double()
+            want[:L] += sums
+            close_sums(got[b, h], npy(want), npy(acc[b, h]), G * l, terms, e)
+            assert torch.equal(got[b, h, L:], acc[b, h, L:])
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("kind", ["random", "ties"])
+@pytest.mark.parametrize("cap,lens,budget,recent", [
+    (8192, (8192, 5000), 2048, 64), (8193, (8193, 8192), 4000, 0), (12000, (11999, 9000), 1000, 1000),
+    (16384, (16384, 16383), 8192, 128), (16384, (16384, 16384), 1, 0), (16385, (16385, 16000), 8192, 128), (20000, (20000, 600), 333, 7),
+])
+def test_kv_evict_of_long_caches(cuda, cap, lens, budget, recent, kind, inplace):
+    # 8 and 16 slots a thread in registers, and slots read again in every pass
+    n, hkv, g = 2, 2, np.random.default_rng(cap)
+    acc = (g.random((n, hkv, cap)) ** 4 * 10).astype(np.float32)
+    if kind == "ties":
+        acc = np.floor(acc)
+        acc[acc == 1] = -0.0
+    pos = np.stack([[g.permutation(cap) for _ in range(hkv)] for _ in range(n)]).astype(np.int32)
+    k, v = g.integers(0, 99, (n, hkv, cap, 8)).astype(np.float32), g.integers(0, 99, (n, hkv, cap, 16)).astype(np.float32)
+    ref = O.kv_evict(k, v, acc, pos, lens, budget, recent)
+    d = [torch.from_numpy(x).to(cuda) for x in (k, v, acc, pos, np.array(lens, np.int32))]
+    outs = {} if inplace else dict(acc_out=torch.full_like(d[2], 7), pos_out=torch.full_like(d[3], 7), len_out=torch.full_like(d[4], 7))
+    got = ops.kv_evict(*d, budget, recent, **outs)
+    for a, r in zip((d[0], d[1], *got), ref):
+        np.testing.assert_array_equal(a.cpu().numpy(), r)
+
+
+def test_in_place_operators_through_a_compiled_function(cuda):
+    # functionalised by the tracer: what the calls change has to come out as the direct calls leave it
+    from kuillm_amd import library  # noqa: F401
+    op = torch.ops.kuiops
+
+    def serve(q, k, v, acc, pos, lens, path):
+        ends = op.kv_tree_commit(k, v, path, lens, 5)
+        out, lse = op.sdpa_decode_accum(q, k, v, acc, ends)
+        op.kv_evict(k, v, acc, pos, ends, 20, 4)
+        return out, lse, ends, acc * 2
+
+    def state():
+        q, k, v = (x.to(cuda) for x in (gen((2, 4, 1, 64), BF, 1), gen((2, 2, 60, 64), BF, 2), gen((2, 2, 60, 64), BF, 3)))
+        acc = torch.rand(2, 2, 60, generator=torch.Generator().manual_seed(4)).to(cuda)
+        pos = torch.arange(60, dtype=torch.int32, device=cuda).repeat(2, 2, 1)
+        path = torch.tensor([[0, 2, 4, -1, -1], [0, 1, -1, -1, -1]], dtype=torch.int32, device=cuda)
+        return q, k, v, acc, pos, torch.tensor([60, 33], dtype=torch.int32, device=cuda), path
+    traced = torch.compile(serve, backend="aot_eager", fullgraph=True)
+    for _ in range(2):
+        mine, theirs = state(), state()
+        for a, b in zip(serve(*mine), traced(*theirs)):
+            assert torch.equal(a, b)
+        for a, b in zip(mine, theirs):
+            assert torch.equal(a, b)
