@@ -496,7 +496,7 @@ extern "C" int kuiops_kv_tree_commit(int64_t batch, int64_t n, int64_t hkv, int6
                                      const int32_t *path, int64_t t, const int32_t *kv_len, int32_t *len_out, void *stream) {
     if (batch < 0 || n < 0 || hkv < 0 || cap < 0 || p < 0 || t <= 0 || !sk || !sv) return KUIOPS_E_INVALID;
     if (n == 0 || batch == 0) return batch == n ? KUIOPS_OK : KUIOPS_E_INVALID;
-    if (batch % n || hkv == 0 || !path || !kv_len || !len_out || len_out == kv_len) return KUIOPS_E_INVALID;
+    if (batch % n || hkv == 0 || (p > 0 && !path) || !kv_len || !len_out || len_out == kv_len) return KUIOPS_E_INVALID;
     if (cap > 0 && (!K || !V || K == V)) return KUIOPS_E_INVALID;
     if (p > t) return KUIOPS_E_INVALID;
     if (p > kMaxTree || batch > 65535 || hkv > 65535 || cap >= ((int64_t)1 << 31)) return KUIOPS_E_UNSUPPORTED;

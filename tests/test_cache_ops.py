@@ -293,3 +293,13 @@ def test_weights_of_caches_past_a_launch_are_refused_before_anything_runs(lib, e
         got = lib.kuiops_sdpa_decode_accum(1, 1, 1, l, (1 << 30) - 1, e, e, _lib.BF16, p, s3, p, s3, p, s3, p, s3, p, 0.1, 1, null, p, s2,
                                            p, 1 << 50, null)
         assert got == UNSUPPORTED
+
+
+def test_kv_tree_commit_of_a_path_without_entries(lib):
+    # nothing was accepted: no path to read, so none is asked for; the call goes as far as the device
+    p, q, null, r3 = ctypes.c_void_p(1 << 20), ctypes.c_void_p(1 << 21), None, _lib.strides3(0, 0, 128)
+    for entries, status in ((3, INVALID), (0, UNSUPPORTED)):
+        # (rows of 120 bytes: refused behind the check of the path)
+        assert lib.kuiops_kv_tree_commit(1, 1, 2, 40, 120, 128, p, r3, q, r3, entries, null, 4, p, q, null) == status
+    _, k, v = attn()
+    refuses(UNSUPPORTED, ops.kv_tree_commit, k, v, torch.zeros(2, 0, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 3)

@@ -270,3 +270,11 @@ def test_in_place_operators_through_a_compiled_function(cuda):
             assert torch.equal(a, b)
         for a, b in zip(mine, theirs):
             assert torch.equal(a, b)
+
+
+def test_kv_tree_commit_of_a_path_without_entries(cuda):
+    k = torch.randn(2, 2, 30, 64, device=cuda).to(BF)
+    kd, vd = k.clone(), k.clone()
+    lens = torch.tensor([20, 3], dtype=torch.int32, device=cuda)
+    ends = ops.kv_tree_commit(kd, vd, torch.zeros(2, 0, dtype=torch.int32, device=cuda), lens, 7)
+    assert ends.tolist() == [13, 3] and torch.equal(kd, k) and torch.equal(vd, k)
