@@ -153,11 +153,13 @@ __global__ __launch_bounds__(kCommitWaves * 64) void tree_commit_kernel(CommitAr
 // one as of the other, and the i-th kept row goes to the i-th freed slot.  Sources
 // are at or behind the budget and destinations below it, so the moves need no
 // order.  Slots of 1024 x IPT keys stay in registers (thread t has t, t + 1024,
-// ...); longer caches are read again (from L2) in each of the six passes.
+// ...); longer caches are read again (from L2) in each of the five passes (newest
+// position, three digits, ranks).
 // evict_move_kernel moves the rows of K and V (few of them move in the first kernel).
-// What bounds them: a few hundred slots, one work-group's latency (576 keys: 8.0 us with
-// the move); 64 heads of 8000, select 13.3 us, of it the histograms about half; the moves
-// the memory, 91 MB read and written in 20 us.
+// What bounds them: a few hundred slots, one work-group's latency (576 keys: 8.2 us with
+// the move); 64 heads of 8000, select 15 us (13.3 with the slots in L2), of it the
+// histograms about half, on 64 of the 256 CUs; the moves, 91 MB read and written in 20 us,
+// 4.5 TB/s: row by row they stay 12% below a large copy.
 constexpr int kEvictThreads = 1024;
 struct EvictArgs {
     int n, hkv, budget, recent;
@@ -560,7 +562,8 @@ extern "C" int kuiops_kv_evict(int64_t n, int64_t hkv, int64_t cap, int64_t krow
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min(per, cdiv(most, 256))), (unsigned)(n * hkv));
     const dim3 heads((unsigned)(n * hkv)), threads(kEvictThreads);
     // (slots of registers as the capacity needs: 8000 slots, 16 against 8 per thread 16.1 / 13.3 us;
-    // 2000, 4 against 2 10.9 / 10.0)
+    // 2000, 4 against 2 10.9 / 10.0, the same slots over and over; the device lengths may be
+    // far below the capacity, which the host cannot see)
     if (cap <= kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<1>), heads, threads, 0, as_stream(stream), a);
     else if (cap <= 2 * kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<2>), heads, threads, 0, as_stream(stream), a);
     else if (cap <= 4 * kEvictThreads) hipLaunchKernelGGL((evict_select_kernel<4>), heads, threads, 0, as_stream(stream), a);

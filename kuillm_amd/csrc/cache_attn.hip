@@ -245,7 +245,7 @@ __device__ __forceinline__ void store_row(const CacheAttnArgs &a, int64_t b, int
 //   rows over 500 keys 11.1 / 11.1, 16 sequences of 4000 keys with weights 54.5 / 54.6).
 // K needs no LDS because a wave shares its keys with no other; V does, as the MFMA
 // wants 8 keys of a column in a lane.  Measured: 4 sequences of 1153 to 2013 keys, 32 / 32
-// heads of 128, 13 rows: 24.5 us, 4.3 TB/s; 8 rows over 500 keys, one sequence: 7.8 us, all
+// heads of 128, 13 rows: 24.7 us, 4.2 TB/s; 8 rows over 500 keys, one sequence: 7.9 us, all
 // of it latency (key count, query, first keys, three steps of them, waves' merge).
 // A part that is 0 times an infinite value is NaN, so is a masked NaN: a wave
 // whose sums are not finite goes over its keys again with the row maxima that
@@ -551,12 +551,15 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
 // prompt with weights 61 / 69.
 // With two key groups (KG) 8 waves take blocks 2 j and 2 j + 1 and join their sums
 // through LDS in the end, half the columns each, in a fixed order.
-// Measured: 256 rows per head over 60000 keys, 8 heads of 128: 78 us, 800 TFLOP/s
-// and 3.1 TB/s; with all blocks in L2 it takes as long, and the MFMA pipes are
-// busy 36% of the time with one or two waves a SIMD: a step of 64 keys is 1024 cycles of MFMA
-// and about 900 of exponentials and other vector instructions, which overlap only in
-// part.  Deeper prefetch from LDS changed nothing; 512 registers and one wave a SIMD cost
-// 15 to 35% (accumulators copied to and fro).
+// Measured: 256 rows per head over 60000 keys, 8 heads of 128: 126 us, 500 TFLOP/s of the
+// two products and 2.0 TB/s.  What bounds it: a step of 64 keys is 2048 cycles of MFMA
+// (three parts; f16's two: 1536) and about 1200 of exponentials, maxima and the parts'
+// splitting, and every wave reads all 32 KB of the step's K and V from LDS for its 32
+// rows.  They overlap only in part, as the step's one barrier keeps all waves in the same
+// phase: the MFMA pipes are busy 50% of the time (bf16, two key groups; f16 at head dim 64
+// 29%), the waves wait 31%.  Found with one part: with all blocks in L2 it took as long,
+// deeper prefetch from LDS changed nothing, 512 registers and one wave a SIMD cost 15 to
+// 35% (accumulators copied to and fro).
 template <typename T, int HD, int KG>
 __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2, 2))) void cache_rows_kernel(CacheAttnArgs a) {
     constexpr int NWV = 4, KB = 64, R = 32 * NWV;
@@ -950,7 +953,7 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
 // accum_merge_kernel -- the weights of a few rows' keys from the scores that
 // cache_attn_kernel kept, and the merge of its splits: a work-group has 512 keys
 // of a KV head and its share of the rows' outputs.  (Writing and reading the
-// scores costs 8 bytes a row and key, reading K again 2 e a key.)  7.1 us for 16 sequences
+// scores costs 8 bytes a row and key, reading K again 2 e a key.)  7.9 us for 16 sequences
 // of 8 heads, 4 rows, 4000 keys: of which 8 MB of scores take about 2.
 constexpr int kScoreRows = 32;
 template <typename T, int HD>
@@ -1029,9 +1032,13 @@ __global__ __launch_bounds__(256) void accum_merge_kernel(CacheAttnArgs a) {
 // memory into the operand's lanes, 16 bytes of 32 rows each, their addresses alone
 // took three times the arithmetic's time.  A work-group takes tiles p and last - p:
 // causal keys are seen by the fewer rows the later they are, and two such tiles
-// always by about as many.  What bounds it: the exponentials (a turn of 32 rows and 64
-// keys, head dim 64: about 770 cycles of vector instructions, 256 of MFMA), and for
-// 32-key tiles the rows' traffic from L2, 8 to 10 TB/s.  With `parts` > 1 that many
+// always by about as many.  What bounds it: waiting and the exponentials (a turn of 32
+// rows and 64 keys, head dim 64: about 770 cycles of vector instructions, 256 of MFMA), and
+// for 32-key tiles the rows' traffic from L2, 8 to 10 TB/s.  Waves wait 42% of their cycles:
+// the turns' lse values are loads kept in registers across turns, and for the last of a
+// group of NS turns the compiler waits for all loads, the next stages' DMA with them; the
+// counted wait holds for the others.  33 us for a 1999-token prompt of 32 / 8 heads of 64,
+// f16.  With `parts` > 1 that many
 // work-groups share a tile's rows, and sum_parts_kernel adds up their sums.
 template <typename T, int HD, int KT>
 __global__ __launch_bounds__(HD <= 128 ? 512 : 256) void key_weights_kernel(CacheAttnArgs a, int tiles, int parts) {
@@ -1205,12 +1212,14 @@ struct Plan {
 // Which kernel.  16-row groups are several work-groups for more rows, each of
 // which reads the keys (from L2 behind the first), which fills the GPU soonest;
 // 128-row ones read them once and do far less per row.  The 16-row form wins up
-// to about 2^25 = (KV heads x 16-row groups x keys x head dim).  Measured around
-// it, us, best split counts, 16 against 128 rows: head dim 128, 8 KV heads, 256
-// rows, 2048 / 4096 keys 19.5 / 20.0 and 28.3 / 24.7; 32 heads, 64 rows, 1024 / 4096
-// 14.6 / 15.6 and 29.1 / 22.4; head dim 64, 32 heads, 256 rows, 1024 / 2048 15.1 / 16.4
-// and 23.3 / 19.2; 8 heads, 32 rows, 256 keys 6.1 / 8.3; 64 heads, 64 rows, 4000 keys
-// of 128 42.4 / 30.5.
+// to about 2^25 = (KV heads x 16-row groups x keys x head dim).  Measured around it, us
+// with the merge, best split counts, 16 against 128 rows, bf16: head dim 128, 8 KV heads, 256
+// rows, 1024 / 2048 / 4096 keys 15.3 / 19.6, 19.7 / 23.3 and 29.7 / 27.4; 32 heads, 64 rows, the
+// same keys 15.6 / 18.4, 20.7 / 22.0 and 30.0 / 28.1; 64 heads, 64 rows, 1024 and 4000 keys 17.2 /
+// 22.2 and 43.5 / 41.0; 16 heads, 104 rows, 3000 keys 24.7 / 23.7; head dim 64, 32 heads, 256 rows,
+// 512 / 1024 / 2048 10.4 / 15.1, 15.1 / 19.2 and 24.3 / 21.8; 8 heads, 32 rows, 256 keys of 128 9.4 /
+// 12.3.  f16's two parts: 128 rows 0 to 4 us less.  Rows that fill a quarter of a 128-row group
+// cross later: 64 heads, 32 rows, 4000 and 8000 keys of 128 31.2 / 33.3 and 62.5 / 62.2.
 //
 // How many splits.  About one work-group per CU (of 16-row ones twice that while each
 // still has 2048 keys), of at
@@ -1222,11 +1231,15 @@ struct Plan {
 //
 // How many key groups.  A 128-row work-group that has a CU for itself takes the keys
 // with two groups of 4 waves, unless its keys are few, as the second group's first
-// loads and the joining of the sums take their time: one / two groups, kernel alone, 16 row
-// groups over 60000 keys of 128 in 16 splits 83.4 / 78.2; a 1999-token prompt, 32 / 8
-// heads of 64 39.5 / 35.7; 64 row groups, 1000 keys each 33.4 / 36.0; 256 row groups of 8000
-// keys 163 / 145 (one group and two splits 137 and 12 of merge).  With more work-groups
-// two of them share a CU: 512 of 4000 keys 137 / 150.
+// loads and the joining of the sums take their time.  One / two groups, us with the merge,
+// at 700, 1000, 1300, 1600, 2000, 2600 and 4000 keys a work-group: bf16, 16 row groups in 16
+// splits, 256 rows a head, of 128: 40.3 / 41.5, 47.8 / 47.7, 55.9 / 56.7, 64.0 / 63.3, 78.8 / 76.0, 100 / 94,
+// 143 / 136; 104 rows a head: 36.1 / 39.6, 45.6 / 47.2, 56.4 / 58.8, 67.0 / 67.4, 84.0 / 77.8, 105 / 98, 154 /
+// 149; 64 row groups in 4 splits, 35.2 / 37.4 to 57.2 / 58.5, 69.7 / 70.2, 90.5 / 87.5, 134 / 129;
+// head dim 64, 16 row groups: 27.0 / 26.7, 31.1 / 29.9, 36.1 / 35.1, 41.1 / 38.8 to 83.2 / 75.0; f16
+// alike (two groups gain up to 17% at 4000 keys of 64).  So they are equal near 1600 at head
+// dim 128 and near 700 at 64, where one group costs 9% at most up to the limit.  With more
+// work-groups two of them share a CU: 512 of 4000 keys, one part, 137 / 150.
 constexpr int kCUs = 256;
 Plan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t s, int64_t e, int64_t ev, int mode, bool accum) {
     Plan p{};
