@@ -60,7 +60,8 @@ typedef enum kuiops_dtype {
     KUIOPS_I16 = 6,
     KUIOPS_I8 = 7,
     KUIOPS_U8 = 8,
-    KUIOPS_BOOL = 9
+    KUIOPS_BOOL = 9,
+    KUIOPS_F8E4M3 = 10         /* paged caches only                          */
 } kuiops_dtype;
 
 /* Storage of the [K, N] right-hand operand B of a GEMM.
@@ -745,6 +746,71 @@ KUIOPS_API int kuiops_kv_evict(int64_t n, int64_t hkv, int64_t cap, int64_t krow
                     const int32_t *pos, const int64_t sp[2], const int32_t *kv_len, int64_t budget,
                     int64_t recent, float *acc_out, const int64_t sao[2], int32_t *pos_out, const int64_t spo[2],
                     int32_t *len_out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------ paged KV caches --
+ * No reference counterpart: its app keeps one contiguous cache per sequence
+ * (infer.py:57-89).  Sequences share a pool of pages: slot j of sequence b is
+ * row j % page of page table[b][j / page].  A table entry outside 0 .. pages - 1
+ * is no page: what would be stored there is dropped, it reads as zeros, and
+ * attention does not see its slots.
+ *
+ * The layout (host memory, read during the call): K / V elements of `dtype` at
+ * page * s[0] + head * s[1] + row * s[2], rows of hd contiguous ones that do not
+ * overlap; fp32 scales of 8-bit pages at page * ss[0] + head * ss[1] + row; table
+ * (device int32) rows of `width` entries, ld_table apart.  dtype BF16, F16, or
+ * I8 / F8E4M3: a row is then scale * stored, scale = max |x| / M, stored =
+ * nearest(x M / max |x|) with ties to even, M = 127 / 448, and a row with a NaN
+ * or an infinity reads back as NaN.  hd: multiples of 16 up to 128; page:
+ * multiples of 16 up to 2^20; width * page below 2^30.  K, V and the scales 16-byte
+ * aligned, strides multiples of 16 bytes, row strides below 2^24.            */
+typedef struct kuiops_paged_layout {
+    int64_t pages, page, hkv, hd, width, ld_table;
+    int64_t sk[3], sv[3], sks[2], svs[2];
+    int dtype;
+} kuiops_paged_layout;
+
+/* Per-head norm and rotation of new tokens, and their store into the pages.
+ * qkv: [n][t] rows of (hq + 2 hkv) * hd elements (q heads, k heads, v heads) at
+ * b * ld_batch + i * ld_tok.  Token i of sequence b goes to slot and position
+ * pos0[b] + i (device int32[n], null: 0); slots outside the table are dropped.
+ * lens (device int32[n], taken as 0 .. t; null: t): tokens i >= lens[b] are not
+ * there: nothing of them is read or stored and their q_out is 0.  Queries and keys
+ * become y = x * rsqrt(mean(x^2) + eps) * w with the weights q_norm / k_norm
+ * ([hd], of dtype; null: y = x), then turn by the angles pos * inv_freq[i]: the
+ * pairs (y_i, y_{i + hd/2}) -> (y_i cos - y_{i+hd/2} sin, y_{i+hd/2} cos + y_i
+ * sin), angles in 64 bits, one rounding at the end.  q_out: strides sq = batch,
+ * head, token.  Slots that receive a token must not be named by two sequences'
+ * tables.  dtype BF16 / F16, equal to the pages' unless those are of 8 bits.     */
+KUIOPS_API int kuiops_kv_paged_append(int64_t n, int64_t t, int64_t hq, int dtype, const void *qkv, int64_t ld_tok,
+                           int64_t ld_batch, const int32_t *lens, const int32_t *pos0, const float *inv_freq,
+                           const void *q_norm, const void *k_norm, double eps, void *q_out, const int64_t sq[3],
+                           const kuiops_paged_layout *at, void *K, void *V, float *k_scale, float *v_scale,
+                           const int32_t *table, void *stream);
+
+/* The first min(s, kv_len[b]) slots (kv_len: device int32[n], taken as 0 .. width *
+ * page) gathered into k_out / v_out (strides batch, head, slot; contiguous rows).
+ * Rows behind them are left as they are, or become 0 with `fill`.  dtype: that of
+ * 16-bit pages; BF16, F16 or F32 for 8-bit ones (stored * scale, one rounding).   */
+KUIOPS_API int kuiops_kv_paged_read(int64_t n, int64_t s, int dtype, const kuiops_paged_layout *at, const void *K,
+                         const void *V, const float *k_scale, const float *v_scale, const int32_t *table,
+                         const int32_t *kv_len, void *k_out, const int64_t sko[3], void *v_out,
+                         const int64_t svo[3], int fill, void *stream);
+
+/* Attention of the newest tokens over the pages: query i of sequence b is slot
+ * kv_len[b] - l + i and sees the slots up to its own that have a page (none: output
+ * 0, lse -inf).  What lies elsewhere in the pages, NaN and infinities included,
+ * stays out of it.  kv_len: device int32[n], taken as 0 .. width * page.  Q / O:
+ * strides batch, head, query; O must not overlap an input.  lse: fp32 [n][hq][l]
+ * (natural log) or null.  scale > 0.  Workspace (slots = width * page): may be 0
+ * bytes, 16-byte aligned; its contents must be zero before the first call with
+ * it, and every call leaves them fit for the next one, of any sizes.  Calls that
+ * share one must not run at the same time.                                   */
+KUIOPS_API size_t kuiops_sdpa_paged_workspace(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t slots, int64_t hd);
+KUIOPS_API int kuiops_sdpa_paged(int64_t n, int64_t hq, int64_t l, int dtype, const void *Q, const int64_t sq[3],
+                      const kuiops_paged_layout *at, const void *K, const void *V, const float *k_scale,
+                      const float *v_scale, const int32_t *table, const int32_t *kv_len, void *O,
+                      const int64_t so[3], float *lse, float scale, void *workspace, size_t workspace_bytes,
+                      void *stream);
 
 #ifdef __cplusplus
 }

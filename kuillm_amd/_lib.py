@@ -22,7 +22,7 @@ E_HIP = -3
 E_WORKSPACE = -4
 
 # kuiops_dtype
-F32, F16, BF16, F64, I64, I32, I16, I8, U8, BOOL = range(10)
+F32, F16, BF16, F64, I64, I32, I16, I8, U8, BOOL, F8E4M3 = range(11)
 # kuiops_b_layout
 B_ROW, B_COL = 0, 1
 # kuiops_c_kind
@@ -40,6 +40,15 @@ _dbl = ctypes.c_double
 _flt = ctypes.c_float
 _sz = ctypes.c_size_t
 _i64p = ctypes.POINTER(ctypes.c_int64)
+
+
+class PagedLayout(ctypes.Structure):
+    """kuiops_paged_layout"""
+    _fields_ = [(name, _i64) for name in ("pages", "page", "hkv", "hd", "width", "ld_table")] + \
+        [("sk", _i64 * 3), ("sv", _i64 * 3), ("sks", _i64 * 2), ("svs", _i64 * 2), ("dtype", _int)]
+
+
+_layoutp = ctypes.POINTER(PagedLayout)
 
 # name -> (restype, argtypes); mirrors include/kuiops.h one to one.
 X_PLAIN, X_RMSNORM, X_SWIGLU = 1, 2, 3
@@ -115,6 +124,12 @@ SIGNATURES = {
     "kuiops_kv_evict_workspace": (_sz, [_i64, _i64, _i64]),
     "kuiops_kv_evict": (_int, [_i64, _i64, _i64, _i64, _i64, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp,
                                _i64, _i64, _vp, _i64p, _vp, _i64p, _vp, _vp, _sz, _vp]),
+    "kuiops_kv_paged_append": (_int, [_i64, _i64, _i64, _int, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _dbl, _vp, _i64p,
+                                      _layoutp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "kuiops_kv_paged_read": (_int, [_i64, _i64, _int, _layoutp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64p, _vp, _i64p, _int, _vp]),
+    "kuiops_sdpa_paged_workspace": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "kuiops_sdpa_paged": (_int, [_i64, _i64, _i64, _int, _vp, _i64p, _layoutp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64p, _vp,
+                                 _flt, _vp, _sz, _vp]),
 }
 
 

@@ -1,0 +1,467 @@
+// Rows into and out of a paged KV cache, gfx950.
+//
+//   kuiops_kv_paged_append  per-head norm and rotation of new tokens' queries and keys,
+//       keys and values into the sequences' pages, quantised as they are written
+//   kuiops_kv_paged_read    the sequences' rows gathered out of their pages as numbers
+//
+// 8-bit pages hold a row x as x_i = scale * s_i with scale = m / M, s_i = nearest(x_i M / m),
+// m = max |x_i|, M the type's largest value (int8 127, e4m3 448).
+#include <algorithm>
+
+#include "paged.hpp"
+
+namespace kuiops {
+
+int check_cache(const kuiops_paged_layout *at, int dtype, const void *K, const void *V, const float *ks, const float *vs,
+                const int32_t *table, PagedCache &c) {
+    if (at->pages < 0 || at->page <= 0 || at->hkv <= 0 || at->hd <= 0 || at->width < 0) return KUIOPS_E_INVALID;
+    if (at->width > 0 && !table) return KUIOPS_E_INVALID;
+    if (at->pages > 0 && (!K || !V)) return KUIOPS_E_INVALID;
+    if (dtype != KUIOPS_BF16 && dtype != KUIOPS_F16) return KUIOPS_E_UNSUPPORTED;
+    const bool bytes = at->dtype == KUIOPS_I8 || at->dtype == KUIOPS_F8E4M3;
+    if (!bytes && at->dtype != KUIOPS_BF16 && at->dtype != KUIOPS_F16) return KUIOPS_E_UNSUPPORTED;
+    if (!bytes && at->dtype != dtype) return KUIOPS_E_INVALID;
+    if (bytes && at->pages > 0 && (!ks || !vs)) return KUIOPS_E_INVALID;
+    // rows in 16-byte pieces, 16 rows of a page at a time, 32-bit slots
+    if (at->hd % 16 || at->hd > 128 || at->page % 16 || at->page > (1 << 20) || at->pages >= ((int64_t)1 << 31) ||
+        at->width * at->page >= ((int64_t)1 << 30) || at->hkv >= (1 << 20))
+        return KUIOPS_E_UNSUPPORTED;
+    const int64_t unit = bytes ? 16 : 8;
+    if (!aligned16(K) || !aligned16(V) || (bytes && (!aligned16(ks) || !aligned16(vs)))) return KUIOPS_E_UNSUPPORTED;
+    for (int i = 0; i < 3; ++i)
+        if (at->sk[i] % unit || at->sv[i] % unit || at->sk[i] < 0 || at->sv[i] < 0) return KUIOPS_E_UNSUPPORTED;
+    if (at->sk[2] < at->hd || at->sv[2] < at->hd || at->sk[2] >= (1 << 24) || at->sv[2] >= (1 << 24)) return KUIOPS_E_UNSUPPORTED;
+    for (int i = 0; i < 2 && bytes; ++i)
+        if (at->sks[i] % 4 || at->svs[i] % 4 || at->sks[i] < 0 || at->svs[i] < 0) return KUIOPS_E_UNSUPPORTED;
+    if (at->ld_table < 0) return KUIOPS_E_UNSUPPORTED;
+    c = PagedCache{K, V, bytes ? ks : nullptr, bytes ? vs : nullptr, table,
+                   at->sk[0], at->sk[1], at->sk[2], at->sv[0], at->sv[1], at->sv[2],
+                   at->sks[0], at->sks[1], at->svs[0], at->svs[1], at->ld_table,
+                   (int)at->pages, (int)at->page, (int)at->hkv, (int)at->hd, (int)at->width, at->dtype};
+    return KUIOPS_OK;
+}
+
+namespace {
+
+struct AppendArgs {
+    PagedCache c;
+    int n, t, hq;
+    const void *qkv;
+    int64_t ld_tok, ld_batch;
+    const int32_t *lens, *pos0;
+    const float *inv_freq;
+    const void *q_norm, *k_norm;
+    double eps;
+    void *q;
+    int64_t sq0, sq1, sq2;
+    int heads;                 // heads that a work-group takes
+};
+
+// cos and sin of pos * freq, 64-bit: the angle less the nearest multiple of pi / 2 (in two
+// parts, whose product with the multiple is exact enough far past any position), then Taylor's
+// series on +- pi / 4, whose first term left out is below 2^-53.
+__device__ __forceinline__ void turn_of(int64_t pos, float freq, double &c, double &s) {
+    const double a = (double)pos * (double)freq;
+    const double n = rint(a * 0.63661977236758134308);
+    double r = fma(-n, 1.57079632679489655800, a);
+    r = fma(-n, 6.12323399573676603587e-17, r);
+    const double x = r * r;
+    double sn = -1.0 / 1307674368000.0;
+    sn = fma(sn, x, 1.0 / 6227020800.0);
+    sn = fma(sn, x, -1.0 / 39916800.0);
+    sn = fma(sn, x, 1.0 / 362880.0);
+    sn = fma(sn, x, -1.0 / 5040.0);
+    sn = fma(sn, x, 1.0 / 120.0);
+    sn = fma(sn, x, -1.0 / 6.0);
+    sn = fma(sn * x, r, r);
+    double cs = 1.0 / 20922789888000.0;
+    cs = fma(cs, x, -1.0 / 87178291200.0);
+    cs = fma(cs, x, 1.0 / 479001600.0);
+    cs = fma(cs, x, -1.0 / 3628800.0);
+    cs = fma(cs, x, 1.0 / 40320.0);
+    cs = fma(cs, x, -1.0 / 720.0);
+    cs = fma(cs, x, 1.0 / 24.0);
+    cs = fma(cs, x, -1.0 / 2.0);
+    cs = fma(cs, x, 1.0);
+    const int64_t quarter = (int64_t)n & 3;
+    c = quarter == 0 ? cs : quarter == 1 ? -sn : quarter == 2 ? -cs : sn;
+    s = quarter == 0 ? sn : quarter == 1 ? cs : quarter == 2 ? -sn : -cs;
+}
+
+// The value of the lane D away within a group of lanes (the same moves as group_sum's)
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+template <int CTRL> __device__ __forceinline__ double dpp(double v) {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    const u32x2 r = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[0], CTRL, 0xF, 0xF, false),
+                     (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[1], CTRL, 0xF, 0xF, false)};
+    return __builtin_bit_cast(double, r);
+}
+template <int N, typename F, typename Op>
+__device__ __forceinline__ F over_group(F v, Op op) {
+    static_assert(N == 4 || N == 8, "group size");
+    v = op(v, dpp<0xB1>(v));
+    v = op(v, dpp<0x4E>(v));
+    if (N == 8) v = op(v, dpp<0x141>(v));
+    return v;
+}
+
+// Eight values s = nearest(x * r) of the 8-bit type, r = M / m: x M / m in 64 bits, where the
+// product's last bit may miss a tie that the quotient hits, so what 32 bits hold to 2^-45 is
+// taken to be that (a tie is: it has 9 bits).  e4m3: the rest goes through 32 bits cut off
+// with the last bit set, which rounds as the 64-bit value does.
+template <bool INT8, typename F>
+__device__ __forceinline__ u32x2 to_bytes(const F (&x)[8], double r) {
+    u32x2 w;
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+        uint32_t got = 0;
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const double y = (double)x[e + i] * r;
+            float z = (float)y;
+            const double off = y - (double)z;
+            if (fabs(off) > fabs(y) * 0x1p-45) {
+                // the neighbour nearer to zero, its last bit set
+                uint32_t u = __float_as_uint(z);
+                if ((off < 0) == (y > 0)) u -= 1;
+                z = __uint_as_float(u | 1);
+            }
+            f[i] = z;
+            if constexpr (INT8) got |= ((uint32_t)(int)rintf(z) & 0xffu) << (8 * i);
+        }
+        if constexpr (!INT8) {
+            got = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+            got = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], (int)got, true);
+        }
+        w[e / 4] = got;
+    }
+    return w;
+}
+
+// ------------------------------------------------------------------------
+// paged_append_kernel -- a work-group has TB tokens and some of their heads.  The tokens'
+// cos / sin are worked out once for all heads (64 bits, in LDS); HD / 16 lanes have a head, 8
+// values i and their partners i + hd / 2 each, so a row is read and written in 16-byte
+// pieces and the rotation needs no exchange.  Queries, and keys of 16-bit pages, are computed
+// in 32 bits and rounded once; keys of 8-bit pages in 64, so that a value next to a border
+// between two quantised ones falls on its own side of it.
+template <typename T, int PK, int HD, int TB>
+__global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    constexpr int LPH = HD / 16, HALF = HD / 2;
+    typedef typename std::conditional<PK == 0, float, double>::type K;      // what keys are computed in
+    __shared__ __attribute__((aligned(16))) K s_cos[TB][HALF], s_sin[TB][HALF];
+    const int tid = threadIdx.x, half = a.c.hd / 2;
+    const int64_t b = blockIdx.y;
+    const int t0 = blockIdx.x * TB;
+    const int there = a.lens ? max(0, min(a.lens[b], a.t)) : a.t;
+    const int64_t first = a.pos0 ? a.pos0[b] : 0;
+    for (int x = tid; x < TB * HALF; x += 256) {
+        const int k = x / HALF, i = x % HALF;
+        if (i < half && t0 + k < there) {
+            double c, s;
+            turn_of(first + t0 + k, a.inv_freq[i], c, s);
+            s_cos[k][i] = (K)c;
+            s_sin[k][i] = (K)s;
+        }
+    }
+    __syncthreads();
+    const int hkv = a.c.hkv, h0 = blockIdx.z * a.heads, h1 = min(h0 + a.heads, a.hq + 2 * hkv);
+    const int tasks = TB * (h1 - h0) * LPH;
+    for (int x = tid; x < tasks; x += 256) {
+        // (the lanes of a head are in one wave, and all of them or none are here)
+        const int hx = x / LPH, k = hx / (h1 - h0), h = h0 + hx - k * (h1 - h0), d = x % LPH * 8;
+        const int t = t0 + k;
+        if (t >= a.t) continue;
+        const bool mine = d < half;
+        const int64_t slot = first + t;
+        T *q = reinterpret_cast<T *>(a.q) + b * a.sq0 + h * a.sq1 + t * a.sq2 + d;
+        if (t >= there) {
+            // a token that is not there: nothing of it is read, its query is 0
+            if (h < a.hq && mine) {
+                *reinterpret_cast<u32x4 *>(q) = u32x4{0, 0, 0, 0};
+                *reinterpret_cast<u32x4 *>(q + half) = u32x4{0, 0, 0, 0};
+            }
+            continue;
+        }
+        const T *row = reinterpret_cast<const T *>(a.qkv) + b * a.ld_batch + t * a.ld_tok + (int64_t)h * a.c.hd + d;
+        const t8 v1 = __builtin_bit_cast(t8, mine ? *reinterpret_cast<const u32x4 *>(row) : u32x4{0, 0, 0, 0});
+        const t8 v2 = __builtin_bit_cast(t8, mine ? *reinterpret_cast<const u32x4 *>(row + half) : u32x4{0, 0, 0, 0});
+        auto turned = [&](auto one, const void *norm, auto (&x1)[8], auto (&x2)[8]) __attribute__((always_inline)) {
+            typedef decltype(one) F;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x1[e] = (F)to_f32(v1[e]);
+                x2[e] = (F)to_f32(v2[e]);
+            }
+            if (norm) {
+                F sum = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum += x1[e] * x1[e] + x2[e] * x2[e];
+                sum = over_group<LPH>(sum, [](F u, F w) { return u + w; });
+                const F r = F(1) / sqrt(sum / (F)a.c.hd + (F)a.eps);
+                const T *w = reinterpret_cast<const T *>(norm) + d;
+                const t8 w1 = __builtin_bit_cast(t8, mine ? *reinterpret_cast<const u32x4 *>(w) : u32x4{0, 0, 0, 0});
+                const t8 w2 = __builtin_bit_cast(t8, mine ? *reinterpret_cast<const u32x4 *>(w + half) : u32x4{0, 0, 0, 0});
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x1[e] *= r * (F)to_f32(w1[e]);
+                    x2[e] *= r * (F)to_f32(w2[e]);
+                }
+            }
+            if (!mine) return;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const F c = (F)s_cos[k][d + e], s = (F)s_sin[k][d + e], y1 = x1[e], y2 = x2[e];
+                x1[e] = y1 * c - y2 * s;
+                x2[e] = y2 * c + y1 * s;
+            }
+        };
+        auto rounded = [&](const float (&y)[8]) __attribute__((always_inline)) {
+            t8 w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = from_f32<T>(y[e]);
+            return __builtin_bit_cast(u32x4, w);
+        };
+        if (h < a.hq) {
+            float x1[8], x2[8];
+            turned(1.f, a.q_norm, x1, x2);
+            if (mine) {
+                *reinterpret_cast<u32x4 *>(q) = rounded(x1);
+                *reinterpret_cast<u32x4 *>(q + half) = rounded(x2);
+            }
+            continue;
+        }
+        const bool key = h < a.hq + hkv;
+        const int hk = h - a.hq - (key ? 0 : hkv);
+        K x1[8], x2[8];
+        if (key) turned(K(1), a.k_norm, x1, x2);
+        else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x1[e] = (K)to_f32(v1[e]);
+                x2[e] = (K)to_f32(v2[e]);
+            }
+        }
+        int at = 0;
+        const int id = slot >= 0 && slot < (int64_t)a.c.width * a.c.page ? page_of(a.c, b, (int)slot, at) : -1;
+        if (id < 0) continue;                         // the slot has no page
+        const int64_t off = key ? id * a.c.sk0 + hk * a.c.sk1 + at * a.c.sk2 : id * a.c.sv0 + hk * a.c.sv1 + at * a.c.sv2;
+        char *dst = reinterpret_cast<char *>(const_cast<void *>(key ? a.c.K : a.c.V)) + (off + d) * (PK == 0 ? 2 : 1);
+        if constexpr (PK == 0) {
+            if (mine) {
+                *reinterpret_cast<u32x4 *>(dst) = key ? rounded(x1) : __builtin_bit_cast(u32x4, v1);
+                *reinterpret_cast<u32x4 *>(dst + half * 2) = key ? rounded(x2) : __builtin_bit_cast(u32x4, v2);
+            }
+        } else {
+            constexpr bool INT8 = PK == 1;
+            constexpr double M = INT8 ? 127.0 : 448.0;
+            double top = 0.0;
+            float odd = 0.f;                          // NaN if the row has one, or an infinity
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                top = fmax(top, fmax(fabs(x1[e]), fabs(x2[e])));
+                odd += (float)(x1[e] * 0.0) + (float)(x2[e] * 0.0);
+            }
+            top = over_group<LPH>(top, [](double u, double w) { return fmax(u, w); });
+            odd = over_group<LPH>(odd, [](float u, float w) { return u + w; });
+            // a row that is not finite reads back as NaN
+            const bool fine = odd == 0.f;
+            const double r = fine && top > 0.0 ? M / top : 0.0;
+            if (mine) {
+                if (!fine) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x1[e] = x2[e] = 0;
+                }
+                *reinterpret_cast<u32x2 *>(dst) = to_bytes<INT8>(x1, r);
+                *reinterpret_cast<u32x2 *>(dst + half) = to_bytes<INT8>(x2, r);
+            }
+            if (d == 0) {
+                float *sc = const_cast<float *>(key ? a.c.ks : a.c.vs);
+                sc[key ? id * a.c.sks0 + hk * a.c.sks1 + at : id * a.c.svs0 + hk * a.c.svs1 + at] =
+                    fine ? (float)(top / M) : __uint_as_float(0x7fc00000u);
+            }
+        }
+    }
+}
+
+struct ReadArgs {
+    PagedCache c;
+    int s;
+    const int32_t *kv_len;
+    void *k, *v;
+    int64_t ko0, ko1, ko2, vo0, vo1, vo2;
+    int fill;
+};
+
+// ------------------------------------------------------------------------
+// paged_read_kernel -- a work-group has ROWS slots of one KV head, keys and values; 16 bytes
+// of a page a lane.
+template <typename T, int PK, int HD>
+__global__ __launch_bounds__(256) void paged_read_kernel(ReadArgs a) {
+    constexpr int E = PK == 0 ? 8 : 16, LPR = HD / E, RPI = 256 / LPR, ROWS = 128, IT = ROWS / RPI;
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    const int tid = threadIdx.x, d = tid % LPR * E;
+    const int64_t bh = blockIdx.y, b = bh / a.c.hkv, hk = bh % a.c.hkv;
+    const int L = min(a.s, paged_len(a.c, a.kv_len, b)), s0 = blockIdx.x * ROWS;
+    if (s0 >= (a.fill ? a.s : L) || d >= a.c.hd) return;
+    constexpr int B = PK == 0 ? 2 : 1;
+    int id[IT], at[IT];
+#pragma unroll
+    for (int j = 0; j < IT; ++j) {
+        const int slot = s0 + j * RPI + tid / LPR;
+        id[j] = slot < L ? page_of(a.c, b, slot, at[j]) : -1;
+    }
+    u32x4 w[2][IT];
+    float sc[2][IT];
+#pragma unroll
+    for (int j = 0; j < IT; ++j) {
+        w[0][j] = w[1][j] = u32x4{0, 0, 0, 0};
+        sc[0][j] = sc[1][j] = 0.f;
+        if (id[j] >= 0) {
+            w[0][j] = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const char *>(a.c.K) + (id[j] * a.c.sk0 + hk * a.c.sk1 + at[j] * a.c.sk2 + d) * B);
+            w[1][j] = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const char *>(a.c.V) + (id[j] * a.c.sv0 + hk * a.c.sv1 + at[j] * a.c.sv2 + d) * B);
+            if constexpr (PK != 0) {
+                sc[0][j] = a.c.ks[id[j] * a.c.sks0 + hk * a.c.sks1 + at[j]];
+                sc[1][j] = a.c.vs[id[j] * a.c.svs0 + hk * a.c.svs1 + at[j]];
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int j = 0; j < IT; ++j) {
+            const int slot = s0 + j * RPI + tid / LPR;
+            if (slot >= (a.fill ? a.s : L)) continue;
+            T *dst = reinterpret_cast<T *>(x ? a.v : a.k) +
+                     (x ? b * a.vo0 + hk * a.vo1 + slot * a.vo2 : b * a.ko0 + hk * a.ko1 + slot * a.ko2) + d;
+            if constexpr (PK == 0) *reinterpret_cast<u32x4 *>(dst) = w[x][j];
+            else {
+#pragma unroll
+                for (int e = 0; e < E; e += 4) {
+                    const uint32_t u = w[x][j][e / 4];
+                    float f[4];
+                    if constexpr (PK == 1) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(u >> (8 * i));
+                    } else {
+                        f[0] = __builtin_amdgcn_cvt_f32_fp8((int)u, 0);
+                        f[1] = __builtin_amdgcn_cvt_f32_fp8((int)u, 1);
+                        f[2] = __builtin_amdgcn_cvt_f32_fp8((int)u, 2);
+                        f[3] = __builtin_amdgcn_cvt_f32_fp8((int)u, 3);
+                    }
+                    typedef T t4 __attribute__((ext_vector_type(4)));
+                    t4 y;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = from_f32<T>(f[i] * sc[x][j]);
+                    *reinterpret_cast<t4 *>(dst + e) = y;
+                }
+            }
+        }
+}
+
+// ------------------------------------------------------------- host side
+
+template <typename T, int PK, int HD>
+void launch_append(AppendArgs &a, hipStream_t st) {
+    const int heads = a.hq + 2 * a.c.hkv;
+    // tokens enough for every CU: 4 of them share a work-group's tables; fewer: the heads are
+    // spread over work-groups
+    if ((int64_t)a.n * a.t >= 1024) {
+        a.heads = heads;
+        hipLaunchKernelGGL((paged_append_kernel<T, PK, HD, 4>), dim3((unsigned)cdiv(a.t, 4), (unsigned)a.n, 1), dim3(256), 0, st, a);
+        return;
+    }
+    const int per = 256 / (HD / 16);                  // heads that a work-group's threads have at once
+    const int parts = (int)cdiv(heads, per);
+    a.heads = (int)cdiv(heads, parts);
+    hipLaunchKernelGGL((paged_append_kernel<T, PK, HD, 1>), dim3((unsigned)a.t, (unsigned)a.n, (unsigned)parts), dim3(256), 0, st, a);
+}
+
+template <typename T>
+void launch_append_kind(AppendArgs &a, hipStream_t st) {
+    const bool small = a.c.hd <= 64;
+    if (a.c.dtype == KUIOPS_I8) small ? launch_append<T, 1, 64>(a, st) : launch_append<T, 1, 128>(a, st);
+    else if (a.c.dtype == KUIOPS_F8E4M3) small ? launch_append<T, 2, 64>(a, st) : launch_append<T, 2, 128>(a, st);
+    else small ? launch_append<T, 0, 64>(a, st) : launch_append<T, 0, 128>(a, st);
+}
+
+template <typename T, int PK>
+void launch_read(const ReadArgs &a, unsigned heads, hipStream_t st) {
+    const dim3 grid((unsigned)cdiv(a.s, 128), heads);
+    if (a.c.hd <= 64) hipLaunchKernelGGL((paged_read_kernel<T, PK, 64>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_read_kernel<T, PK, 128>), grid, dim3(256), 0, st, a);
+}
+
+template <typename T>
+void launch_read_kind(const ReadArgs &a, unsigned heads, hipStream_t st) {
+    if (a.c.dtype == KUIOPS_I8) launch_read<T, 1>(a, heads, st);
+    else if (a.c.dtype == KUIOPS_F8E4M3) launch_read<T, 2>(a, heads, st);
+    else launch_read<T, 0>(a, heads, st);
+}
+
+}  // namespace
+
+}  // namespace kuiops
+
+using namespace kuiops;
+
+extern "C" int kuiops_kv_paged_append(int64_t n, int64_t t, int64_t hq, int dtype, const void *qkv, int64_t ld_tok,
+                                      int64_t ld_batch, const int32_t *lens, const int32_t *pos0, const float *inv_freq,
+                                      const void *q_norm, const void *k_norm, double eps, void *q_out, const int64_t sq[3],
+                                      const kuiops_paged_layout *at, void *K, void *V, float *k_scale, float *v_scale,
+                                      const int32_t *table, void *stream) {
+    if (n < 0 || t < 0 || hq < 0 || !at || !sq) return KUIOPS_E_INVALID;
+    AppendArgs a{};
+    if (n == 0 || t == 0) return KUIOPS_OK;
+    const int bad = check_cache(at, dtype, K, V, k_scale, v_scale, table, a.c);
+    if (bad) return bad;
+    if (!qkv || !inv_freq || (hq > 0 && !q_out) || !(eps >= 0.0)) return KUIOPS_E_INVALID;
+    if (ld_tok % 8 || ld_batch % 8 || sq[0] % 8 || sq[1] % 8 || sq[2] % 8) return KUIOPS_E_UNSUPPORTED;
+    if (!aligned16(qkv) || !aligned16(q_out) || (q_norm && !aligned16(q_norm)) || (k_norm && !aligned16(k_norm)))
+        return KUIOPS_E_UNSUPPORTED;
+    // grid axes, launches below 2^32 threads
+    if (n > 65535 || t >= (1 << 24) || hq + 2 * at->hkv >= (1 << 16) || n * t * cdiv(hq + 2 * at->hkv, 32) >= (1 << 24))
+        return KUIOPS_E_UNSUPPORTED;
+    a.n = (int)n; a.t = (int)t; a.hq = (int)hq;
+    a.qkv = qkv; a.ld_tok = ld_tok; a.ld_batch = ld_batch;
+    a.lens = lens; a.pos0 = pos0; a.inv_freq = inv_freq;
+    a.q_norm = q_norm; a.k_norm = k_norm; a.eps = eps;
+    a.q = q_out; a.sq0 = sq[0]; a.sq1 = sq[1]; a.sq2 = sq[2];
+    if (dtype == KUIOPS_BF16) launch_append_kind<bf16_t>(a, as_stream(stream));
+    else launch_append_kind<f16_t>(a, as_stream(stream));
+    return launch_status();
+}
+
+extern "C" int kuiops_kv_paged_read(int64_t n, int64_t s, int dtype, const kuiops_paged_layout *at, const void *K, const void *V,
+                                    const float *k_scale, const float *v_scale, const int32_t *table, const int32_t *kv_len,
+                                    void *k_out, const int64_t sko[3], void *v_out, const int64_t svo[3], int fill, void *stream) {
+    if (n < 0 || s < 0 || !at || !sko || !svo) return KUIOPS_E_INVALID;
+    if (n == 0 || s == 0) return KUIOPS_OK;
+    ReadArgs a{};
+    // (8-bit pages as fp32 too; the cache's check knows the 16-bit types)
+    const bool wide = dtype == KUIOPS_F32;
+    if (wide && at->dtype != KUIOPS_I8 && at->dtype != KUIOPS_F8E4M3) return KUIOPS_E_UNSUPPORTED;
+    const int bad = check_cache(at, wide ? KUIOPS_BF16 : dtype, K, V, k_scale, v_scale, table, a.c);
+    if (bad) return bad;
+    if (!kv_len || !k_out || !v_out) return KUIOPS_E_INVALID;
+    const int64_t unit = wide ? 4 : 8;
+    for (int i = 0; i < 3; ++i)
+        if (sko[i] % unit || svo[i] % unit) return KUIOPS_E_UNSUPPORTED;
+    if (!aligned16(k_out) || !aligned16(v_out)) return KUIOPS_E_UNSUPPORTED;
+    const int64_t heads = n * at->hkv;
+    if (s >= (1 << 30) || heads > 65535 || cdiv(s, 128) * heads >= (1 << 24)) return KUIOPS_E_UNSUPPORTED;
+    a.s = (int)s; a.kv_len = kv_len;
+    a.k = k_out; a.v = v_out;
+    a.ko0 = sko[0]; a.ko1 = sko[1]; a.ko2 = sko[2];
+    a.vo0 = svo[0]; a.vo1 = svo[1]; a.vo2 = svo[2];
+    a.fill = fill;
+    hipStream_t st = as_stream(stream);
+    if (wide) at->dtype == KUIOPS_I8 ? launch_read<float, 1>(a, (unsigned)heads, st) : launch_read<float, 2>(a, (unsigned)heads, st);
+    else if (dtype == KUIOPS_BF16) launch_read_kind<bf16_t>(a, (unsigned)heads, st);
+    else launch_read_kind<f16_t>(a, (unsigned)heads, st);
+    return launch_status();
+}

@@ -14,8 +14,9 @@ Schemas follow the aten ops they replace (mm, addmm, bmm, _softmax over the
 last dim, scaled-dot-product attention returning (out, lse), topk, gather,
 index, the elementwise maps, last-axis mean, cat) with the reference's argument meaning
 (kuipy/kuiops.py:403-754).  The drafted-tree and bounded-cache ops (sdpa_tree,
-tree_accept, kv_tree_commit, sdpa_decode_accum, kv_evict) have no aten counterpart;
-those that change a cache in place say so in their schemas.
+tree_accept, kv_tree_commit, sdpa_decode_accum, kv_evict) and those of a paged cache
+(kv_paged_append, kv_paged_read, sdpa_paged) have no aten counterpart; those that change
+a cache in place say so in their schemas.
 """
 from __future__ import annotations
 
@@ -53,6 +54,13 @@ _SCHEMAS = {
                          "float? scale=None, bool causal=True) -> (Tensor, Tensor)",
     "kv_evict": "kv_evict(Tensor(a!) k, Tensor(b!) v, Tensor(c!) acc, Tensor(d!) pos, Tensor(e!) kv_len, int budget, "
                 "int recent=0) -> ()",
+    "kv_paged_append": "kv_paged_append(Tensor qkv, Tensor inv_freq, Tensor? pos0, Tensor(a!) k_pages, Tensor(b!) v_pages, "
+                       "Tensor table, Tensor(c!)? k_scale=None, Tensor(d!)? v_scale=None, Tensor? q_norm=None, "
+                       "Tensor? k_norm=None, float eps=1e-6, Tensor? lens=None) -> Tensor",
+    "kv_paged_read": "kv_paged_read(Tensor k_pages, Tensor v_pages, Tensor table, Tensor kv_len, int length, "
+                     "Tensor? k_scale=None, Tensor? v_scale=None, ScalarType? dtype=None) -> (Tensor, Tensor)",
+    "sdpa_paged": "sdpa_paged(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor kv_len, Tensor? k_scale=None, "
+                  "Tensor? v_scale=None, float? scale=None) -> (Tensor, Tensor)",
 }
 for _s in _SCHEMAS.values():
     _LIB.define(_s)
@@ -143,13 +151,22 @@ def _kv_evict(k, v, acc, pos, kv_len, budget, recent=0):
     ops.kv_evict(k, v, acc, pos, kv_len, budget, recent)
 
 
+def _kv_paged_read(k_pages, v_pages, table, kv_len, length, k_scale=None, v_scale=None, dtype=None):
+    return ops.kv_paged_read(k_pages, v_pages, table, kv_len, length, k_scale, v_scale, dtype)
+
+
+def _sdpa_paged(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=None, scale=None):
+    return ops.sdpa_paged(q, k_pages, v_pages, table, kv_len, k_scale, v_scale, scale, return_lse=True)
+
+
 for _name, _fn in (("mm", _mm), ("addmm", _addmm), ("bmm", _bmm), ("softmax", _softmax),
                    ("sdpa", _sdpa), ("sdpa_decode", _sdpa_decode), ("topk", _topk),
                    ("gather", _gather), ("index", _index), ("index_multi", _index_multi), ("scatter", _scatter), ("sort", _sort),
                    ("cumsum", _cumsum), ("multinomial", _multinomial), ("elementwise", _elementwise),
                    ("mean_lastdim", _mean_lastdim), ("cat", _cat), ("sdpa_tree", _sdpa_tree),
                    ("tree_accept", ops.tree_accept), ("kv_tree_commit", ops.kv_tree_commit),
-                   ("sdpa_decode_accum", _sdpa_decode_accum), ("kv_evict", _kv_evict)):
+                   ("sdpa_decode_accum", _sdpa_decode_accum), ("kv_evict", _kv_evict),
+                   ("kv_paged_append", ops.kv_paged_append), ("kv_paged_read", _kv_paged_read), ("sdpa_paged", _sdpa_paged)):
     _LIB.impl(_name, _fn, "CUDA")
 
 
@@ -280,3 +297,23 @@ def _sdpa_decode_accum_fake(q, k, v, acc, kv_len=None, scale=None, causal=True):
 @_fake("kv_evict")
 def _kv_evict_fake(k, v, acc, pos, kv_len, budget, recent=0):
     return None
+
+
+@_fake("kv_paged_append")
+def _kv_paged_append_fake(qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale=None, v_scale=None, q_norm=None, k_norm=None,
+                          eps=1e-6, lens=None):
+    hkv, hd = k_pages.shape[1], k_pages.shape[3]
+    return qkv.new_empty((qkv.shape[0], qkv.shape[2] // hd - 2 * hkv, qkv.shape[1], hd))
+
+
+@_fake("kv_paged_read")
+def _kv_paged_read_fake(k_pages, v_pages, table, kv_len, length, k_scale=None, v_scale=None, dtype=None):
+    if dtype is None:
+        dtype = k_pages.dtype if k_scale is None else torch.bfloat16
+    shape = (table.shape[0], k_pages.shape[1], length, k_pages.shape[3])
+    return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+
+
+@_fake("sdpa_paged")
+def _sdpa_paged_fake(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=None, scale=None):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:3], dtype=torch.float32)

@@ -1509,3 +1509,230 @@ def kv_evict(k, v, acc, pos, kv_len, budget, recent=0, acc_out=None, pos_out=Non
         n, hkv, cap, p.krow, p.vrow, k.data_ptr(), p.sk, v.data_ptr(), p.sv, acc_at, sa, pos_at, sp, len_at, budget,
         min(recent, budget), acc_to, sao, pos_to, spo, len_to, ws.data_ptr(), 4 * moves))
     return acc_out, pos_out, len_out
+
+
+# ------------------------------------------------------ paged KV caches
+# Sequences share a pool of pages, k_pages / v_pages (pages, hkv, page, hd); slot j of
+# sequence b is row j % page of page table[b, j // page] (int32 [n, width]).  An entry
+# outside 0 .. pages - 1 (-1, say) is no page: stores there are dropped, it reads as
+# zeros, attention does not see it.  Pages are bf16 / f16, or int8 / float8_e4m3fn with
+# an fp32 scale per row (k_scale / v_scale, (pages, hkv, page)).
+
+_PAGE_BYTES = {torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.F8E4M3}
+
+
+class _PagedPlan:
+    __slots__ = ("layout", "n", "bytes", "slots")
+
+
+@functools.lru_cache(maxsize=2048)
+def _paged_plan(name, k, v, k_scale, v_scale, table) -> _PagedPlan:
+    """Checks the (shape, stride, dtype) of a paged cache's tensors."""
+    (ks, kst, kd), (vs, vst, vd) = k, v
+    if len(ks) != 4 or ks != vs or kd != vd or ks[1] == 0 or ks[2] == 0 or ks[3] == 0 \
+            or len(table[0]) != 2 or table[2] != torch.int32:
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    p = _PagedPlan()
+    p.bytes = kd in _PAGE_BYTES
+    if p.bytes != (k_scale is not None) or p.bytes != (v_scale is not None):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if not p.bytes and kd not in HALF:
+        raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
+    pages, hkv, page, hd = ks
+    p.n, width = table[0]
+    if any(not _own_rows(shape, stride) for shape, stride in ((ks, kst), (vs, vst))):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if width > 1 and table[1][1] != 1:
+        raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
+    at = p.layout = _lib.PagedLayout(pages=pages, page=page, hkv=hkv, hd=hd, width=width,
+                                     ld_table=table[1][0] if p.n > 1 else 0,
+                                     dtype=_PAGE_BYTES[kd] if p.bytes else _dt(kd))
+    at.sk, at.sv = _c_strides(ks, kst, 3), _c_strides(vs, vst, 3)
+    if page == 1:
+        at.sk[2] = at.sv[2] = hd
+    for scale, st in ((k_scale, at.sks), (v_scale, at.svs)):
+        if scale is not None:
+            if scale[0] != ks[:3] or scale[2] != torch.float32 or not _own_rows(*scale[:2]):
+                raise _lib.KuiopsError(name, _lib.E_INVALID)
+            st[:] = _c_strides(*scale[:2], 2)
+    p.slots = width * page
+    return p
+
+
+def _paged_cache(name, k, v, k_scale, v_scale, table):
+    return _paged_plan(name, _meta(k), _meta(v), _meta(k_scale), _meta(v_scale), _meta(table))
+
+
+def _readable(t):
+    """t, or a copy where the kernels cannot read its rows in place: 16-byte pieces."""
+    st = t.stride()
+    if (t.shape[-1] <= 1 or st[-1] == 1) and t.data_ptr() % 16 == 0 and \
+            not any(s % 8 for s, size in zip(st[:-1], t.shape) if size > 1):
+        return t
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+
+
+def _apart(name, out, *others):
+    if out.numel():
+        at = out.data_ptr()
+        for o in others:
+            if o is not None and o.numel() and o.data_ptr() == at:
+                raise _lib.KuiopsError(name, _lib.E_INVALID)
+
+
+@functools.lru_cache(maxsize=2048)
+def _append_plan(qkv, hkv, hd, inv_freq, q_norm, k_norm, q_out):
+    """(hq, C strides of q_out) from the (shape, stride, dtype) of kv_paged_append's other tensors."""
+    name, (shape, _, dtype) = "kv_paged_append", qkv
+    if len(shape) != 3 or hd % 2 or shape[2] % hd or shape[2] // hd < 2 * hkv or inv_freq[0] != (hd // 2,) \
+            or inv_freq[2] != torch.float32 or any(w is not None and (w[0] != (hd,) or w[2] != dtype) for w in (q_norm, k_norm)):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if dtype not in HALF:
+        raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
+    n, t, hq = shape[0], shape[1], shape[2] // hd - 2 * hkv
+    if q_out is None:
+        return hq, _c_strides((n, hq, t, hd), (hq * t * hd, t * hd, hd, 1), 3)
+    if q_out[0] != (n, hq, t, hd) or q_out[2] != dtype or not _own_rows(*q_out[:2]):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    return hq, _c_strides(*q_out[:2], 3)
+
+
+def kv_paged_append(qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale=None, v_scale=None, q_norm=None, k_norm=None,
+                    eps=1e-6, lens=None, q_out=None):
+    """Norms and rotates the queries and keys of new tokens and stores their keys and
+    values in a paged cache, quantised if its pages are of 8 bits -> q (n, hq, t, hd).
+
+    qkv (n, t, (hq + 2 hkv) hd) is the fused projection's output (q, k, v heads).  Token
+    i of sequence b goes to slot and position ``pos0[b]`` + i (int32 [n] on the device;
+    None: 0); slots that the table does not reach are dropped.  Tokens from ``lens[b]``
+    on (int32 [n]; None: t) are padding: nothing of them is read or stored, their q is 0.
+    With ``q_norm`` / ``k_norm`` ([hd], qkv's type) a head becomes x * rsqrt(mean(x^2) +
+    eps) * weight; then queries and keys turn by the angles position * ``inv_freq``
+    (fp32 [hd / 2]), in 64 bits, and are rounded once.  8-bit pages get a row x as
+    stored * scale, scale = max |x| / M, stored = nearest(x M / max |x|), M = 127 (int8)
+    or 448 (float8_e4m3fn); a row that is not finite reads back as NaN.  A slot that
+    receives a token must belong to one sequence.  bf16 / f16; hd a multiple of 16 up to
+    128, pages of multiples of 16 rows.  ``q_out`` receives q in place."""
+    name = "kv_paged_append"
+    p = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
+    hq, sq = _append_plan(_meta(qkv), k_pages.shape[1], k_pages.shape[3], _meta(inv_freq), _meta(q_norm), _meta(k_norm), _meta(q_out))
+    n, t, _ = qkv.shape
+    if n != p.n or not (p.bytes or k_pages.dtype == qkv.dtype):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    for x in (pos0, lens):
+        if x is not None and not _flat_ints(x, n):
+            raise _lib.KuiopsError(name, _lib.E_INVALID)
+    _apart(name, k_pages, v_pages)
+    if q_out is not None:
+        _apart(name, q_out, qkv, k_pages, v_pages)
+    device = _gpu_of(name, qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale, v_scale, q_norm, k_norm, lens, q_out)
+    qkv, inv_freq = _readable(qkv), inv_freq.contiguous()
+    q_norm, k_norm = (w if w is None else _readable(w) for w in (q_norm, k_norm))
+    if q_out is None:
+        q_out = qkv.new_empty((n, hq, t, k_pages.shape[3]))
+    ld_batch, ld_tok, _ = qkv.stride()
+    _enqueue("kuiops_kv_paged_append", device, (
+        n, t, hq, _dt(qkv.dtype), qkv.data_ptr(), ld_tok if t > 1 else 0, ld_batch if n > 1 else 0, _ptr(lens), _ptr(pos0),
+        inv_freq.data_ptr(), _ptr(q_norm), _ptr(k_norm), float(eps), q_out.data_ptr(), sq, p.layout, k_pages.data_ptr(),
+        v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr()))
+    return q_out
+
+
+@functools.lru_cache(maxsize=2048)
+def _read_strides(shape, out, dtype):
+    if out[0] != shape or out[2] != dtype or not _own_rows(*out[:2]):
+        raise _lib.KuiopsError("kv_paged_read", _lib.E_INVALID)
+    return _c_strides(*out[:2], 3)
+
+
+def kv_paged_read(k_pages, v_pages, table, kv_len, length=None, k_scale=None, v_scale=None, dtype=None, k_out=None, v_out=None):
+    """The cached rows of the sequences, gathered out of their pages -> (k, v)
+    (n, hkv, length, hd): slots 0 .. ``kv_len[b]`` - 1 (int32 [n] on the device), as far as
+    ``length`` (default: all that the table reaches) goes.  For prompt attention over
+    what the cache holds (:func:`sdpa_decode_accum`, :func:`sdpa`).
+
+    ``dtype``: 16-bit pages come as they are, 8-bit ones as stored * scale in bf16
+    (default), f16 or fp32.  Rows behind a sequence are 0, or left as they are in
+    ``k_out`` / ``v_out`` (given together; (n, hkv, length, hd), unit last stride)."""
+    name = "kv_paged_read"
+    p = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
+    n, hkv, hd = p.n, k_pages.shape[1], k_pages.shape[3]
+    if (k_out is None) != (v_out is None) or not _flat_ints(kv_len, n):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if dtype is None:
+        dtype = k_out.dtype if k_out is not None else torch.bfloat16 if p.bytes else k_pages.dtype
+    if not p.bytes and dtype != k_pages.dtype or dtype not in (*HALF, torch.float32):
+        raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
+    if length is None:
+        length = k_out.shape[2] if k_out is not None and k_out.dim() == 4 else p.slots
+    if int(length) < 0:
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    shape, fill = torch.Size((n, hkv, int(length), hd)), k_out is None
+    if not fill:
+        sk, sv = _read_strides(shape, _meta(k_out), dtype), _read_strides(shape, _meta(v_out), dtype)
+        _apart(name, k_out, v_out, k_pages, v_pages)
+        _apart(name, v_out, k_pages, v_pages)
+    device = _gpu_of(name, k_pages, v_pages, table, kv_len, k_scale, v_scale, k_out, v_out)
+    if fill:
+        k_out, v_out = k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+        sk = sv = _read_strides(shape, _meta(k_out), dtype)
+    _enqueue("kuiops_kv_paged_read", device, (
+        n, shape[2], _dt(dtype), p.layout, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(),
+        kv_len.data_ptr(), k_out.data_ptr(), sk, v_out.data_ptr(), sv, 1 if fill else 0))
+    return k_out, v_out
+
+
+@functools.lru_cache(maxsize=2048)
+def _paged_attn_plan(q, hkv, hd, slots, out):
+    """(C strides of q, those of its copy, of out, bytes of the workspace, default scale)."""
+    name, (shape, stride, dtype) = "sdpa_paged", q
+    if len(shape) != 4 or shape[3] != hd or shape[1] % hkv:
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if dtype not in HALF:
+        raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
+    n, hq, l, _ = shape
+    flat = (hq * l * hd, l * hd, hd, 1)
+    if out is not None and (out[0] != shape or out[2] != dtype or not _own_rows(*out[:2])):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    return (_c_strides(shape, stride, 3), _c_strides(shape, flat, 3), _c_strides(shape, flat if out is None else out[1], 3),
+            _lib_handle().kuiops_sdpa_paged_workspace(n, hq, hkv, l, slots, hd), 1.0 / math.sqrt(hd))
+
+
+def _zeroed_workspace(device, nbytes):
+    """sdpa_paged's workspace: the current stream's own, or memory of its own (and its
+    zero fill) in a graph that is being captured, so that two graphs may run at once."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return workspace(device, nbytes, "paged")
+
+
+def sdpa_paged(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=None, scale=None, return_lse=False, out=None):
+    """Attention of the newest tokens over a paged KV cache -> (out, lse).
+
+    q (n, hq, l, hd): query i of sequence b is slot ``kv_len[b]`` - l + i (int32 [n] on the
+    device, read when the kernel runs; its own key among the slots, so appended before)
+    and sees the slots up to its own that have a page; one that sees none gives 0 and
+    lse -inf.  For decoding (l = 1) and a few drafted tokens: up to 16 rows of l * hq /
+    hkv share a pass over the cache (longer pieces of a prompt: :func:`kv_paged_read` and
+    :func:`sdpa_decode_accum`).  bf16 / f16; hd a multiple of 16 up to 128; scale > 0.
+    ``out`` ((n, hq, l, hd), unit last stride) receives the result in place; it must not
+    overlap q or the cache."""
+    name = "sdpa_paged"
+    p = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
+    sq, sq_copy, so, nbytes, default = _paged_attn_plan(_meta(q), k_pages.shape[1], k_pages.shape[3], p.slots, _meta(out))
+    n, hq, l, _ = q.shape
+    if n != p.n or not (p.bytes or k_pages.dtype == q.dtype) or not _flat_ints(kv_len, n):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    if out is not None:
+        _apart(name, out, q, k_pages, v_pages)
+    device = _gpu_of(name, q, k_pages, v_pages, table, kv_len, k_scale, v_scale, out)
+    given, q = q, _readable(q)
+    if out is None:
+        out = q.new_empty((n, hq, l, k_pages.shape[3]))
+    lse = q.new_empty((n, hq, l), dtype=torch.float32) if return_lse else None
+    ws = _zeroed_workspace(q.device, nbytes) if nbytes else None
+    _enqueue("kuiops_sdpa_paged", device, (
+        n, hq, l, _dt(q.dtype), q.data_ptr(), sq if q is given else sq_copy, p.layout, k_pages.data_ptr(), v_pages.data_ptr(),
+        _ptr(k_scale), _ptr(v_scale), table.data_ptr(), kv_len.data_ptr(), out.data_ptr(), so, _ptr(lse),
+        default if scale is None else float(scale), _ptr(ws), nbytes))
+    return out, lse

@@ -733,3 +733,82 @@ def kv_evict(k, v, acc, pos, kv_len, budget, recent=0):
                 c[b, g, :m] = c[b, g, slots]
             acc_out[b, g, :m], pos_out[b, g, :m] = np.asarray(acc)[b, g, slots], np.asarray(pos)[b, g, slots]
     return k, v, acc_out, pos_out, np.minimum(lens, budget).astype(np.int32)
+
+
+# ------------------------------------------------------ paged KV caches
+
+
+def paged_slot(row, page, pages, slot):
+    """(page, row in it) of a sequence's slot, None where it has no page; ``row`` is
+    its row of the table."""
+    p = slot // page
+    if slot < 0 or p >= len(row) or not 0 <= int(row[p]) < pages:
+        return None
+    return int(row[p]), slot % page
+
+
+def nearest_e4m3(y):
+    """The nearest value of 4 exponent and 3 fraction bits, ties to even (|y| <= 448)."""
+    y = np.asarray(y, np.float64)
+    step = np.exp2(np.floor(np.log2(np.maximum(np.abs(y), 2.0 ** -6))) - 3)
+    return np.rint(y / step) * step
+
+
+def quantise_rows(x, kind):
+    """Rows [..., hd] in 8 bits, "int8" or "e4m3": (stored values, scales, how far each
+    value lies from the nearest border between two stored ones, in steps)."""
+    M = 127.0 if kind == "int8" else 448.0
+    x = np.asarray(x, np.float64)
+    fine = np.isfinite(x).all(-1, keepdims=True)
+    top = np.where(fine, np.abs(np.where(fine, x, 0)).max(-1, keepdims=True), 0.0)
+    y = np.where(fine & (top > 0), np.where(fine, x, 0) * M / np.where(top > 0, top, 1), 0.0)
+    if kind == "int8":
+        step = np.ones_like(y)
+    else:
+        step = np.exp2(np.floor(np.log2(np.maximum(np.abs(y), 2.0 ** -6))) - 3)
+    off = np.abs(np.abs(y / step - np.floor(y / step)) - 0.5)
+    stored = np.rint(y) if kind == "int8" else nearest_e4m3(y)
+    return stored, np.where(fine, top / M, np.nan)[..., 0], off
+
+
+def norm_rope(x, w, eps, pos, inv_freq):
+    """Heads x [..., hd] at position ``pos``, normed (weights w, or None) and rotated
+    in 64 bits: (values, sums of absolute terms)."""
+    x = np.asarray(x, np.float64)
+    if w is not None:
+        x = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * np.asarray(w, np.float64)
+    a = float(pos) * np.asarray(inv_freq, np.float64)
+    h = x.shape[-1] // 2
+    u, v, c, s = x[..., :h], x[..., h:], np.cos(a), np.sin(a)
+    return (np.concatenate([u * c - v * s, v * c + u * s], -1),
+            np.concatenate([np.abs(u * c) + np.abs(v * s), np.abs(v * c) + np.abs(u * s)], -1))
+
+
+def paged_rows(pages, scale, table, length):
+    """Values [n, hkv, length, hd] of the slots below ``length`` (0 where there is no page),
+    and which have one [n, length]."""
+    pages = np.asarray(pages, np.float64)
+    P, hkv, page, hd = pages.shape
+    out, there = np.zeros((len(table), hkv, length, hd)), np.zeros((len(table), length), bool)
+    for b, row in enumerate(table):
+        for slot in range(length):
+            at = paged_slot(row, page, P, slot)
+            if at is not None:
+                there[b, slot] = True
+                out[b, :, slot] = pages[at[0], :, at[1]] * (1 if scale is None else np.asarray(scale, np.float64)[at[0], :, at[1], None])
+    return out, there
+
+
+def sdpa_paged(q, k, v, table, kv_len, k_scale=None, v_scale=None, scale=None):
+    """Attention of the newest tokens over a paged cache (kuiops_sdpa_paged): (out, lse,
+    sums of absolute output terms, largest sum of absolute score terms)."""
+    n, _, l, e = q.shape
+    page, width = k.shape[2], np.shape(table)[1]
+    scale = 1.0 / np.sqrt(e) if scale is None else scale
+    lens = [min(max(int(x), 0), width * page) for x in kv_len]
+    kk, there = paged_rows(k, k_scale, table, max(lens, default=0))
+    vv, _ = paged_rows(v, v_scale, table, max(lens, default=0))
+    got = []
+    for b, L in enumerate(lens):
+        got.append(_attend_rows(q[b], kk[b], vv[b], lambda i, b=b, L=L: [j for j in range(max(0, L - l + i + 1)) if there[b, j]], scale))
+    return np.stack([x[0] for x in got]), np.stack([x[1] for x in got]), np.stack([x[3] for x in got]), max(x[4] for x in got)
