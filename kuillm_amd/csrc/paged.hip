@@ -37,7 +37,7 @@ int check_cache(const kuiops_paged_layout *at, int dtype, const void *K, const v
     c = PagedCache{K, V, bytes ? ks : nullptr, bytes ? vs : nullptr, table,
                    at->sk[0], at->sk[1], at->sk[2], at->sv[0], at->sv[1], at->sv[2],
                    at->sks[0], at->sks[1], at->svs[0], at->svs[1], at->ld_table,
-                   (int)at->pages, (int)at->page, (int)at->hkv, (int)at->hd, (int)at->width, at->dtype};
+                   (int)at->pages, (int)at->page, (int)at->hkv, (int)at->hd, (int)at->width, paged_div((int)at->page / 16), at->dtype};
     return KUIOPS_OK;
 }
 
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
             }
         }
         int at = 0;
-        const int id = slot >= 0 && slot < (int64_t)a.c.width * a.c.page ? page_of(a.c, b, (int)slot, at) : -1;
+        const int id = slot >= 0 && slot < (1 << 30) ? page_of(a.c, b, (int)slot, at) : -1;
         if (id < 0) continue;                         // the slot has no page
         const int64_t off = key ? id * a.c.sk0 + hk * a.c.sk1 + at * a.c.sk2 : id * a.c.sv0 + hk * a.c.sv1 + at * a.c.sv2;
         char *dst = reinterpret_cast<char *>(const_cast<void *>(key ? a.c.K : a.c.V)) + (off + d) * (PK == 0 ? 2 : 1);

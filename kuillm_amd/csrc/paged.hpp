@@ -15,11 +15,12 @@ struct PagedCache {
     const int32_t *table;
     int64_t sk0, sk1, sk2, sv0, sv1, sv2, sks0, sks1, svs0, svs1, ld_table;
     int pages, page, hkv, hd, width;
+    PageDiv div;                       // by a page's 16-slot groups
     int dtype;
 };
 
 __device__ __forceinline__ int page_of(const PagedCache &c, int64_t b, int slot, int &at) {
-    return paged_find(c.table + b * c.ld_table, c.width, c.page, c.pages, slot, at);
+    return paged_find(c.table + b * c.ld_table, c.width, c.page, c.div, c.pages, slot, at);
 }
 
 __device__ __forceinline__ int paged_len(const PagedCache &c, const int32_t *kv_len, int64_t b) {

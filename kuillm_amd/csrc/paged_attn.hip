@@ -15,27 +15,35 @@ namespace kuiops {
 namespace {
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// (the same in all lanes, said so: a size that came out of a vector minimum puts a loop over
+// the lanes' descriptors around every load)
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void *base, uint32_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)bytes, 0x00020000);
+    const uint64_t p = reinterpret_cast<uint64_t>(base);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>((uint64_t)hi << 32 | lo), (short)0,
+                                             __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
 constexpr float kLn2 = 0.69314718055994530942f, kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kOut = 0x80000000u;        // an offset past every descriptor
 constexpr float kSlack = 8.f;                 // a row's maximum may grow by 2^8 before its sums are rescaled
-constexpr int kMaxSplits = 64;                // (the merge has a lane for each)
 constexpr int kCounterStride = 16;            // words: a cache line's atomics serialise
+constexpr int kTile = 32;                     // slots that a wave takes at once
+constexpr int kSwitch = 12, kLeast = 16;      // tiles that going on to another unit takes the time of; of a work-group, at least
+constexpr int kWhole = 24, kPiece = 8;        // tiles that are not worth a merge; of a piece, at least
 
 struct PagedArgs {
     PagedCache c;
-    int n, hq, l, splits, row_groups;
+    int n, hq, l, groups, row_groups;      // groups: work-groups that share the keys
+    int apart;                 // a work-group has one piece
     const void *Q;
     void *O;
     int64_t sq0, sq1, sq2, so0, so1, so2;
     float *lse;                // [n][hq][l], or null
     float scale_log2;          // softmax scale * log2(e), > 0
     const int32_t *kv_len;
-    // splits > 1: per (sequence, KV head, row group) a counter that is zero between calls, and
-    // per split 16 rows of (maximum in the log2 domain, sum) and of the unnormalised output
+    // per work-group a counter that is zero between calls, and for two pieces 16 rows of
+    // (maximum in the log2 domain, sum) and of the unnormalised output
     unsigned *counters;
     float *ws_ml, *ws_o;
 };
@@ -105,13 +113,52 @@ __device__ __forceinline__ typename Words<W>::type load_words(__amdgpu_buffer_rs
 __device__ __forceinline__ uint32_t word(uint32_t v, int) { return v; }
 template <typename V> __device__ __forceinline__ uint32_t word(const V &v, int i) { return v[i]; }
 
+// The schedule.  A unit is one sequence's KV head; its slots are tiles of 32.
+//   Few units: a work-group has one piece of a unit, all pieces of about the same size; a
+//   short unit is one piece.
+//   Others: the tiles of all units stand in one list, sequence after sequence, of which a
+//   work-group has `per` adjacent places, so the work is even whatever the sequences' lengths;
+//   it goes through pieces of one or more units.
+// A unit that lies in one work-group is finished there; the pieces of the others are merged
+// by the last of its work-groups to arrive.
+struct Piece {
+    int b, hk, L;              // the unit, and its sequence's length
+    int t0, t1;                // its tiles
+    int first, pieces, late;   // the unit's first work-group and number of pieces; `late`: the first
+                               // piece is its work-group's last one, not its first
+};
+
+// Tiles of a sequence; an empty one has one too, whose rows see nothing.
+__device__ __forceinline__ int paged_tiles(int len) { return max(1, (len + kTile - 1) / kTile); }
+// The sum over this lane and those before it (lane moves within rows of 16, then the rows'
+// last lanes to the rows behind)
+template <int CTRL, int ROWS> __device__ __forceinline__ int from_before(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_prefix(int v) {
+    v += from_before<0x111, 0xF>(v);
+    v += from_before<0x112, 0xF>(v);
+    v += from_before<0x114, 0xF>(v);
+    v += from_before<0x118, 0xF>(v);
+    v += from_before<0x142, 0xA>(v);
+    v += from_before<0x143, 0xC>(v);
+    return v;
+}
+// The arguments, read again where they are used: held in scalar registers over the loop they
+// would be spilled into vector lanes.
+template <typename A> __device__ __forceinline__ const A &late_args() {
+    typedef const A __attribute__((address_space(4))) *ptr;
+    ptr p = (ptr)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const A *)p;
+}
+
 // ------------------------------------------------------------------------
-// paged_attn_kernel -- a work-group has up to 16 query rows of a KV head and a run of its
-// slots; its 4 waves take 32 slots in turn.  Pages are multiples of 16 rows, so 16 slots
-// lie in one page: every load has its page's address in scalar registers, and a buffer
-// descriptor that ends with the page's (or the sequence's) last row, so rows behind it and
-// absent pages read as zeros and nothing is read there.  The pages' numbers of 32 turns are
-// fetched at once, a lane each.
+// paged_attn_kernel -- up to 16 query rows of a KV head; the waves take a piece's tiles in
+// turn.  Pages are multiples of 16 rows, so 16 slots lie in one page: every load has its
+// page's address in scalar registers, and a buffer descriptor that ends with the last row
+// that is there, so rows behind it and absent pages read as zeros and nothing is read
+// there.  The pages' numbers of 32 turns are fetched at once, a lane each.
 //   S = K Q^T (16x16x32 MFMA): K straight to registers, 16 bytes a lane; a lane then holds
 //   8 scores of one row, keys 16 t + 4 G + i (G = lane / 16): the row's maximum crosses
 //   lanes 16 and 32 apart only.
@@ -121,69 +168,108 @@ template <typename V> __device__ __forceinline__ uint32_t word(const V &v, int i
 // A part that is 0 times an infinite value is NaN, so is a masked NaN: a wave whose sums
 // are not finite goes over its keys again with the row maxima that it found, value by value
 // for the rows that see them.
-template <typename T, int PK, int HD>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
+template <typename T, int PK, int HD, int NWV>
+__global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
     typedef typename std::conditional<PK == kSame, T, bf16_t>::type C;       // the products' type
     typedef typename Mfma<C>::frag frag;
     typedef C c8 __attribute__((ext_vector_type(8)));
-    constexpr int NWV = 4, KB = 32, R = 16, NP = Parts<C>::N;
+    constexpr int KB = kTile, R = 16, NT = 64 * NWV, NP = Parts<C>::N;
     constexpr int B = PK == kSame ? 2 : 1;            // bytes of a cached value
     constexpr int KK = HD / 32, KL = HD * B / 64;     // MFMAs over a key, loads of 16 keys
     constexpr int DT = HD / 16, VW = DT * B / 4;      // columns of V a lane has, in dwords
     constexpr int NQ = PK != kSame && sizeof(T) == 2 && !std::is_same<T, bf16_t>::value ? 2 : 1;
     typedef typename Words<VW>::type vwords;
     constexpr int LD = HD + 4;                        // row stride of the waves' sums in LDS
-    __shared__ float so[NWV][R][LD], sm[NWV][R], sl[NWV][R];
+    __shared__ __attribute__((aligned(16))) float so[NWV][R][LD];
+    __shared__ float sm[NWV][R], sl[NWV][R];
+    __shared__ int s_last;
+    // (one word of each of the arguments' lines: they arrive together, not one after another)
+    asm volatile("" ::"s"(a.c.K), "s"(a.c.sv0), "s"(a.c.pages), "s"(a.Q), "s"(a.so1), "s"(a.ws_o));
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lr = lane & 15, G4 = lane >> 4;
 
-    // the row groups of a (sequence, KV head, split) run on one XCD, whose L2 then has the
-    // keys for all but the first
-    const int idx = blockIdx.x >> 3, unit = idx / a.row_groups * 8 + (blockIdx.x & 7), rg = idx % a.row_groups;
-    if (unit >= a.n * a.c.hkv * a.splits) return;
-    const int split = unit % a.splits, bh = unit / a.splits, b = bh / a.c.hkv, hk = bh % a.c.hkv;
+    // the row groups of a work-group's keys run on one XCD, whose L2 then has them for all but
+    // the first
+    const int idx = blockIdx.x >> 3, me = idx / a.row_groups * 8 + (blockIdx.x & 7), rg = idx % a.row_groups;
+    if (me >= a.groups) return;
     const int G = a.hq / a.c.hkv, rows_kv = G * a.l, r0 = rg * R, nrows = min(R, rows_kv - r0);
 
-    const int L = paged_len(a.c, a.kv_len, b);
-    // whole turns of the work-group, spread evenly over the sequence's splits
-    const int turns = (L + NWV * KB - 1) / (NWV * KB);
-    const int per = max(1, (turns + a.splits - 1) / a.splits), used = max(1, (turns + per - 1) / per);
-    if (split >= used) return;
-    const int kbeg = split * per * NWV * KB, kend = min(L, kbeg + per * NWV * KB);
-    const int free_end = L - a.l + 1;                 // slots below are seen by every row
+    // a lane has the lengths of 64 sequences at a time
+    auto len_of = [&](int x) __attribute__((always_inline)) { return x < a.n ? paged_len(a.c, a.kv_len, x) : 0; };
+    auto tiles_of = [&](int x, int len) __attribute__((always_inline)) { return x < a.n ? paged_tiles(len) : 0; };
+    int lens = len_of(lane), here = tiles_of(lane, lens), upto = wave_prefix(here);
+    int all = __builtin_amdgcn_readlane(upto, 63);
+    int per, cur = 0, stop = 0, x0 = 0, before = 0;
+    Piece p;
+    if (a.apart) {                                    // (n <= 64)
+        per = max(kPiece, (all * a.c.hkv + a.groups - a.n * a.c.hkv - 1) / (a.groups - a.n * a.c.hkv));
+        const int cut = here <= kWhole ? min(here, 1) : (here + per - 1) / per, ends = wave_prefix(cut);
+        if (me >= __builtin_amdgcn_readlane(ends, 63) * a.c.hkv) return;
+        p.b = __builtin_ctzll(__ballot(ends * a.c.hkv > me));
+        p.pieces = __builtin_amdgcn_readlane(cut, p.b);
+        p.L = __builtin_amdgcn_readlane(lens, p.b);
+        const int at = me - __builtin_amdgcn_readlane(ends - cut, p.b) * a.c.hkv, tiles = paged_tiles(p.L);
+        p.hk = at / p.pieces;
+        const int z = at - p.hk * p.pieces;
+        p.first = me - z;
+        p.late = 0;
+        p.t0 = (int)((int64_t)z * tiles / p.pieces);
+        p.t1 = (int)((int64_t)(z + 1) * tiles / p.pieces);
+    } else {
+        // (a unit begins with kSwitch places that no tile has)
+        for (int x = 64; x < a.n; x += 64) all += __builtin_amdgcn_readlane(wave_prefix(tiles_of(x + lane, len_of(x + lane))), 63);
+        all = (all + a.n * kSwitch) * a.c.hkv;
+        per = max(kSwitch + kLeast, (all + a.groups - 1) / a.groups);
+        cur = me * per;
+        if (cur >= all) return;
+        stop = cur + per;                             // (past the last tile for the last work-group)
+        uint64_t past;
+        auto places = [&](int x, int t) __attribute__((always_inline)) { return t + (min(x, a.n) - x0) * kSwitch; };
+        while (!(past = __ballot((before + places(x0 + lane + 1, upto)) * a.c.hkv > cur))) {      // (ends: cur < all)
+            before += places(x0 + 64, __builtin_amdgcn_readlane(upto, 63));
+            x0 += 64;
+            lens = len_of(x0 + lane);
+            here = tiles_of(x0 + lane, lens);
+            upto = wave_prefix(here);
+        }
+        p.b = x0 + __builtin_ctzll(past);
+        before += places(p.b, __builtin_amdgcn_readlane(upto - here, p.b - x0));
+        p.L = __builtin_amdgcn_readlane(lens, p.b - x0);
+        p.hk = (cur - before * a.c.hkv) / (paged_tiles(p.L) + kSwitch);
+    }
+    // the tiles of u among the places cur .. stop - 1
+    auto cut_out = [&](Piece &u) __attribute__((always_inline)) {
+        const int tiles = paged_tiles(u.L), unit0 = before * a.c.hkv + u.hk * (tiles + kSwitch), tile0 = unit0 + kSwitch;
+        u.t0 = max(cur - tile0, 0);
+        u.t1 = min(tiles, stop - tile0);
+        u.first = tile0 / per;
+        u.pieces = (tile0 + tiles - 1) / per - u.first + 1;
+        u.late = unit0 > u.first * per;
+        cur = tile0 + u.t1;
+    };
+    if (!a.apart) cut_out(p);
+    // the piece behind u, false if there is none
+    auto next_piece = [&](Piece &u) __attribute__((always_inline)) {
+        if (cur + kSwitch >= stop) return false;
+        if (++u.hk == a.c.hkv) {
+            before += paged_tiles(u.L) + kSwitch;
+            u.hk = 0;
+            if (++u.b == a.n) return false;
+            if (u.b == x0 + 64) {
+                x0 = u.b;
+                lens = len_of(x0 + lane);
+            }
+            u.L = __builtin_amdgcn_readlane(lens, u.b - x0);
+        }
+        cut_out(u);
+        return true;
+    };
 
-    // the query: row r0 + lr
+    // row r0 + lr of the KV head's list
     const int rr = r0 + lr;
     const bool row_ok = rr < rows_kv;
     const int h = row_ok ? rr / a.l : 0, pos = row_ok ? rr - h * a.l : 0;
-    const int last = L - a.l + pos;                   // the row's last slot
-    frag qf[NQ][KK];
-    {
-        const T *q = reinterpret_cast<const T *>(a.Q) + b * a.sq0 + (hk * G + h) * a.sq1 + pos * a.sq2;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            // (columns in the order of K's loads: 8-bit ones bring 16 columns, for two MFMAs)
-            const int d = B == 2 ? kk * 32 + G4 * 8 : (kk >> 1) * 64 + G4 * 16 + (kk & 1) * 8;
-            const u32x4 raw = row_ok && d < a.c.hd ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0};
-            if constexpr (NQ == 1) qf[0][kk] = as_frag<frag>(raw);
-            else {
-                // f16 as two bf16: 8 bits and the 3 behind them
-                typedef T t8 __attribute__((ext_vector_type(8)));
-                const t8 v = __builtin_bit_cast(t8, raw);
-                c8 hi, lo;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = to_f32(v[e]), top = Parts<bf16_t>::cut(x);
-                    hi[e] = (C)top;
-                    lo[e] = (C)(fabsf(x) < INFINITY ? x - top : 0.f);
-                }
-                qf[0][kk] = __builtin_bit_cast(frag, hi);
-                qf[1][kk] = __builtin_bit_cast(frag, lo);
-            }
-        }
-    }
-
     uint32_t offK[KL];
 #pragma unroll
     for (int j = 0; j < KL; ++j) {
@@ -194,64 +280,141 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) offV[i] = lr * DT < a.c.hd ? (uint32_t)(((4 * G4 + i) * a.c.sv2 + lr * DT) * B) : kOut;
 
-    // page numbers (-1: none) and rows of the 16-slot groups of 32 turns, a lane each
-    auto group_key = [&](int turn, int g) __attribute__((always_inline)) { return kbeg + (turn * NWV + wave) * KB + 16 * g; };
-    auto fetch = [&](int turn0, int &id, int &row) __attribute__((always_inline)) {
-        id = paged_find16(a.c.table + b * a.c.ld_table, a.c.page, a.c.pages, group_key(turn0 + (lane >> 1), lane & 1), kend, row);
-    };
-    int id_now, row_now, id_next, row_next, turn0 = 0;
-    fetch(0, id_now, row_now);
-    fetch(32, id_next, row_next);
+    const int64_t rowK = a.c.sk2 * B, rowV = a.c.sv2 * B;
+    constexpr int D4 = HD / 4;
 
-    struct Stage {
-        u32x4 k[2][KL];
-        vwords v[8];
-        f32x4 ks[2], vs[2];
-        int n[2];                                     // rows of the two groups that are there
+    // Where the 16-slot groups of 32 turns lie, a lane each: the rows that are there, the
+    // addresses of the first one's key, value and scales.  The next 32 turns' page numbers
+    // are on their way meanwhile.
+    auto group_key = [&](const Piece &u, int turn, int g) __attribute__((always_inline)) { return (u.t0 + turn * NWV + wave) * KB + 16 * g; };
+    int turn0 = 0;
+    struct Entries {
+        int entry, row;
+    } soon;
+    auto fetch = [&](const Piece &u, int from) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t rs_t = make_rsrc(a.c.table + u.b * a.c.ld_table, a.c.width * 4);
+        const int key = group_key(u, from + (lane >> 1), lane & 1);
+        Entries x;
+        const int at = paged_entry(key, a.c.page, a.c.div, x.row);
+        // (an entry behind the piece is out of the descriptor's reach: nothing is fetched)
+        x.entry = __builtin_amdgcn_raw_buffer_load_b32(rs_t, key < min(u.L, u.t1 * KB) ? at * 4 : (int)kOut, 0, 0);
+        return x;
     };
-    Stage st[2];
-    const char *Kp = reinterpret_cast<const char *>(a.c.K) + hk * a.c.sk1 * B, *Vp = reinterpret_cast<const char *>(a.c.V) + hk * a.c.sv1 * B;
-    auto issue = [&](int turn, Stage &s) __attribute__((always_inline)) {
+    u32x4 qr[KK];
+    auto load_q = [&](const Piece &u) __attribute__((always_inline)) {
+        const T *q = reinterpret_cast<const T *>(a.Q) + u.b * a.sq0 + (u.hk * G + h) * a.sq1 + pos * a.sq2;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            // (columns in the order of K's loads: 8-bit ones bring 16 columns, for two MFMAs)
+            const int d = B == 2 ? kk * 32 + G4 * 8 : (kk >> 1) * 64 + G4 * 16 + (kk & 1) * 8;
+            qr[kk] = row_ok && d < a.c.hd ? *reinterpret_cast<const u32x4 *>(q + d) : u32x4{0, 0, 0, 0};
+        }
+    };
+    struct Groups {
+        int n;
+        uint64_t k, v, ks, vs;
+    } now;
+    auto locate = [&](const Piece &u, const Entries &x) __attribute__((always_inline)) {
+        const int key = group_key(u, turn0 + (lane >> 1), lane & 1), id = paged_id(x.entry, a.c.pages);
+        const int64_t page = max(id, 0);
+        now.n = paged_rows16(id, key, min(u.L, u.t1 * KB));
+        now.k = reinterpret_cast<uint64_t>(a.c.K) + (page * a.c.sk0 + u.hk * a.c.sk1 + x.row * a.c.sk2) * B;
+        now.v = reinterpret_cast<uint64_t>(a.c.V) + (page * a.c.sv0 + u.hk * a.c.sv1 + x.row * a.c.sv2) * B;
+        if constexpr (PK != kSame) {
+            now.ks = reinterpret_cast<uint64_t>(a.c.ks + page * a.c.sks0 + u.hk * a.c.sks1 + x.row);
+            now.vs = reinterpret_cast<uint64_t>(a.c.vs + page * a.c.svs0 + u.hk * a.c.svs1 + x.row);
+        }
+        soon = fetch(u, turn0 + 32);
+    };
+    auto address = [&](uint64_t x, int from) __attribute__((always_inline)) {
+        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, from), hi = __builtin_amdgcn_readlane((uint32_t)(x >> 32), from);
+        return reinterpret_cast<const char *>((uint64_t)hi << 32 | lo);
+    };
+
+    // One tile of keys and of values: a tile's registers are loaded again as soon as its
+    // product has read them.
+    u32x4 kr[2][KL];
+    vwords vr[8];
+    f32x4 ks[2], vs[2];
+    int there[2];                                     // rows of the two groups that are there
+    auto issue_k = [&](int turn) __attribute__((always_inline)) {
         if (turn >= turn0 + 32) {
             turn0 += 32;
-            id_now = id_next;
-            row_now = row_next;
-            fetch(turn0 + 32, id_next, row_next);
+            locate(p, soon);
         }
-        __amdgpu_buffer_rsrc_t rv[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int from = 2 * (turn - turn0) + t;
-            const int id = __builtin_amdgcn_readlane(id_now, from), row = __builtin_amdgcn_readlane(row_now, from);
-            const int m = s.n[t] = paged_rows16(id, group_key(turn, t), kend);
-            const int64_t page = max(id, 0);
-            const __amdgpu_buffer_rsrc_t rk =
-                make_rsrc(Kp + (page * a.c.sk0 + row * a.c.sk2) * B, m ? (uint32_t)(((m - 1) * a.c.sk2 + a.c.hd) * B) : 0u);
-            rv[t] = make_rsrc(Vp + (page * a.c.sv0 + row * a.c.sv2) * B, m ? (uint32_t)(((m - 1) * a.c.sv2 + a.c.hd) * B) : 0u);
+            const int m = there[t] = __builtin_amdgcn_readlane(now.n, from);
+            const __amdgpu_buffer_rsrc_t rk = make_rsrc(address(now.k, from), m ? (uint32_t)((m - 1) * rowK) + a.c.hd * B : 0u);
 #pragma unroll
-            for (int j = 0; j < KL; ++j) s.k[t][j] = load_words<4>(rk, offK[j]);
-            if constexpr (PK != kSame) {
-                s.ks[t] = __builtin_bit_cast(f32x4, load_words<4>(make_rsrc(a.c.ks + page * a.c.sks0 + hk * a.c.sks1 + row, m * 4), G4 * 16));
-                s.vs[t] = __builtin_bit_cast(f32x4, load_words<4>(make_rsrc(a.c.vs + page * a.c.svs0 + hk * a.c.svs1 + row, m * 4), G4 * 16));
-            }
+            for (int j = 0; j < KL; ++j) kr[t][j] = load_words<4>(rk, offK[j]);
+            if constexpr (PK != kSame)
+                ks[t] = __builtin_bit_cast(f32x4, load_words<4>(make_rsrc(address(now.ks, from), m * 4), G4 * 16));
         }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // (behind issue_k of the same turn)
+    auto issue_v = [&](int turn) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s.v[j] = load_words<VW>(rv[j >> 2], offV[j & 3]);
+        for (int t = 0; t < 2; ++t) {
+            const int from = 2 * (turn - turn0) + t, m = there[t];
+            const __amdgpu_buffer_rsrc_t rv = make_rsrc(address(now.v, from), m ? (uint32_t)((m - 1) * rowV) + a.c.hd * B : 0u);
+            if constexpr (PK != kSame)
+                vs[t] = __builtin_bit_cast(f32x4, load_words<4>(make_rsrc(address(now.vs, from), m * 4), G4 * 16));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) vr[4 * t + j] = load_words<VW>(rv, offV[j]);
+        }
         __builtin_amdgcn_sched_barrier(0);
     };
 
+    {
+        const Entries x = fetch(p, 0);
+        load_q(p);
+        locate(p, x);
+        issue_k(0);
+        issue_v(0);
+    }
+    for (;;) {
+    Piece then = p;
+    const bool more = !a.apart && next_piece(then);
+    Entries later{};
+    if (more) later = fetch(then, 0);
+    const int free_end = p.L - a.l + 1;               // slots below are seen by every row
+    const int last = p.L - a.l + pos;                 // the row's last slot
+    const int mine = (p.t1 - p.t0 - wave + NWV - 1) / NWV;  // turns of this wave
+    frag qf[NQ][KK];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+        if constexpr (NQ == 1) qf[0][kk] = as_frag<frag>(qr[kk]);
+        else {
+            // f16 as two bf16: 8 bits and the 3 behind them
+            typedef T t8 __attribute__((ext_vector_type(8)));
+            const t8 v = __builtin_bit_cast(t8, qr[kk]);
+            c8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = to_f32(v[e]), top = Parts<bf16_t>::cut(x);
+                hi[e] = (C)top;
+                lo[e] = (C)(fabsf(x) < INFINITY ? x - top : 0.f);
+            }
+            qf[0][kk] = __builtin_bit_cast(frag, hi);
+            qf[1][kk] = __builtin_bit_cast(frag, lo);
+        }
+    }
+
     // scores of a turn, scales of K in them: (t, i) is slot k0 + 16 t + 4 G4 + i; unseen ones -inf
-    auto scores = [&](int turn, const Stage &s, f32x4 *sc) __attribute__((always_inline)) {
-        const int k0 = group_key(turn, 0);
+    auto scores = [&](int turn, f32x4 *sc) __attribute__((always_inline)) {
+        const int k0 = group_key(p, turn, 0);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
                 u32x4 kw;
-                if constexpr (PK == kSame) kw = s.k[t][kk];
+                if constexpr (PK == kSame) kw = kr[t][kk];
                 else {
-                    const uint32_t w0 = s.k[t][kk >> 1][2 * (kk & 1)], w1 = s.k[t][kk >> 1][2 * (kk & 1) + 1];
+                    const uint32_t w0 = kr[t][kk >> 1][2 * (kk & 1)], w1 = kr[t][kk >> 1][2 * (kk & 1) + 1];
                     kw = u32x4{pair_of<PK, 0>(w0), pair_of<PK, 1>(w0), pair_of<PK, 0>(w1), pair_of<PK, 1>(w1)};
                 }
 #pragma unroll
@@ -259,15 +422,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             }
             if constexpr (PK != kSame) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sc[t][i] *= s.ks[t][i];
+                for (int i = 0; i < 4; ++i) sc[t][i] *= ks[t][i];
             }
         }
-        if (k0 + KB > free_end || s.n[0] + s.n[1] < KB) {
+        if (k0 + KB > free_end || there[0] + there[1] < KB) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (4 * G4 + i >= s.n[t] || k0 + 16 * t + 4 * G4 + i > last) sc[t][i] = -INFINITY;
+                    if (4 * G4 + i >= there[t] || k0 + 16 * t + 4 * G4 + i > last) sc[t][i] = -INFINITY;
         }
     };
 
@@ -275,9 +438,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     float m_used = -INFINITY, l_run = 0.f;
 #pragma unroll
     for (int c = 0; c < DT; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto step = [&](int turn, const Stage &s) __attribute__((always_inline)) {
+    for (int turn = 0; turn < mine; ++turn) {
         f32x4 sc[2];
-        scores(turn, s, sc);
+        scores(turn, sc);
+        __builtin_amdgcn_sched_barrier(0);
+        issue_k(turn + 1);
         float mx = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -302,7 +467,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             for (int i = 0; i < 4; ++i) {
                 float p = fast_exp2(__builtin_fmaf(sc[t][i], a.scale_log2, -mref));
                 l_run += p;
-                if constexpr (PK != kSame) p *= s.vs[t][i];
+                if constexpr (PK != kSame) p *= vs[t][i];
                 C x[NP];
                 Parts<C>::split(p, x);
 #pragma unroll
@@ -314,10 +479,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if constexpr (PK == kSame) {
-                    const uint32_t lo = word(s.v[2 * e], c >> 1), hi = word(s.v[2 * e + 1], c >> 1);
+                    const uint32_t lo = word(vr[2 * e], c >> 1), hi = word(vr[2 * e + 1], c >> 1);
                     w[e] = c & 1 ? __builtin_amdgcn_perm(hi, lo, 0x07060302u) : __builtin_amdgcn_perm(hi, lo, 0x05040100u);
                 } else {
-                    const uint32_t lo = word(s.v[2 * e], c >> 2), hi = word(s.v[2 * e + 1], c >> 2);
+                    const uint32_t lo = word(vr[2 * e], c >> 2), hi = word(vr[2 * e + 1], c >> 2);
                     switch (c & 3) {
                         case 0: w[e] = pair_across<PK, 0>(lo, hi); break;
                         case 1: w[e] = pair_across<PK, 1>(lo, hi); break;
@@ -329,18 +494,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
 #pragma unroll
             for (int y = 0; y < NP; ++y) o[c] = Mfma<C>::m16(as_frag<frag>(w), __builtin_bit_cast(frag, part[y]), o[c]);
         }
-    };
-
-    // turns of this wave whose first slot is below kend
-    const int mine = (kend - kbeg - wave * KB + NWV * KB - 1) / (NWV * KB);
-    issue(0, st[0]);
-    for (int turn = 0; turn < mine; turn += 2) {
-        issue(turn + 1, st[1]);
-        step(turn, st[0]);
         __builtin_amdgcn_sched_barrier(0);
-        issue(turn + 2, st[0]);
-        if (turn + 1 < mine) step(turn + 1, st[1]);
-        __builtin_amdgcn_sched_barrier(0);
+        issue_v(turn + 1);
     }
 
     float z = 0.f;                  // stays 0 if every sum is finite
@@ -353,25 +508,24 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
         for (int c = 0; c < DT; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
         const float mref = m_used == -INFINITY ? 0.f : m_used + Shift<C>::value;
         turn0 = 0;
-        fetch(0, id_now, row_now);
-        fetch(32, id_next, row_next);
+        locate(p, fetch(p, 0));
         for (int turn = 0; turn < mine; ++turn) {
-            issue(turn, st[0]);
+            issue_k(turn);
+            issue_v(turn);
             f32x4 sc[2];
-            scores(turn, st[0], sc);
-            const int k0 = group_key(turn, 0);
+            scores(turn, sc);
+            const int k0 = group_key(p, turn, 0);
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
                 float p = fast_exp2(__builtin_fmaf(sc[x >> 2][x & 3], a.scale_log2, -mref));
-                if constexpr (PK != kSame) p *= st[0].vs[x >> 2][x & 3];
+                if constexpr (PK != kSame) p *= vs[x >> 2][x & 3];
                 const int from = 2 * (turn - turn0) + (x >> 2);
-                const int64_t page = max(0, __builtin_amdgcn_readlane(id_now, from));
-                const int row = __builtin_amdgcn_readlane(row_now, from);
+                const char *vfirst = address(now.v, from);
                 for (int g = 0; g < 4; ++g) {
                     const int at = 4 * g + (x & 3);
                     const float pk = __shfl(p, g * 16 + lr, 64);
-                    if (at >= st[0].n[x >> 2] || !row_ok || k0 + 16 * (x >> 2) + at > last) continue;
-                    const char *vp = Vp + (page * a.c.sv0 + (int64_t)(row + at) * a.c.sv2) * B;
+                    if (at >= there[x >> 2] || !row_ok || k0 + 16 * (x >> 2) + at > last) continue;
+                    const char *vp = vfirst + at * rowV;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -386,6 +540,16 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                 }
             }
         }
+    }
+
+    // the next piece's query, addresses and (behind the stores below) first keys are on their
+    // way while this one is finished
+    const Piece u = p;
+    if (more) {
+        p = then;
+        turn0 = 0;
+        load_q(p);
+        locate(p, later);
     }
 
     // the waves' sums merge through LDS; lanes of a row hold disjoint keys
@@ -403,27 +567,31 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     }
     __syncthreads();
 
-    constexpr int D4 = HD / 4;
+    const PagedArgs &e = late_args<PagedArgs>();
     auto store_row = [&](int r, int d, f32x4 v, float m, float ls) __attribute__((always_inline)) {
         typedef T t4 __attribute__((ext_vector_type(4)));
-        const int head = hk * G + (r0 + r) / a.l, i = (r0 + r) % a.l;
+        const int head = u.hk * G + (r0 + r) / e.l, i = (r0 + r) % e.l;
         const float inv = ls != 0.f ? 1.f / ls : 0.f;
-        if (d < a.c.hd) {
+        if (d < e.c.hd) {
             t4 w;
 #pragma unroll
             for (int y = 0; y < 4; ++y) w[y] = from_f32<T>(v[y] * inv);
-            *reinterpret_cast<t4 *>(reinterpret_cast<T *>(a.O) + b * a.so0 + head * a.so1 + i * a.so2 + d) = w;
+            *reinterpret_cast<t4 *>(reinterpret_cast<T *>(e.O) + u.b * e.so0 + head * e.so1 + i * e.so2 + d) = w;
         }
-        if (a.lse && d == 0) a.lse[((int64_t)b * a.hq + head) * a.l + i] = ls != 0.f ? (m + __log2f(ls)) * kLn2 : -INFINITY;
+        if (e.lse && d == 0) e.lse[((int64_t)u.b * e.hq + head) * e.l + i] = ls != 0.f ? (m + __log2f(ls)) * kLn2 : -INFINITY;
     };
-    // the splits' states of this row group, agent-coherent (sc1): written through the XCD's L2
-    // and read past it, as the work-group that merges them may run on another XCD
-    const int group = bh * a.row_groups + rg;
-    const int64_t slot0 = (int64_t)group * a.splits * R;
-    const bool alone = used == 1;
-    const __amdgpu_buffer_rsrc_t rs_o = make_rsrc(alone ? nullptr : a.ws_o + slot0 * HD, alone ? 0u : (uint32_t)a.splits * R * HD * 4);
-    const __amdgpu_buffer_rsrc_t rs_ml = make_rsrc(alone ? nullptr : a.ws_ml + slot0 * 2, alone ? 0u : (uint32_t)a.splits * R * 8);
-    for (int x = tid; x < nrows * D4; x += NWV * 64) {
+
+    // Pieces of a unit that several work-groups have: their states, agent-coherent (sc1), are
+    // written through the XCD's L2 and read past it, as the work-group that merges them may
+    // run on another XCD.  A work-group has two such pieces at most, its first and its last.
+    const bool alone = u.pieces == 1;
+    const __amdgpu_buffer_rsrc_t rs_o = make_rsrc(alone ? nullptr : e.ws_o, alone ? 0u : 0x7fffffffu);
+    const __amdgpu_buffer_rsrc_t rs_ml = make_rsrc(alone ? nullptr : e.ws_ml, alone ? 0u : 0x7fffffffu);
+    // the rows of piece z: its owner's first piece, unless the unit begins behind the owner's first tile
+    auto state = [&](int z) __attribute__((always_inline)) {
+        return (((u.first + z) * e.row_groups + rg) * 2 + (z == 0 ? u.late : 0)) * R;
+    };
+    for (int x = tid; x < nrows * D4; x += NT) {
         const int r = x / D4, d = x % D4 * 4;
         float mm = -INFINITY;
 #pragma unroll
@@ -443,93 +611,126 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             store_row(r, d, oo, mm, ll);
             continue;
         }
-        const int at = split * R + r;
+        const int at = state(me - u.first) + r;
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, oo), rs_o, (at * HD + d) * 4, 0, kSc1Aux);
         if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{mm, ll}), rs_ml, at * 8, 0, kSc1Aux);
     }
-    if (alone) return;
-
-    // The last of the row group's work-groups to arrive merges the splits, in their order
-    // (the same bits whatever the order of arrival).  Every thread waits for its stores'
-    // acknowledgements before the barrier that precedes the counter's agent-scope addition.
-    __shared__ int s_last;
-    __shared__ float s_w[R][kMaxSplits], s_M[R], s_L[R];
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    unsigned *ctr = a.counters + (int64_t)group * kCounterStride;
-    if (tid == 0) s_last = __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(used - 1);
-    __syncthreads();
-    if (!s_last) return;
-    for (int r = wave; r < nrows; r += NWV) {
-        u32x2 ml = {__float_as_uint(-INFINITY), 0u};
-        if (lane < used) ml = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs_ml, (lane * R + r) * 8, 0, kSc1Aux));
-        const float mz = __uint_as_float(ml[0]), M = wave_max(mz), Mu = M == -INFINITY ? 0.f : M;
-        const float w = fast_exp2(mz - Mu);
-        s_w[r][lane] = w;
-        const float Ls = wave_sum(w * __uint_as_float(ml[1]));
-        if (lane == 0) {
-            s_M[r] = M;
-            s_L[r] = Ls;
-        }
+    if (!alone) {
+        // Every thread waits for its stores' acknowledgements before the barrier that precedes
+        // the counter's agent-scope addition.
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_s_waitcnt(0);
     }
-    __syncthreads();
-    for (int x = tid; x < nrows * D4; x += NWV * 64) {
-        const int r = x / D4, d = x % D4 * 4;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int z0 = 0; z0 < used; z0 += 16) {
-            f32x4 ov[16];
+    if (more) {
+        issue_k(0);
+        issue_v(0);
+    }
+    if (!alone) {
+        __syncthreads();
+        unsigned *ctr = e.counters + (int64_t)(u.first * e.row_groups + rg) * kCounterStride;
+        if (tid == 0) s_last = __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(u.pieces - 1);
+        __syncthreads();
+        if (s_last) {
+            // Merged in the pieces' order, the same bits whatever the order of arrival.  A thread
+            // has 4 columns of a row; threads to spare share the pieces and join through LDS.
+            const int items = nrows * D4, share = max(1, min(NT / items, u.pieces / 2));
+            for (int x0 = 0; x0 < items; x0 += NT) {
+                const int zg = share > 1 ? tid / items : 0, x = x0 + tid - zg * items;
+                const int r = x / D4, d = x % D4 * 4;
+                const bool on = x < items && zg < share;
+                float m = -INFINITY, ls = 0.f;
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                constexpr int Z = 8;
+                for (int z0 = zg; on && z0 < u.pieces; z0 += Z * share) {
+                    f32x4 ov[Z];
+                    f32x2 ml[Z];
 #pragma unroll
-            for (int z = 0; z < 16; ++z)
-                // (splits that are not there: past the end of the descriptor, no memory is read)
-                ov[z] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                      rs_o, z0 + z < used ? (((z0 + z) * R + r) * HD + d) * 4 : (int)kOut, 0, kSc1Aux));
+                    for (int z = 0; z < Z; ++z) {
+                        // (pieces that are not there: past the end of the descriptor, no memory is read)
+                        const int y = z0 + z * share, at = state(y) + r;
+                        ov[z] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs_o, y < u.pieces ? (at * HD + d) * 4 : (int)kOut, 0, kSc1Aux));
+                        ml[z] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rs_ml, y < u.pieces ? at * 8 : (int)kOut, 0, kSc1Aux));
+                    }
+                    float mx = m;
 #pragma unroll
-            for (int z = 0; z < 16; ++z) {
-                const float w = z0 + z < used ? s_w[r][z0 + z] : 0.f;
+                    for (int z = 0; z < Z; ++z) {
+                        if (z0 + z * share >= u.pieces) ml[z][0] = -INFINITY;
+                        mx = fmaxf(mx, ml[z][0]);
+                    }
+                    const float mu = mx == -INFINITY ? 0.f : mx, keep = fast_exp2(m - mu);
+                    ls *= keep;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(w, ov[z][i], acc[i]);
+                    for (int i = 0; i < 4; ++i) acc[i] *= keep;
+#pragma unroll
+                    for (int z = 0; z < Z; ++z) {
+                        const float w = fast_exp2(ml[z][0] - mu);
+                        ls = __builtin_fmaf(w, ml[z][1], ls);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(w, ov[z][i], acc[i]);
+                    }
+                    m = mx;
+                }
+                if (share > 1) {
+                    // (the waves' sums there were read before the counter's barrier)
+                    float *slots = &so[0][0][0];
+                    static_assert(sizeof(so) >= NT * 32, "8 words a thread");
+                    *reinterpret_cast<f32x4 *>(slots + tid * 8) = acc;
+                    *reinterpret_cast<f32x2 *>(slots + tid * 8 + 4) = f32x2{m, ls};
+                    __syncthreads();
+                    for (int g = 1; g < share && tid < items; ++g) {
+                        const f32x4 ov = *reinterpret_cast<const f32x4 *>(slots + (tid + g * items) * 8);
+                        const f32x2 ml = *reinterpret_cast<const f32x2 *>(slots + (tid + g * items) * 8 + 4);
+                        const float mx = fmaxf(m, ml[0]), mu = mx == -INFINITY ? 0.f : mx;
+                        const float w0 = fast_exp2(m - mu), w1 = fast_exp2(ml[0] - mu);
+                        ls = ls * w0 + ml[1] * w1;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[i] = acc[i] * w0 + ov[i] * w1;
+                        m = mx;
+                    }
+                }
+                if (x < items && zg == 0) store_row(r, d, acc, m, ls);
             }
+            if (tid == 0) __hip_atomic_store(ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        store_row(r, d, acc, s_M[r], s_L[r]);
     }
-    if (tid == 0) __hip_atomic_store(ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!more) break;
+    __syncthreads();
+    }
 }
 
 // ------------------------------------------------------------- host side
 
 struct PagedPlan {
-    int row_groups, splits;
-    int64_t units;
+    int row_groups, groups, apart;
     size_t counter_bytes, ml_bytes, o_bytes;
 };
 
-constexpr int kCUs = 256;
-// The counters' part of a workspace, the same for calls of all sizes: groups that are split
-// are at most one a CU.
-constexpr size_t kCounterBytes = (size_t)kCUs * kCounterStride * 4;
+constexpr int kWaves = 4;
+constexpr int kMaxGroups = 256;
+// The counters' part of a workspace, the same for calls of all sizes
+constexpr size_t kCounterBytes = (size_t)kMaxGroups * kCounterStride * 4;
 
 PagedPlan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t slots, int64_t hd) {
     PagedPlan p{};
-    const int64_t rows = hq / hkv * l;
-    p.row_groups = (int)cdiv(rows, 16);
-    const int64_t groups = n * hkv * p.row_groups;
-    // two work-groups a CU, of a turn (128 slots) at least
-    p.splits = (int)std::max<int64_t>(1, std::min({(int64_t)kMaxSplits, 2 * kCUs / std::max<int64_t>(groups, 1), cdiv(slots, 128)}));
-    p.units = n * hkv * p.splits;
-    if (p.splits > 1) {
+    p.row_groups = (int)cdiv(hq / hkv * l, 16);
+    // no more work-groups than full tables have tiles for
+    const int64_t tiles = n * hkv * std::max<int64_t>(1, cdiv(slots, kTile));
+    p.groups = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxGroups / p.row_groups, tiles));
+    p.apart = n * hkv * 8 <= p.groups;
+    if (p.groups > 1) {
+        const size_t states = (size_t)p.groups * p.row_groups * 2 * 16;
         p.counter_bytes = kCounterBytes;
-        p.ml_bytes = (size_t)groups * p.splits * 16 * 8;
-        p.o_bytes = (size_t)groups * p.splits * 16 * (hd <= 64 ? 64 : 128) * 4;
+        p.ml_bytes = states * 8;
+        p.o_bytes = states * (hd <= 64 ? 64 : 128) * 4;
     }
     return p;
 }
 
 template <typename T, int PK>
 void launch_paged(const PagedArgs &a, const PagedPlan &p, hipStream_t st) {
-    const dim3 grid((unsigned)(cdiv(p.units, 8) * 8 * p.row_groups));
-    if (a.c.hd <= 64) hipLaunchKernelGGL((paged_attn_kernel<T, PK, 64>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_attn_kernel<T, PK, 128>), grid, dim3(256), 0, st, a);
+    const dim3 grid((unsigned)(cdiv(p.groups, 8) * 8 * p.row_groups));
+    if (a.c.hd <= 64) hipLaunchKernelGGL((paged_attn_kernel<T, PK, 64, kWaves>), grid, dim3(64 * kWaves), 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<T, PK, 128, kWaves>), grid, dim3(64 * kWaves), 0, st, a);
 }
 
 template <typename T>
@@ -565,14 +766,15 @@ extern "C" int kuiops_sdpa_paged(int64_t n, int64_t hq, int64_t l, int dtype, co
     if (!aligned16(Q) || (reinterpret_cast<uintptr_t>(O) & 7)) return KUIOPS_E_UNSUPPORTED;
     for (int i = 0; i < 3; ++i)
         if (sq[i] % 8 || so[i] % 4) return KUIOPS_E_UNSUPPORTED;
-    // 32-bit indices of rows and work-groups, launches below 2^32 threads
-    const int64_t rows = hq / at->hkv * l;
-    if (l >= (1 << 24) || rows >= (1 << 24) || n * hq * l >= ((int64_t)1 << 31) || n * at->hkv >= (1 << 20)) return KUIOPS_E_UNSUPPORTED;
-    const PagedPlan p = plan_of(n, hq, at->hkv, l, at->width * at->page, at->hd);
-    if (cdiv(p.units, 8) * 8 * p.row_groups >= ((int64_t)1 << 24)) return KUIOPS_E_UNSUPPORTED;
+    // 32-bit indices of rows and tiles, launches below 2^32 threads
+    const int64_t rows = hq / at->hkv * l, slots = at->width * at->page;
+    if (l >= (1 << 24) || rows >= (1 << 24) || n * hq * l >= ((int64_t)1 << 31) ||
+        n * at->hkv >= (1 << 20) || n * at->hkv * (slots / kTile + 1 + kSwitch) >= ((int64_t)1 << 30))
+        return KUIOPS_E_UNSUPPORTED;
+    const PagedPlan p = plan_of(n, hq, at->hkv, l, slots, at->hd);
     const size_t need = p.counter_bytes + p.ml_bytes + p.o_bytes;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KUIOPS_E_WORKSPACE;
-    a.n = (int)n; a.hq = (int)hq; a.l = (int)l; a.splits = p.splits; a.row_groups = p.row_groups;
+    a.n = (int)n; a.hq = (int)hq; a.l = (int)l; a.groups = p.groups; a.apart = p.apart; a.row_groups = p.row_groups;
     a.Q = Q; a.O = O;
     a.sq0 = sq[0]; a.sq1 = sq[1]; a.sq2 = sq[2];
     a.so0 = so[0]; a.so1 = so[1]; a.so2 = so[2];

@@ -21,19 +21,33 @@ KUIOPS_HOST_DEVICE int paged_slots(int len, int width, int page) {
 // An entry of the table that is no page of the pool is -1.
 KUIOPS_HOST_DEVICE int paged_id(int entry, int pages) { return (unsigned)entry < (unsigned)pages ? entry : -1; }
 
-// The page of a slot (-1: none) and its row there.  Nothing behind the table's row is read.
-KUIOPS_HOST_DEVICE int paged_find(const int32_t *row, int width, int page, int pages, int slot, int &at) {
-    const int p = slot / page;
+// x / d as (x * mul) >> shift for x below 2^26: mul = ceil(2^shift / d) with shift = 26 + ceil(log2 d),
+// whose excess mul * d - 2^shift < d <= 2^(shift - 26) never reaches the next quotient.
+struct PageDiv {
+    uint32_t mul;
+    int32_t shift;
+};
+inline PageDiv paged_div(int d) {
+    int s = 0;
+    while ((1 << s) < d) ++s;
+    return {(uint32_t)((((uint64_t)1 << (26 + s)) + d - 1) / d), 26 + s};
+}
+KUIOPS_HOST_DEVICE int paged_quotient(int x, PageDiv d) { return (int)((uint64_t)(uint32_t)x * d.mul >> d.shift); }
+
+// Which entry of its row of the table a slot (>= 0) has, and which row of that page; `div`
+// divides by a page's 16-slot groups.  For 16 slots from a multiple of 16 on it is the same
+// page, whose size is a multiple too.
+KUIOPS_HOST_DEVICE int paged_entry(int slot, int page, PageDiv div, int &at) {
+    const int p = paged_quotient(slot >> 4, div);
     at = slot - p * page;
-    return slot >= 0 && p < width ? paged_id(row[p], pages) : -1;
+    return p;
 }
 
-// The same for the 16 slots from `slot` on (a multiple of 16, pages are too), as long as some
-// of them lie below `end` (at most the sequence's slots).
-KUIOPS_HOST_DEVICE int paged_find16(const int32_t *row, int page, int pages, int slot, int end, int &at) {
-    const int gpp = page / 16, g = slot / 16, p = g / gpp;
-    at = (g - p * gpp) * 16;
-    return slot >= 0 && slot < end ? paged_id(row[p], pages) : -1;
+// The page of a slot (-1: none) and its row there.  Nothing outside the table's row is read.
+KUIOPS_HOST_DEVICE int paged_find(const int32_t *row, int width, int page, PageDiv div, int pages, int slot, int &at) {
+    const bool in = slot >= 0 && slot < width * page;
+    const int p = paged_entry(in ? slot : 0, page, div, at);
+    return in ? paged_id(row[p], pages) : -1;
 }
 
 // How many of the 16 slots from `slot` on are there.

@@ -82,8 +82,10 @@ def index(tmp_path_factory):
     (at / "index.cpp").write_text('#include "paged_index.hpp"\nextern "C" {\n'
                                   "int slots(int a, int b, int c) { return kuiops::paged_slots(a, b, c); }\n"
                                   "int rows16(int a, int b, int c) { return kuiops::paged_rows16(a, b, c); }\n"
-                                  "int find(const int32_t *r, int w, int p, int n, int s, int *at) { return kuiops::paged_find(r, w, p, n, s, *at); }\n"
-                                  "int find16(const int32_t *r, int p, int n, int s, int e, int *at) { return kuiops::paged_find16(r, p, n, s, e, *at); }\n}\n")
+                                  "int find(const int32_t *r, int w, int p, int n, int s, int *at) { return kuiops::paged_find(r, w, p, kuiops::paged_div(p / 16), n, s, *at); }\n"
+                                  "int entry(int s, int p, int *at) { return kuiops::paged_entry(s, p, kuiops::paged_div(p / 16), *at); }\n"
+                                  "int id(int e, int n) { return kuiops::paged_id(e, n); }\n"
+                                  "int quotient(int x, int d) { return kuiops::paged_quotient(x, kuiops::paged_div(d)); }\n}\n")
     subprocess.run([gxx, "-std=c++17", "-shared", "-fPIC", f"-I{C.CSRC}", "-o", str(at / "index.so"), str(at / "index.cpp")], check=True)
     return ctypes.CDLL(str(at / "index.so"))
 
@@ -110,7 +112,9 @@ def test_every_slot_lies_in_the_pool_or_nowhere(index, page, width, pages):
         end = index.slots(length, width, page)
         assert end == min(max(length, 0), width * page)
         for slot in [s // 16 * 16 for s in slots]:
-            got = index.find16(ptr, page, pages, slot, end, ctypes.byref(at))
+            # (as the attention does: the entry of a slot at or behind the end is not fetched)
+            p = index.entry(max(slot, 0), page, ctypes.byref(at))
+            got = index.id(int(row[p]), pages) if 0 <= slot < end else -1
             n = index.rows16(got, slot, end)
             assert 0 <= n <= 16
             if got >= 0:
@@ -119,6 +123,16 @@ def test_every_slot_lies_in_the_pool_or_nowhere(index, page, width, pages):
                 assert O.paged_slot(row, page, pages, slot + i) == (got, at.value + i) and slot + i < end
             for i in range(n, 16):          # the others have no page or lie behind the sequence
                 assert slot + i >= end or slot < 0 or O.paged_slot(row, page, pages, slot + i) is None
+
+
+def test_the_quotient_is_exact(index):
+    # below 2^26 (2^30 slots in groups of 16), by up to 2^16 groups of a page
+    g = np.random.default_rng(0)
+    for d in [1, 2, 3, 5, 7, 31, 32, 33, 1000, 4095, 4097, 32768, 32769, 65535, 65536] + g.integers(1, 65537, 200).tolist():
+        top = 2 ** 26 - 1
+        for x in [0, 1, d - 1, d, d + 1, top, top // d * d, top // d * d - 1] + g.integers(0, top + 1, 50).tolist():
+            if 0 <= x <= top:
+                assert index.quotient(x, d) == x // d, (x, d)
 
 
 # ---------------------------------------------------------------- refusals
@@ -280,7 +294,7 @@ def test_c_entries_refuse_on_the_host(lib):
     assert attn(hq=3) == attn(q=null) == attn(ln=null) == INVALID
     assert attn(sm=0.0) == attn(sm=-1.0) == attn(sm=float("nan")) == attn(sm=float("inf")) == UNSUPPORTED
     assert attn(q=off) == attn(sq=_lib.strides3(0, 0, 60)) == UNSUPPORTED
-    assert attn(n=1 << 19) == attn(l=1 << 24) == attn(hq=1 << 20, l=1 << 10) == UNSUPPORTED
+    assert attn(n=1 << 19) == attn(n=1 << 18, width=1 << 16) == attn(l=1 << 24) == attn(hq=1 << 20, l=1 << 10) == UNSUPPORTED
     assert attn(l=0) == attn(hq=0) == append(t=0) == read(s=0) == _lib.OK
     assert append(x=null) == append(f=null) == append(eps=-1.0) == append(eps=float("nan")) == INVALID
     assert append(ld=500) == append(x=off) == append(w=off) == append(n=1 << 16) == append(t=1 << 24) == UNSUPPORTED
@@ -294,9 +308,9 @@ def test_c_entries_refuse_on_the_host(lib):
 
 def test_workspace_sizes(lib):
     f = lib.kuiops_sdpa_paged_workspace
-    for args in ((0, 4, 2, 1, 48, 64), (2, 4, 2, 1, 0, 64), (2, 3, 2, 1, 48, 64), (2, 4, 0, 1, 48, 64), (64, 32, 8, 1, 8000, 128), (1, 4, 4, 1, 128, 64)):
+    for args in ((0, 4, 2, 1, 48, 64), (2, 4, 2, 1, 0, 64), (2, 3, 2, 1, 48, 64), (2, 4, 0, 1, 48, 64), (1, 4, 1, 1, 32, 64)):
         assert f(*args) == 0
-    assert f(1, 32, 8, 1, 1 << 20, 128) <= 8 << 20
+    assert f(1, 32, 8, 1, 1 << 20, 128) <= 10 << 20
 
 
 # ------------------------------------------------------------- custom ops
