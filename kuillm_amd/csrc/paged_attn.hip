@@ -7,6 +7,7 @@
 // per row.  Rows of the query heads that share a KV head are one list (row = head in
 // group * l + position), so K and V are read once for all of them.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.hpp"
 
@@ -30,12 +31,15 @@ constexpr float kSlack = 8.f;                 // a row's maximum may grow by 2^8
 constexpr int kCounterStride = 16;            // words: a cache line's atomics serialise
 constexpr int kTile = 32;                     // slots that a wave takes at once
 constexpr int kSwitch = 12, kLeast = 16;      // tiles that going on to another unit takes the time of; of a work-group, at least
-constexpr int kWhole = 24, kPiece = 8;        // tiles that are not worth a merge; of a piece, at least
+constexpr int kWhole = 12, kPiece = 4;        // tiles that are not worth a merge; of a piece, at least
+// tiles of a work-group from which on the work is spread evenly; with two units a work-group and more
+constexpr int kEven = 16, kEvenMany = 64;
 
 struct PagedArgs {
     PagedCache c;
-    int n, hq, l, groups, row_groups;      // groups: work-groups that share the keys
-    int apart;                 // a work-group has one piece
+    int n, hq, l, groups, row_groups;      // groups: work-groups that share the keys evenly
+    int launched;
+    int may_part;              // there are work-groups enough for a piece each
     const void *Q;
     void *O;
     int64_t sq0, sq1, sq2, so0, so1, so2;
@@ -104,23 +108,30 @@ template <int W> struct Words;
 template <> struct Words<1> { typedef uint32_t type; };
 template <> struct Words<2> { typedef u32x2 type; };
 template <> struct Words<4> { typedef u32x4 type; };
-template <int W>
+// AUX: the cache policy, 2 for non-temporal
+template <int W, int AUX = 0>
 __device__ __forceinline__ typename Words<W>::type load_words(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
-    if constexpr (W == 1) return __builtin_amdgcn_raw_buffer_load_b32(r, (int)voff, 0, 0);
-    else if constexpr (W == 2) return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)voff, 0, 0));
-    else return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, 0, 0));
+    if constexpr (W == 1) return __builtin_amdgcn_raw_buffer_load_b32(r, (int)voff, 0, AUX);
+    else if constexpr (W == 2) return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)voff, 0, AUX));
+    else return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, 0, AUX));
 }
 __device__ __forceinline__ uint32_t word(uint32_t v, int) { return v; }
 template <typename V> __device__ __forceinline__ uint32_t word(const V &v, int i) { return v[i]; }
 
 // The schedule.  A unit is one sequence's KV head; its slots are tiles of 32.
-//   Few units: a work-group has one piece of a unit, all pieces of about the same size; a
-//   short unit is one piece.
-//   Others: the tiles of all units stand in one list, sequence after sequence, of which a
+//   Short caches (`apart`): a work-group has one piece of a unit, the pieces of a unit all of
+//   about the same size and a short unit one piece.
+//   Long ones: the tiles of all units stand in one list, sequence after sequence, of which a
 //   work-group has `per` adjacent places, so the work is even whatever the sequences' lengths;
 //   it goes through pieces of one or more units.
 // A unit that lies in one work-group is finished there; the pieces of the others are merged
 // by the last of its work-groups to arrive.
+// Where they cross: a piece that follows another in its work-group costs 5 us (drained loads,
+// the waves' merge, the unit's), uneven pieces up to their difference.  Pieces apart / even
+// list, us, 8 KV heads of 128, with tiles a work-group if even: 8 sequences of 500 (3) 11.8 / 17.4,
+// 5 of 3000 (11) 15.4 / 18.4, 8 of 2000 (12) 18.9 / 18.3, 64 of 600 (28) 26.6 / 31.5, 16 of 2000
+// (23) 25.6 / 22.9, 8 of 6000 (35) 43.7 / 34.9, 16 of 4000 (47) 50.7 / 42.9, 64 of 2000 (94) 76.1 / 76.2,
+// 32 of 8000 in e4m3 (141) 102 / 80.5.
 struct Piece {
     int b, hk, L;              // the unit, and its sequence's length
     int t0, t1;                // its tiles
@@ -168,7 +179,7 @@ template <typename A> __device__ __forceinline__ const A &late_args() {
 // A part that is 0 times an infinite value is NaN, so is a masked NaN: a wave whose sums
 // are not finite goes over its keys again with the row maxima that it found, value by value
 // for the rows that see them.
-template <typename T, int PK, int HD, int NWV>
+template <typename T, int PK, int HD, int NWV, int AUX>
 __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
     typedef typename std::conditional<PK == kSame, T, bf16_t>::type C;       // the products' type
     typedef typename Mfma<C>::frag frag;
@@ -192,51 +203,54 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
     // the row groups of a work-group's keys run on one XCD, whose L2 then has them for all but
     // the first
     const int idx = blockIdx.x >> 3, me = idx / a.row_groups * 8 + (blockIdx.x & 7), rg = idx % a.row_groups;
-    if (me >= a.groups) return;
+    if (me >= a.launched) return;
     const int G = a.hq / a.c.hkv, rows_kv = G * a.l, r0 = rg * R, nrows = min(R, rows_kv - r0);
 
-    // a lane has the lengths of 64 sequences at a time
+    // Places in the list (`apart`: pieces) of a sequence's KV head.  A unit begins with kSwitch
+    // places that no tile has.
+    int per = 0, x0 = 0, before = 0, lens, all = 0;
     auto len_of = [&](int x) __attribute__((always_inline)) { return x < a.n ? paged_len(a.c, a.kv_len, x) : 0; };
-    auto tiles_of = [&](int x, int len) __attribute__((always_inline)) { return x < a.n ? paged_tiles(len) : 0; };
-    int lens = len_of(lane), here = tiles_of(lane, lens), upto = wave_prefix(here);
-    int all = __builtin_amdgcn_readlane(upto, 63);
-    int per, cur = 0, stop = 0, x0 = 0, before = 0;
+    // a lane has the lengths of 64 sequences at a time
+    for (x0 = 0; x0 < a.n; x0 += 64) {
+        lens = len_of(x0 + lane);
+        all += __builtin_amdgcn_readlane(wave_prefix(x0 + lane < a.n ? paged_tiles(lens) : 0), 63);
+    }
+    all *= a.c.hkv;
+    const bool apart = a.may_part && all < (a.n * a.c.hkv < 2 * a.groups ? kEven : kEvenMany) * a.groups;
+    if (!apart && me >= a.groups) return;
+    per = apart ? max(kPiece, (all + a.groups - 1) / a.groups)
+                : max(kSwitch + kLeast, (all + a.n * a.c.hkv * kSwitch + a.groups - 1) / a.groups);
+    int cur = apart ? me : me * per;
+    auto weight = [&](int len) __attribute__((always_inline)) {
+        const int t = paged_tiles(len);
+        return !apart ? t + kSwitch : t <= kWhole ? 1 : (t + per - 1) / per;
+    };
+    const int stop = cur + per;                       // (past the last tile for the last work-group)
     Piece p;
-    if (a.apart) {                                    // (n <= 64)
-        per = max(kPiece, (all * a.c.hkv + a.groups - a.n * a.c.hkv - 1) / (a.groups - a.n * a.c.hkv));
-        const int cut = here <= kWhole ? min(here, 1) : (here + per - 1) / per, ends = wave_prefix(cut);
-        if (me >= __builtin_amdgcn_readlane(ends, 63) * a.c.hkv) return;
-        p.b = __builtin_ctzll(__ballot(ends * a.c.hkv > me));
-        p.pieces = __builtin_amdgcn_readlane(cut, p.b);
-        p.L = __builtin_amdgcn_readlane(lens, p.b);
-        const int at = me - __builtin_amdgcn_readlane(ends - cut, p.b) * a.c.hkv, tiles = paged_tiles(p.L);
-        p.hk = at / p.pieces;
-        const int z = at - p.hk * p.pieces;
+    for (x0 = 0;; x0 += 64) {
+        if (x0 >= a.n) return;                        // nothing for this work-group
+        if (a.n > 64) lens = len_of(x0 + lane);
+        const int here = x0 + lane < a.n ? weight(lens) : 0, upto = wave_prefix(here);
+        const uint64_t past = __ballot((before + upto) * a.c.hkv > cur);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            p.b = x0 + at;
+            before += __builtin_amdgcn_readlane(upto - here, at);
+            p.pieces = __builtin_amdgcn_readlane(here, at);
+            p.L = __builtin_amdgcn_readlane(lens, at);
+            break;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    // (in a unit of the sequence: its KV head, and the piece of an `apart` one)
+    const int inside = cur - before * a.c.hkv;
+    p.hk = inside / p.pieces;
+    if (apart) {
+        const int z = inside - p.hk * p.pieces, tiles = paged_tiles(p.L);
         p.first = me - z;
         p.late = 0;
         p.t0 = (int)((int64_t)z * tiles / p.pieces);
         p.t1 = (int)((int64_t)(z + 1) * tiles / p.pieces);
-    } else {
-        // (a unit begins with kSwitch places that no tile has)
-        for (int x = 64; x < a.n; x += 64) all += __builtin_amdgcn_readlane(wave_prefix(tiles_of(x + lane, len_of(x + lane))), 63);
-        all = (all + a.n * kSwitch) * a.c.hkv;
-        per = max(kSwitch + kLeast, (all + a.groups - 1) / a.groups);
-        cur = me * per;
-        if (cur >= all) return;
-        stop = cur + per;                             // (past the last tile for the last work-group)
-        uint64_t past;
-        auto places = [&](int x, int t) __attribute__((always_inline)) { return t + (min(x, a.n) - x0) * kSwitch; };
-        while (!(past = __ballot((before + places(x0 + lane + 1, upto)) * a.c.hkv > cur))) {      // (ends: cur < all)
-            before += places(x0 + 64, __builtin_amdgcn_readlane(upto, 63));
-            x0 += 64;
-            lens = len_of(x0 + lane);
-            here = tiles_of(x0 + lane, lens);
-            upto = wave_prefix(here);
-        }
-        p.b = x0 + __builtin_ctzll(past);
-        before += places(p.b, __builtin_amdgcn_readlane(upto - here, p.b - x0));
-        p.L = __builtin_amdgcn_readlane(lens, p.b - x0);
-        p.hk = (cur - before * a.c.hkv) / (paged_tiles(p.L) + kSwitch);
     }
     // the tiles of u among the places cur .. stop - 1
     auto cut_out = [&](Piece &u) __attribute__((always_inline)) {
@@ -248,7 +262,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
         u.late = unit0 > u.first * per;
         cur = tile0 + u.t1;
     };
-    if (!a.apart) cut_out(p);
+    if (!apart) cut_out(p);
     // the piece behind u, false if there is none
     auto next_piece = [&](Piece &u) __attribute__((always_inline)) {
         if (cur + kSwitch >= stop) return false;
@@ -348,7 +362,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
             const int m = there[t] = __builtin_amdgcn_readlane(now.n, from);
             const __amdgpu_buffer_rsrc_t rk = make_rsrc(address(now.k, from), m ? (uint32_t)((m - 1) * rowK) + a.c.hd * B : 0u);
 #pragma unroll
-            for (int j = 0; j < KL; ++j) kr[t][j] = load_words<4>(rk, offK[j]);
+            for (int j = 0; j < KL; ++j) kr[t][j] = load_words<4, AUX>(rk, offK[j]);
             if constexpr (PK != kSame)
                 ks[t] = __builtin_bit_cast(f32x4, load_words<4>(make_rsrc(address(now.ks, from), m * 4), G4 * 16));
         }
@@ -363,7 +377,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
             if constexpr (PK != kSame)
                 vs[t] = __builtin_bit_cast(f32x4, load_words<4>(make_rsrc(address(now.vs, from), m * 4), G4 * 16));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) vr[4 * t + j] = load_words<VW>(rv, offV[j]);
+            for (int j = 0; j < 4; ++j) vr[4 * t + j] = load_words<VW, AUX>(rv, offV[j]);
         }
         __builtin_amdgcn_sched_barrier(0);
     };
@@ -377,7 +391,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
     }
     for (;;) {
     Piece then = p;
-    const bool more = !a.apart && next_piece(then);
+    const bool more = !apart && next_piece(then);
     Entries later{};
     if (more) later = fetch(then, 0);
     const int free_end = p.L - a.l + 1;               // slots below are seen by every row
@@ -701,14 +715,17 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
 // ------------------------------------------------------------- host side
 
 struct PagedPlan {
-    int row_groups, groups, apart;
+    int row_groups, groups, may_part, launched;
     size_t counter_bytes, ml_bytes, o_bytes;
 };
 
 constexpr int kWaves = 4;
+// work-groups that share the keys evenly (512, two a CU: 16 sequences of 4000 44.2 -> 46.4 us), and
+// units that have work-groups of their own
 constexpr int kMaxGroups = 256;
 // The counters' part of a workspace, the same for calls of all sizes
-constexpr size_t kCounterBytes = (size_t)kMaxGroups * kCounterStride * 4;
+constexpr int kApart = 2048;
+constexpr size_t kCounterBytes = (size_t)(kApart + kMaxGroups) * kCounterStride * 4;
 
 PagedPlan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t slots, int64_t hd) {
     PagedPlan p{};
@@ -716,9 +733,10 @@ PagedPlan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t slots, 
     // no more work-groups than full tables have tiles for
     const int64_t tiles = n * hkv * std::max<int64_t>(1, cdiv(slots, kTile));
     p.groups = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxGroups / p.row_groups, tiles));
-    p.apart = n * hkv * 8 <= p.groups;
-    if (p.groups > 1) {
-        const size_t states = (size_t)p.groups * p.row_groups * 2 * 16;
+    p.may_part = n * hkv * p.row_groups <= kApart;
+    p.launched = p.groups + (p.may_part ? (int)(n * hkv) : 0);
+    if (tiles > n * hkv) {
+        const size_t states = (size_t)p.launched * p.row_groups * 2 * 16;
         p.counter_bytes = kCounterBytes;
         p.ml_bytes = states * 8;
         p.o_bytes = states * (hd <= 64 ? 64 : 128) * 4;
@@ -726,11 +744,23 @@ PagedPlan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t slots, 
     return p;
 }
 
+// Keys and values of pools (or full tables) of this many bytes pass by the caches
+// (non-temporal loads); those of smaller ones may be found in the 256 MB of memory-side cache the
+// next time: us without / with, 52 MB read 18.1 / 22.2, 119 MB 31.4 / 31.7, 145 MB 34.4 / 32.4, 204
+// MB 42.4 / 39.8, 394 MB 75.5 / 71.0.
+constexpr int64_t kStreamBytes = 120 << 20;
+
+template <typename T, int PK, int AUX>
+void launch_paged(const PagedArgs &a, const PagedPlan &p, hipStream_t st) {
+    const dim3 grid((unsigned)(cdiv(p.launched, 8) * 8 * p.row_groups));
+    if (a.c.hd <= 64) hipLaunchKernelGGL((paged_attn_kernel<T, PK, 64, kWaves, AUX>), grid, dim3(64 * kWaves), 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<T, PK, 128, kWaves, AUX>), grid, dim3(64 * kWaves), 0, st, a);
+}
 template <typename T, int PK>
 void launch_paged(const PagedArgs &a, const PagedPlan &p, hipStream_t st) {
-    const dim3 grid((unsigned)(cdiv(p.groups, 8) * 8 * p.row_groups));
-    if (a.c.hd <= 64) hipLaunchKernelGGL((paged_attn_kernel<T, PK, 64, kWaves>), grid, dim3(64 * kWaves), 0, st, a);
-    else hipLaunchKernelGGL((paged_attn_kernel<T, PK, 128, kWaves>), grid, dim3(64 * kWaves), 0, st, a);
+    const int64_t rows = std::min<int64_t>(a.c.pages, (int64_t)a.n * a.c.width) * a.c.page * a.c.hkv;
+    if (rows * a.c.hd * 2 * (PK == kSame ? 2 : 1) >= kStreamBytes) launch_paged<T, PK, 2>(a, p, st);
+    else launch_paged<T, PK, 0>(a, p, st);
 }
 
 template <typename T>
@@ -774,7 +804,7 @@ extern "C" int kuiops_sdpa_paged(int64_t n, int64_t hq, int64_t l, int dtype, co
     const PagedPlan p = plan_of(n, hq, at->hkv, l, slots, at->hd);
     const size_t need = p.counter_bytes + p.ml_bytes + p.o_bytes;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KUIOPS_E_WORKSPACE;
-    a.n = (int)n; a.hq = (int)hq; a.l = (int)l; a.groups = p.groups; a.apart = p.apart; a.row_groups = p.row_groups;
+    a.n = (int)n; a.hq = (int)hq; a.l = (int)l; a.groups = p.groups; a.may_part = p.may_part; a.launched = p.launched; a.row_groups = p.row_groups;
     a.Q = Q; a.O = O;
     a.sq0 = sq[0]; a.sq1 = sq[1]; a.sq2 = sq[2];
     a.so0 = so[0]; a.so1 = so[1]; a.so2 = so[2];
