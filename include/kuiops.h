@@ -774,7 +774,7 @@ typedef struct kuiops_paged_layout {
  * b * ld_batch + i * ld_tok.  Token i of sequence b goes to slot and position
  * pos0[b] + i (device int32[n], null: 0); slots outside the table are dropped.
  * lens (device int32[n], taken as 0 .. t; null: t): tokens i >= lens[b] are not
- * there: nothing of them is read or stored and their q_out is 0.  Queries and keys
+ * there: nothing of them is used or stored and their q_out is 0.  Queries and keys
  * become y = x * rsqrt(mean(x^2) + eps) * w with the weights q_norm / k_norm
  * ([hd], of dtype; null: y = x), then turn by the angles pos * inv_freq[i]: the
  * pairs (y_i, y_{i + hd/2}) -> (y_i cos - y_{i+hd/2} sin, y_{i+hd/2} cos + y_i

@@ -7,6 +7,7 @@
 // 8-bit pages hold a row x as x_i = scale * s_i with scale = m / M, s_i = nearest(x_i M / m),
 // m = max |x_i|, M the type's largest value (int8 127, e4m3 448).
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.hpp"
 
@@ -107,183 +108,241 @@ __device__ __forceinline__ F over_group(F v, Op op) {
     return v;
 }
 
-// Eight values s = nearest(x * r) of the 8-bit type, r = M / m: x M / m in 64 bits, where the
-// product's last bit may miss a tie that the quotient hits, so what 32 bits hold to 2^-45 is
-// taken to be that (a tie is: it has 9 bits).  e4m3: the rest goes through 32 bits cut off
-// with the last bit set, which rounds as the 64-bit value does.
-template <bool INT8, typename F>
-__device__ __forceinline__ u32x2 to_bytes(const F (&x)[8], double r) {
-    u32x2 w;
+// Eight values s = nearest(x M / m) of the 8-bit type, four a dword.
+//
+// Keys, 64 bits: y = x * r with r = M / m, whose last bit may miss a border that the quotient
+// hits, so y is taken to be what lies within 2^-38 of it (int8) or what 32 bits hold to 2^-45
+// of it (e4m3).  int8: two additions of a power of two round to those steps and then to a whole
+// number, which is the low word of the second.  e4m3: the conversion starts at 32 bits, which
+// must not turn y into a border; if one of a wave's values lies on one (or below the type's
+// normal ones, where borders are elsewhere), they are cut off with the last bit set instead,
+// which rounds as the 64-bit value does.
+template <bool INT8>
+__device__ __forceinline__ void to_bytes(const double (&x)[8], double r, u32x2 &w) {
+    if constexpr (INT8) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            uint32_t got = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const double y = fma(x[e + i], r, 0x1.8p14) - 0x1.8p14;
+                got |= ((uint32_t)__double2loint(y + 0x1.8p52) & 0xffu) << (8 * i);
+            }
+            w[e / 4] = got;
+        }
+    } else {
+        float f[8];
+        bool border = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            f[e] = (float)(x[e] * r);
+            border |= (__float_as_uint(f[e]) & 0xfffffu) == 0x80000u || fabsf(f[e]) < 0x1p-6f;
+        }
+        if (__any(border)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const double y = x[e] * r, off = y - (double)f[e];
+                if (fabs(off) > fabs(y) * 0x1p-45) {
+                    uint32_t u = __float_as_uint(f[e]);
+                    if ((off < 0) == (y > 0)) u -= 1;            // the neighbour nearer to zero
+                    f[e] = __uint_as_float(u | 1);
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+            w[e / 4] = __builtin_amdgcn_cvt_pk_fp8_f32(f[e + 2], f[e + 3], __builtin_amdgcn_cvt_pk_fp8_f32(f[e], f[e + 1], 0, false), true);
+    }
+}
+// Values, which come in 16 bits: x M is exact in 32, and its quotient by m, rounded once, is a
+// border only where the exact one is (that lies a 2^-12th of a step away from any other, at
+// least).  Rows near the type's end are scaled down first.
+template <bool INT8>
+__device__ __forceinline__ void to_bytes(const float (&x)[8], float m, u32x2 &w) {
+    const float down = m > 0x1p100f ? 0x1p-16f : 1.f, M = (INT8 ? 127.f : 448.f) * down, by = m > 0.f ? m * down : 1.f;
 #pragma unroll
     for (int e = 0; e < 8; e += 4) {
-        uint32_t got = 0;
         float f[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const double y = (double)x[e + i] * r;
-            float z = (float)y;
-            const double off = y - (double)z;
-            if (fabs(off) > fabs(y) * 0x1p-45) {
-                // the neighbour nearer to zero, its last bit set
-                uint32_t u = __float_as_uint(z);
-                if ((off < 0) == (y > 0)) u -= 1;
-                z = __uint_as_float(u | 1);
-            }
-            f[i] = z;
-            if constexpr (INT8) got |= ((uint32_t)(int)rintf(z) & 0xffu) << (8 * i);
+        for (int i = 0; i < 4; ++i) f[i] = x[e + i] * M / by;
+        if constexpr (INT8) {
+            uint32_t got = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) got |= ((uint32_t)(int)rintf(f[i]) & 0xffu) << (8 * i);
+            w[e / 4] = got;
+        } else {
+            w[e / 4] = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false), true);
         }
-        if constexpr (!INT8) {
-            got = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-            got = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], (int)got, true);
-        }
-        w[e / 4] = got;
     }
-    return w;
 }
 
 // ------------------------------------------------------------------------
-// paged_append_kernel -- a work-group has TB tokens and some of their heads.  The tokens'
-// cos / sin are worked out once for all heads (64 bits, in LDS); HD / 16 lanes have a head, 8
-// values i and their partners i + hd / 2 each, so a row is read and written in 16-byte
-// pieces and the rotation needs no exchange.  Queries, and keys of 16-bit pages, are computed
-// in 32 bits and rounded once; keys of 8-bit pages in 64, so that a value next to a border
-// between two quantised ones falls on its own side of it.
-template <typename T, int PK, int HD, int TB>
-__global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
+// paged_append_kernel -- a work-group has one token and `heads` of its heads, one pass:
+// HD / 16 lanes have a head, 8 values i and their partners i + hd / 2 each, so a row is read
+// and written in 16-byte pieces and the rotation needs no exchange.  The row is on its way
+// while its cos / sin are computed for all heads (64 bits, in LDS) and its page looked up.
+// Queries, and keys of 16-bit pages, are computed in 32 bits and rounded once; keys of 8-bit
+// pages in 64, so that a value next to a border between two quantised ones falls on its own
+// side of it.
+// What bounds it: the bytes, and for 8 bits the arithmetic about as much; waves at work hide
+// both, so registers are kept few (4 ragged prompts of 4001 tokens, 32 + 8 heads of 128, normed:
+// 7 waves a SIMD 69 us, 4.8 TB/s, 5 waves 82; two tokens a work-group 74, four 78; heads handed
+// out over the threads in turn, 4 tokens a work-group, 73; 6150 tokens in e4m3: 8 / 7 / 6 / 5 waves 55 / 44 / 45 / 49).
+constexpr int kAppendThreads = 512;
+template <typename T, int PK, int HD>
+__global__ __launch_bounds__(kAppendThreads, PK == 0 ? 7 : 6) void paged_append_kernel(AppendArgs a) {
     typedef T t8 __attribute__((ext_vector_type(8)));
     constexpr int LPH = HD / 16, HALF = HD / 2;
     typedef typename std::conditional<PK == 0, float, double>::type K;      // what keys are computed in
-    __shared__ __attribute__((aligned(16))) K s_cos[TB][HALF], s_sin[TB][HALF];
-    const int tid = threadIdx.x, half = a.c.hd / 2;
+    __shared__ __attribute__((aligned(16))) K s_cos[HALF], s_sin[HALF];
+    __shared__ int s_id, s_at;
+    const int tid = threadIdx.x, hd = a.c.hd, half = hd / 2, hkv = a.c.hkv;
     const int64_t b = blockIdx.y;
-    const int t0 = blockIdx.x * TB;
+    const int t = blockIdx.x, h = blockIdx.z * a.heads + tid / LPH, d = tid % LPH * 8;
+    // (the lanes of a head are in one wave, and all of them or none are at work; those past the
+    // head's end go along without a value)
+    const bool mine = d < half, on = tid / LPH < a.heads && h < a.hq + 2 * hkv;
+    u32x4 r1 = {0, 0, 0, 0}, r2 = {0, 0, 0, 0};
+    if (mine && on) {
+        const T *row = reinterpret_cast<const T *>(a.qkv) + b * a.ld_batch + t * a.ld_tok + (h * hd + d);
+        r1 = *reinterpret_cast<const u32x4 *>(row);
+        r2 = *reinterpret_cast<const u32x4 *>(row + half);
+    }
+    const bool query = h < a.hq, key = !query && h < a.hq + hkv;
+    const void *norm = query ? a.q_norm : key ? a.k_norm : nullptr;
+    u32x4 n1 = {0, 0, 0, 0}, n2 = {0, 0, 0, 0};
+    if (norm && mine && on) {
+        n1 = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const T *>(norm) + d);
+        n2 = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const T *>(norm) + d + half);
+    }
     const int there = a.lens ? max(0, min(a.lens[b], a.t)) : a.t;
     const int64_t first = a.pos0 ? a.pos0[b] : 0;
-    for (int x = tid; x < TB * HALF; x += 256) {
-        const int k = x / HALF, i = x % HALF;
-        if (i < half && t0 + k < there) {
+    if (t < there) {
+        for (int i = tid; i < half; i += blockDim.x) {
             double c, s;
-            turn_of(first + t0 + k, a.inv_freq[i], c, s);
-            s_cos[k][i] = (K)c;
-            s_sin[k][i] = (K)s;
+            turn_of(first + t, a.inv_freq[i], c, s);
+            s_cos[i] = (K)c;
+            s_sin[i] = (K)s;
         }
     }
-    __syncthreads();
-    const int hkv = a.c.hkv, h0 = blockIdx.z * a.heads, h1 = min(h0 + a.heads, a.hq + 2 * hkv);
-    const int tasks = TB * (h1 - h0) * LPH;
-    for (int x = tid; x < tasks; x += 256) {
-        // (the lanes of a head are in one wave, and all of them or none are here)
-        const int hx = x / LPH, k = hx / (h1 - h0), h = h0 + hx - k * (h1 - h0), d = x % LPH * 8;
-        const int t = t0 + k;
-        if (t >= a.t) continue;
-        const bool mine = d < half;
+    if (tid == 0) {
         const int64_t slot = first + t;
-        T *q = reinterpret_cast<T *>(a.q) + b * a.sq0 + h * a.sq1 + t * a.sq2 + d;
-        if (t >= there) {
-            // a token that is not there: nothing of it is read, its query is 0
-            if (h < a.hq && mine) {
-                *reinterpret_cast<u32x4 *>(q) = u32x4{0, 0, 0, 0};
-                *reinterpret_cast<u32x4 *>(q + half) = u32x4{0, 0, 0, 0};
-            }
-            continue;
-        }
-        const T *row = reinterpret_cast<const T *>(a.qkv) + b * a.ld_batch + t * a.ld_tok + (int64_t)h * a.c.hd + d;
-        const t8 v1 = __builtin_bit_cast(t8, mine ? *reinterpret_cast<const u32x4 *>(row) : u32x4{0, 0, 0, 0});
-        const t8 v2 = __builtin_bit_cast(t8, mine ? *reinterpret_cast<const u32x4 *>(row + half) : u32x4{0, 0, 0, 0});
-        auto turned = [&](auto one, const void *norm, auto (&x1)[8], auto (&x2)[8]) __attribute__((always_inline)) {
-            typedef decltype(one) F;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x1[e] = (F)to_f32(v1[e]);
-                x2[e] = (F)to_f32(v2[e]);
-            }
-            if (norm) {
-                F sum = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum += x1[e] * x1[e] + x2[e] * x2[e];
-                sum = over_group<LPH>(sum, [](F u, F w) { return u + w; });
-                const F r = F(1) / sqrt(sum / (F)a.c.hd + (F)a.eps);
-                const T *w = reinterpret_cast<const T *>(norm) + d;
-                const t8 w1 = __builtin_bit_cast(t8, mine ? *reinterpret_cast<const u32x4 *>(w) : u32x4{0, 0, 0, 0});
-                const t8 w2 = __builtin_bit_cast(t8, mine ? *reinterpret_cast<const u32x4 *>(w + half) : u32x4{0, 0, 0, 0});
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x1[e] *= r * (F)to_f32(w1[e]);
-                    x2[e] *= r * (F)to_f32(w2[e]);
-                }
-            }
-            if (!mine) return;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const F c = (F)s_cos[k][d + e], s = (F)s_sin[k][d + e], y1 = x1[e], y2 = x2[e];
-                x1[e] = y1 * c - y2 * s;
-                x2[e] = y2 * c + y1 * s;
-            }
-        };
-        auto rounded = [&](const float (&y)[8]) __attribute__((always_inline)) {
-            t8 w;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = from_f32<T>(y[e]);
-            return __builtin_bit_cast(u32x4, w);
-        };
-        if (h < a.hq) {
-            float x1[8], x2[8];
-            turned(1.f, a.q_norm, x1, x2);
-            if (mine) {
-                *reinterpret_cast<u32x4 *>(q) = rounded(x1);
-                *reinterpret_cast<u32x4 *>(q + half) = rounded(x2);
-            }
-            continue;
-        }
-        const bool key = h < a.hq + hkv;
-        const int hk = h - a.hq - (key ? 0 : hkv);
-        K x1[8], x2[8];
-        if (key) turned(K(1), a.k_norm, x1, x2);
-        else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x1[e] = (K)to_f32(v1[e]);
-                x2[e] = (K)to_f32(v2[e]);
-            }
-        }
         int at = 0;
-        const int id = slot >= 0 && slot < (1 << 30) ? page_of(a.c, b, (int)slot, at) : -1;
-        if (id < 0) continue;                         // the slot has no page
-        const int64_t off = key ? id * a.c.sk0 + hk * a.c.sk1 + at * a.c.sk2 : id * a.c.sv0 + hk * a.c.sv1 + at * a.c.sv2;
-        char *dst = reinterpret_cast<char *>(const_cast<void *>(key ? a.c.K : a.c.V)) + (off + d) * (PK == 0 ? 2 : 1);
-        if constexpr (PK == 0) {
-            if (mine) {
-                *reinterpret_cast<u32x4 *>(dst) = key ? rounded(x1) : __builtin_bit_cast(u32x4, v1);
-                *reinterpret_cast<u32x4 *>(dst + half * 2) = key ? rounded(x2) : __builtin_bit_cast(u32x4, v2);
+        s_id = slot >= 0 && slot < (1 << 30) ? page_of(a.c, b, (int)slot, at) : -1;
+        s_at = at;
+    }
+    __syncthreads();
+    if (!on) return;
+    T *q = reinterpret_cast<T *>(a.q) + b * a.sq0 + h * a.sq1 + t * a.sq2 + d;
+    if (t >= there) {
+        // a token that is not there: its query is 0
+        if (query && mine) {
+            *reinterpret_cast<u32x4 *>(q) = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4 *>(q + half) = u32x4{0, 0, 0, 0};
+        }
+        return;
+    }
+    const t8 v1 = __builtin_bit_cast(t8, r1), v2 = __builtin_bit_cast(t8, r2), w1 = __builtin_bit_cast(t8, n1), w2 = __builtin_bit_cast(t8, n2);
+    auto turned = [&](auto one, auto (&x1)[8], auto (&x2)[8]) __attribute__((always_inline)) {
+        typedef decltype(one) F;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x1[e] = (F)to_f32(v1[e]);
+            x2[e] = (F)to_f32(v2[e]);
+        }
+        if (norm) {
+            F sum = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += x1[e] * x1[e] + x2[e] * x2[e];
+            sum = over_group<LPH>(sum, [](F u, F w) { return u + w; });
+            const F r = F(1) / sqrt(sum / (F)hd + (F)a.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x1[e] *= r * (F)to_f32(w1[e]);
+                x2[e] *= r * (F)to_f32(w2[e]);
             }
-        } else {
-            constexpr bool INT8 = PK == 1;
-            constexpr double M = INT8 ? 127.0 : 448.0;
-            double top = 0.0;
-            float odd = 0.f;                          // NaN if the row has one, or an infinity
+        }
+        if (!mine) return;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const F c = (F)s_cos[d + e], s = (F)s_sin[d + e], y1 = x1[e], y2 = x2[e];
+            x1[e] = y1 * c - y2 * s;
+            x2[e] = y2 * c + y1 * s;
+        }
+    };
+    auto rounded = [&](const float (&y)[8]) __attribute__((always_inline)) {
+        t8 w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = from_f32<T>(y[e]);
+        return __builtin_bit_cast(u32x4, w);
+    };
+    if (query || (PK == 0 && key)) {
+        float x1[8], x2[8];
+        turned(1.f, x1, x2);
+        r1 = rounded(x1);
+        r2 = rounded(x2);
+    }
+    if (query) {
+        if (mine) {
+            *reinterpret_cast<u32x4 *>(q) = r1;
+            *reinterpret_cast<u32x4 *>(q + half) = r2;
+        }
+        return;
+    }
+    const int id = __builtin_amdgcn_readfirstlane(s_id), at = __builtin_amdgcn_readfirstlane(s_at);
+    if (id < 0) return;                           // the slot has no page
+    const int hk = h - a.hq - (key ? 0 : hkv);
+    const int64_t off = key ? id * a.c.sk0 + hk * a.c.sk1 + at * a.c.sk2 : id * a.c.sv0 + hk * a.c.sv1 + at * a.c.sv2;
+    char *dst = reinterpret_cast<char *>(const_cast<void *>(key ? a.c.K : a.c.V)) + (off + d) * (PK == 0 ? 2 : 1);
+    if constexpr (PK == 0) {
+        if (mine) {
+            *reinterpret_cast<u32x4 *>(dst) = r1;
+            *reinterpret_cast<u32x4 *>(dst + half * 2) = r2;
+        }
+    } else {
+        constexpr bool INT8 = PK == 1;
+        constexpr double M = INT8 ? 127.0 : 448.0;
+        u32x2 b1, b2;
+        float scale;                              // NaN for a row that has one, or an infinity
+        bool fine;
+        if (key) {
+            double x1[8], x2[8], top = 0.0, odd = 0.0;
+            turned(1.0, x1, x2);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 top = fmax(top, fmax(fabs(x1[e]), fabs(x2[e])));
-                odd += (float)(x1[e] * 0.0) + (float)(x2[e] * 0.0);
+                odd += x1[e] + x2[e];
             }
             top = over_group<LPH>(top, [](double u, double w) { return fmax(u, w); });
-            odd = over_group<LPH>(odd, [](float u, float w) { return u + w; });
-            // a row that is not finite reads back as NaN
-            const bool fine = odd == 0.f;
+            odd = over_group<LPH>(odd, [](double u, double w) { return u + w; });
+            fine = odd * 0.0 == 0.0;
             const double r = fine && top > 0.0 ? M / top : 0.0;
-            if (mine) {
-                if (!fine) {
+            scale = (float)(top / M);
+            to_bytes<INT8>(x1, r, b1);
+            to_bytes<INT8>(x2, r, b2);
+        } else {
+            float x1[8], x2[8], top = 0.f, odd = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x1[e] = x2[e] = 0;
-                }
-                *reinterpret_cast<u32x2 *>(dst) = to_bytes<INT8>(x1, r);
-                *reinterpret_cast<u32x2 *>(dst + half) = to_bytes<INT8>(x2, r);
+            for (int e = 0; e < 8; ++e) {
+                x1[e] = to_f32(v1[e]);
+                x2[e] = to_f32(v2[e]);
+                top = fmaxf(top, fmaxf(fabsf(x1[e]), fabsf(x2[e])));
+                odd = __builtin_fmaf(x1[e], 0.f, __builtin_fmaf(x2[e], 0.f, odd));
             }
-            if (d == 0) {
-                float *sc = const_cast<float *>(key ? a.c.ks : a.c.vs);
-                sc[key ? id * a.c.sks0 + hk * a.c.sks1 + at : id * a.c.svs0 + hk * a.c.svs1 + at] =
-                    fine ? (float)(top / M) : __uint_as_float(0x7fc00000u);
-            }
+            top = over_group<LPH>(top, [](float u, float w) { return fmaxf(u, w); });
+            odd = over_group<LPH>(odd, [](float u, float w) { return u + w; });
+            fine = odd == 0.f;
+            scale = (float)((double)top / M);
+            to_bytes<INT8>(x1, top, b1);
+            to_bytes<INT8>(x2, top, b2);
+        }
+        if (mine) {
+            *reinterpret_cast<u32x2 *>(dst) = fine ? b1 : u32x2{0, 0};
+            *reinterpret_cast<u32x2 *>(dst + half) = fine ? b2 : u32x2{0, 0};
+        }
+        if (d == 0) {
+            float *sc = const_cast<float *>(key ? a.c.ks : a.c.vs);
+            sc[key ? id * a.c.sks0 + hk * a.c.sks1 + at : id * a.c.svs0 + hk * a.c.svs1 + at] = fine ? scale : __uint_as_float(0x7fc00000u);
         }
     }
 }
@@ -298,32 +357,32 @@ struct ReadArgs {
 };
 
 // ------------------------------------------------------------------------
-// paged_read_kernel -- a work-group has ROWS slots of one KV head, keys and values; 16 bytes
-// of a page a lane.
+// paged_read_kernel -- a work-group has 128 slots of one KV head, keys and values; 8 values of
+// a row a lane, so that what is written, the larger part, goes out in 16-byte pieces that
+// follow one another.  All loads of a thread are on their way at once, behind its page numbers.
 template <typename T, int PK, int HD>
 __global__ __launch_bounds__(256) void paged_read_kernel(ReadArgs a) {
-    constexpr int E = PK == 0 ? 8 : 16, LPR = HD / E, RPI = 256 / LPR, ROWS = 128, IT = ROWS / RPI;
-    typedef T t8 __attribute__((ext_vector_type(8)));
-    const int tid = threadIdx.x, d = tid % LPR * E;
+    constexpr int LPR = HD / 8, RPI = 256 / LPR, ROWS = 128, IT = ROWS / RPI, B = PK == 0 ? 2 : 1;
+    typedef typename std::conditional<PK == 0, u32x4, u32x2>::type words;
+    const int tid = threadIdx.x, d = tid % LPR * 8;
     const int64_t bh = blockIdx.y, b = bh / a.c.hkv, hk = bh % a.c.hkv;
-    const int L = min(a.s, paged_len(a.c, a.kv_len, b)), s0 = blockIdx.x * ROWS;
-    if (s0 >= (a.fill ? a.s : L) || d >= a.c.hd) return;
-    constexpr int B = PK == 0 ? 2 : 1;
+    const int L = min(a.s, paged_len(a.c, a.kv_len, b)), s0 = blockIdx.x * ROWS, end = a.fill ? a.s : L;
+    if (s0 >= end || d >= a.c.hd) return;
     int id[IT], at[IT];
 #pragma unroll
     for (int j = 0; j < IT; ++j) {
         const int slot = s0 + j * RPI + tid / LPR;
         id[j] = slot < L ? page_of(a.c, b, slot, at[j]) : -1;
     }
-    u32x4 w[2][IT];
+    words w[2][IT];
     float sc[2][IT];
 #pragma unroll
     for (int j = 0; j < IT; ++j) {
-        w[0][j] = w[1][j] = u32x4{0, 0, 0, 0};
+        w[0][j] = w[1][j] = words{};
         sc[0][j] = sc[1][j] = 0.f;
         if (id[j] >= 0) {
-            w[0][j] = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const char *>(a.c.K) + (id[j] * a.c.sk0 + hk * a.c.sk1 + at[j] * a.c.sk2 + d) * B);
-            w[1][j] = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const char *>(a.c.V) + (id[j] * a.c.sv0 + hk * a.c.sv1 + at[j] * a.c.sv2 + d) * B);
+            w[0][j] = *reinterpret_cast<const words *>(reinterpret_cast<const char *>(a.c.K) + (id[j] * a.c.sk0 + hk * a.c.sk1 + at[j] * a.c.sk2 + d) * B);
+            w[1][j] = *reinterpret_cast<const words *>(reinterpret_cast<const char *>(a.c.V) + (id[j] * a.c.sv0 + hk * a.c.sv1 + at[j] * a.c.sv2 + d) * B);
             if constexpr (PK != 0) {
                 sc[0][j] = a.c.ks[id[j] * a.c.sks0 + hk * a.c.sks1 + at[j]];
                 sc[1][j] = a.c.vs[id[j] * a.c.svs0 + hk * a.c.svs1 + at[j]];
@@ -335,50 +394,46 @@ __global__ __launch_bounds__(256) void paged_read_kernel(ReadArgs a) {
 #pragma unroll
         for (int j = 0; j < IT; ++j) {
             const int slot = s0 + j * RPI + tid / LPR;
-            if (slot >= (a.fill ? a.s : L)) continue;
+            if (slot >= end) continue;
             T *dst = reinterpret_cast<T *>(x ? a.v : a.k) +
                      (x ? b * a.vo0 + hk * a.vo1 + slot * a.vo2 : b * a.ko0 + hk * a.ko1 + slot * a.ko2) + d;
             if constexpr (PK == 0) *reinterpret_cast<u32x4 *>(dst) = w[x][j];
             else {
+                typedef T t8 __attribute__((ext_vector_type(8)));
+                t8 y;
 #pragma unroll
-                for (int e = 0; e < E; e += 4) {
+                for (int e = 0; e < 8; ++e) {
                     const uint32_t u = w[x][j][e / 4];
-                    float f[4];
-                    if constexpr (PK == 1) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(u >> (8 * i));
-                    } else {
-                        f[0] = __builtin_amdgcn_cvt_f32_fp8((int)u, 0);
-                        f[1] = __builtin_amdgcn_cvt_f32_fp8((int)u, 1);
-                        f[2] = __builtin_amdgcn_cvt_f32_fp8((int)u, 2);
-                        f[3] = __builtin_amdgcn_cvt_f32_fp8((int)u, 3);
-                    }
-                    typedef T t4 __attribute__((ext_vector_type(4)));
-                    t4 y;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = from_f32<T>(f[i] * sc[x][j]);
-                    *reinterpret_cast<t4 *>(dst + e) = y;
+                    float f;
+                    if constexpr (PK == 1) f = (float)(int8_t)(u >> (8 * (e % 4)));
+                    else switch (e % 4) {
+                            case 0: f = __builtin_amdgcn_cvt_f32_fp8((int)u, 0); break;
+                            case 1: f = __builtin_amdgcn_cvt_f32_fp8((int)u, 1); break;
+                            case 2: f = __builtin_amdgcn_cvt_f32_fp8((int)u, 2); break;
+                            default: f = __builtin_amdgcn_cvt_f32_fp8((int)u, 3); break;
+                        }
+                    y[e] = from_f32<T>(f * sc[x][j]);
                 }
+                *reinterpret_cast<t8 *>(dst) = y;
             }
         }
 }
 
 // ------------------------------------------------------------- host side
 
+constexpr int64_t kCUs = 256;
+
 template <typename T, int PK, int HD>
 void launch_append(AppendArgs &a, hipStream_t st) {
+    // up to 512 threads, for 8 bits 256 (6150 tokens of 48 heads of 128, e4m3: 44 -> 42 us)
+    constexpr int LPH = HD / 16, most = (PK == 0 ? kAppendThreads : kAppendThreads / 2) / LPH;
     const int heads = a.hq + 2 * a.c.hkv;
-    // tokens enough for every CU: 4 of them share a work-group's tables; fewer: the heads are
-    // spread over work-groups
-    if ((int64_t)a.n * a.t >= 1024) {
-        a.heads = heads;
-        hipLaunchKernelGGL((paged_append_kernel<T, PK, HD, 4>), dim3((unsigned)cdiv(a.t, 4), (unsigned)a.n, 1), dim3(256), 0, st, a);
-        return;
-    }
-    const int per = 256 / (HD / 16);                  // heads that a work-group's threads have at once
-    const int parts = (int)cdiv(heads, per);
+    // few tokens: the heads are spread over work-groups until each CU has one, a wave of heads each
+    // at least
+    const int64_t parts = std::max(cdiv(heads, most), std::min(cdiv(heads * LPH, 64), kCUs / ((int64_t)a.n * a.t)));
     a.heads = (int)cdiv(heads, parts);
-    hipLaunchKernelGGL((paged_append_kernel<T, PK, HD, 1>), dim3((unsigned)a.t, (unsigned)a.n, (unsigned)parts), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)a.t, (unsigned)a.n, (unsigned)cdiv(heads, a.heads)), threads((unsigned)(cdiv(a.heads * LPH, 64) * 64));
+    hipLaunchKernelGGL((paged_append_kernel<T, PK, HD>), grid, threads, 0, st, a);
 }
 
 template <typename T>
@@ -424,7 +479,7 @@ extern "C" int kuiops_kv_paged_append(int64_t n, int64_t t, int64_t hq, int dtyp
     if (!aligned16(qkv) || !aligned16(q_out) || (q_norm && !aligned16(q_norm)) || (k_norm && !aligned16(k_norm)))
         return KUIOPS_E_UNSUPPORTED;
     // grid axes, launches below 2^32 threads
-    if (n > 65535 || t >= (1 << 24) || hq + 2 * at->hkv >= (1 << 16) || n * t * cdiv(hq + 2 * at->hkv, 32) >= (1 << 24))
+    if (n > 65535 || t >= (1 << 24) || hq + 2 * at->hkv >= (1 << 16) || n * t * cdiv(hq + 2 * at->hkv, 32) >= (1 << 23))
         return KUIOPS_E_UNSUPPORTED;
     a.n = (int)n; a.t = (int)t; a.hq = (int)hq;
     a.qkv = qkv; a.ld_tok = ld_tok; a.ld_batch = ld_batch;

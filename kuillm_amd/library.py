@@ -303,7 +303,7 @@ def _kv_evict_fake(k, v, acc, pos, kv_len, budget, recent=0):
 def _kv_paged_append_fake(qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale=None, v_scale=None, q_norm=None, k_norm=None,
                           eps=1e-6, lens=None):
     hkv, hd = k_pages.shape[1], k_pages.shape[3]
-    return qkv.new_empty((qkv.shape[0], qkv.shape[2] // hd - 2 * hkv, qkv.shape[1], hd))
+    return qkv.new_empty((qkv.shape[0], qkv.shape[1], qkv.shape[2] // hd - 2 * hkv, hd)).transpose(1, 2)
 
 
 @_fake("kv_paged_read")

@@ -1522,7 +1522,7 @@ _PAGE_BYTES = {torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.F8E4M3}
 
 
 class _PagedPlan:
-    __slots__ = ("layout", "n", "bytes", "slots")
+    __slots__ = ("layout", "n", "hkv", "hd", "bytes", "slots", "holds")
 
 
 @functools.lru_cache(maxsize=2048)
@@ -1533,13 +1533,14 @@ def _paged_plan(name, k, v, k_scale, v_scale, table) -> _PagedPlan:
             or len(table[0]) != 2 or table[2] != torch.int32:
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     p = _PagedPlan()
-    p.bytes = kd in _PAGE_BYTES
+    p.bytes, p.holds = kd in _PAGE_BYTES, math.prod(ks) > 0
     if p.bytes != (k_scale is not None) or p.bytes != (v_scale is not None):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     if not p.bytes and kd not in HALF:
         raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
     pages, hkv, page, hd = ks
     p.n, width = table[0]
+    p.hkv, p.hd = hkv, hd
     if any(not _own_rows(shape, stride) for shape, stride in ((ks, kst), (vs, vst))):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     if width > 1 and table[1][1] != 1:
@@ -1563,49 +1564,59 @@ def _paged_cache(name, k, v, k_scale, v_scale, table):
     return _paged_plan(name, _meta(k), _meta(v), _meta(k_scale), _meta(v_scale), _meta(table))
 
 
-def _readable(t):
-    """t, or a copy where the kernels cannot read its rows in place: 16-byte pieces."""
-    st = t.stride()
-    if (t.shape[-1] <= 1 or st[-1] == 1) and t.data_ptr() % 16 == 0 and \
-            not any(s % 8 for s, size in zip(st[:-1], t.shape) if size > 1):
-        return t
+def _in_pieces(shape, stride) -> bool:
+    """Whether the kernels can read rows of these strides in place, in 16-byte pieces
+    (from an address that is a multiple of 16)."""
+    return (shape[-1] <= 1 or stride[-1] == 1) and not any(st % 8 for st, size in zip(stride[:-1], shape) if size > 1)
+
+
+def _copied(t):
     return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
-def _apart(name, out, *others):
-    if out.numel():
-        at = out.data_ptr()
-        for o in others:
-            if o is not None and o.numel() and o.data_ptr() == at:
-                raise _lib.KuiopsError(name, _lib.E_INVALID)
+class _AppendPlan:
+    __slots__ = ("dims", "dtype", "ld", "ld_copy", "in_place", "weights_in_place", "sq", "q_layout")
 
 
 @functools.lru_cache(maxsize=2048)
-def _append_plan(qkv, hkv, hd, inv_freq, q_norm, k_norm, q_out):
-    """(hq, C strides of q_out) from the (shape, stride, dtype) of kv_paged_append's other tensors."""
-    name, (shape, _, dtype) = "kv_paged_append", qkv
+def _append_plan(qkv, n, hkv, hd, pages, inv_freq, q_norm, k_norm, q_out) -> _AppendPlan:
+    """Checks the (shape, stride, dtype) of kv_paged_append's other tensors; `pages`: the type
+    of 16-bit pages, None for 8 bits."""
+    name, (shape, stride, dtype) = "kv_paged_append", qkv
     if len(shape) != 3 or hd % 2 or shape[2] % hd or shape[2] // hd < 2 * hkv or inv_freq[0] != (hd // 2,) \
             or inv_freq[2] != torch.float32 or any(w is not None and (w[0] != (hd,) or w[2] != dtype) for w in (q_norm, k_norm)):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     if dtype not in HALF:
         raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
-    n, t, hq = shape[0], shape[1], shape[2] // hd - 2 * hkv
-    if q_out is None:
-        return hq, _c_strides((n, hq, t, hd), (hq * t * hd, t * hd, hd, 1), 3)
-    if q_out[0] != (n, hq, t, hd) or q_out[2] != dtype or not _own_rows(*q_out[:2]):
+    if shape[0] != n or pages not in (None, dtype):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
-    return hq, _c_strides(*q_out[:2], 3)
+    p = _AppendPlan()
+    t, w = shape[1], shape[2]
+    hq = w // hd - 2 * hkv
+    p.dims, p.dtype = (n, t, hq), _dt(dtype)
+    p.in_place = _in_pieces(shape, stride)
+    p.ld, p.ld_copy = (stride[1] if t > 1 else 0, stride[0] if n > 1 else 0), (w, t * w)
+    p.weights_in_place = all(x is None or x[1] == (1,) for x in (q_norm, k_norm))
+    p.q_layout = (n, hq, t, hd), (hq * t * hd, hd, hq * hd, 1)          # token by token, as the rows arrive
+    if q_out is None:
+        p.sq = _c_strides(*p.q_layout, 3)
+    elif q_out[0] != (n, hq, t, hd) or q_out[2] != dtype or not _own_rows(*q_out[:2]):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    else:
+        p.sq = _c_strides(*q_out[:2], 3)
+    return p
 
 
 def kv_paged_append(qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale=None, v_scale=None, q_norm=None, k_norm=None,
                     eps=1e-6, lens=None, q_out=None):
     """Norms and rotates the queries and keys of new tokens and stores their keys and
-    values in a paged cache, quantised if its pages are of 8 bits -> q (n, hq, t, hd).
+    values in a paged cache, quantised if its pages are of 8 bits -> q (n, hq, t, hd), a
+    transposed view of (n, t, hq, hd).
 
     qkv (n, t, (hq + 2 hkv) hd) is the fused projection's output (q, k, v heads).  Token
     i of sequence b goes to slot and position ``pos0[b]`` + i (int32 [n] on the device;
     None: 0); slots that the table does not reach are dropped.  Tokens from ``lens[b]``
-    on (int32 [n]; None: t) are padding: nothing of them is read or stored, their q is 0.
+    on (int32 [n]; None: t) are padding: nothing of them is used or stored, their q is 0.
     With ``q_norm`` / ``k_norm`` ([hd], qkv's type) a head becomes x * rsqrt(mean(x^2) +
     eps) * weight; then queries and keys turn by the angles position * ``inv_freq``
     (fp32 [hd / 2]), in 64 bits, and are rounded once.  8-bit pages get a row x as
@@ -1614,28 +1625,42 @@ def kv_paged_append(qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale=None, 
     receives a token must belong to one sequence.  bf16 / f16; hd a multiple of 16 up to
     128, pages of multiples of 16 rows.  ``q_out`` receives q in place."""
     name = "kv_paged_append"
-    p = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
-    hq, sq = _append_plan(_meta(qkv), k_pages.shape[1], k_pages.shape[3], _meta(inv_freq), _meta(q_norm), _meta(k_norm), _meta(q_out))
-    n, t, _ = qkv.shape
-    if n != p.n or not (p.bytes or k_pages.dtype == qkv.dtype):
-        raise _lib.KuiopsError(name, _lib.E_INVALID)
+    c = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
+    p = _append_plan(_meta(qkv), c.n, c.hkv, c.hd, None if c.bytes else k_pages.dtype, _meta(inv_freq), _meta(q_norm), _meta(k_norm),
+                     _meta(q_out))
     for x in (pos0, lens):
-        if x is not None and not _flat_ints(x, n):
+        if x is not None and not _flat_ints(x, c.n):
             raise _lib.KuiopsError(name, _lib.E_INVALID)
-    _apart(name, k_pages, v_pages)
-    if q_out is not None:
-        _apart(name, q_out, qkv, k_pages, v_pages)
+    k_at, v_at = k_pages.data_ptr(), v_pages.data_ptr()
+    if c.holds and (k_at == v_at or (q_out is not None and q_out.data_ptr() in (qkv.data_ptr(), k_at, v_at))):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
     device = _gpu_of(name, qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale, v_scale, q_norm, k_norm, lens, q_out)
-    qkv, inv_freq = _readable(qkv), inv_freq.contiguous()
-    q_norm, k_norm = (w if w is None else _readable(w) for w in (q_norm, k_norm))
+    ld = p.ld
+    if not p.in_place or qkv.data_ptr() % 16:
+        qkv, ld = _copied(qkv), p.ld_copy
+    if not inv_freq.is_contiguous():
+        inv_freq = inv_freq.contiguous()
+    if q_norm is not None and (not p.weights_in_place or q_norm.data_ptr() % 16):
+        q_norm = _copied(q_norm)
+    if k_norm is not None and (not p.weights_in_place or k_norm.data_ptr() % 16):
+        k_norm = _copied(k_norm)
     if q_out is None:
-        q_out = qkv.new_empty((n, hq, t, k_pages.shape[3]))
-    ld_batch, ld_tok, _ = qkv.stride()
+        q_out = qkv.new_empty_strided(*p.q_layout)
     _enqueue("kuiops_kv_paged_append", device, (
-        n, t, hq, _dt(qkv.dtype), qkv.data_ptr(), ld_tok if t > 1 else 0, ld_batch if n > 1 else 0, _ptr(lens), _ptr(pos0),
-        inv_freq.data_ptr(), _ptr(q_norm), _ptr(k_norm), float(eps), q_out.data_ptr(), sq, p.layout, k_pages.data_ptr(),
-        v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr()))
+        *p.dims, p.dtype, qkv.data_ptr(), *ld, _ptr(lens), _ptr(pos0), inv_freq.data_ptr(), _ptr(q_norm), _ptr(k_norm), float(eps),
+        q_out.data_ptr(), p.sq, c.layout, k_at, v_at, _ptr(k_scale), _ptr(v_scale), table.data_ptr()))
     return q_out
+
+
+@functools.lru_cache(maxsize=2048)
+def _read_plan(n, hkv, length, hd, dtype, pages):
+    """(shape, C type, C strides) of kv_paged_read's outputs; `pages` as in _append_plan."""
+    if length < 0:
+        raise _lib.KuiopsError("kv_paged_read", _lib.E_INVALID)
+    if pages not in (None, dtype) or dtype not in (*HALF, torch.float32):
+        raise _lib.Unsupported("kv_paged_read", _lib.E_UNSUPPORTED)
+    shape = torch.Size((n, hkv, length, hd))
+    return shape, _dt(dtype), _c_strides(shape, (hkv * length * hd, length * hd, hd, 1), 3)
 
 
 @functools.lru_cache(maxsize=2048)
@@ -1655,55 +1680,64 @@ def kv_paged_read(k_pages, v_pages, table, kv_len, length=None, k_scale=None, v_
     (default), f16 or fp32.  Rows behind a sequence are 0, or left as they are in
     ``k_out`` / ``v_out`` (given together; (n, hkv, length, hd), unit last stride)."""
     name = "kv_paged_read"
-    p = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
-    n, hkv, hd = p.n, k_pages.shape[1], k_pages.shape[3]
-    if (k_out is None) != (v_out is None) or not _flat_ints(kv_len, n):
+    c = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
+    if (k_out is None) != (v_out is None) or not _flat_ints(kv_len, c.n):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     if dtype is None:
-        dtype = k_out.dtype if k_out is not None else torch.bfloat16 if p.bytes else k_pages.dtype
-    if not p.bytes and dtype != k_pages.dtype or dtype not in (*HALF, torch.float32):
-        raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
+        dtype = k_out.dtype if k_out is not None else torch.bfloat16 if c.bytes else k_pages.dtype
     if length is None:
-        length = k_out.shape[2] if k_out is not None and k_out.dim() == 4 else p.slots
-    if int(length) < 0:
-        raise _lib.KuiopsError(name, _lib.E_INVALID)
-    shape, fill = torch.Size((n, hkv, int(length), hd)), k_out is None
-    if not fill:
+        length = k_out.shape[2] if k_out is not None and k_out.dim() == 4 else c.slots
+    shape, code, flat = _read_plan(c.n, c.hkv, int(length), c.hd, dtype, None if c.bytes else k_pages.dtype)
+    k_at, v_at, fill = k_pages.data_ptr(), v_pages.data_ptr(), k_out is None
+    if fill:
+        sk = sv = flat
+    else:
         sk, sv = _read_strides(shape, _meta(k_out), dtype), _read_strides(shape, _meta(v_out), dtype)
-        _apart(name, k_out, v_out, k_pages, v_pages)
-        _apart(name, v_out, k_pages, v_pages)
+        ko, vo = k_out.data_ptr(), v_out.data_ptr()
+        if k_out.numel() and (ko == vo or ko in (k_at, v_at) or vo in (k_at, v_at)):
+            raise _lib.KuiopsError(name, _lib.E_INVALID)
     device = _gpu_of(name, k_pages, v_pages, table, kv_len, k_scale, v_scale, k_out, v_out)
     if fill:
-        k_out, v_out = k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
-        sk = sv = _read_strides(shape, _meta(k_out), dtype)
+        k_out = k_pages.new_empty(shape, dtype=dtype)
+        v_out = torch.empty_like(k_out)
     _enqueue("kuiops_kv_paged_read", device, (
-        n, shape[2], _dt(dtype), p.layout, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(),
-        kv_len.data_ptr(), k_out.data_ptr(), sk, v_out.data_ptr(), sv, 1 if fill else 0))
+        c.n, shape[2], code, c.layout, k_at, v_at, _ptr(k_scale), _ptr(v_scale), table.data_ptr(), kv_len.data_ptr(), k_out.data_ptr(),
+        sk, v_out.data_ptr(), sv, 1 if fill else 0))
     return k_out, v_out
 
 
+class _PagedAttnPlan:
+    __slots__ = ("dims", "dtype", "sq", "sq_copy", "in_place", "so", "ws", "scale")
+
+
 @functools.lru_cache(maxsize=2048)
-def _paged_attn_plan(q, hkv, hd, slots, out):
-    """(C strides of q, those of its copy, of out, bytes of the workspace, default scale)."""
+def _paged_attn_plan(q, n, hkv, hd, pages, slots, out) -> _PagedAttnPlan:
+    """Checks the (shape, stride, dtype) of sdpa_paged's other tensors; `pages` as in _append_plan."""
     name, (shape, stride, dtype) = "sdpa_paged", q
     if len(shape) != 4 or shape[3] != hd or shape[1] % hkv:
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     if dtype not in HALF:
         raise _lib.Unsupported(name, _lib.E_UNSUPPORTED)
-    n, hq, l, _ = shape
-    flat = (hq * l * hd, l * hd, hd, 1)
-    if out is not None and (out[0] != shape or out[2] != dtype or not _own_rows(*out[:2])):
+    if shape[0] != n or pages not in (None, dtype) or (out is not None and (out[0] != shape or out[2] != dtype or not _own_rows(*out[:2]))):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
-    return (_c_strides(shape, stride, 3), _c_strides(shape, flat, 3), _c_strides(shape, flat if out is None else out[1], 3),
-            _lib_handle().kuiops_sdpa_paged_workspace(n, hq, hkv, l, slots, hd), 1.0 / math.sqrt(hd))
+    p = _PagedAttnPlan()
+    _, hq, l, _ = shape
+    flat = (hq * l * hd, l * hd, hd, 1)
+    p.dims, p.dtype = (n, hq, l), _dt(dtype)
+    p.sq, p.sq_copy, p.in_place = _c_strides(shape, stride, 3), _c_strides(shape, flat, 3), _in_pieces(shape, stride)
+    p.so = _c_strides(shape, flat if out is None else out[1], 3)
+    p.ws = _lib_handle().kuiops_sdpa_paged_workspace(n, hq, hkv, l, slots, hd)
+    p.scale = 1.0 / math.sqrt(hd)
+    return p
 
 
-def _zeroed_workspace(device, nbytes):
+def _zeroed_workspace(device, index, nbytes):
     """sdpa_paged's workspace: the current stream's own, or memory of its own (and its
     zero fill) in a graph that is being captured, so that two graphs may run at once."""
     if torch.cuda.is_current_stream_capturing():
         return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return workspace(device, nbytes, "paged")
+    buf = _WS.get((index, _raw_stream(index), "paged"))
+    return buf if buf is not None and buf.numel() >= nbytes else workspace(device, nbytes, "paged")
 
 
 def sdpa_paged(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=None, scale=None, return_lse=False, out=None):
@@ -1718,21 +1752,22 @@ def sdpa_paged(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=None, s
     ``out`` ((n, hq, l, hd), unit last stride) receives the result in place; it must not
     overlap q or the cache."""
     name = "sdpa_paged"
-    p = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
-    sq, sq_copy, so, nbytes, default = _paged_attn_plan(_meta(q), k_pages.shape[1], k_pages.shape[3], p.slots, _meta(out))
-    n, hq, l, _ = q.shape
-    if n != p.n or not (p.bytes or k_pages.dtype == q.dtype) or not _flat_ints(kv_len, n):
+    c = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
+    p = _paged_attn_plan(_meta(q), c.n, c.hkv, c.hd, None if c.bytes else k_pages.dtype, c.slots, _meta(out))
+    if not _flat_ints(kv_len, c.n):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
-    if out is not None:
-        _apart(name, out, q, k_pages, v_pages)
+    k_at, v_at = k_pages.data_ptr(), v_pages.data_ptr()
+    if out is not None and out.numel() and out.data_ptr() in (q.data_ptr(), k_at, v_at):
+        raise _lib.KuiopsError(name, _lib.E_INVALID)
     device = _gpu_of(name, q, k_pages, v_pages, table, kv_len, k_scale, v_scale, out)
-    given, q = q, _readable(q)
     if out is None:
-        out = q.new_empty((n, hq, l, k_pages.shape[3]))
-    lse = q.new_empty((n, hq, l), dtype=torch.float32) if return_lse else None
-    ws = _zeroed_workspace(q.device, nbytes) if nbytes else None
+        out = q.new_empty(q.shape)
+    sq = p.sq
+    if not p.in_place or q.data_ptr() % 16:
+        q, sq = _copied(q), p.sq_copy
+    lse = q.new_empty(p.dims, dtype=torch.float32) if return_lse else None
+    ws = _zeroed_workspace(q.device, device, p.ws) if p.ws else None
     _enqueue("kuiops_sdpa_paged", device, (
-        n, hq, l, _dt(q.dtype), q.data_ptr(), sq if q is given else sq_copy, p.layout, k_pages.data_ptr(), v_pages.data_ptr(),
-        _ptr(k_scale), _ptr(v_scale), table.data_ptr(), kv_len.data_ptr(), out.data_ptr(), so, _ptr(lse),
-        default if scale is None else float(scale), _ptr(ws), nbytes))
+        *p.dims, p.dtype, q.data_ptr(), sq, c.layout, k_at, v_at, _ptr(k_scale), _ptr(v_scale), table.data_ptr(), kv_len.data_ptr(),
+        out.data_ptr(), p.so, _ptr(lse), p.scale if scale is None else float(scale), _ptr(ws), p.ws))
     return out, lse

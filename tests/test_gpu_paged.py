@@ -99,6 +99,17 @@ def test_sdpa_paged(cuda, n, hq, hkv, l, hd, page, lens, dtype, kind):
     attends(c, gen((n, hq, l, hd), dtype, 1), lens)
 
 
+def some_of(c, q, lens, picked):
+    """Attention of all sequences, checked for the picked ones."""
+    out, lse = ops.sdpa_paged(q.to(c.device), **c.args(), kv_len=ints(lens, c.device), return_lse=True)
+    for b in picked:
+        own = torch.from_numpy(c.table[b].astype(np.int64)).to(c.device)
+        k, v, ks, vs = (None if x is None else npy(x[own]) for x in c.pages + c.scales)
+        ref, lref, size, terms = O.sdpa_paged(npy(q[b:b + 1]), k, v, [np.arange(len(own))], lens[b:b + 1], ks, vs)
+        close_out(out[b:b + 1], ref, size, terms, q.shape[-1], False)
+        close_lse(lse[b:b + 1], lref, terms, q.shape[-1])
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_sdpa_paged_over_turns_of_page_numbers(cuda, kind):
     # the numbers of 32 turns (4096 slots) of a work-group are fetched at once: 70 sequences' heads leave one split
@@ -106,12 +117,40 @@ def test_sdpa_paged_over_turns_of_page_numbers(cuda, kind):
     g = np.random.default_rng(0)
     lens = [int(x) for x in g.integers(1, 200, 70)]
     lens[0], lens[1], lens[69] = 8561, 4096, 4129
-    q = gen((70, 4, 1, 64), BF, 1)
-    out, _ = ops.sdpa_paged(q.to(cuda), **c.args(), kv_len=ints(lens, cuda))
-    (k, v), (ks, vs) = c.numbers()
-    for b in (0, 1, 5, 69):
-        ref, _, size, terms = O.sdpa_paged(npy(q[b:b + 1]), k, v, c.table[b:b + 1], lens[b:b + 1], ks, vs)
-        close_out(out[b:b + 1], ref, size, terms, 64, False)
+    some_of(c, gen((70, 4, 1, 64), BF, 1), lens, (0, 1, 5, 69))
+
+
+# From 16 tiles of 32 slots a work-group on (256 of them over the 16-row groups) the tiles of all
+# sequences and KV heads are one list: pieces end anywhere in a sequence, units of one tile and
+# empty sequences lie between others.
+EVEN = [  # n, hq, hkv, l, hd, page, lens, checked
+    (9, 8, 8, 1, 64, 64, (3200, 0, 1, 3199, 2377, 33, 2800, 3200, 2900), (0, 1, 2, 3, 4, 5, 8)),
+    (2, 16, 16, 1, 128, 48, (6000, 5000), (0, 1)),
+    (1, 20, 1, 2, 64, 16, (50000,), (0,)),                          # three row groups of 40 rows
+    (130, 2, 2, 1, 64, 32, tuple(700 - 3 * (b % 90) for b in range(130)), (0, 1, 63, 64, 65, 127, 128, 129)),    # past 64 sequences
+    (70, 8, 8, 1, 64, 16, tuple(1300 - b * (b % 3) for b in range(70)), (0, 2, 40, 64, 69)),                     # two units a work-group and more
+]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,hq,hkv,l,hd,page,lens,checked", EVEN)
+def test_sdpa_paged_even_pieces(cuda, n, hq, hkv, l, hd, page, lens, checked, kind):
+    row_groups = -(-(hq // hkv * l) // 16)
+    tiles = hkv * sum(max(1, -(-x // 32)) for x in lens)
+    assert tiles >= (16 if n * hkv < 512 // row_groups else 64) * (256 // row_groups)
+    c = Cache(cuda, BF, kind, n, hkv, hd, page, -(-max(lens) // page), seed=31)
+    some_of(c, gen((n, hq, l, hd), BF, 1), lens, checked)
+
+
+def test_large_pools_pass_by_the_caches(cuda):
+    # (pools of 120 MB and more are read with other loads)
+    for kind, dtype, hd, n in (("same", BF, 128, 8), ("int8", HF, 64, 32), ("e4m3", BF, 128, 16), ("same", HF, 64, 16)):
+        page, width, hkv = 64, 66 if n < 32 else 62, 8
+        lens = [width * page - 31 * b for b in range(n)]
+        bytes_ = 2 * n * width * page * hkv * hd * (2 if kind == "same" else 1)
+        c = Cache(cuda, dtype, kind, n, hkv, hd, page, width, seed=32)
+        assert bytes_ >= 120 << 20
+        some_of(c, gen((n, hkv, 1, hd), dtype, 1), lens, (0, n - 1))
 
 
 @pytest.mark.parametrize("kind", KINDS)
