@@ -92,10 +92,12 @@ __device__ __forceinline__ float byte_value(uint32_t w) {
     if constexpr (PK == kInt8) return (float)(int8_t)(w >> (8 * I));
     else return __builtin_amdgcn_cvt_f32_fp8((int)w, I);
 }
-// Bytes 0, 1 (H = 0) or 2, 3 (H = 1) of w as two bf16.
+// Bytes 0, 1 (H = 0) or 2, 3 (H = 1) of w as two bf16 (e4m3: one conversion; two and a
+// permute took 77.2 us where this takes 75.0).
 template <int PK, int H>
 __device__ __forceinline__ uint32_t pair_of(uint32_t w) {
-    return upper_halves(byte_value<PK, 2 * H>(w), byte_value<PK, 2 * H + 1>(w));
+    if constexpr (PK == kE4M3) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, H));
+    else return upper_halves(byte_value<PK, 2 * H>(w), byte_value<PK, 2 * H + 1>(w));
 }
 // Byte I of two words as two bf16.
 template <int PK, int I>
@@ -179,6 +181,13 @@ template <typename A> __device__ __forceinline__ const A &late_args() {
 // A part that is 0 times an infinite value is NaN, so is a masked NaN: a wave whose sums
 // are not finite goes over its keys again with the row maxima that it found, value by value
 // for the rows that see them.
+// What bounds it: the K / V stream (a plain read of as much reaches 5.4 to 6.1 TB/s with the
+// launch) and what lies around it: arguments, lengths, page numbers and first keys one after
+// another 3 us, the waves' merge 0.9, pieces stored, counted and merged 2.  Kernel alone: 16
+// sequences of 2000 to 4000 keys, 32 / 8 heads of 128, bf16 39.5 us, 5.2 TB/s; 32 of 4000 to
+// 8000 in e4m3 75 us, 5.5 TB/s; 60001 keys of one sequence in int8 31 us, 4.1 TB/s; 600 keys of
+// one sequence, heads of 64: 8.7 us.  Two tiles in flight a wave took longer (16 sequences 45.8
+// against 44.2), with 214 instead of 256 registers; so did 8 waves.
 template <typename T, int PK, int HD, int NWV, int AUX>
 __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
     typedef typename std::conditional<PK == kSame, T, bf16_t>::type C;       // the products' type
@@ -294,7 +303,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) offV[i] = lr * DT < a.c.hd ? (uint32_t)(((4 * G4 + i) * a.c.sv2 + lr * DT) * B) : kOut;
 
-    const int64_t rowK = a.c.sk2 * B, rowV = a.c.sv2 * B;
+    const uint32_t rowK = (uint32_t)a.c.sk2 * B, rowV = (uint32_t)a.c.sv2 * B;        // (below 2^25)
     constexpr int D4 = HD / 4;
 
     // Where the 16-slot groups of 32 turns lie, a lane each: the rows that are there, the
@@ -360,7 +369,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
         for (int t = 0; t < 2; ++t) {
             const int from = 2 * (turn - turn0) + t;
             const int m = there[t] = __builtin_amdgcn_readlane(now.n, from);
-            const __amdgpu_buffer_rsrc_t rk = make_rsrc(address(now.k, from), m ? (uint32_t)((m - 1) * rowK) + a.c.hd * B : 0u);
+            const __amdgpu_buffer_rsrc_t rk = make_rsrc(address(now.k, from), m ? (m - 1) * rowK + a.c.hd * B : 0u);
 #pragma unroll
             for (int j = 0; j < KL; ++j) kr[t][j] = load_words<4, AUX>(rk, offK[j]);
             if constexpr (PK != kSame)
@@ -373,7 +382,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int from = 2 * (turn - turn0) + t, m = there[t];
-            const __amdgpu_buffer_rsrc_t rv = make_rsrc(address(now.v, from), m ? (uint32_t)((m - 1) * rowV) + a.c.hd * B : 0u);
+            const __amdgpu_buffer_rsrc_t rv = make_rsrc(address(now.v, from), m ? (m - 1) * rowV + a.c.hd * B : 0u);
             if constexpr (PK != kSame)
                 vs[t] = __builtin_bit_cast(f32x4, load_words<4>(make_rsrc(address(now.vs, from), m * 4), G4 * 16));
 #pragma unroll
@@ -479,11 +488,11 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float p = fast_exp2(__builtin_fmaf(sc[t][i], a.scale_log2, -mref));
-                l_run += p;
-                if constexpr (PK != kSame) p *= vs[t][i];
+                float w = fast_exp2(__builtin_fmaf(sc[t][i], a.scale_log2, -mref));
+                l_run += w;
+                if constexpr (PK != kSame) w *= vs[t][i];
                 C x[NP];
-                Parts<C>::split(p, x);
+                Parts<C>::split(w, x);
 #pragma unroll
                 for (int y = 0; y < NP; ++y) part[y][4 * t + i] = x[y];
             }
@@ -496,12 +505,18 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
                     const uint32_t lo = word(vr[2 * e], c >> 1), hi = word(vr[2 * e + 1], c >> 1);
                     w[e] = c & 1 ? __builtin_amdgcn_perm(hi, lo, 0x07060302u) : __builtin_amdgcn_perm(hi, lo, 0x05040100u);
                 } else {
-                    const uint32_t lo = word(vr[2 * e], c >> 2), hi = word(vr[2 * e + 1], c >> 2);
-                    switch (c & 3) {
-                        case 0: w[e] = pair_across<PK, 0>(lo, hi); break;
-                        case 1: w[e] = pair_across<PK, 1>(lo, hi); break;
-                        case 2: w[e] = pair_across<PK, 2>(lo, hi); break;
-                        default: w[e] = pair_across<PK, 3>(lo, hi); break;
+                    const uint32_t a0 = word(vr[2 * e], c >> 2), a1 = word(vr[2 * e + 1], c >> 2);
+                    if constexpr (PK == kInt8) {
+                        switch (c & 3) {
+                            case 0: w[e] = pair_across<PK, 0>(a0, a1); break;
+                            case 1: w[e] = pair_across<PK, 1>(a0, a1); break;
+                            case 2: w[e] = pair_across<PK, 2>(a0, a1); break;
+                            default: w[e] = pair_across<PK, 3>(a0, a1); break;
+                        }
+                    } else {
+                        // (columns c and c ^ 1 of a key in one conversion)
+                        const uint32_t lo = c & 2 ? pair_of<PK, 1>(a0) : pair_of<PK, 0>(a0), hi = c & 2 ? pair_of<PK, 1>(a1) : pair_of<PK, 0>(a1);
+                        w[e] = c & 1 ? __builtin_amdgcn_perm(hi, lo, 0x07060302u) : __builtin_amdgcn_perm(hi, lo, 0x05040100u);
                     }
                 }
             }
@@ -531,13 +546,13 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
             const int k0 = group_key(p, turn, 0);
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-                float p = fast_exp2(__builtin_fmaf(sc[x >> 2][x & 3], a.scale_log2, -mref));
-                if constexpr (PK != kSame) p *= vs[x >> 2][x & 3];
+                float w = fast_exp2(__builtin_fmaf(sc[x >> 2][x & 3], a.scale_log2, -mref));
+                if constexpr (PK != kSame) w *= vs[x >> 2][x & 3];
                 const int from = 2 * (turn - turn0) + (x >> 2);
                 const char *vfirst = address(now.v, from);
                 for (int g = 0; g < 4; ++g) {
                     const int at = 4 * g + (x & 3);
-                    const float pk = __shfl(p, g * 16 + lr, 64);
+                    const float pk = __shfl(w, g * 16 + lr, 64);
                     if (at >= there[x >> 2] || !row_ok || k0 + 16 * (x >> 2) + at > last) continue;
                     const char *vp = vfirst + at * rowV;
 #pragma unroll
