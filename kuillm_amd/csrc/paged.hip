@@ -187,7 +187,7 @@ __device__ __forceinline__ void to_bytes(const float (&x)[8], float m, u32x2 &w)
 // What bounds it: the bytes, and for 8 bits the arithmetic about as much; waves at work hide
 // both, so registers are kept few (4 ragged prompts of 4001 tokens, 32 + 8 heads of 128, normed:
 // 7 waves a SIMD 69 us, 4.8 TB/s, 5 waves 82; two tokens a work-group 74, four 78; heads handed
-// out over the threads in turn, 4 tokens a work-group, 73; 6150 tokens in e4m3: 8 / 7 / 6 / 5 waves 55 / 44 / 45 / 49).
+// out over the threads in turn, 4 tokens a work-group, 73; 6297 tokens in e4m3: 8 / 7 / 6 / 5 waves 55 / 44 / 45 / 49).
 constexpr int kAppendThreads = 512;
 template <typename T, int PK, int HD>
 __global__ __launch_bounds__(kAppendThreads, PK == 0 ? 7 : 6) void paged_append_kernel(AppendArgs a) {
@@ -360,8 +360,8 @@ struct ReadArgs {
 // paged_read_kernel -- a work-group has 128 slots of one KV head, keys and values; 8 values of
 // a row a lane, so that what is written, the larger part, goes out in 16-byte pieces that
 // follow one another.  All loads of a thread are on their way at once, behind its page numbers.
-// What bounds it: the bytes; 8 sequences of 4000 to 8000 rows, 8 heads of 128 in int8, to bf16 with
-// the rows behind them cleared 78.5 us, 4.8 TB/s read and written (a large copy 5.1); 16 values
+// What bounds it: the bytes; 8 sequences of 4583 to 8000 rows, 8 heads of 128 in int8, to bf16 with
+// the rows behind them cleared 78.5 us, 4.7 TB/s read and written (a large copy 5.1); 16 values
 // a lane, stored 8 bytes at a time, 85.6.
 template <typename T, int PK, int HD>
 __global__ __launch_bounds__(256) void paged_read_kernel(ReadArgs a) {
@@ -428,7 +428,7 @@ constexpr int64_t kCUs = 256;
 
 template <typename T, int PK, int HD>
 void launch_append(AppendArgs &a, hipStream_t st) {
-    // up to 512 threads, for 8 bits 256 (6150 tokens of 48 heads of 128, e4m3: 44 -> 42 us)
+    // up to 512 threads, for 8 bits 256 (6297 tokens of 48 heads of 128, e4m3: 44 -> 42 us)
     constexpr int LPH = HD / 16, most = (PK == 0 ? kAppendThreads : kAppendThreads / 2) / LPH;
     const int heads = a.hq + 2 * a.c.hkv;
     // few tokens: the heads are spread over work-groups until each CU has one, a wave of heads each

@@ -184,7 +184,7 @@ template <typename A> __device__ __forceinline__ const A &late_args() {
 // What bounds it: the K / V stream (a plain read of as much reaches 5.4 to 6.1 TB/s with the
 // launch) and what lies around it: arguments, lengths, page numbers and first keys one after
 // another 3 us, the waves' merge 0.9, pieces stored, counted and merged 2.  Kernel alone: 16
-// sequences of 2000 to 4000 keys, 32 / 8 heads of 128, bf16 39.5 us, 5.2 TB/s; 32 of 4000 to
+// sequences of 2111 to 4000 keys, 32 / 8 heads of 128, bf16 39.7 us, 5.1 TB/s; 32 of 4085 to
 // 8000 in e4m3 75 us, 5.5 TB/s; 60001 keys of one sequence in int8 31 us, 4.1 TB/s; 600 keys of
 // one sequence, heads of 64: 8.7 us.  Two tiles in flight a wave took longer (16 sequences 45.8
 // against 44.2), with 214 instead of 256 registers; so did 8 waves.
