@@ -779,8 +779,7 @@ typedef struct kuiops_paged_layout {
  * ([hd], of dtype; null: y = x), then turn by the angles pos * inv_freq[i]: the
  * pairs (y_i, y_{i + hd/2}) -> (y_i cos - y_{i+hd/2} sin, y_{i+hd/2} cos + y_i
  * sin), angles in 64 bits, one rounding at the end.  q_out: strides sq = batch,
- * head, token.  Slots that receive a token must not be named by two sequences'
- * tables.  dtype BF16 / F16, equal to the pages' unless those are of 8 bits.     */
+ * head, token.  A page that receives tokens must be named once in the table.  dtype BF16 / F16, equal to the pages' unless those are of 8 bits.     */
 KUIOPS_API int kuiops_kv_paged_append(int64_t n, int64_t t, int64_t hq, int dtype, const void *qkv, int64_t ld_tok,
                            int64_t ld_batch, const int32_t *lens, const int32_t *pos0, const float *inv_freq,
                            const void *q_norm, const void *k_norm, double eps, void *q_out, const int64_t sq[3],
@@ -802,9 +801,10 @@ KUIOPS_API int kuiops_kv_paged_read(int64_t n, int64_t s, int dtype, const kuiop
  * stays out of it.  kv_len: device int32[n], taken as 0 .. width * page.  Q / O:
  * strides batch, head, query; O must not overlap an input.  lse: fp32 [n][hq][l]
  * (natural log) or null.  scale > 0.  Workspace (slots = width * page): may be 0
- * bytes, 16-byte aligned; its contents must be zero before the first call with
- * it, and every call leaves them fit for the next one, of any sizes.  Calls that
- * share one must not run at the same time.                                   */
+ * bytes, 16-byte aligned; its first KUIOPS_SDPA_PAGED_ZEROED bytes must be zero
+ * before the first call with it, and every call leaves them zero, whatever its sizes.
+ * Calls that share one must not run at the same time.                       */
+#define KUIOPS_SDPA_PAGED_ZEROED 147456
 KUIOPS_API size_t kuiops_sdpa_paged_workspace(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t slots, int64_t hd);
 KUIOPS_API int kuiops_sdpa_paged(int64_t n, int64_t hq, int64_t l, int dtype, const void *Q, const int64_t sq[3],
                       const kuiops_paged_layout *at, const void *K, const void *V, const float *k_scale,

@@ -23,6 +23,8 @@ E_WORKSPACE = -4
 
 # kuiops_dtype
 F32, F16, BF16, F64, I64, I32, I16, I8, U8, BOOL, F8E4M3 = range(11)
+# bytes at the head of a kuiops_sdpa_paged workspace that start at zero
+SDPA_PAGED_ZEROED = 147456
 # kuiops_b_layout
 B_ROW, B_COL = 0, 1
 # kuiops_c_kind

@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(ReadArgs a) {
     constexpr int LPR = HD / 8, RPI = 256 / LPR, ROWS = 128, IT = ROWS / RPI, B = PK == 0 ? 2 : 1;
     typedef typename std::conditional<PK == 0, u32x4, u32x2>::type words;
     const int tid = threadIdx.x, d = tid % LPR * 8;
-    const int64_t bh = blockIdx.y, b = bh / a.c.hkv, hk = bh % a.c.hkv;
+    const int64_t b = blockIdx.z, hk = blockIdx.y;
     const int L = min(a.s, paged_len(a.c, a.kv_len, b)), s0 = blockIdx.x * ROWS, end = a.fill ? a.s : L;
     if (s0 >= end || d >= a.c.hd) return;
     int id[IT], at[IT];
@@ -448,17 +448,17 @@ void launch_append_kind(AppendArgs &a, hipStream_t st) {
 }
 
 template <typename T, int PK>
-void launch_read(const ReadArgs &a, unsigned heads, hipStream_t st) {
-    const dim3 grid((unsigned)cdiv(a.s, 128), heads);
+void launch_read(const ReadArgs &a, unsigned n, hipStream_t st) {
+    const dim3 grid((unsigned)cdiv(a.s, 128), (unsigned)a.c.hkv, n);
     if (a.c.hd <= 64) hipLaunchKernelGGL((paged_read_kernel<T, PK, 64>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((paged_read_kernel<T, PK, 128>), grid, dim3(256), 0, st, a);
 }
 
 template <typename T>
-void launch_read_kind(const ReadArgs &a, unsigned heads, hipStream_t st) {
-    if (a.c.dtype == KUIOPS_I8) launch_read<T, 1>(a, heads, st);
-    else if (a.c.dtype == KUIOPS_F8E4M3) launch_read<T, 2>(a, heads, st);
-    else launch_read<T, 0>(a, heads, st);
+void launch_read_kind(const ReadArgs &a, unsigned n, hipStream_t st) {
+    if (a.c.dtype == KUIOPS_I8) launch_read<T, 1>(a, n, st);
+    else if (a.c.dtype == KUIOPS_F8E4M3) launch_read<T, 2>(a, n, st);
+    else launch_read<T, 0>(a, n, st);
 }
 
 }  // namespace
@@ -510,16 +510,16 @@ extern "C" int kuiops_kv_paged_read(int64_t n, int64_t s, int dtype, const kuiop
     for (int i = 0; i < 3; ++i)
         if (sko[i] % unit || svo[i] % unit) return KUIOPS_E_UNSUPPORTED;
     if (!aligned16(k_out) || !aligned16(v_out)) return KUIOPS_E_UNSUPPORTED;
-    const int64_t heads = n * at->hkv;
-    if (s >= (1 << 30) || heads > 65535 || cdiv(s, 128) * heads >= (1 << 24)) return KUIOPS_E_UNSUPPORTED;
+    // grid axes, launches below 2^32 threads
+    if (s >= (1 << 30) || n > 65535 || at->hkv > 65535 || cdiv(s, 128) * n * at->hkv >= (1 << 24)) return KUIOPS_E_UNSUPPORTED;
     a.s = (int)s; a.kv_len = kv_len;
     a.k = k_out; a.v = v_out;
     a.ko0 = sko[0]; a.ko1 = sko[1]; a.ko2 = sko[2];
     a.vo0 = svo[0]; a.vo1 = svo[1]; a.vo2 = svo[2];
     a.fill = fill;
     hipStream_t st = as_stream(stream);
-    if (wide) at->dtype == KUIOPS_I8 ? launch_read<float, 1>(a, (unsigned)heads, st) : launch_read<float, 2>(a, (unsigned)heads, st);
-    else if (dtype == KUIOPS_BF16) launch_read_kind<bf16_t>(a, (unsigned)heads, st);
-    else launch_read_kind<f16_t>(a, (unsigned)heads, st);
+    if (wide) at->dtype == KUIOPS_I8 ? launch_read<float, 1>(a, (unsigned)n, st) : launch_read<float, 2>(a, (unsigned)n, st);
+    else if (dtype == KUIOPS_BF16) launch_read_kind<bf16_t>(a, (unsigned)n, st);
+    else launch_read_kind<f16_t>(a, (unsigned)n, st);
     return launch_status();
 }

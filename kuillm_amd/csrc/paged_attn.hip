@@ -38,7 +38,8 @@ constexpr int kEven = 16, kEvenMany = 64;
 struct PagedArgs {
     PagedCache c;
     int n, hq, l, groups, row_groups;      // groups: work-groups that share the keys evenly
-    int launched;
+    int launched, G;           // query heads of a KV head
+    float share;               // 1 / groups, a little more
     int may_part;              // there are work-groups enough for a piece each
     const void *Q;
     void *O;
@@ -211,9 +212,11 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
 
     // the row groups of a work-group's keys run on one XCD, whose L2 then has them for all but
     // the first
-    const int idx = blockIdx.x >> 3, me = idx / a.row_groups * 8 + (blockIdx.x & 7), rg = idx % a.row_groups;
+    // (what would be divided by 1 mostly is not: 40 instructions one after another)
+    const int idx = blockIdx.x >> 3, of = a.row_groups == 1 ? idx : idx / a.row_groups, rg = idx - of * a.row_groups;
+    const int me = of * 8 + (blockIdx.x & 7);
     if (me >= a.launched) return;
-    const int G = a.hq / a.c.hkv, rows_kv = G * a.l, r0 = rg * R, nrows = min(R, rows_kv - r0);
+    const int G = a.G, rows_kv = G * a.l, r0 = rg * R, nrows = min(R, rows_kv - r0);
 
     // Places in the list (`apart`: pieces) of a sequence's KV head.  A unit begins with kSwitch
     // places that no tile has.
@@ -227,8 +230,9 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
     all *= a.c.hkv;
     const bool apart = a.may_part && all < (a.n * a.c.hkv < 2 * a.groups ? kEven : kEvenMany) * a.groups;
     if (!apart && me >= a.groups) return;
-    per = apart ? max(kPiece, (all + a.groups - 1) / a.groups)
-                : max(kSwitch + kLeast, (all + a.n * a.c.hkv * kSwitch + a.groups - 1) / a.groups);
+    // (more than a share of the places, by 2^-20 of it and one: the same in all work-groups)
+    per = apart ? max(kPiece, (int)((float)all * a.share) + 1)
+                : max(kSwitch + kLeast, (int)((float)(all + a.n * a.c.hkv * kSwitch) * a.share) + 1);
     int cur = apart ? me : me * per;
     auto weight = [&](int len) __attribute__((always_inline)) {
         const int t = paged_tiles(len);
@@ -253,13 +257,14 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
     }
     // (in a unit of the sequence: its KV head, and the piece of an `apart` one)
     const int inside = cur - before * a.c.hkv;
-    p.hk = inside / p.pieces;
+    p.hk = p.pieces == 1 ? inside : inside / p.pieces;
     if (apart) {
         const int z = inside - p.hk * p.pieces, tiles = paged_tiles(p.L);
+        const int each = p.pieces == 1 ? tiles : tiles / p.pieces, longer = tiles - each * p.pieces;      // the first ones have one more
         p.first = me - z;
         p.late = 0;
-        p.t0 = (int)((int64_t)z * tiles / p.pieces);
-        p.t1 = (int)((int64_t)(z + 1) * tiles / p.pieces);
+        p.t0 = z * each + min(z, longer);
+        p.t1 = p.t0 + each + (z < longer ? 1 : 0);
     }
     // the tiles of u among the places cur .. stop - 1
     auto cut_out = [&](Piece &u) __attribute__((always_inline)) {
@@ -292,7 +297,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
     // row r0 + lr of the KV head's list
     const int rr = r0 + lr;
     const bool row_ok = rr < rows_kv;
-    const int h = row_ok ? rr / a.l : 0, pos = row_ok ? rr - h * a.l : 0;
+    const int h = !row_ok ? 0 : a.l == 1 ? rr : rr / a.l, pos = row_ok ? rr - h * a.l : 0;
     uint32_t offK[KL];
 #pragma unroll
     for (int j = 0; j < KL; ++j) {
@@ -599,7 +604,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
     const PagedArgs &e = late_args<PagedArgs>();
     auto store_row = [&](int r, int d, f32x4 v, float m, float ls) __attribute__((always_inline)) {
         typedef T t4 __attribute__((ext_vector_type(4)));
-        const int head = u.hk * G + (r0 + r) / e.l, i = (r0 + r) % e.l;
+        const int hr = e.l == 1 ? r0 + r : (r0 + r) / e.l, head = u.hk * G + hr, i = r0 + r - hr * e.l;
         const float inv = ls != 0.f ? 1.f / ls : 0.f;
         if (d < e.c.hd) {
             t4 w;
@@ -741,6 +746,7 @@ constexpr int kMaxGroups = 256;
 // The counters' part of a workspace, the same for calls of all sizes
 constexpr int kApart = 2048;
 constexpr size_t kCounterBytes = (size_t)(kApart + kMaxGroups) * kCounterStride * 4;
+static_assert(kCounterBytes == KUIOPS_SDPA_PAGED_ZEROED, "what callers clear");
 
 PagedPlan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t slots, int64_t hd) {
     PagedPlan p{};
@@ -819,7 +825,7 @@ extern "C" int kuiops_sdpa_paged(int64_t n, int64_t hq, int64_t l, int dtype, co
     const PagedPlan p = plan_of(n, hq, at->hkv, l, slots, at->hd);
     const size_t need = p.counter_bytes + p.ml_bytes + p.o_bytes;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KUIOPS_E_WORKSPACE;
-    a.n = (int)n; a.hq = (int)hq; a.l = (int)l; a.groups = p.groups; a.may_part = p.may_part; a.launched = p.launched; a.row_groups = p.row_groups;
+    a.n = (int)n; a.hq = (int)hq; a.l = (int)l; a.groups = p.groups; a.may_part = p.may_part; a.launched = p.launched; a.G = (int)(hq / at->hkv); a.share = (1.f + 0x1p-20f) / (float)p.groups; a.row_groups = p.row_groups;
     a.Q = Q; a.O = O;
     a.sq0 = sq[0]; a.sq1 = sq[1]; a.sq2 = sq[2];
     a.so0 = so[0]; a.so1 = so[1]; a.so2 = so[2];

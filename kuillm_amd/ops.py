@@ -1621,8 +1621,8 @@ def kv_paged_append(qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale=None, 
     eps) * weight; then queries and keys turn by the angles position * ``inv_freq``
     (fp32 [hd / 2]), in 64 bits, and are rounded once.  8-bit pages get a row x as
     stored * scale, scale = max |x| / M, stored = nearest(x M / max |x|), M = 127 (int8)
-    or 448 (float8_e4m3fn); a row that is not finite reads back as NaN.  A slot that
-    receives a token must belong to one sequence.  bf16 / f16; hd a multiple of 16 up to
+    or 448 (float8_e4m3fn); a row that is not finite reads back as NaN.  A page that
+    receives tokens must be named once in the table.  bf16 / f16; hd a multiple of 16 up to
     128, pages of multiples of 16 rows.  ``q_out`` receives q in place."""
     name = "kv_paged_append"
     c = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
@@ -1731,11 +1731,14 @@ def _paged_attn_plan(q, n, hkv, hd, pages, slots, out) -> _PagedAttnPlan:
     return p
 
 
-def _zeroed_workspace(device, index, nbytes):
-    """sdpa_paged's workspace: the current stream's own, or memory of its own (and its
-    zero fill) in a graph that is being captured, so that two graphs may run at once."""
+def _paged_workspace(device, index, nbytes):
+    """sdpa_paged's workspace: the current stream's own, or memory of its own (and the
+    zero fill of its counters) in a graph that is being captured, so that two graphs may
+    run at once."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:_lib.SDPA_PAGED_ZEROED].zero_()
+        return ws
     buf = _WS.get((index, _raw_stream(index), "paged"))
     return buf if buf is not None and buf.numel() >= nbytes else workspace(device, nbytes, "paged")
 
@@ -1766,7 +1769,7 @@ def sdpa_paged(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=None, s
     if not p.in_place or q.data_ptr() % 16:
         q, sq = _copied(q), p.sq_copy
     lse = q.new_empty(p.dims, dtype=torch.float32) if return_lse else None
-    ws = _zeroed_workspace(q.device, device, p.ws) if p.ws else None
+    ws = _paged_workspace(q.device, device, p.ws) if p.ws else None
     _enqueue("kuiops_sdpa_paged", device, (
         *p.dims, p.dtype, q.data_ptr(), sq, c.layout, k_at, v_at, _ptr(k_scale), _ptr(v_scale), table.data_ptr(), kv_len.data_ptr(),
         out.data_ptr(), p.so, _ptr(lse), p.scale if scale is None else float(scale), _ptr(ws), p.ws))

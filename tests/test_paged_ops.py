@@ -299,7 +299,7 @@ def test_c_entries_refuse_on_the_host(lib):
     assert append(x=null) == append(f=null) == append(eps=-1.0) == append(eps=float("nan")) == INVALID
     assert append(ld=500) == append(x=off) == append(w=off) == append(n=1 << 16) == append(t=1 << 24) == UNSUPPORTED
     assert read(ln=null) == read(out=null) == INVALID
-    assert read(out=off) == read(so=_lib.strides3(0, 0, 60)) == read(s=1 << 30) == read(n=1 << 15) == UNSUPPORTED
+    assert read(out=off) == read(so=_lib.strides3(0, 0, 60)) == read(s=1 << 30) == read(n=1 << 16) == read(n=1 << 15, s=1 << 15) == UNSUPPORTED
     # splits need their workspace
     need = lib.kuiops_sdpa_paged_workspace(2, 4, 2, 1, 4800, 64)
     assert need > 0
@@ -307,6 +307,7 @@ def test_c_entries_refuse_on_the_host(lib):
 
 
 def test_workspace_sizes(lib):
+    assert f"#define KUIOPS_SDPA_PAGED_ZEROED {_lib.SDPA_PAGED_ZEROED}\n" in (C.INCLUDE / "kuiops.h").read_text()
     f = lib.kuiops_sdpa_paged_workspace
     for args in ((0, 4, 2, 1, 48, 64), (2, 4, 2, 1, 0, 64), (2, 3, 2, 1, 48, 64), (2, 4, 0, 1, 48, 64), (1, 4, 1, 1, 32, 64)):
         assert f(*args) == 0
