@@ -798,7 +798,7 @@ KUIOPS_API int kuiops_kv_paged_read(int64_t n, int64_t s, int dtype, const kuiop
 /* Attention of the newest tokens over the pages: query i of sequence b is slot
  * kv_len[b] - l + i and sees the slots up to its own that have a page (none: output
  * 0, lse -inf).  What lies elsewhere in the pages, NaN and infinities included,
- * stays out of it.  kv_len: device int32[n], taken as 0 .. width * page.  Q / O:
+ * stays out of it.  kv_len: device int32[n]; slots past the table have no page.  Q / O:
  * strides batch, head, query; O must not overlap an input.  lse: fp32 [n][hq][l]
  * (natural log) or null.  scale > 0.  Workspace (slots = width * page): may be 0
  * bytes, 16-byte aligned; its first KUIOPS_SDPA_PAGED_ZEROED bytes must be zero

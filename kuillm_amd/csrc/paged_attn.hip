@@ -2,7 +2,7 @@
 //
 //   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i k_j - lse_i)  over the slots j <= L - l + i
 //
-// of the sequence's L = kv_len[b] ones; slot j is row j % page of page
+// of the sequence's L = kv_len[b] ones, as far as its table goes; slot j is row j % page of page
 // table[b][j / page].  8-bit pages: k_j = ks_j * K_j and v_j = vs_j * V_j with a scale
 // per row.  Rows of the query heads that share a KV head are one list (row = head in
 // group * l + position), so K and V are read once for all of them.
@@ -408,8 +408,11 @@ __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
     const bool more = !apart && next_piece(then);
     Entries later{};
     if (more) later = fetch(then, 0);
-    const int free_end = p.L - a.l + 1;               // slots below are seen by every row
-    const int last = p.L - a.l + pos;                 // the row's last slot
+    // (a length may pass its table's end.  Read here, where keys are waited for: 600 slots 8.6 us, as
+    // without it; with the lengths above 8.8)
+    const int told = max(a.kv_len[p.b], p.L);
+    const int free_end = told - a.l + 1;              // slots below are seen by every row
+    const int last = told - a.l + pos;                // the row's last slot
     const int mine = (p.t1 - p.t0 - wave + NWV - 1) / NWV;  // turns of this wave
     frag qf[NQ][KK];
 #pragma unroll

@@ -1748,8 +1748,8 @@ def sdpa_paged(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=None, s
 
     q (n, hq, l, hd): query i of sequence b is slot ``kv_len[b]`` - l + i (int32 [n] on the
     device, read when the kernel runs; its own key among the slots, so appended before)
-    and sees the slots up to its own that have a page; one that sees none gives 0 and
-    lse -inf.  For decoding (l = 1) and a few drafted tokens: up to 16 rows of l * hq /
+    and sees the slots up to its own that have a page (a length may pass the table's
+    end); one that sees none gives 0 and lse -inf.  For decoding (l = 1) and a few drafted tokens: up to 16 rows of l * hq /
     hkv share a pass over the cache (longer pieces of a prompt: :func:`kv_paged_read` and
     :func:`sdpa_decode_accum`).  bf16 / f16; hd a multiple of 16 up to 128; scale > 0.
     ``out`` ((n, hq, l, hd), unit last stride) receives the result in place; it must not

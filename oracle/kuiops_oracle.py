@@ -810,5 +810,5 @@ def sdpa_paged(q, k, v, table, kv_len, k_scale=None, v_scale=None, scale=None):
     vv, _ = paged_rows(v, v_scale, table, max(lens, default=0))
     got = []
     for b, L in enumerate(lens):
-        got.append(_attend_rows(q[b], kk[b], vv[b], lambda i, b=b, L=L: [j for j in range(max(0, L - l + i + 1)) if there[b, j]], scale))
+        got.append(_attend_rows(q[b], kk[b], vv[b], lambda i, b=b, L=L: [j for j in range(min(L, int(kv_len[b]) - l + i + 1)) if there[b, j]], scale))
     return np.stack([x[0] for x in got]), np.stack([x[1] for x in got]), np.stack([x[3] for x in got]), max(x[4] for x in got)

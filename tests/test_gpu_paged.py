@@ -165,6 +165,16 @@ def test_absent_pages_are_not_seen(cuda, dtype, kind):
     attends(c, gen((4, 4, 2, 64), dtype, 2), (600, 640, 635, 500))
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("width,l", [(3, 4), (3, 20), (200, 5)])
+def test_drafted_tokens_that_pass_the_table(cuda, width, l, kind):
+    # the queries of slots that the table has keep them, whatever lies past its end
+    end = 16 * width
+    c = Cache(cuda, BF, kind, 6, 2, 64, 16, width, seed=41)
+    attends(c, gen((6, 4, l, 64), BF, 2), (end, end + 1, end + 3, end + l, end + l + 7, 2 ** 31 - 1))
+    attends(c, gen((6, 4, l, 64), BF, 3), (end + 2, 3, -1, end + 1, 0, -2 ** 31))
+
+
 def test_lengths_outside_the_table(cuda):
     c = Cache(cuda, BF, "same", 4, 2, 64, 16, 3, seed=6)
     attends(c, gen((4, 4, 1, 64), BF, 2), (49, -1, 2 ** 31 - 1, -2 ** 31))

@@ -71,6 +71,16 @@ def test_a_full_table_is_a_cache():
     np.testing.assert_allclose(lse, lref, rtol=1e-12)
 
 
+def test_queries_keep_their_slots_past_the_table():
+    r = np.random.default_rng(2)
+    k, v, q = r.standard_normal((3, 1, 16, 8)), r.standard_normal((3, 1, 16, 8)), r.standard_normal((1, 2, 4, 8))
+    whole, _, _, _ = O.sdpa_paged(q, k, v, [[0, 1, 2]], [34])                # slots 30 .. 33
+    out, _, _, _ = O.sdpa_paged(q, k, v, [[0, 1]], [34])
+    np.testing.assert_array_equal(out[:, :, :2], whole[:, :, :2])
+    without, _, _, _ = O.sdpa_paged(q, k, v, [[0, 1, -1]], [34])
+    np.testing.assert_array_equal(out, without)
+
+
 # ------------------------------------------------- the kernels' arithmetic, on the host
 
 @pytest.fixture(scope="module")
