@@ -1751,7 +1751,9 @@ def sdpa_paged(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=None, s
     and sees the slots up to its own that have a page (a length may pass the table's
     end); one that sees none gives 0 and lse -inf.  For decoding (l = 1) and a few drafted tokens: up to 16 rows of l * hq /
     hkv share a pass over the cache (longer pieces of a prompt: :func:`kv_paged_read` and
-    :func:`sdpa_decode_accum`).  bf16 / f16; hd a multiple of 16 up to 128; scale > 0.
+    :func:`sdpa_decode_accum`).  After :func:`kv_paged_append` of t tokens with ``lens``
+    pass pos0 + t for all: the tokens that are there see what they should, the rows of
+    padding are of no use.  bf16 / f16; hd a multiple of 16 up to 128; scale > 0.
     ``out`` ((n, hq, l, hd), unit last stride) receives the result in place; it must not
     overlap q or the cache."""
     name = "sdpa_paged"

@@ -650,6 +650,32 @@ def test_a_server_of_three_sequences(cuda, kind):
     assert pos.tolist() == [110, 37, 84]
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_drafted_tokens_of_a_padded_batch(cuda, kind):
+    """Fewer drafted tokens than others have: with kv_len = pos0 + t each token sees what it
+    sees alone, whatever lies in the slots of the padding (or past the table's end)."""
+    n, t, hq, hkv, hd, page, width = 5, 4, 8, 2, 64, 16, 6
+    pos0, lens = (90, 95, 0, 33, 92), (4, 1, 2, 0, 3)
+    c = Cache(cuda, BF, kind, n, hkv, hd, page, width, seed=42)
+    for b, (p, m) in enumerate(zip(pos0, lens)):        # not finite where the padding would be
+        for s in range(p + m, min(p + t, page * width)):
+            at = c.table[b, s // page], slice(None), s % page
+            for x in (c.pages if kind == "same" else c.scales):
+                x[at] = NAN
+    a, freq = c.args(), frequencies(hd).to(cuda)
+    qkv = gen((n, t, (hq + 2 * hkv) * hd), BF, 1).to(cuda)
+    start = ints(pos0, cuda)
+    q = ops.kv_paged_append(qkv, freq, start, **a, lens=ints(lens, cuda))
+    out, lse = ops.sdpa_paged(q, **a, kv_len=start + t, return_lse=True)
+    for b, m in enumerate(lens):
+        if m:
+            one = Cache.__new__(Cache)
+            one.__dict__.update(c.__dict__, table=c.table[b:b + 1])
+            ref, lref, size, terms = one.attention(q[b:b + 1, :, :m], [pos0[b] + m])
+            close_out(out[b:b + 1, :, :m], ref, size, terms, hd, False)
+            close_lse(lse[b:b + 1, :, :m], lref, terms, hd)
+
+
 def test_custom_ops_on_the_gpu(cuda):
     from kuillm_amd import library  # noqa: F401
     op = torch.ops.kuiops
