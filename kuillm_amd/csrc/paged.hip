@@ -496,7 +496,7 @@ extern "C" int kuiops_kv_paged_append(int64_t n, int64_t t, int64_t hq, int dtyp
     if (n == 0 || t == 0) return KUIOPS_OK;
     const int bad = check_cache(at, dtype, K, V, k_scale, v_scale, table, a.c);
     if (bad) return bad;
-    if (!qkv || !inv_freq || (hq > 0 && !q_out) || !(eps >= 0.0)) return KUIOPS_E_INVALID;
+    if (!qkv || !inv_freq || (hq > 0 && !q_out) || !(eps >= 0.0 && eps < INFINITY)) return KUIOPS_E_INVALID;
     if (ld_tok % 8 || ld_batch % 8 || sq[0] % 8 || sq[1] % 8 || sq[2] % 8) return KUIOPS_E_UNSUPPORTED;
     if (!aligned16(qkv) || !aligned16(q_out) || (q_norm && !aligned16(q_norm)) || (k_norm && !aligned16(k_norm)))
         return KUIOPS_E_UNSUPPORTED;

@@ -1623,7 +1623,8 @@ def kv_paged_append(qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale=None, 
     stored * scale, scale = max |x| / M, stored = nearest(x M / max |x|), M = 127 (int8)
     or 448 (float8_e4m3fn); a row that is not finite reads back as NaN.  A page that
     receives tokens must be named once in the table.  bf16 / f16; hd a multiple of 16 up to
-    128, pages of multiples of 16 rows.  ``q_out`` receives q in place."""
+    128, pages of multiples of 16 rows.  ``q_out`` receives q in place; it must
+    not overlap qkv or the cache."""
     name = "kv_paged_append"
     c = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
     p = _append_plan(_meta(qkv), c.n, c.hkv, c.hd, None if c.bytes else k_pages.dtype, _meta(inv_freq), _meta(q_norm), _meta(k_norm),

@@ -166,6 +166,24 @@ def test_absent_pages_are_not_seen(cuda, dtype, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_sequences_that_share_pages(cuda, kind):
+    # a prefix in pages that all tables name, and one page over and over
+    c = Cache(cuda, HF, kind, 5, 2, 128, 32, 40, seed=43)
+    c.table[:, :30] = c.table[0, :30]
+    c.table[4] = 7
+    lens = (1000, 1280, 961, 5, 1279)
+    attends(c, gen((5, 8, 2, 128), HF, 2), lens)
+    k, v = ops.kv_paged_read(**c.args(), kv_len=ints(lens, cuda))
+    assert torch.equal(k[0, :, :960], k[2, :, :960]) and torch.equal(v[4, :, :32], v[4, :, 1216:1248])
+
+
+def test_more_rows_than_work_groups(cuda):
+    # 300 groups of 16 rows: each has the whole sequence
+    c = Cache(cuda, BF, "same", 1, 1, 64, 16, 50, seed=44)
+    attends(c, gen((1, 16, 300, 64), BF, 2), (777,))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("width,l", [(3, 4), (3, 20), (200, 5)])
 def test_drafted_tokens_that_pass_the_table(cuda, width, l, kind):
     # the queries of slots that the table has keep them, whatever lies past its end

@@ -306,7 +306,7 @@ def test_c_entries_refuse_on_the_host(lib):
     assert attn(q=off) == attn(sq=_lib.strides3(0, 0, 60)) == UNSUPPORTED
     assert attn(n=1 << 19) == attn(n=1 << 18, width=1 << 16) == attn(l=1 << 24) == attn(hq=1 << 20, l=1 << 10) == UNSUPPORTED
     assert attn(l=0) == attn(hq=0) == append(t=0) == read(s=0) == _lib.OK
-    assert append(x=null) == append(f=null) == append(eps=-1.0) == append(eps=float("nan")) == INVALID
+    assert append(x=null) == append(f=null) == append(eps=-1.0) == append(eps=float("nan")) == append(eps=float("inf")) == INVALID
     assert append(ld=500) == append(x=off) == append(w=off) == append(n=1 << 16) == append(t=1 << 24) == UNSUPPORTED
     assert read(ln=null) == read(out=null) == INVALID
     assert read(out=off) == read(so=_lib.strides3(0, 0, 60)) == read(s=1 << 30) == read(n=1 << 16) == read(n=1 << 15, s=1 << 15) == UNSUPPORTED
