@@ -91,15 +91,14 @@ __device__ __forceinline__ void turn_of(int64_t pos, float freq, double &c, doub
 
 // 1 / sqrt(x) and 1 / x in 64 bits: the hardware's first values and Newton's iteration, whose
 // error squares from 2^-14 or better each time. (Correctly rounded roots and quotients instead:
-// 64 tokens of 32 + 8 heads, normed, 3.85 for 3.77 us, 512 tokens in int8 5.1 for 5.0.) A row
-// with an infinity gets NaN from the first form's 0 * inf; for pages of 8 bits, the one form
-// in 64 bits, such a row is NaN as a whole anyway.
+// 64 tokens of 32 + 8 heads, normed, 3.85 for 3.77 us, 512 tokens in int8 5.1 for 5.0.) The
+// root of an infinity is kept from the iteration's 0 * inf.
 __device__ __forceinline__ float inverse_root(float x) { return rsqrtf(x); }
 __device__ __forceinline__ double inverse_root(double x) {
     double r = __builtin_amdgcn_rsq(x);
 #pragma unroll
     for (int i = 0; i < 3; ++i) r = fma(r * 0.5, fma(-x * r, r, 1.0), r);
-    return r;
+    return x < INFINITY || x != x ? r : 0.0;
 }
 __device__ __forceinline__ double inverse(double x) {
     double r = __builtin_amdgcn_rcp(x);
@@ -274,11 +273,28 @@ __global__ __launch_bounds__(kAppendThreads, PK == 0 ? 7 : 6) void paged_append_
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum += x1[e] * x1[e] + x2[e] * x2[e];
             sum = over_group<LPH>(sum, [](F u, F w) { return u + w; });
-            const F r = inverse_root(sum * (F)a.inv_hd + (F)a.eps);
+            const F ms = sum * (F)a.inv_hd + (F)a.eps;
+            // bf16's squares leave fp32's range from 2^64 on and lose bits from 2^-63 down (the
+            // latter only seen where eps is as small): such a row's norm in 64 bits.  The same
+            // in all lanes of a head.
+            if (sizeof(F) == 4 && !(ms > (F)0x1p-100 && ms < (F)0x1p100)) {
+                double wide = 0.0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x1[e] *= r * (F)to_f32(w1[e]);
-                x2[e] *= r * (F)to_f32(w2[e]);
+                for (int e = 0; e < 8; ++e) wide += (double)x1[e] * (double)x1[e] + (double)x2[e] * (double)x2[e];
+                wide = over_group<LPH>(wide, [](double u, double w) { return u + w; });
+                const double r = inverse_root(wide * a.inv_hd + a.eps);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x1[e] = (F)((double)x1[e] * (r * (double)to_f32(w1[e])));
+                    x2[e] = (F)((double)x2[e] * (r * (double)to_f32(w2[e])));
+                }
+            } else {
+                const F r = inverse_root(ms);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x1[e] *= r * (F)to_f32(w1[e]);
+                    x2[e] *= r * (F)to_f32(w2[e]);
+                }
             }
         }
         if (!mine) return;

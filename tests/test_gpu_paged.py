@@ -522,6 +522,46 @@ def test_append_of_rows_that_are_zero_tiny_or_not_finite(cuda, kind):
     assert torch.isfinite(k[0, 0, [0, 1, 2, 4, 5]]).all() and torch.isfinite(v[0, 0, [0, 1, 2, 3, 5]]).all()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-6, 1e12])
+def test_append_norms_rows_of_any_size(cuda, eps, hd, kind):
+    # squares past fp32's range on both sides, rows of different sizes in one wave
+    c = Cache(cuda, BF, kind, 1, 2, hd, 16, 1, seed=26)
+    sizes = (-75, -70, -64, -40, 0, 50, 62, 64, 70, 115)
+    qkv = gen((1, len(sizes), 7 * hd), BF, 1) * 2.0 ** torch.tensor(sizes, dtype=torch.float32).to(BF)[:, None]
+    qkv[0, :, hd:2 * hd] = gen((len(sizes), hd), BF, 4)          # one head of each as it mostly is
+    w = [(1 + gen((hd,), torch.float32, 2 + i, 0.3)).to(BF) for i in range(2)]
+    appends(c, qkv, 3, 2, hd, frequencies(hd), (3,), None, *w, eps=eps)
+
+
+def test_append_norms_the_smallest_and_largest(cuda, monkeypatch):
+    # bf16's denormals; an eps past fp32's range beside large rows.  Below 2^-126 bf16's step is 2^-126 2^-7
+    # whatever the value, so that half a step, what a rounding is off by, is 2^-134 there, not u |ref|.
+    relative = rotated_tolerance
+    monkeypatch.setitem(globals(), "rotated_tolerance", lambda *a: relative(*a) + 2.0 ** -134)
+    c = Cache(cuda, BF, "same", 1, 1, 64, 16, 1, seed=27)
+    w = torch.ones(64, dtype=BF)
+    for size, eps in ((2.0 ** -128, 0.0), (2.0 ** -128, 1e-6), (2.0 ** 64, 1e40), (2.0 ** 110, 1e60)):
+        appends(c, gen((1, 3, 3 * 64), BF, 1) * size, 1, 1, 64, frequencies(64), (3,), None, w, w, eps=eps)
+
+
+def test_append_norms_of_rows_that_are_not_finite(cuda):
+    # as the formula gives: a number over an infinite root is 0, an infinity over it NaN; with a NaN all are
+    c = Cache(cuda, BF, "same", 1, 1, 64, 16, 1, seed=28)
+    qkv = gen((1, 3, 3 * 64), BF, 1)
+    for at in (0, 64):                      # the query, the key
+        qkv[0, 0, at + 5], qkv[0, 1, at + 40] = math.inf, NAN
+    w = torch.ones(64, dtype=BF, device=cuda)
+    fine = ops.kv_paged_append(qkv[:, 2:].to(cuda), frequencies(64).to(cuda), ints([2], cuda), **c.args(), q_norm=w, k_norm=w)
+    q = ops.kv_paged_append(qkv.to(cuda), frequencies(64).to(cuda), None, **c.args(), q_norm=w, k_norm=w)
+    k = c.pages[0][int(c.table[0, 0]), 0, :3]
+    for x in (q[0, 0], k):
+        assert torch.isnan(x[0, [5, 37]]).all() and x[0].isnan().sum() == 2 and (x[0, [*range(5), *range(6, 37), *range(38, 64)]] == 0).all()
+        assert torch.isnan(x[1]).all() and torch.isfinite(x[2]).all()
+    assert torch.equal(q[:, :, 2:], fine)
+
+
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
 def test_append_ties_go_to_even(cuda, kind):
     # values at every border of the type (x / 2 of its largest and so on): exact in bf16
