@@ -1521,8 +1521,58 @@ def kv_evict(k, v, acc, pos, kv_len, budget, recent=0, acc_out=None, pos_out=Non
 _PAGE_BYTES = {torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.F8E4M3}
 
 
+def _extent(meta):
+    """(shape, stride, bytes of an element, bytes from the first to behind the last element)
+    of a (shape, stride, dtype)."""
+    if meta is None:
+        return None
+    shape, stride, dtype = meta
+    return shape, stride, dtype.itemsize, _span(shape, stride) * dtype.itemsize
+
+
+@functools.lru_cache(maxsize=2048)
+def _meet(a, b, ahead) -> bool:
+    """Whether an element of b, which begins ``ahead`` bytes behind a, lies on one of a (both
+    from _extent, neither empty): whether an offset in a less one in b, a sum of strides
+    times digits of either sign, is ``ahead`` to within an element.  Layouts whose strides
+    do not nest and take too long to decide count as meeting."""
+    digits = {}
+    for (shape, stride, size, _), sign in ((a, 1), (b, -1)):
+        for count, st in zip(shape, stride):
+            if count > 1 and st:
+                d = digits.setdefault(st * size, [0, 0])
+                d[sign > 0] += sign * (count - 1)
+    steps = sorted(((st, *d) for st, d in digits.items()), reverse=True)
+    rest = [(0, 0)]                      # what the smaller strides reach
+    for st, lo, hi in reversed(steps):
+        rest.append((rest[-1][0] + st * lo, rest[-1][1] + st * hi))
+    rest.reverse()
+    todo, looked = [(0, ahead - a[2] + 1, ahead + b[2] - 1)], 0
+    while todo:
+        i, least, most = todo.pop()
+        if i == len(steps):
+            if least <= 0 <= most:
+                return True
+            continue
+        looked += 1
+        if looked > 4096:
+            return True
+        st, lo, hi = steps[i]
+        low, high = rest[i + 1]
+        for d in range(max(lo, -((high - least) // st)), min(hi, (most - low) // st) + 1):
+            todo.append((i + 1, least - d * st, most - d * st))
+            if len(todo) > 4096:
+                return True
+    return False
+
+
+def _apart(a_at, a, b_at, b) -> bool:
+    """Whether tensors of these addresses and extents share no memory (a or b None: no tensor)."""
+    return a is None or b is None or a_at + a[3] <= b_at or b_at + b[3] <= a_at or not a[3] or not b[3] or not _meet(a, b, b_at - a_at)
+
+
 class _PagedPlan:
-    __slots__ = ("layout", "n", "hkv", "hd", "bytes", "slots", "holds")
+    __slots__ = ("layout", "n", "hkv", "hd", "bytes", "slots", "k", "v", "k_scale", "v_scale")
 
 
 @functools.lru_cache(maxsize=2048)
@@ -1533,7 +1583,8 @@ def _paged_plan(name, k, v, k_scale, v_scale, table) -> _PagedPlan:
             or len(table[0]) != 2 or table[2] != torch.int32:
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     p = _PagedPlan()
-    p.bytes, p.holds = kd in _PAGE_BYTES, math.prod(ks) > 0
+    p.bytes = kd in _PAGE_BYTES
+    p.k, p.v, p.k_scale, p.v_scale = _extent(k), _extent(v), _extent(k_scale), _extent(v_scale)
     if p.bytes != (k_scale is not None) or p.bytes != (v_scale is not None):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     if not p.bytes and kd not in HALF:
@@ -1564,6 +1615,12 @@ def _paged_cache(name, k, v, k_scale, v_scale, table):
     return _paged_plan(name, _meta(k), _meta(v), _meta(k_scale), _meta(v_scale), _meta(table))
 
 
+def _off_cache(c, at, t, k_at, v_at, k_scale, v_scale) -> bool:
+    """Whether an output of extent t at this address shares no memory with the cache c."""
+    return _apart(at, t, k_at, c.k) and _apart(at, t, v_at, c.v) \
+        and (not c.bytes or (_apart(at, t, k_scale.data_ptr(), c.k_scale) and _apart(at, t, v_scale.data_ptr(), c.v_scale)))
+
+
 def _in_pieces(shape, stride) -> bool:
     """Whether the kernels can read rows of these strides in place, in 16-byte pieces
     (from an address that is a multiple of 16)."""
@@ -1575,7 +1632,7 @@ def _copied(t):
 
 
 class _AppendPlan:
-    __slots__ = ("dims", "dtype", "ld", "ld_copy", "in_place", "weights_in_place", "sq", "q_layout")
+    __slots__ = ("dims", "dtype", "ld", "ld_copy", "in_place", "weights_in_place", "sq", "q_layout", "x", "out")
 
 
 @functools.lru_cache(maxsize=2048)
@@ -1594,6 +1651,7 @@ def _append_plan(qkv, n, hkv, hd, pages, inv_freq, q_norm, k_norm, q_out) -> _Ap
     t, w = shape[1], shape[2]
     hq = w // hd - 2 * hkv
     p.dims, p.dtype = (n, t, hq), _dt(dtype)
+    p.x, p.out = _extent(qkv), _extent(q_out)
     p.in_place = _in_pieces(shape, stride)
     p.ld, p.ld_copy = (stride[1] if t > 1 else 0, stride[0] if n > 1 else 0), (w, t * w)
     p.weights_in_place = all(x is None or x[1] == (1,) for x in (q_norm, k_norm))
@@ -1624,7 +1682,8 @@ def kv_paged_append(qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale=None, 
     or 448 (float8_e4m3fn); a row that is not finite reads back as NaN.  A page that
     receives tokens must be named once in the table.  bf16 / f16; hd a multiple of 16 up to
     128, pages of multiples of 16 rows.  ``q_out`` receives q in place; it must
-    not overlap qkv or the cache."""
+    not overlap qkv or the cache, nor k_pages v_pages, nor k_scale v_scale (other parts of
+    one buffer are taken)."""
     name = "kv_paged_append"
     c = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
     p = _append_plan(_meta(qkv), c.n, c.hkv, c.hd, None if c.bytes else k_pages.dtype, _meta(inv_freq), _meta(q_norm), _meta(k_norm),
@@ -1633,7 +1692,9 @@ def kv_paged_append(qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale=None, 
         if x is not None and not _flat_ints(x, c.n):
             raise _lib.KuiopsError(name, _lib.E_INVALID)
     k_at, v_at = k_pages.data_ptr(), v_pages.data_ptr()
-    if c.holds and (k_at == v_at or (q_out is not None and q_out.data_ptr() in (qkv.data_ptr(), k_at, v_at))):
+    if not _apart(k_at, c.k, v_at, c.v) or (c.bytes and not _apart(k_scale.data_ptr(), c.k_scale, v_scale.data_ptr(), c.v_scale)) \
+            or (q_out is not None and not (_apart(q_out.data_ptr(), p.out, qkv.data_ptr(), p.x)
+                                           and _off_cache(c, q_out.data_ptr(), p.out, k_at, v_at, k_scale, v_scale))):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     device = _gpu_of(name, qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale, v_scale, q_norm, k_norm, lens, q_out)
     ld = p.ld
@@ -1666,9 +1727,10 @@ def _read_plan(n, hkv, length, hd, dtype, pages):
 
 @functools.lru_cache(maxsize=2048)
 def _read_strides(shape, out, dtype):
+    """(C strides, extent) of an output of kv_paged_read that the caller gives."""
     if out[0] != shape or out[2] != dtype or not _own_rows(*out[:2]):
         raise _lib.KuiopsError("kv_paged_read", _lib.E_INVALID)
-    return _c_strides(*out[:2], 3)
+    return _c_strides(*out[:2], 3), _extent(out)
 
 
 def kv_paged_read(k_pages, v_pages, table, kv_len, length=None, k_scale=None, v_scale=None, dtype=None, k_out=None, v_out=None):
@@ -1679,7 +1741,8 @@ def kv_paged_read(k_pages, v_pages, table, kv_len, length=None, k_scale=None, v_
 
     ``dtype``: 16-bit pages come as they are, 8-bit ones as stored * scale in bf16
     (default), f16 or fp32.  Rows behind a sequence are 0, or left as they are in
-    ``k_out`` / ``v_out`` (given together; (n, hkv, length, hd), unit last stride)."""
+    ``k_out`` / ``v_out`` (given together; (n, hkv, length, hd), unit last stride, not
+    overlapping each other or the cache)."""
     name = "kv_paged_read"
     c = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
     if (k_out is None) != (v_out is None) or not _flat_ints(kv_len, c.n):
@@ -1693,9 +1756,10 @@ def kv_paged_read(k_pages, v_pages, table, kv_len, length=None, k_scale=None, v_
     if fill:
         sk = sv = flat
     else:
-        sk, sv = _read_strides(shape, _meta(k_out), dtype), _read_strides(shape, _meta(v_out), dtype)
+        (sk, kx), (sv, vx) = _read_strides(shape, _meta(k_out), dtype), _read_strides(shape, _meta(v_out), dtype)
         ko, vo = k_out.data_ptr(), v_out.data_ptr()
-        if k_out.numel() and (ko == vo or ko in (k_at, v_at) or vo in (k_at, v_at)):
+        if not _apart(ko, kx, vo, vx) or not _off_cache(c, ko, kx, k_at, v_at, k_scale, v_scale) \
+                or not _off_cache(c, vo, vx, k_at, v_at, k_scale, v_scale):
             raise _lib.KuiopsError(name, _lib.E_INVALID)
     device = _gpu_of(name, k_pages, v_pages, table, kv_len, k_scale, v_scale, k_out, v_out)
     if fill:
@@ -1708,7 +1772,7 @@ def kv_paged_read(k_pages, v_pages, table, kv_len, length=None, k_scale=None, v_
 
 
 class _PagedAttnPlan:
-    __slots__ = ("dims", "dtype", "sq", "sq_copy", "in_place", "so", "ws", "scale")
+    __slots__ = ("dims", "dtype", "sq", "sq_copy", "in_place", "so", "ws", "scale", "q", "out")
 
 
 @functools.lru_cache(maxsize=2048)
@@ -1725,6 +1789,7 @@ def _paged_attn_plan(q, n, hkv, hd, pages, slots, out) -> _PagedAttnPlan:
     _, hq, l, _ = shape
     flat = (hq * l * hd, l * hd, hd, 1)
     p.dims, p.dtype = (n, hq, l), _dt(dtype)
+    p.q, p.out = _extent(q), _extent(out)
     p.sq, p.sq_copy, p.in_place = _c_strides(shape, stride, 3), _c_strides(shape, flat, 3), _in_pieces(shape, stride)
     p.so = _c_strides(shape, flat if out is None else out[1], 3)
     p.ws = _lib_handle().kuiops_sdpa_paged_workspace(n, hq, hkv, l, slots, hd)
@@ -1763,7 +1828,8 @@ def sdpa_paged(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=None, s
     if not _flat_ints(kv_len, c.n):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     k_at, v_at = k_pages.data_ptr(), v_pages.data_ptr()
-    if out is not None and out.numel() and out.data_ptr() in (q.data_ptr(), k_at, v_at):
+    if out is not None and not (_apart(out.data_ptr(), p.out, q.data_ptr(), p.q)
+                                and _off_cache(c, out.data_ptr(), p.out, k_at, v_at, k_scale, v_scale)):
         raise _lib.KuiopsError(name, _lib.E_INVALID)
     device = _gpu_of(name, q, k_pages, v_pages, table, kv_len, k_scale, v_scale, out)
     if out is None:

@@ -266,6 +266,110 @@ def test_sdpa_paged_refuses_its_query_as_output():
     refuses(INVALID, ops.sdpa_paged, **a, out=a["q"])
 
 
+def test_what_shares_memory():
+    # against the sets of bytes, over small layouts of any strides
+    g = np.random.default_rng(5)
+
+    def some():
+        size = int(g.choice([1, 2, 4]))
+        shape = tuple(int(x) for x in g.integers(1, 4, g.integers(1, 4)))
+        return shape, tuple(int(x) for x in g.integers(0, 9, len(shape))), {1: torch.int8, 2: BF, 4: torch.float32}[size]
+
+    def places(x, at):
+        own = {0}
+        for count, st in zip(*x[:2]):
+            own = {o + i * st for o in own for i in range(count)}
+        return {at + o * x[2].itemsize + i for o in own for i in range(x[2].itemsize)}
+    seen = [0, 0]
+    for _ in range(4000):
+        a, b, to = some(), some(), int(g.integers(-30, 40))
+        shared = bool(places(a, 0) & places(b, to))
+        assert ops._apart(100, ops._extent(a), 100 + to, ops._extent(b)) != shared, (a, b, to)
+        seen[shared] += 1
+    assert min(seen) > 500
+    empty = ops._extent(((3, 0), (4, 1), BF))
+    assert ops._apart(0, empty, 0, ops._extent(((4,), (1,), BF))) and ops._apart(0, None, 0, empty)
+    # strides that do not nest, as large as tensors are: an answer, and soon
+    x = ops._extent(((1 << 20, 1 << 20), (7, 3), BF))
+    assert not ops._apart(0, x, 1, x)
+
+
+def takes(fn, **a):
+    refuses(UNSUPPORTED, fn, **a)              # all that is left to refuse: it is not on a GPU
+
+
+def test_kv_paged_append_refuses_shared_scales_and_pools_that_overlap():
+    for dtype in (torch.int8, F8):
+        a = append_args(dtype)
+        refuses(INVALID, ops.kv_paged_append, **{**a, "v_scale": a["k_scale"]})
+        scales = torch.zeros(7, 2, 16)
+        refuses(INVALID, ops.kv_paged_append, **{**a, "k_scale": scales[:6], "v_scale": scales[1:]})
+        both = torch.zeros(6, 2, 2, 16)
+        takes(ops.kv_paged_append, **{**a, "k_scale": both[:, 0], "v_scale": both[:, 1]})
+    a = append_args()
+    pool = torch.zeros(12, 2, 16, 64, dtype=BF)
+    refuses(INVALID, ops.kv_paged_append, **{**a, "k_pages": pool[:6], "v_pages": pool[1:7]})
+    refuses(INVALID, ops.kv_paged_append, **{**a, "k_pages": pool[5:11], "v_pages": pool[:6]})
+    takes(ops.kv_paged_append, **{**a, "k_pages": pool[:6], "v_pages": pool[6:]})
+    takes(ops.kv_paged_append, **{**a, "k_pages": pool[::2], "v_pages": pool[1::2]})
+    heads = torch.zeros(6, 4, 16, 64, dtype=BF)
+    takes(ops.kv_paged_append, **{**a, "k_pages": heads[:, :2], "v_pages": heads[:, 2:]})
+    refuses(INVALID, ops.kv_paged_append, **{**a, "k_pages": heads[:, :2], "v_pages": heads[:, 1:3]})
+    rows = torch.zeros(6, 2, 16, 128, dtype=BF)
+    takes(ops.kv_paged_append, **{**a, "k_pages": rows[..., 64:], "v_pages": rows[..., :64]})
+    # one pool to read keys and values from is no mistake
+    for fn, args in ENTRIES[1:]:
+        b = args()
+        takes(fn, **{**b, "v_pages": b["k_pages"]})
+
+
+def test_kv_paged_append_refuses_a_query_output_on_its_inputs():
+    a = append_args()
+    wide = torch.zeros(2, 3, 800, dtype=BF)
+    a["qkv"] = wide[..., :512]
+    for first, fn in ((0, refuses), (256, refuses), (511, refuses), (512, None), (544, None)):
+        view = wide[..., first:first + 256].view(2, 3, 4, 64).transpose(1, 2)
+        takes(ops.kv_paged_append, **a, q_out=view) if fn is None else fn(INVALID, ops.kv_paged_append, **a, q_out=view)
+    for pool in (a["k_pages"], a["v_pages"]):
+        refuses(INVALID, ops.kv_paged_append, **a, q_out=pool.view(-1)[-2 * 4 * 3 * 64:].view(2, 4, 3, 64))
+    a = append_args(torch.int8)
+    scales = torch.zeros(1000)
+    refuses(INVALID, ops.kv_paged_append, **{**a, "v_scale": scales[:192].view(6, 2, 16)},
+            q_out=scales.view(BF)[380:380 + 1536].view(2, 4, 3, 64))
+
+
+def test_kv_paged_read_refuses_outputs_that_overlap():
+    a = read_args()
+    out = torch.zeros(2, 2, 97, 64, dtype=BF)
+    refuses(INVALID, ops.kv_paged_read, **a, k_out=out[:, :, :48], v_out=out[:, :, 47:95])
+    takes(ops.kv_paged_read, **a, k_out=out[:, :, :48], v_out=out[:, :, 48:96])
+    for dtype in (BF, torch.int8):
+        a = read_args(dtype)
+        far = torch.zeros(2, 2, 8, 64, dtype=BF)
+        for name in ("k_pages", "v_pages") + (("k_scale", "v_scale") if dtype != BF else ()):
+            base = torch.zeros(64 << 10, dtype=torch.uint8)
+            x = a[name]
+            b = {**a, name: base[:x.numel() * x.element_size()].view(x.dtype).view(x.shape)}
+            at = x.numel() * x.element_size() - 16
+            on, off = (base[i:i + 4096].view(BF).view(2, 2, 8, 64) for i in (at, at + 16))
+            for outs in ((on, far), (far, on)):
+                refuses(INVALID, ops.kv_paged_read, **b, k_out=outs[0], v_out=outs[1])
+            takes(ops.kv_paged_read, **b, k_out=off, v_out=far)
+
+
+def test_sdpa_paged_refuses_an_output_on_its_inputs():
+    a = attn_args()
+    buf = torch.zeros(2, 8, 1, 64, dtype=BF)
+    refuses(INVALID, ops.sdpa_paged, **{**a, "q": buf[:, :4]}, out=buf[:, 1:5])
+    takes(ops.sdpa_paged, **{**a, "q": buf[:, :4]}, out=buf[:, 4:])
+    for name in ("k_pages", "v_pages"):
+        refuses(INVALID, ops.sdpa_paged, **a, out=a[name].view(-1)[-512:].view(2, 4, 1, 64))
+    b = attn_args(F8)
+    scales = torch.zeros(512)
+    refuses(INVALID, ops.sdpa_paged, **{**b, "k_scale": scales[:192].view(6, 2, 16)}, out=scales.view(BF)[382:894].view(2, 4, 1, 64))
+    takes(ops.sdpa_paged, **{**b, "k_scale": scales[:192].view(6, 2, 16)}, out=scales.view(BF)[384:896].view(2, 4, 1, 64))
+
+
 def layout(pages=6, page=16, hkv=2, hd=64, width=3, dtype=_lib.BF16, row=64, scale=16):
     at = _lib.PagedLayout(pages=pages, page=page, hkv=hkv, hd=hd, width=width, ld_table=width, dtype=dtype)
     at.sk[:] = at.sv[:] = (hkv * page * row, page * row, row)
