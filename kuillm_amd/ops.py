@@ -1737,7 +1737,11 @@ def kv_paged_read(k_pages, v_pages, table, kv_len, length=None, k_scale=None, v_
     """The cached rows of the sequences, gathered out of their pages -> (k, v)
     (n, hkv, length, hd): slots 0 .. ``kv_len[b]`` - 1 (int32 [n] on the device), as far as
     ``length`` (default: all that the table reaches) goes.  For prompt attention over
-    what the cache holds (:func:`sdpa_decode_accum`, :func:`sdpa`).
+    what the cache holds: after :func:`kv_paged_append` of t tokens read with kv_len =
+    pos0 + t, or pos0 + lens where a batch is padded, and a ``length`` that no pos0 + t
+    passes.  Then :func:`sdpa` with an additive mask that shows query i the slots up to
+    pos0 + i, or for short pieces (head dims 64 and 128) :func:`sdpa_decode` with kv_len =
+    pos0 + t for all sequences.  The rows from lens[b] on are of no use.
 
     ``dtype``: 16-bit pages come as they are, 8-bit ones as stored * scale in bf16
     (default), f16 or fp32.  Rows behind a sequence are 0, or left as they are in
@@ -1816,8 +1820,7 @@ def sdpa_paged(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=None, s
     device, read when the kernel runs; its own key among the slots, so appended before)
     and sees the slots up to its own that have a page (a length may pass the table's
     end); one that sees none gives 0 and lse -inf.  For decoding (l = 1) and a few drafted tokens: up to 16 rows of l * hq /
-    hkv share a pass over the cache (longer pieces of a prompt: :func:`kv_paged_read` and
-    :func:`sdpa_decode_accum`).  After :func:`kv_paged_append` of t tokens with ``lens``
+    hkv share a pass over the cache (longer pieces of a prompt: see :func:`kv_paged_read`).  After :func:`kv_paged_append` of t tokens with ``lens``
     pass pos0 + t for all: the tokens that are there see what they should, the rows of
     padding are of no use.  bf16 / f16; hd a multiple of 16 up to 128; scale > 0.
     ``out`` ((n, hq, l, hd), unit last stride) receives the result in place; it must not

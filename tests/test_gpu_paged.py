@@ -734,6 +734,40 @@ def test_drafted_tokens_of_a_padded_batch(cuda, kind):
             close_lse(lse[b:b + 1, :, :m], lref, terms, hd)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("t,hd", [(24, 64), (130, 128)])
+def test_prompt_pieces_of_a_padded_batch(cuda, t, hd, dtype, kind):
+    """Append, read back with kv_len = pos0 + lens and attend to the slots up to each token's, all
+    sequences in one call: each token sees what it sees alone, whatever the pages hold behind it."""
+    n, hq, hkv, page, width = 4, 8, 2, 16, 8 if t < 100 else 16
+    pos0, lens = (0, 40, 7, 16 * width - 25), (t, 5, 0, min(t, 25))        # the last one's padding passes the table
+    c = Cache(cuda, dtype, kind, n, hkv, hd, page, width, seed=45)
+    for b, (p, m) in enumerate(zip(pos0, lens)):
+        for s in range(p + m, min(p + t, page * width)):
+            at = c.table[b, s // page], slice(None), s % page
+            for x in (c.pages if kind == "same" else c.scales):
+                x[at] = NAN
+    a, freq = c.args(), frequencies(hd).to(cuda)
+    qkv, w = gen((n, t, (hq + 2 * hkv) * hd), dtype, 1).to(cuda), (1 + gen((hd,), torch.float32, 2, 0.3)).to(dtype).to(cuda)
+    start, there = ints(pos0, cuda), ints(lens, cuda)
+    longest = max(pos0) + t
+    q = ops.kv_paged_append(qkv, freq, start, **a, q_norm=w, k_norm=w, lens=there)
+    k, v = ops.kv_paged_read(**a, kv_len=start + there, length=longest, dtype=dtype)
+    acc = torch.zeros(n, hkv, longest, device=cuda)
+    seen = torch.arange(longest, device=cuda) <= (start[:, None] + torch.arange(t, device=cuda))[:, :, None]
+    mask = torch.where(seen, 0.0, -math.inf).to(dtype)[:, None]
+    calls = [(True, ops.sdpa(q, k, v, bias=mask)), (False, ops.sdpa_decode(q, k, v, kv_len=start + t, return_lse=True)),
+             (False, ops.sdpa_decode_accum(q, k, v, acc, start + t, return_lse=True))]
+    for b, (p, m) in enumerate(zip(pos0, lens)):
+        if m:
+            kk, vv = npy(k[b:b + 1, :, :p + m]), npy(v[b:b + 1, :, :p + m])
+            ref, lref, _, size, terms = O.sdpa_decode_accum(npy(q[b:b + 1, :, :m]), kk, vv, np.zeros((1, hkv, p + m)))
+            for one_part, (out, lse) in calls:
+                close_out(out[b:b + 1, :, :m], ref, size, terms, hd, one_part)
+                close_lse(lse[b:b + 1, :, :m], lref, terms, hd)
+
+
 def test_custom_ops_on_the_gpu(cuda):
     from kuillm_amd import library  # noqa: F401
     op = torch.ops.kuiops
