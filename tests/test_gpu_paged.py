@@ -142,6 +142,71 @@ def test_sdpa_paged_even_pieces(cuda, n, hq, hkv, l, hd, page, lens, checked, ki
     some_of(c, gen((n, hq, l, hd), BF, 1), lens, checked)
 
 
+def longest_piece(lens, hkv, row_groups):
+    """Tiles of 32 slots of the longest piece that a work-group has, for lengths that make one list
+    of all tiles (a unit, a sequence's KV head, begins with 12 places that no tile has)."""
+    groups, switch = max(1, 256 // row_groups), 12
+    tiles = [max(1, -(-x // 32)) for x in lens for _ in range(hkv)]
+    assert sum(tiles) >= (16 if len(tiles) < 2 * groups else 64) * groups
+    per = max(switch + 16, int((sum(tiles) + len(tiles) * switch) / groups) + 1)
+    best, at = 0, 0
+    for t in tiles:
+        first, end = at + switch, at + switch + t
+        best = max([best] + [min(end, (w + 1) * per) - max(first, w * per) for w in range(first // per, (end - 1) // per + 1)])
+        at = end
+    return best
+
+
+# A wave takes every fourth tile of a piece; where its tiles lie is fetched for 32 of them at a time,
+# so a piece of 128 tiles and more goes on to the next 32 (many rows a KV head leave few work-groups
+# for the tiles, so long pieces need no large cache)
+TURNS = [  # n, hq, hkv, l, hd, page, lens
+    (1, 16, 1, 129, 64, 16, (9000,)),                       # one work-group a row group: 282 tiles
+    (3, 16, 1, 64, 64, 48, (9000, 3, 9001)),                # four: pieces that end anywhere, and another behind them
+    (2, 16, 2, 129, 128, 32, (4097, 4480)),                 # three: two units of 129 tiles and two of 140
+]
+
+
+def rows_of(q, lens, first, count):
+    """(the queries first .. first + count - 1, the lengths with which they are the last ones)"""
+    return q[:, :, first:first + count], [L - q.shape[2] + first + count for L in lens]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,hq,hkv,l,hd,page,lens", TURNS)
+def test_sdpa_paged_goes_on_to_more_page_numbers(cuda, n, hq, hkv, l, hd, page, lens, kind):
+    assert longest_piece(lens, hkv, -(-(hq // hkv * l) // 16)) > 128
+    c = Cache(cuda, BF, kind, n, hkv, hd, page, -(-max(lens) // page), seed=46)
+    q = gen((n, hq, l, hd), BF, 1)
+    out, lse = ops.sdpa_paged(q.to(cuda), **c.args(), kv_len=ints(lens, cuda), return_lse=True)
+    for first in (0, l - 2):
+        some, ends = rows_of(q, lens, first, 2)
+        ref, lref, size, terms = c.attention(some, ends)
+        close_out(out[:, :, first:first + 2], ref, size, terms, hd, False)
+        close_lse(lse[:, :, first:first + 2], lref, terms, hd)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,hq,hkv,l,hd,page,lens", TURNS)
+def test_masked_nan_behind_more_page_numbers(cuda, n, hq, hkv, l, hd, page, lens, kind):
+    # the newest slot of each sequence holds a NaN: the wave that has it goes over all its tiles again
+    # for the queries that do not see it
+    c = Cache(cuda, BF, kind, n, hkv, hd, page, -(-max(lens) // page), seed=47)
+    q = gen((n, hq, l, hd), BF, 1)
+    some, ends = rows_of(q, lens, l - 3, 2)
+    ref, lref, size, terms = c.attention(some, ends)
+    for b, L in enumerate(lens):
+        p, r = O.paged_slot(c.table[b], page, c.pages[1].shape[0], L - 1)
+        if kind == "same":
+            c.pages[1][p, :, r] = NAN
+        else:
+            c.scales[1][p, :, r] = NAN
+    out, lse = ops.sdpa_paged(q.to(cuda), **c.args(), kv_len=ints(lens, cuda), return_lse=True)
+    close_out(out[:, :, l - 3:l - 1], ref, size, terms, hd, False)
+    close_lse(lse[:, :, l - 3:l - 1], lref, terms, hd)
+    assert torch.isnan(out[:, :, l - 1]).all() and torch.isfinite(out[:, :, :l - 1]).all()
+
+
 def test_large_pools_pass_by_the_caches(cuda):
     # (pools of 120 MB and more are read with other loads)
     for kind, dtype, hd, n in (("same", BF, 128, 8), ("int8", HF, 64, 32), ("e4m3", BF, 128, 16), ("same", HF, 64, 16)):
