@@ -759,7 +759,8 @@ PagedPlan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t slots, 
     p.groups = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxGroups / p.row_groups, tiles));
     p.may_part = n * hkv * p.row_groups <= kApart;
     p.launched = p.groups + (p.may_part ? (int)(n * hkv) : 0);
-    if (tiles > n * hkv) {
+    // (a single work-group for the keys has every unit whole, as has one tile a unit)
+    if (tiles > n * hkv && p.groups > 1) {
         const size_t states = (size_t)p.launched * p.row_groups * 2 * 16;
         p.counter_bytes = kCounterBytes;
         p.ml_bytes = states * 8;

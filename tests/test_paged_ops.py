@@ -428,6 +428,17 @@ def test_workspace_sizes(lib):
     assert f(1, 32, 8, 1, 1 << 20, 128) <= 10 << 20
 
 
+def test_many_query_rows_need_no_workspace(lib):
+    # a piece of a work-group for each 16 rows of a KV head: from 129 groups of rows on a work-group has all
+    # keys, nothing is split, and the states' space does not grow with the rows
+    f = lib.kuiops_sdpa_paged_workspace
+    assert f(1, 16, 1, 128, 8000, 128) > 0
+    for l in (129, 300, 8192, 1 << 20):
+        assert f(1, 16, 1, l, 8000, 128) == f(2, 128, 8, l, 1 << 20, 128) == 0
+    most = max(f(n, 16 * g, g, l, 1 << 16, 128) for n in (1, 2, 16, 64, 300) for g in (1, 8) for l in (1, 2, 5, 16, 100, 128, 129, 1000))
+    assert most <= 40 << 20
+
+
 # ------------------------------------------------------------- custom ops
 
 def test_custom_ops_trace_without_a_device():
