@@ -1600,8 +1600,6 @@ def _paged_plan(name, k, v, k_scale, v_scale, table) -> _PagedPlan:
                                      ld_table=table[1][0] if p.n > 1 else 0,
                                      dtype=_PAGE_BYTES[kd] if p.bytes else _dt(kd))
     at.sk, at.sv = _c_strides(ks, kst, 3), _c_strides(vs, vst, 3)
-    if page == 1:
-        at.sk[2] = at.sv[2] = hd
     for scale, st in ((k_scale, at.sks), (v_scale, at.svs)):
         if scale is not None:
             if scale[0] != ks[:3] or scale[2] != torch.float32 or not _own_rows(*scale[:2]):

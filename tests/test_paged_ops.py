@@ -420,6 +420,16 @@ def test_c_entries_refuse_on_the_host(lib):
     assert attn(width=300, ws=null, nb=0) == attn(width=300, nb=need - 1) == attn(width=300, ws=off) == _lib.E_WORKSPACE
 
 
+def test_pages_of_one_row_are_refused_whatever_their_strides(lib):
+    # (torch lets the stride of an axis of one entry be anything; the layout has 0 for it)
+    p, null, s3 = ctypes.c_void_p(1 << 20), None, _lib.strides3(0, 0, 64)
+    for row in (0, 64, 128):
+        at = layout(page=1)
+        at.sk[2] = at.sv[2] = row
+        assert lib.kuiops_kv_paged_read(2, 40, _lib.BF16, at, p, p, null, null, p, p, p, s3, p, s3, 0, null) == UNSUPPORTED
+        assert lib.kuiops_sdpa_paged(2, 4, 1, _lib.BF16, p, s3, at, p, p, null, null, p, p, p, s3, null, 0.1, p, 1 << 30, null) == UNSUPPORTED
+
+
 def test_workspace_sizes(lib):
     assert f"#define KUIOPS_SDPA_PAGED_ZEROED {_lib.SDPA_PAGED_ZEROED}\n" in (C.INCLUDE / "kuiops.h").read_text()
     f = lib.kuiops_sdpa_paged_workspace
