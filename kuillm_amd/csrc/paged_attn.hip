@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "paged.hpp"
+#include "prob_parts.hpp"
 
 namespace kuiops {
 
@@ -27,7 +28,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void *base, ui
 
 constexpr float kLn2 = 0.69314718055994530942f, kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kOut = 0x80000000u;        // an offset past every descriptor
-constexpr float kSlack = 8.f;                 // a row's maximum may grow by 2^8 before its sums are rescaled
 constexpr int kCounterStride = 16;            // words: a cache line's atomics serialise
 constexpr int kTile = 32;                     // slots that a wave takes at once
 constexpr int kSwitch = 12, kLeast = 16;      // tiles that going on to another unit takes the time of; of a work-group, at least
@@ -55,33 +55,8 @@ struct PagedArgs {
 
 enum PageKind { kSame = 0, kInt8 = 1, kE4M3 = 2 };
 
-// A probability as a sum of 16-bit parts, one MFMA each, which keeps fp32's bits: bf16
-// three parts, each the leading 8 bits of what is left, cut off; f16 two, rounded, 2^-23
-// of it lost and no more than half of f16's smallest step (see Shift).  With the few rows
-// of this kernel the K / V stream takes the time, not the MFMAs.
-template <typename T> struct Parts;
-template <> struct Parts<bf16_t> {
-    static constexpr int N = 3;
-    static __device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-    static __device__ __forceinline__ void split(float p, bf16_t (&x)[N]) {
-        const float h = cut(p), r = p - h, m = cut(r);
-        x[0] = (bf16_t)h;
-        x[1] = (bf16_t)m;
-        x[2] = (bf16_t)(r - m);
-    }
-};
-template <> struct Parts<f16_t> {
-    static constexpr int N = 2;
-    static __device__ __forceinline__ void split(float p, f16_t (&x)[N]) {
-        x[0] = from_f32<f16_t>(p);
-        x[1] = from_f32<f16_t>(p - to_f32(x[0]));
-    }
-};
-// probabilities are relative to 2^(maximum + value): f16's smallest step is then 2^-39 to
-// 2^-31 of the row's largest
-template <typename T> struct Shift;
-template <> struct Shift<bf16_t> { static constexpr float value = 0.f; };
-template <> struct Shift<f16_t> { static constexpr float value = -7.f; };
+// Probabilities as sums of 16-bit parts (Parts): with the few rows of this kernel the K / V
+// stream takes the time, not the MFMAs.
 
 // Two bf16 (the upper halves of lo and hi) in a dword.
 __device__ __forceinline__ uint32_t upper_halves(float lo, float hi) {
