@@ -106,10 +106,10 @@ template <typename V> __device__ __forceinline__ uint32_t word(const V &v, int i
 // by the last of its work-groups to arrive.
 // Where they cross: a piece that follows another in its work-group costs 5 us (drained loads,
 // the waves' merge, the unit's), uneven pieces up to their difference.  Pieces apart / even
-// list, us, 8 KV heads of 128, with tiles a work-group if even: 8 sequences of 500 (3) 11.8 / 17.4,
-// 5 of 3000 (11) 15.4 / 18.4, 8 of 2000 (12) 18.9 / 18.3, 64 of 600 (28) 26.6 / 31.5, 16 of 2000
-// (23) 25.6 / 22.9, 8 of 6000 (35) 43.7 / 34.9, 16 of 4000 (47) 50.7 / 42.9, 64 of 2000 (94) 76.1 / 76.2,
-// 32 of 8000 in e4m3 (141) 102 / 80.5.
+// list, us, 8 KV heads of 128, with tiles a work-group if even: 8 sequences of 500 (3) 11.3 / 17.3,
+// 5 of 3000 (11) 15.3 / 18.5, 8 of 2000 (12) 18.6 / 17.6, 64 of 600 (28) 25.4 / 31.8, 16 of 2000
+// (23) 30.9 / 25.7, 8 of 6000 (35) 43.7 / 32.8, 16 of 4000 (47) 52.0 / 40.0, 64 of 2000 (94) 70.0 / 70.7,
+// 32 of 8000 in int8 (141) 100 / 75.8.
 struct Piece {
     int b, hk, L;              // the unit, and its sequence's length
     int t0, t1;                // its tiles
@@ -160,10 +160,11 @@ template <typename A> __device__ __forceinline__ const A &late_args() {
 // What bounds it: the K / V stream (a plain read of as much reaches 5.4 to 6.1 TB/s with the
 // launch) and what lies around it: arguments, lengths, page numbers and first keys one after
 // another 3 us, the waves' merge 0.9, pieces stored, counted and merged 2.  Kernel alone: 16
-// sequences of 2111 to 4000 keys, 32 / 8 heads of 128, bf16 39.7 us, 5.1 TB/s; 32 of 4085 to
+// sequences of 2111 to 4000 keys, 32 / 8 heads of 128, bf16 40 us, 5.1 TB/s; 32 of 4085 to
 // 8000 in e4m3 75 us, 5.5 TB/s; 60001 keys of one sequence in int8 31 us, 4.1 TB/s; 600 keys of
-// one sequence, heads of 64: 8.7 us.  Two tiles in flight a wave took longer (16 sequences 45.8
-// against 44.2), with 214 instead of 256 registers; so did 8 waves.
+// one sequence, heads of 64: 8.7 us.  Two tiles in flight a wave took longer, with 214 instead of
+// 256 registers, in an earlier form of the loop and in bf16 (16 sequences 45.8 against 44.2 then;
+// not tried in 8 bits); so did 8 waves.
 template <typename T, int PK, int HD, int NWV, int AUX>
 __global__ __launch_bounds__(64 * NWV, 2) void paged_attn_kernel(PagedArgs a) {
     typedef typename std::conditional<PK == kSame, T, bf16_t>::type C;       // the products' type
@@ -718,8 +719,9 @@ struct PagedPlan {
 };
 
 constexpr int kWaves = 4;
-// work-groups that share the keys evenly (512, two a CU: 16 sequences of 4000 44.2 -> 46.4 us), and
-// units that have work-groups of their own
+// work-groups that share the keys evenly (512, two a CU: 16 sequences of 4000 39.8 -> 42.7 us, 60001
+// keys of one in int8 31.4 -> 34.4, 32 of 8000 in e4m3 75.1 -> 77.0), and units that have work-groups
+// of their own
 constexpr int kMaxGroups = 256;
 // The counters' part of a workspace, the same for calls of all sizes
 constexpr int kApart = 2048;
@@ -746,8 +748,10 @@ PagedPlan plan_of(int64_t n, int64_t hq, int64_t hkv, int64_t l, int64_t slots, 
 
 // Keys and values of pools (or full tables) of this many bytes pass by the caches
 // (non-temporal loads); those of smaller ones may be found in the 256 MB of memory-side cache the
-// next time: us without / with, 52 MB read 18.1 / 22.2, 119 MB 31.4 / 31.7, 145 MB 34.4 / 32.4, 204
-// MB 42.4 / 39.8, 394 MB 75.5 / 71.0.
+// next time: us without / with, 52 MB read 17.7 / 19.5, 119 MB 28.4 / 27.8, 145 MB 33.1 / 31.5, 204
+// MB 43.2 / 39.9, 394 MB 74.6 / 66.9.  The lengths are not known here: short contexts whose tables
+// could hold more (16 sequences, tables of 32768 slots over a pool of 2 GB) take 15.6 us instead of
+// 14.6 for up to 600 slots, 21.6 instead of 19.5 for 1200, 25.8 instead of 25.7 for 2000.
 constexpr int64_t kStreamBytes = 120 << 20;
 
 template <typename T, int PK, int AUX>

@@ -1675,7 +1675,8 @@ def kv_paged_append(qkv, inv_freq, pos0, k_pages, v_pages, table, k_scale=None, 
     on (int32 [n]; None: t) are padding: nothing of them is used or stored, their q is 0.
     With ``q_norm`` / ``k_norm`` ([hd], qkv's type) a head becomes x * rsqrt(mean(x^2) +
     eps) * weight; then queries and keys turn by the angles position * ``inv_freq``
-    (fp32 [hd / 2]), in 64 bits, and are rounded once.  8-bit pages get a row x as
+    (fp32 [hd / 2]; angles in 64 bits, the rest in fp32, for the keys of 8-bit pages in 64
+    bits too) and are rounded to their type.  8-bit pages get a row x as
     stored * scale, scale = max |x| / M, stored = nearest(x M / max |x|), M = 127 (int8)
     or 448 (float8_e4m3fn); a row that is not finite reads back as NaN.  A page that
     receives tokens must be named once in the table.  bf16 / f16; hd a multiple of 16 up to
@@ -1741,8 +1742,8 @@ def kv_paged_read(k_pages, v_pages, table, kv_len, length=None, k_scale=None, v_
     pos0 + i, or for short pieces (head dims 64 and 128) :func:`sdpa_decode` with kv_len =
     pos0 + t for all sequences.  The rows from lens[b] on are of no use.
 
-    ``dtype``: 16-bit pages come as they are, 8-bit ones as stored * scale in bf16
-    (default), f16 or fp32.  Rows behind a sequence are 0, or left as they are in
+    ``dtype``: 16-bit pages come as they are, 8-bit ones as stored * scale, an
+    fp32 product rounded to bf16 (default), f16 or fp32.  Rows behind a sequence are 0, or left as they are in
     ``k_out`` / ``v_out`` (given together; (n, hkv, length, hd), unit last stride, not
     overlapping each other or the cache)."""
     name = "kv_paged_read"
