@@ -780,9 +780,9 @@ typedef struct kuiops_paged_layout {
  * pairs (y_i, y_{i + hd/2}) -> (y_i cos - y_{i+hd/2} sin, y_{i+hd/2} cos + y_i
  * sin), the angles in 64 bits, the rest in fp32 (keys of 8-bit pages, and norms whose mean
  * square lies outside 2^-100 .. 2^100: in 64 bits), rounded to their type at the end.
- * q_out: strides sq = batch, head, token.  A page that receives tokens must be named once in the table.  K, V, the
- * scales and q_out must not overlap one another or an input.  dtype BF16 / F16, equal to
- * the pages' unless those are of 8 bits.                                     */
+ * q_out: strides sq = batch, head, token.  A page that receives tokens must be named
+ * once in the table.  K, V, the scales and q_out must not overlap one another or an
+ * input.  dtype BF16 / F16, equal to the pages' unless those are of 8 bits.  */
 KUIOPS_API int kuiops_kv_paged_append(int64_t n, int64_t t, int64_t hq, int dtype, const void *qkv, int64_t ld_tok,
                            int64_t ld_batch, const int32_t *lens, const int32_t *pos0, const float *inv_freq,
                            const void *q_norm, const void *k_norm, double eps, void *q_out, const int64_t sq[3],
@@ -792,9 +792,8 @@ KUIOPS_API int kuiops_kv_paged_append(int64_t n, int64_t t, int64_t hq, int dtyp
 /* The first min(s, kv_len[b]) slots (kv_len: device int32[n], taken as 0 .. width *
  * page) gathered into k_out / v_out (strides batch, head, slot; contiguous rows).
  * Rows behind them are left as they are, or become 0 with `fill`.  The outputs must not
- * overlap each other or an input.  dtype: that of
- * 16-bit pages; BF16, F16 or F32 for 8-bit ones (stored * scale in fp32, then rounded
- * to dtype).                                                                 */
+ * overlap each other or an input.  dtype: that of 16-bit pages; BF16, F16 or F32 for
+ * 8-bit ones (stored * scale in fp32, then rounded to dtype).                */
 KUIOPS_API int kuiops_kv_paged_read(int64_t n, int64_t s, int dtype, const kuiops_paged_layout *at, const void *K,
                          const void *V, const float *k_scale, const float *v_scale, const int32_t *table,
                          const int32_t *kv_len, void *k_out, const int64_t sko[3], void *v_out,

@@ -396,7 +396,7 @@ struct ReadArgs {
 // a row a lane, so that what is written, the larger part, goes out in 16-byte pieces that
 // follow one another.  All loads of a thread are on their way at once, behind its page numbers.
 // What bounds it: the bytes; 8 sequences of 4583 to 8000 rows, 8 heads of 128 in int8, to bf16 with
-// the rows behind them cleared 78 to 80 us, 4.7 TB/s read and written (a large copy 5.1); 16 values
+// the rows behind them cleared 78 us, 4.7 TB/s read and written (a large copy 5.1); 16 values
 // a lane, stored 8 bytes at a time, 85.6.
 template <typename T, int PK, int HD>
 __global__ __launch_bounds__(256) void paged_read_kernel(ReadArgs a) {

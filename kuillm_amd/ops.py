@@ -1742,10 +1742,10 @@ def kv_paged_read(k_pages, v_pages, table, kv_len, length=None, k_scale=None, v_
     pos0 + i, or for short pieces (head dims 64 and 128) :func:`sdpa_decode` with kv_len =
     pos0 + t for all sequences.  The rows from lens[b] on are of no use.
 
-    ``dtype``: 16-bit pages come as they are, 8-bit ones as stored * scale, an
-    fp32 product rounded to bf16 (default), f16 or fp32.  Rows behind a sequence are 0, or left as they are in
-    ``k_out`` / ``v_out`` (given together; (n, hkv, length, hd), unit last stride, not
-    overlapping each other or the cache)."""
+    ``dtype``: 16-bit pages come as they are, 8-bit ones as stored * scale, an fp32
+    product rounded to bf16 (default), f16 or fp32.  Rows behind a sequence are 0, or
+    left as they are in ``k_out`` / ``v_out`` (given together; (n, hkv, length, hd), unit
+    last stride, not overlapping each other or the cache)."""
     name = "kv_paged_read"
     c = _paged_cache(name, k_pages, v_pages, k_scale, v_scale, table)
     if (k_out is None) != (v_out is None) or not _flat_ints(kv_len, c.n):
