@@ -1547,21 +1547,22 @@ def _meet(a, b, ahead) -> bool:
     for st, lo, hi in reversed(steps):
         rest.append((rest[-1][0] + st * lo, rest[-1][1] + st * hi))
     rest.reverse()
-    todo, looked = [(0, ahead - a[2] + 1, ahead + b[2] - 1)], 0
+    todo, seen = [(0, ahead - a[2] + 1)], set()
     while todo:
-        i, least, most = todo.pop()
+        i, least = at = todo.pop()
+        most = least + a[2] + b[2] - 2
         if i == len(steps):
             if least <= 0 <= most:
                 return True
             continue
-        looked += 1
-        if looked > 4096:
-            return True
+        if at in seen:
+            continue
+        seen.add(at)
         st, lo, hi = steps[i]
         low, high = rest[i + 1]
         for d in range(max(lo, -((high - least) // st)), min(hi, (most - low) // st) + 1):
-            todo.append((i + 1, least - d * st, most - d * st))
-            if len(todo) > 4096:
+            todo.append((i + 1, least - d * st))
+            if len(todo) + len(seen) > 1 << 16:
                 return True
     return False
 

@@ -317,6 +317,16 @@ def test_kv_paged_append_refuses_shared_scales_and_pools_that_overlap():
     refuses(INVALID, ops.kv_paged_append, **{**a, "k_pages": heads[:, :2], "v_pages": heads[:, 1:3]})
     rows = torch.zeros(6, 2, 16, 128, dtype=BF)
     takes(ops.kv_paged_append, **{**a, "k_pages": rows[..., 64:], "v_pages": rows[..., :64]})
+    # halves of the same rows, the heads of one in the order of the other's slots
+    rows = torch.zeros(6, 64, 2, 128, dtype=BF)
+    mixed = rows.view(6, 2, 64, 128)
+    for page in (16, 64):
+        k, v = rows[:, :page, :, :64].transpose(1, 2), mixed[:, :, :page, 64:]
+        takes(ops.kv_paged_append, **{**a, "k_pages": k, "v_pages": v})
+        refuses(INVALID, ops.kv_paged_append, **{**a, "k_pages": k, "v_pages": mixed[:, :, :page, 63:127]})
+    large = torch.empty(10, 4096, 8, 256, dtype=BF, device="meta")
+    k, v = (ops._extent(ops._meta(x)) for x in (large[..., :128].transpose(1, 2), large.view(10, 8, 4096, 256)[..., 128:]))
+    assert ops._apart(0, k, 256, v) and not ops._apart(0, k, 254, v)
     # one pool to read keys and values from is no mistake
     for fn, args in ENTRIES[1:]:
         b = args()
