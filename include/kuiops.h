@@ -802,9 +802,10 @@ KUIOPS_API int kuiops_kv_paged_read(int64_t n, int64_t s, int dtype, const kuiop
 /* Attention of the newest tokens over the pages: query i of sequence b is slot
  * kv_len[b] - l + i and sees the slots up to its own that have a page (none: output
  * 0, lse -inf).  What lies elsewhere in the pages, NaN and infinities included,
- * stays out of it.  kv_len: device int32[n]; slots past the table have no page.  Q / O:
- * strides batch, head, query; O must not overlap an input.  lse: fp32 [n][hq][l]
- * (natural log) or null.  scale > 0.  Workspace (slots = width * page): may be 0
+ * stays out of it.  Scores and sums are fp32, whose range values of 2^90 and more, or
+ * scores of 2^127, may pass.  kv_len: device int32[n]; slots past the table have no
+ * page.  Q / O: strides batch, head, query; O must not overlap an input.  lse: fp32
+ * [n][hq][l] (natural log) or null.  scale > 0.  Workspace (slots = width * page): may be 0
  * bytes, 16-byte aligned; its first KUIOPS_SDPA_PAGED_ZEROED bytes must be zero
  * before the first call with it, and every call leaves them zero, whatever its sizes.
  * Calls that share one must not run at the same time.                       */

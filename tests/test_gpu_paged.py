@@ -628,6 +628,23 @@ def test_append_norms_of_rows_that_are_not_finite(cuda):
 
 
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_append_norms_of_rows_that_are_not_finite_in_8_bits(cuda, kind):
+    c = Cache(cuda, BF, kind, 1, 1, 128, 16, 1, seed=29)
+    qkv = gen((1, 4, 3 * 128), BF, 1)
+    for at in (0, 128):                     # the query, the key
+        qkv[0, 0, at + 5], qkv[0, 1, at + 70] = -math.inf, NAN
+        qkv[0, 2, at:at + 128] *= 2.0 ** 100
+    w, freq = torch.ones(128, dtype=BF, device=cuda), frequencies(128).to(cuda)
+    q = ops.kv_paged_append(qkv.to(cuda), freq, None, **c.args(), q_norm=w, k_norm=w)
+    k, v = ops.kv_paged_read(**c.args(), kv_len=ints([4], cuda), length=4)
+    assert torch.isnan(k[0, 0, :2]).all() and torch.isfinite(k[0, 0, 2:]).all() and torch.isfinite(v).all()
+    assert torch.isnan(q[0, 0, 0, [5, 69]]).all() and q[0, 0, 0].isnan().sum() == 2 and torch.isnan(q[0, 0, 1]).all()
+    # a normed row's mean square is 1: values off by 2^-4 (e4m3) and less, their squares by (1 + 2^-4)^2 - 1 < 0.13
+    for x in (q[0, 0, 2:], k[0, 0, 2:]):
+        assert ((x.float().square().mean(-1) - 1).abs() < 0.13).all()
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
 def test_append_ties_go_to_even(cuda, kind):
     # values at every border of the type (x / 2 of its largest and so on): exact in bf16
     c = Cache(cuda, BF, kind, 1, 1, 128, 16, 1, seed=23)
